@@ -41,6 +41,8 @@ BUCKET_DTYPE = np.dtype(
         "itemsize": 40,
     }
 )
+# struct eth_packed_tile (16 bytes)
+PACKED_TILE_DTYPE = np.dtype([("begin", "<i4"), ("len", "<i4"), ("start", "<i4"), ("reserved", "<i4")])
 # struct eth_adam_tensor (64 bytes)
 ADAM_TENSOR_DTYPE = np.dtype(
     {
@@ -102,6 +104,9 @@ SIGNATURES["eth_synthetic_batch"] = [_P, _I64, _I64, _I64, _P, _P, _P, _P]
 SIGNATURES["eth_attn_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["eth_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
 
+SIGNATURES["eth_packed_attn_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["eth_packed_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+
 
 class AttnDesc(ctypes.Structure):
     """struct eth_attn_desc (include/eth_amd.h)."""
@@ -123,6 +128,32 @@ class AttnDesc(ctypes.Structure):
     ]
 
 
+class PackedAttnDesc(ctypes.Structure):
+    """struct eth_packed_attn_desc (include/eth_amd.h)."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("q_strides", ctypes.c_int64 * 2),
+        ("k_strides", ctypes.c_int64 * 2),
+        ("v_strides", ctypes.c_int64 * 2),
+        ("o_strides", ctypes.c_int64 * 2),
+        ("do_strides", ctypes.c_int64 * 2),
+        ("dq_strides", ctypes.c_int64 * 2),
+        ("dk_strides", ctypes.c_int64 * 2),
+        ("dv_strides", ctypes.c_int64 * 2),
+        ("q_tiles", ctypes.c_void_p),
+        ("k_tiles", ctypes.c_void_p),
+        ("n_q_tiles", ctypes.c_int32),
+        ("n_k_tiles", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 # functions returning a value instead of a status
 VALUE_SIGNATURES = {
     "eth_ln_bwd_workspace": ([_I64, _I64], _I64),
@@ -132,6 +163,7 @@ VALUE_SIGNATURES = {
     "eth_gemm_splitk_workspace": ([_I64, _I64, _I32], _I64),
     "eth_gemm_splitk_pays": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32], _I64),
     "eth_embedding_bwd_workspace": ([_I64, _I64], _I64),
+    "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
 }
 GEMM_ACCUMULATE, GEMM_BIAS = 1, 2
 

@@ -1,0 +1,1063 @@
+// Causal attention over sequences of different lengths packed into one row
+// dimension, with query heads that share key and value heads, forward and
+// backward, on CDNA4 matrix cores (v_mfma_f32_32x32x16_{bf16,f16}).
+//
+// Rows [begin, begin + len) of q [T, n, hd], k and v [T, m, hd] are one
+// sequence, n = m * group; query head h reads key/value head h / group:
+//   S_ij = scale q_i . k_j (j <= i in the sequence), P = softmax_j S, O = P V
+//   delta_i = sum dO_i . O_i,  dV_j = sum_i P_ij dO_i
+//   dS = P (dO V^T - delta),   dQ = scale dS K,  dK = scale dS^T Q
+// with dK and dV summed over the queries of all heads of the group.
+//
+// The host lists the tiles (blocks of queries, blocks of keys, blocks of rows
+// that no sequence covers) once for a batch, longest chains first; a workgroup
+// takes one tile of the list and one head or group of heads.
+//
+// Arithmetic and layouts are those of attention.hip: S^T = K Q^T with K rows
+// read in swizzled order, so that P^T stays in registers as the operand of
+// O^T = V^T P^T; 64-row blocks go global->LDS by direct loads into XOR-swizzled
+// images a block ahead; fp32 base-2 softmax.  P and dS are rounded to the
+// inputs' type for the second product, as the matrix cores take it.
+//
+// A block's buffer resource starts at its first row and ends with its
+// sequence's last element, so that rows past the sequence read zeros without a
+// comparison (a neighbour's infinities never meet a zero probability), and
+// offsets within it fit 32 bits whatever the tensors' size.
+#include "attention_tiles.h"
+
+namespace eth {
+
+struct PackIn {
+  const uint16_t* p;
+  int64_t ss, sh;  // strides of row and head (elements); dim contiguous
+};
+struct PackOut {
+  uint16_t* p;
+  int64_t ss, sh;
+};
+
+struct PackArgs {
+  PackIn q, k, v, o, dout;
+  PackOut out, dq, dk, dv;
+  float* lse;    // [n, T] log2-domain: m2 + log2(l)
+  float* delta;  // [n, T] rowsum(dO * O)
+  const eth_packed_tile_t* q_tiles;
+  const eth_packed_tile_t* k_tiles;
+  int64_t T;
+  int n, m, group;
+  int hp;  // query heads per workgroup (1, 2 or 4; divides group)
+  int hd;  // head dim (<= the kernel's D; columns hd..D-1 are zero padding)
+  float scale_log2;  // scale * log2(e)
+  float scale;
+};
+
+__device__ __forceinline__ const uint16_t* row_ptr(const PackIn& t, int64_t row, int h) {
+  return t.p + row * t.ss + (int64_t)h * t.sh;
+}
+__device__ __forceinline__ uint16_t* row_ptr(const PackOut& t, int64_t row, int h) {
+  return t.p + row * t.ss + (int64_t)h * t.sh;
+}
+
+// Direct loads of 64-row blocks of one head of one sequence by four waves:
+// unit u (16 bytes) of the image holds row u / CPR, chunk (u % CPR) ^
+// img_swz(row).  Rows past the sequence and columns past the head dim read
+// zeros (the latter have offsets past any range).
+template <int D>
+struct SeqCopy {
+  static constexpr int CPR = D / 8;  // 16-byte chunks per row
+  static constexpr int PW = D / 32;  // 1 KB pieces per wave
+  int32_t off[PW];
+  const char* base;    // the sequence's first row of head 0
+  int64_t row_bytes, range;
+  int w;
+  __device__ __forceinline__ void init(const PackIn& t, int64_t begin, int len, int hd, int wave, int lane) {
+    base = reinterpret_cast<const char*>(t.p + begin * t.ss);
+    row_bytes = t.ss * 2;
+    range = (int64_t)(len - 1) * row_bytes + hd * 2;
+    w = wave;
+#pragma unroll
+    for (int j = 0; j < PW; ++j) {
+      const int u = (w * PW + j) * 64 + lane;
+      const int r = u / CPR, c = (u % CPR) ^ img_swz<D>(r);
+      off[j] = c * 8 < hd ? (int32_t)(r * row_bytes + c * 16) : kAttnOob;
+    }
+  }
+  // rows r0 .. r0 + 63 of the head at `head` (bytes)
+  __device__ __forceinline__ void issue(uint16_t* S, int r0, int64_t head) const {
+    const int64_t at = r0 * row_bytes;
+    int64_t left = range - at;
+    left = left < 0 ? 0 : (left > 0x7fffffff ? 0x7fffffff : left);
+    const a_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + head + at), (short)0, (int)left,
+                                                          0x00020000);
+#pragma unroll
+    for (int j = 0; j < PW; ++j) {
+      const int32_t o = off[j];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(S + (w * PW + j) * 512),
+                                               16, o, 0, 0, 0);
+    }
+  }
+};
+
+// zeros into `rows` rows from `row0` on of heads h0 .. h0 + nh - 1 (a tile of
+// rows that no sequence covers), by `threads` threads
+__device__ __forceinline__ void zero_rows(const PackOut& t, int64_t row0, int rows, int h0, int nh, int hd,
+                                          int threads) {
+  const int cpr = hd / 8, per = rows * cpr;
+  for (int i = threadIdx.x; i < nh * per; i += threads) {
+    const int h = i / per, r = (i - h * per) / cpr, c = i % cpr;
+    *reinterpret_cast<uint4*>(row_ptr(t, row0 + r, h0 + h) + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// ------------------------------------------------------------------ forward --
+// 4 waves x 32 rows; a row is a (query, head) pair: hp heads of a group share
+// the workgroup's K and V blocks, 128 / hp queries each, so that a short
+// sequence wastes less of a tile and the waves' chains are of equal length.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a) {
+  constexpr int KS = D / 16;  // k-steps over the head dim
+  constexpr int DT = D / 32;  // 32-row tiles over the head dim
+  constexpr int IMG = kBKV * D;  // elements of one image
+  __shared__ __attribute__((aligned(16))) uint16_t K0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t K1[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t V0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t V1[IMG];
+
+  // workgroups of one key/value head a multiple of m apart: on one die for
+  // m % 8 == 0, whose L2 then serves the shared rows
+  const int hbs = a.n / a.hp, hb = blockIdx.x % hbs;
+  const int kvh = hb % a.m, h0 = kvh * a.group + hb / a.m * a.hp;
+  const eth_packed_tile_t tile = a.q_tiles[blockIdx.x / hbs];
+  const int64_t begin = tile.begin;
+  if (tile.len < 0) {
+    zero_rows(a.out, begin, -tile.len, h0, a.hp, a.hd, kAttnThreads);
+    for (int i = threadIdx.x; i < a.hp * -tile.len; i += kAttnThreads)
+      a.lse[(int64_t)(h0 + i / -tile.len) * a.T + begin + i % -tile.len] = -INFINITY;
+    return;
+  }
+  const int len = tile.len, bq = kBQ / a.hp;
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  const int h = h0 + w % a.hp;
+  const int q0 = tile.start + w / a.hp * 32;
+  const int q = q0 + (lane & 31);
+  const bool real = q < len;
+  const float sl2 = a.scale_log2;
+
+  SeqCopy<D> kc, vc;
+  kc.init(a.k, begin, len, a.hd, w, lane);
+  vc.init(a.v, begin, len, a.hd, w, lane);
+  const int64_t kh = kvh * a.k.sh * 2, vh = kvh * a.v.sh * 2;
+  const int qend = min(tile.start + bq, len);  // past the tile's last query
+  const int nkv = (qend + kBKV - 1) / kBKV;
+  kc.issue(K0, 0, kh);
+  vc.issue(V0, 0, vh);
+
+  uint4 qf[KS];
+  {
+    const uint16_t* qp = row_ptr(a.q, begin + q, h);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = load_row16<true>(qp, real, ks * 16 + hl * 8, a.hd);
+  }
+  a_f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = a_f32x16{};
+  // running max (log2 units) and sum for query q; the lowest finite start
+  // keeps exp2(-inf - m) at 0 for masked keys
+  float m = -3.4028234e38f, l = 0.f;
+
+  int aoff[KS], toff[DT][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) aoff[ks] = img_row_off<D>(lane, ks);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) toff[dt][hi] = img_tr_off<D>(lane, dt, hi);
+  vm_wait_all();
+  __syncthreads();
+
+  auto block = [&](int j, auto cur_c) __attribute__((always_inline)) {
+    constexpr int cur = decltype(cur_c)::value;
+    const int kv0 = j * kBKV;
+    if (j + 1 < nkv) {  // the next block, a block ahead
+      kc.issue(cur ? K0 : K1, kv0 + kBKV, kh);
+      vc.issue(cur ? V0 : V1, kv0 + kBKV, vh);
+    }
+    if (kv0 <= q0 + 31 && q0 < len) {  // wave has at least one unmasked key in the block
+      const uint16_t* ki = cur ? K1 : K0;
+      const uint16_t* vi = cur ? V1 : V0;
+      // S^T = K Q^T (raw scores; lane = query, registers = 32 of the keys);
+      // fragment order pinned as in the equal-length kernel
+      a_f32x16 sc[2];
+      {
+        uint4 kr[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kr[ks] = *reinterpret_cast<const uint4*>(ki + aoff[ks]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          sc[0] = mma<FP16>(kr[ks], qf[ks], ks == 0 ? a_f32x16{} : sc[0]);
+          __builtin_amdgcn_sched_barrier(0);
+          kr[ks] = *reinterpret_cast<const uint4*>(ki + 32 * D + aoff[ks]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) sc[1] = mma<FP16>(kr[ks], qf[ks], ks == 0 ? a_f32x16{} : sc[1]);
+      }
+      if (kv0 + kBKV - 1 > q0) {  // diagonal block: mask keys after the query
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (kv0 + t * 32 + swz_row(r, hl) > q) sc[t][r] = -INFINITY;
+      }
+      float mx = sc[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mnew = fmaxf(m, mx * sl2);
+      // m is the exponent offset, kept within kRescaleLog2 below the running
+      // max (most blocks then skip the rescale); O / l and lse do not depend on it
+      if (__any(mnew > m + kRescaleLog2)) {
+        const float alpha = fast_exp2(m - mnew);
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[t][r] *= alpha;
+        m = mnew;
+      }
+      float rs = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = fast_exp2(__builtin_fmaf(sc[t][r], sl2, -m));
+          sc[t][r] = p;
+          rs += p;
+        }
+      l += rs;
+      // O^T += V^T P^T over the 64 keys (4 k-steps of 16)
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        const int t = kk >> 1, e0 = (kk & 1) * 8;
+        const uint4 pb = make_uint4(pack2<FP16>(sc[t][e0 + 0], sc[t][e0 + 1]), pack2<FP16>(sc[t][e0 + 2], sc[t][e0 + 3]),
+                                    pack2<FP16>(sc[t][e0 + 4], sc[t][e0 + 5]), pack2<FP16>(sc[t][e0 + 6], sc[t][e0 + 7]));
+        const uint16_t* vp = vi + kk * 16 * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mma<FP16>(img_tr(vp, toff[dt][0], toff[dt][1]), pb, o[dt]);
+      }
+    }
+    vm_wait_all();  // the next block's rows have landed
+    __syncthreads();  // this block's images free, the next block's visible
+  };
+  int j = 0;
+  for (; j + 1 < nkv; j += 2) {
+    block(j, std::integral_constant<int, 0>{});
+    block(j + 1, std::integral_constant<int, 1>{});
+  }
+  if (j < nkv) block(j, std::integral_constant<int, 0>{});
+  l += __shfl_xor(l, 32, 64);
+  if (!real) return;  // a row past the sequence
+  const float inv = 1.0f / l;
+  uint16_t* op = row_ptr(a.out, begin + q, h);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (t * 32 + g * 8 >= a.hd) continue;  // hd % 8 == 0: whole 8-column groups
+      uint2 v;
+      v.x = pack2<FP16>(o[t][g * 4 + 0] * inv, o[t][g * 4 + 1] * inv);
+      v.y = pack2<FP16>(o[t][g * 4 + 2] * inv, o[t][g * 4 + 3] * inv);
+      *reinterpret_cast<uint2*>(op + t * 32 + g * 8 + hl * 4) = v;
+    }
+  if (hl == 0) a.lse[(int64_t)h * a.T + begin + q] = m + log2f(l);
+}
+
+// ------------------------------------------------------------ backward: dQ --
+// Workgroups as in the forward.  Runs first: it also writes delta, which the
+// dK/dV kernels read.
+template <int D, bool FP16>
+__global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs a) {
+  constexpr int KS = D / 16, DT = D / 32;
+  constexpr int IMG = kBKV * D;  // elements of one image
+  __shared__ __attribute__((aligned(16))) uint16_t K0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t K1[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t V0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t V1[IMG];
+
+  const int hbs = a.n / a.hp, hb = blockIdx.x % hbs;
+  const int kvh = hb % a.m, h0 = kvh * a.group + hb / a.m * a.hp;
+  const eth_packed_tile_t tile = a.q_tiles[blockIdx.x / hbs];
+  const int64_t begin = tile.begin;
+  if (tile.len < 0) {
+    zero_rows(a.dq, begin, -tile.len, h0, a.hp, a.hd, kAttnThreads);
+    return;
+  }
+  const int len = tile.len, bq = kBQ / a.hp;
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  const int h = h0 + w % a.hp;
+  const int q0 = tile.start + w / a.hp * 32;
+  const int q = q0 + (lane & 31);
+  const bool real = q < len;
+
+  SeqCopy<D> kc, vc;
+  kc.init(a.k, begin, len, a.hd, w, lane);
+  vc.init(a.v, begin, len, a.hd, w, lane);
+  const int64_t kh = kvh * a.k.sh * 2, vh = kvh * a.v.sh * 2;
+  const int qend = min(tile.start + bq, len);
+  const int nkv = (qend + kBKV - 1) / kBKV;
+  kc.issue(K0, 0, kh);
+  vc.issue(V0, 0, vh);
+
+  uint4 qf[KS], of[KS];
+  {
+    const uint16_t* qp = row_ptr(a.q, begin + q, h);
+    const uint16_t* op = row_ptr(a.dout, begin + q, h);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = load_row16<true>(qp, real, ks * 16 + hl * 8, a.hd);
+      of[ks] = load_row16<true>(op, real, ks * 16 + hl * 8, a.hd);
+    }
+  }
+  const int64_t srow = (int64_t)h * a.T + begin + q;
+  const float lse = real ? a.lse[srow] : 1e30f;
+  // delta = rowsum(dO * O) for this query, from the dO fragments already in
+  // registers (the two half-waves hold alternate 8-element chunks of the row)
+  float del = 0.f;
+  {
+    const uint16_t* opp = row_ptr(a.o, begin + q, h);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const uint4 ov = load_row16<true>(opp, real, ks * 16 + hl * 8, a.hd);
+      const uint32_t ow[4] = {ov.x, ov.y, ov.z, ov.w};
+      const uint32_t dw[4] = {of[ks].x, of[ks].y, of[ks].z, of[ks].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        del += to_f<FP16>((uint16_t)(ow[e] & 0xffffu)) * to_f<FP16>((uint16_t)(dw[e] & 0xffffu));
+        del += to_f<FP16>((uint16_t)(ow[e] >> 16)) * to_f<FP16>((uint16_t)(dw[e] >> 16));
+      }
+    }
+    del += __shfl_xor(del, 32, 64);
+    if (hl == 0 && real) a.delta[srow] = del;
+  }
+  a_f32x16 dq[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) dq[t] = a_f32x16{};
+
+  int aoff[KS], toff[DT][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) aoff[ks] = img_row_off<D>(lane, ks);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) toff[dt][hi] = img_tr_off<D>(lane, dt, hi);
+  vm_wait_all();
+  __syncthreads();
+
+  auto block = [&](int j, auto cur_c) __attribute__((always_inline)) {
+    constexpr int cur = decltype(cur_c)::value;
+    const int kv0 = j * kBKV;
+    if (j + 1 < nkv) {  // the next block, a block ahead
+      kc.issue(cur ? K0 : K1, kv0 + kBKV, kh);
+      vc.issue(cur ? V0 : V1, kv0 + kBKV, vh);
+    }
+    const uint16_t* ki = cur ? K1 : K0;
+    const uint16_t* vi = cur ? V1 : V0;
+    // one 32-key tile at a time: S^T = K Q^T, dP^T = V dO^T (lane = query),
+    // dS^T, then dQ^T += K^T dS^T over those 32 keys
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int kt0 = kv0 + t * 32;
+      if (kt0 > q0 + 31 || q0 >= len) continue;  // every key of the tile follows the wave's queries
+      a_f32x16 s = a_f32x16{}, dp = a_f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = mma<FP16>(*reinterpret_cast<const uint4*>(ki + t * 32 * D + aoff[ks]), qf[ks], s);
+        dp = mma<FP16>(*reinterpret_cast<const uint4*>(vi + t * 32 * D + aoff[ks]), of[ks], dp);
+      }
+      // causal mask only on the tiles that cross the diagonal
+      auto dsoft = [&](auto masked) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lse));
+          dp[r] = p * (dp[r] - del);
+          // (the product: a masked key's own infinities stay out of it)
+          if (decltype(masked)::value && kt0 + swz_row(r, hl) > q) dp[r] = 0.f;
+        }
+      };
+      if (kt0 + 31 > q0)
+        dsoft(std::true_type{});
+      else
+        dsoft(std::false_type{});
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        const int kk = t * 2 + k2, e0 = k2 * 8;
+        const uint4 sb = make_uint4(pack2<FP16>(dp[e0 + 0], dp[e0 + 1]), pack2<FP16>(dp[e0 + 2], dp[e0 + 3]),
+                                    pack2<FP16>(dp[e0 + 4], dp[e0 + 5]), pack2<FP16>(dp[e0 + 6], dp[e0 + 7]));
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+          dq[dt] = mma<FP16>(img_tr(ki + kk * 16 * D, toff[dt][0], toff[dt][1]), sb, dq[dt]);
+      }
+    }
+    vm_wait_all();  // the next block's rows have landed
+    __syncthreads();  // this block's images free, the next block's visible
+  };
+  int j = 0;
+  for (; j + 1 < nkv; j += 2) {
+    block(j, std::integral_constant<int, 0>{});
+    block(j + 1, std::integral_constant<int, 1>{});
+  }
+  if (j < nkv) block(j, std::integral_constant<int, 0>{});
+  if (!real) return;
+  uint16_t* dqp = row_ptr(a.dq, begin + q, h);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (t * 32 + g * 8 >= a.hd) continue;
+      uint2 v;
+      v.x = pack2<FP16>(dq[t][g * 4 + 0] * a.scale, dq[t][g * 4 + 1] * a.scale);
+      v.y = pack2<FP16>(dq[t][g * 4 + 2] * a.scale, dq[t][g * 4 + 3] * a.scale);
+      *reinterpret_cast<uint2*>(dqp + t * 32 + g * 8 + hl * 4) = v;
+    }
+}
+
+// The steps of a key tile: the 64-query blocks from the tile's first query on,
+// of every query head of the group, one head after the other, so that dK and
+// dV of a shared head are summed in registers in a fixed order.
+struct PackStep {
+  int head, block;  // query head within the group, 64-query block
+  __device__ __forceinline__ void next(int first, int nq) {
+    if (++block == nq) {
+      block = first;
+      ++head;
+    }
+  }
+};
+
+// ------------------------------------- backward: dK, dV, head dims to 96 --
+// dK and dV of 32 keys in one wave, four waves per 128 keys, one barrier per
+// 64 queries (see attn_bwd_dkdv_kernel).
+template <int D, bool FP16>
+__global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackArgs a) {
+  static_assert(D == 64 || D == 96, "wider heads run on the paired kernel");
+  constexpr int KS = D / 16, DT = D / 32, CPR = D / 8;
+  constexpr int IMG = kBQ2 * D;  // elements of one image
+  // an array per image, so the compiler can tell the direct loads into one
+  // from the fragment reads of another
+  __shared__ __attribute__((aligned(16))) uint16_t Q0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t Q1[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t O0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t O1[IMG];
+  __shared__ __attribute__((aligned(16))) float lse_s[2][kBQ2];
+  __shared__ __attribute__((aligned(16))) float del_s[2][kBQ2];
+
+  const int kvh = blockIdx.x % a.m;
+  const eth_packed_tile_t tile = a.k_tiles[blockIdx.x / a.m];
+  const int64_t begin = tile.begin;
+  if (tile.len < 0) {
+    zero_rows(a.dk, begin, -tile.len, kvh, 1, a.hd, kAttnThreads);
+    zero_rows(a.dv, begin, -tile.len, kvh, 1, a.hd, kAttnThreads);
+    return;
+  }
+  const int len = tile.len;
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  const int rt = threadIdx.x;
+  const int k0 = tile.start + w * 32;
+  const int key = k0 + (lane & 31);
+
+  SeqCopy<D> qc, oc;
+  qc.init(a.q, begin, len, a.hd, w, lane);
+  oc.init(a.dout, begin, len, a.hd, w, lane);
+  // per-query statistics: threads 0-63 lse, 64-127 delta (a row past the
+  // sequence gets lse = 1e30, so P = 0); delta is negated when it is stored,
+  // not here, where the use would wait for every load in flight
+  const float* stats = rt < 64 ? a.lse : a.delta;
+  const int si = rt & 63;
+  auto stat = [&](const PackStep& st) __attribute__((always_inline)) {
+    float v = rt < 64 ? 1e30f : 0.f;
+    const int qi = st.block * kBQ2 + si;
+    if (qi < len) v = stats[(int64_t)(kvh * a.group + st.head) * a.T + begin + qi];
+    return v;
+  };
+  auto stat_store = [&](int p, float v) __attribute__((always_inline)) {
+    if (rt < 64)
+      lse_s[p][rt] = v;
+    else if (rt < 128)
+      del_s[p][rt - 64] = -v;
+  };
+  auto issue = [&](uint16_t* qi, uint16_t* oi, const PackStep& st) __attribute__((always_inline)) {
+    const int64_t h = kvh * a.group + st.head;
+    qc.issue(qi, st.block * kBQ2, h * a.q.sh * 2);
+    oc.issue(oi, st.block * kBQ2, h * a.dout.sh * 2);
+  };
+  const int first = tile.start / kBQ2, nq = (len + kBQ2 - 1) / kBQ2;
+  const int steps = (nq - first) * a.group;
+  PackStep cur{0, first}, nxt = cur;
+  nxt.next(first, nq);
+  float stat_n = 0.f;
+  issue(Q0, O0, cur);
+  if (rt < 128) stat_n = stat(cur);
+
+  uint4 kf[KS], vf[KS];  // this lane's key: K and V rows, the B operands of S and dP
+  {
+    const uint16_t* kp = row_ptr(a.k, begin + key, kvh);
+    const uint16_t* vp = row_ptr(a.v, begin + key, kvh);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      kf[ks] = load_row16<true>(kp, key < len, ks * 16 + hl * 8, a.hd);
+      vf[ks] = load_row16<true>(vp, key < len, ks * 16 + hl * 8, a.hd);
+    }
+  }
+  a_f32x16 dk[DT], dv[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) dk[t] = dv[t] = a_f32x16{};
+
+  int aoff[KS], toff[DT][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) aoff[ks] = img_row_off<D>(lane, ks);
+#pragma unroll
+  for (int d2 = 0; d2 < DT; ++d2)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) toff[d2][hi] = img_tr_off<D>(lane, d2, hi);
+  auto bfrag = [&](const uint16_t* img, int kk, int d2) __attribute__((always_inline)) {
+    return img_tr(img + kk * 16 * D, toff[d2][0], toff[d2][1]);
+  };
+  vm_wait_all();
+  stat_store(0, stat_n);
+  __syncthreads();
+
+  auto step = [&](int i, auto par_c) __attribute__((always_inline)) {
+    constexpr int P = decltype(par_c)::value;
+    const int qs0 = cur.block * kBQ2;
+    const bool more = i + 1 < steps;
+    if (more) {  // the next step's rows into the other images, a step ahead
+      issue(P ? Q0 : Q1, P ? O0 : O1, nxt);
+      if (rt < 128) stat_n = stat(nxt);
+    }
+    const uint16_t* qi = P ? Q1 : Q0;
+    const uint16_t* oi = P ? O1 : O0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int qt = qs0 + t * 32;
+      if (qt + 31 < k0 || qt >= len || k0 >= len) continue;  // every query precedes the wave's keys, or no row at all
+      a_f32x16 s = a_f32x16{}, dp;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 d4 = *reinterpret_cast<const float4*>(&del_s[P][t * 32 + swz_row(4 * g, hl)]);
+        dp[4 * g + 0] = d4.x;
+        dp[4 * g + 1] = d4.y;
+        dp[4 * g + 2] = d4.z;
+        dp[4 * g + 3] = d4.w;
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        s = mma<FP16>(*reinterpret_cast<const uint4*>(qi + t * 32 * D + aoff[ks]), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        dp = mma<FP16>(*reinterpret_cast<const uint4*>(oi + t * 32 * D + aoff[ks]), vf[ks], dp);
+      // P; query of register r = qt + swz_row(r, hl); the causal mask only on
+      // the tiles that cross the diagonal
+      auto probs = [&](auto masked) __attribute__((always_inline)) {
+        const int kq = key - qt - 8 * hl;  // masked when > swz_row(r, 0)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 l4 = *reinterpret_cast<const float4*>(&lse_s[P][t * 32 + swz_row(4 * g, hl)]);
+          const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            float p = fast_exp2(__builtin_fmaf(s[r], a.scale_log2, -lv[e]));
+            if (decltype(masked)::value && kq > swz_row(r, 0)) p = 0.f;
+            s[r] = p;
+          }
+        }
+      };
+      if (qt < k0 + 31)
+        probs(std::true_type{});
+      else
+        probs(std::false_type{});
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        const int kk = t * 2 + k2, e0 = k2 * 8;
+        const uint4 pa = make_uint4(pack2<FP16>(s[e0 + 0], s[e0 + 1]), pack2<FP16>(s[e0 + 2], s[e0 + 3]),
+                                    pack2<FP16>(s[e0 + 4], s[e0 + 5]), pack2<FP16>(s[e0 + 6], s[e0 + 7]));
+#pragma unroll
+        for (int d2 = 0; d2 < DT; ++d2) dv[d2] = mma<FP16>(pa, bfrag(oi, kk, d2), dv[d2]);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = s[r] * dp[r];
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        const int kk = t * 2 + k2, e0 = k2 * 8;
+        const uint4 sa = make_uint4(pack2<FP16>(dp[e0 + 0], dp[e0 + 1]), pack2<FP16>(dp[e0 + 2], dp[e0 + 3]),
+                                    pack2<FP16>(dp[e0 + 4], dp[e0 + 5]), pack2<FP16>(dp[e0 + 6], dp[e0 + 7]));
+#pragma unroll
+        for (int d2 = 0; d2 < DT; ++d2) dk[d2] = mma<FP16>(sa, bfrag(qi, kk, d2), dk[d2]);
+      }
+    }
+    cur = nxt;
+    nxt.next(first, nq);
+    vm_wait_all();  // the next step's rows and statistics have landed
+    if (more) stat_store(P ^ 1, stat_n);
+    __syncthreads();  // this step's images free, the next step's visible
+  };
+  int i = 0;
+  for (; i + 1 < steps; i += 2) {
+    step(i, std::integral_constant<int, 0>{});
+    step(i + 1, std::integral_constant<int, 1>{});
+  }
+  if (i < steps) step(i, std::integral_constant<int, 0>{});
+
+  // out through LDS in 16-byte row chunks: lane holds d = t*32 + lane%32 for
+  // keys acc_row(r, hl); dV by way of the dO images, dK of the Q images
+  static_assert(2 * 32 * D <= IMG, "two waves' staging fits an image");
+  uint16_t* sv = (w < 2 ? O0 : O1) + (w & 1) * 32 * D;
+  uint16_t* sk = (w < 2 ? Q0 : Q1) + (w & 1) * 32 * D;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int o = acc_row(r, hl) * D + t * 32 + (lane & 31);
+      sv[o] = from_f<FP16>(dv[t][r]);
+      sk[o] = from_f<FP16>(dk[t][r] * a.scale);
+    }
+  wave_lds_fence();  // a wave reads back only its own rows
+#pragma unroll
+  for (int i = 0; i < 32 * CPR / 64; ++i) {
+    const int c = i * 64 + lane, kr = c / CPR, col = (c % CPR) * 8;
+    if (k0 + kr >= len || col >= a.hd) continue;
+    *reinterpret_cast<uint4*>(row_ptr(a.dv, begin + k0 + kr, kvh) + col) =
+        *reinterpret_cast<const uint4*>(sv + kr * D + col);
+    *reinterpret_cast<uint4*>(row_ptr(a.dk, begin + k0 + kr, kvh) + col) =
+        *reinterpret_cast<const uint4*>(sk + kr * D + col);
+  }
+}
+
+// ------------------------------ backward: dK, dV paired, head dims to 128 --
+// Eight waves: wave w < 4 (the dV wave) and wave w + 4 (the dK wave) own the
+// same 32 keys and share a SIMD, skewed by half a step (see
+// attn_bwd_dkdv_x128_kernel): in step j the dV wave computes S(j) and P(j),
+// hands P (fp32) over through LDS and adds P(j)^T dO(j) into dV, while the dK
+// wave first finishes step j-1 and then computes dP(j) - delta.  Three Q
+// images, two dO images and two P buffers (145 KB of LDS).
+template <bool FP16>
+__global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kernel(PackArgs a) {
+  constexpr int D = 128, KS = D / 16, DT = D / 32;
+  constexpr int IMG = kBQ2 * D;  // elements of one image
+  __shared__ __attribute__((aligned(16))) uint16_t Qx[3 * IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t O0[IMG];
+  __shared__ __attribute__((aligned(16))) uint16_t O1[IMG];
+  __shared__ a_u32x4 Ps[2][4][2][4][64];
+  __shared__ __attribute__((aligned(16))) float lse_s[2][kBQ2];
+  __shared__ __attribute__((aligned(16))) float del_s[2][kBQ2];
+
+  const int kvh = blockIdx.x % a.m;
+  const eth_packed_tile_t tile = a.k_tiles[blockIdx.x / a.m];
+  const int64_t begin = tile.begin;
+  if (tile.len < 0) {
+    zero_rows(a.dk, begin, -tile.len, kvh, 1, a.hd, 2 * kAttnThreads);
+    zero_rows(a.dv, begin, -tile.len, kvh, 1, a.hd, 2 * kAttnThreads);
+    return;
+  }
+  const int len = tile.len;
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // wave-uniform
+  const int w = wv & 3;
+  const bool dkw = wv >= 4;  // the dK wave of its pair
+  const int rt = threadIdx.x & (kAttnThreads - 1);
+  const int k0 = tile.start + w * 32;
+  const int key = k0 + (lane & 31);
+
+  // B operands of the first product: K rows (S = Q K^T) in the dV wave, V
+  // rows (dP = dO V^T) in the dK wave
+  uint4 kf[KS];
+  {
+    const uint16_t* kp = row_ptr(dkw ? a.v : a.k, begin + key, kvh);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = load_row16<true>(kp, key < len, ks * 16 + hl * 8, a.hd);
+  }
+  a_f32x16 acc[DT];  // dV in the dV wave, dK in the dK wave
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = a_f32x16{};
+
+  // direct loads: the dV waves move Q, the dK waves dO
+  SeqCopy<D> sc;
+  sc.init(dkw ? a.dout : a.q, begin, len, a.hd, w, lane);
+  const int64_t head_bytes = (dkw ? a.dout.sh : a.q.sh) * 2;
+  auto issue = [&](uint16_t* img, const PackStep& st) __attribute__((always_inline)) {
+    sc.issue(img, st.block * kBQ2, (kvh * a.group + st.head) * head_bytes);
+  };
+  int aoff[KS], toff[DT][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) aoff[ks] = img_row_off<D>(lane, ks);
+#pragma unroll
+  for (int d2 = 0; d2 < DT; ++d2)
+#pragma unroll
+    for (int hi = 0; hi < 2; ++hi) toff[d2][hi] = img_tr_off<D>(lane, d2, hi);
+  auto bfrag = [&](const uint16_t* img, int kk, int d2) __attribute__((always_inline)) {
+    return img_tr(img + kk * 16 * D, toff[d2][0], toff[d2][1]);
+  };
+  // acc += X^T B over a step's 64 queries: X (P or dS, one 32-query tile per
+  // t) as the A operand, B from the transposing reads of `img`, four B
+  // fragments in flight (order pinned: the scheduler otherwise hoists every
+  // read and runs out of registers).  With `pbuf` (the dK wave), tile t's X is
+  // first formed as dS = P (dP - delta) from P in `pbuf`.
+  auto second = [&](a_f32x16 (&x)[2], const uint16_t* img, const a_u32x4 (*pbuf)[2][4][64])
+                    __attribute__((always_inline)) {
+    uint4 fb[DT];
+#pragma unroll
+    for (int d2 = 0; d2 < DT; ++d2) fb[d2] = bfrag(img, 0, d2);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (pbuf) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const a_u32x4 pv = pbuf[w][t][g][lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[t][4 * g + e] = __uint_as_float(pv[e]) * x[t][4 * g + e];
+        }
+      }
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
+        const int kk = t * 2 + k2, e0 = k2 * 8;
+        const uint4 pa = make_uint4(pack2<FP16>(x[t][e0 + 0], x[t][e0 + 1]), pack2<FP16>(x[t][e0 + 2], x[t][e0 + 3]),
+                                    pack2<FP16>(x[t][e0 + 4], x[t][e0 + 5]), pack2<FP16>(x[t][e0 + 6], x[t][e0 + 7]));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d2 = 0; d2 < DT; ++d2) {
+          acc[d2] = mma<FP16>(pa, fb[d2], acc[d2]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (kk < 3) fb[d2] = bfrag(img, kk + 1, d2);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+  };
+  // x = (rows of img) kf^T over the 64 queries of a step, starting at x0(t):
+  // S (dV wave) or dP (dK wave), query of register r of tile t = t*32 +
+  // swz_row(r, hl); a rolling window of four A fragments
+  auto first_product = [&](a_f32x16 (&x)[2], const uint16_t* img, auto x0) __attribute__((always_inline)) {
+    auto afrag = [&](int i) __attribute__((always_inline)) {  // fragment i = t*KS + ks
+      return *reinterpret_cast<const uint4*>(img + (i / KS) * 32 * D + aoff[i % KS]);
+    };
+    uint4 fa[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fa[i] = afrag(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const int i = t * KS + ks;
+        x[t] = mma<FP16>(fa[i & 3], kf[ks], ks == 0 ? x0(t) : x[t]);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 4 < 2 * KS) fa[i & 3] = afrag(i + 4);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+
+  const int first = tile.start / kBQ2, nq = (len + kBQ2 - 1) / kBQ2;
+  const int n = (nq - first) * a.group;
+  auto stat = [&](const PackStep& st) __attribute__((always_inline)) {
+    float v = dkw ? 0.f : 1e30f;
+    const int qi = st.block * kBQ2 + rt;
+    if (qi < len) v = (dkw ? a.delta : a.lse)[(int64_t)(kvh * a.group + st.head) * a.T + begin + qi];
+    return v;
+  };
+  // (delta is negated here: at the load, the use would wait for the step's
+  // direct loads too)
+  auto stat_store = [&](int p, float v) __attribute__((always_inline)) {
+    if (dkw)
+      del_s[p][rt] = -v;
+    else
+      lse_s[p][rt] = v;
+  };
+  PackStep cur{0, first}, nxt = cur;
+  nxt.next(first, nq);
+  float stat_n = 0.f;
+  issue(dkw ? O0 : Qx, cur);
+  if (rt < kBQ2) stat_n = stat(cur);
+  vm_wait_all();
+  if (rt < kBQ2) stat_store(0, stat_n);
+  __syncthreads();
+
+  a_f32x16 x[2];  // S then P (dV wave); dP - delta, then dS (dK wave)
+  const bool any = k0 < len;
+  bool active_prev = false;
+  // step j (Q image j % 3; dO image, P buffer and statistics j % 2 = P, a
+  // template constant)
+  auto step = [&](int j, int qslot, auto par_c, auto role_c) __attribute__((always_inline)) {
+    constexpr int P = decltype(par_c)::value;
+    constexpr bool DKW = decltype(role_c)::value;  // the role, a constant here
+    const int qs0 = cur.block * kBQ2;
+    const int qnext = qslot == 2 ? 0 : qslot + 1, qprev = qslot == 0 ? 2 : qslot - 1;
+    // the next step's rows into idle images; the dV waves issue theirs behind
+    // their reads of this step's Q (one array holds the three Q images, so
+    // the compiler waits for loads in flight to it before a read)
+    auto next = [&]() __attribute__((always_inline)) {
+      if (j + 1 < n) {
+        issue(DKW ? (P ? O0 : O1) : Qx + qnext * IMG, nxt);
+        if (rt < kBQ2) stat_n = stat(nxt);
+      }
+    };
+    if constexpr (DKW) next();
+    // a pair whose keys all follow every query of a step skips its work
+    const bool active = any && qs0 + kBQ2 - 1 >= k0;
+    // the sub-products are fenced from each other: the scheduler otherwise
+    // hoists every fragment read of the next product above the current
+    // one and runs out of registers
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!DKW) {
+      if (active) first_product(x, Qx + qslot * IMG, [](int) { return a_f32x16{}; });
+      __builtin_amdgcn_sched_barrier(0);
+      next();
+      __builtin_amdgcn_sched_barrier(0);
+      if (active) {
+        const bool diag = qs0 < k0 + 31;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          auto probs = [&](auto masked) __attribute__((always_inline)) {
+            // the causal mask: query qs0 + t*32 + swz_row(r, hl) precedes the
+            // key when kq > t*32 + swz_row(r, 0) (a constant per register)
+            const int kq = key - qs0 - 8 * hl;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              // lse of the 4 queries of registers 4g..4g+3 (consecutive)
+              const float4 l4 = *reinterpret_cast<const float4*>(&lse_s[P][t * 32 + swz_row(4 * g, hl)]);
+              const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int r = 4 * g + e;
+                float p = fast_exp2(__builtin_fmaf(x[t][r], a.scale_log2, -lv[e]));
+                if (decltype(masked)::value && kq > t * 32 + swz_row(r, 0)) p = 0.f;
+                x[t][r] = p;
+              }
+            }
+          };
+          if (diag)
+            probs(std::true_type{});
+          else
+            probs(std::false_type{});
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            Ps[P][w][t][g][lane] = a_u32x4{__float_as_uint(x[t][4 * g]), __float_as_uint(x[t][4 * g + 1]),
+                                           __float_as_uint(x[t][4 * g + 2]), __float_as_uint(x[t][4 * g + 3])};
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        second(x, P ? O1 : O0, nullptr);
+      }
+    } else {
+      if (active_prev)  // finish step j-1: dS = P (dP - delta), dK += dS^T Q
+        second(x, Qx + qprev * IMG, Ps[P ^ 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (active) {
+        // dP - delta: the accumulator starts at -delta (stored negated)
+        first_product(x, P ? O1 : O0, [&](int t) __attribute__((always_inline)) {
+          a_f32x16 d;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float4 d4 = *reinterpret_cast<const float4*>(&del_s[P][t * 32 + swz_row(4 * g, hl)]);
+            d[4 * g + 0] = d4.x;
+            d[4 * g + 1] = d4.y;
+            d[4 * g + 2] = d4.z;
+            d[4 * g + 3] = d4.w;
+          }
+          return d;
+        });
+      }
+    }
+    active_prev = active;
+    cur = nxt;
+    nxt.next(first, nq);
+    __builtin_amdgcn_sched_barrier(0);
+    vm_wait_all();  // the next step's rows and statistics have landed
+    if (j + 1 < n && rt < kBQ2) stat_store(P ^ 1, stat_n);
+    __syncthreads();  // P(j) handed over; images of step j-1 free
+  };
+  // each role runs its own copy of the step loop (the same barriers in the
+  // same order), so neither keeps the other's values alive
+  auto run = [&](auto role_c) __attribute__((always_inline)) {
+    int j = 0, qslot = 0;
+    for (; j + 1 < n; j += 2) {
+      step(j, qslot, std::integral_constant<int, 0>{}, role_c);
+      qslot = qslot == 2 ? 0 : qslot + 1;
+      step(j + 1, qslot, std::integral_constant<int, 1>{}, role_c);
+      qslot = qslot == 2 ? 0 : qslot + 1;
+    }
+    if (j < n) {
+      step(j, qslot, std::integral_constant<int, 0>{}, role_c);
+      qslot = qslot == 2 ? 0 : qslot + 1;
+    }
+    // the dK waves finish the last step (its P is in buffer (n - 1) % 2)
+    if (decltype(role_c)::value && active_prev) {
+      const int pb = (n - 1) & 1, qlast = qslot == 0 ? 2 : qslot - 1;
+      second(x, Qx + qlast * IMG, Ps[pb]);
+    }
+  };
+  if (dkw)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
+  // the 32 x 128 tile of each wave (dV or dK, rounded to 16 bits) through
+  // LDS, then out in 16-byte row chunks: lane holds d = t*32 + lane%32 for
+  // keys acc_row(r, hl); the staging rows are padded by 8 elements
+  constexpr int SL = D + 8;
+  __syncthreads();  // every image and P buffer read
+  // 8.5 KB per wave: the dV waves' in the Q images, the dK waves' in the P buffers
+  uint16_t* stage = (dkw ? reinterpret_cast<uint16_t*>(&Ps[0][0][0][0][0]) : Qx) + w * 32 * SL;
+  static_assert(4 * 32 * SL <= 3 * IMG && 4 * 32 * SL * 2 <= (int)sizeof(Ps), "staging fits");
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      stage[acc_row(r, hl) * SL + t * 32 + (lane & 31)] = from_f<FP16>(dkw ? acc[t][r] * a.scale : acc[t][r]);
+  wave_lds_fence();  // the wave reads back only its own rows
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = i * 64 + lane, kr = c >> 4, col = (c & 15) * 8;  // key row, first column of the chunk
+    if (k0 + kr >= len || col >= a.hd) continue;
+    *reinterpret_cast<uint4*>(row_ptr(dkw ? a.dk : a.dv, begin + k0 + kr, kvh) + col) =
+        *reinterpret_cast<const uint4*>(stage + kr * SL + col);
+  }
+}
+
+}  // namespace eth
+
+using namespace eth;
+
+// heads of a group per workgroup: as many of the four waves as divide it
+static int heads_per_tile(int group) { return group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1; }
+
+extern "C" int eth_packed_attn_tile_rows(int heads, int kv_heads) {
+  if (heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  return kBQ / heads_per_tile(heads / kv_heads);
+}
+
+static bool good_strides(const void* p, const int64_t* st) {
+  // (64 rows of a block within 31-bit offsets)
+  return ((uintptr_t)p & 15) == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[0] >= 0 && st[1] >= 0 &&
+         st[0] < (1LL << 24);
+}
+
+static int packed_check(const eth_packed_attn_desc_t* d) {
+  ETH_CHECK_ARG(d, "packed attention: null descriptor");
+  ETH_CHECK_ARG(d->dtype == ETH_BF16 || d->dtype == ETH_F16, "packed attention: dtype must be bf16/fp16");
+  ETH_CHECK_ARG(d->head_dim >= 8 && d->head_dim <= 128 && d->head_dim % 8 == 0,
+                "packed attention: head_dim must be a multiple of 8 in [8, 128] (got %d)", d->head_dim);
+  ETH_CHECK_ARG(d->heads > 0 && d->kv_heads > 0 && d->heads % d->kv_heads == 0,
+                "packed attention: heads (%d) must be a multiple of kv_heads (%d)", d->heads, d->kv_heads);
+  ETH_CHECK_ARG(d->rows > 0 && d->rows < (1LL << 31), "packed attention: rows must be in [1, 2^31) (got %lld)",
+                (long long)d->rows);
+  ETH_CHECK_ARG(d->q_tiles && d->k_tiles && d->n_q_tiles > 0 && d->n_k_tiles > 0, "packed attention: no tiles");
+  ETH_CHECK_ARG((int64_t)d->n_q_tiles * d->heads < (1LL << 31) && (int64_t)d->n_k_tiles * d->kv_heads < (1LL << 31),
+                "packed attention: too many tiles");
+  // (a positive scale keeps the order of the scores, and a product with -inf is -inf)
+  ETH_CHECK_ARG(d->scale >= 0x1p-100f && d->scale <= 0x1p100f, "packed attention: scale must be positive and finite");
+  return ETH_OK;
+}
+
+static PackArgs packed_args(const eth_packed_attn_desc_t* d) {
+  PackArgs a{};
+  a.q_tiles = d->q_tiles;
+  a.k_tiles = d->k_tiles;
+  a.T = d->rows;
+  a.n = d->heads;
+  a.m = d->kv_heads;
+  a.group = a.n / a.m;
+  a.hp = heads_per_tile(a.group);
+  a.hd = d->head_dim;
+  a.scale = d->scale;
+  a.scale_log2 = a.scale * 1.4426950408889634f;
+  return a;
+}
+static PackIn pin(const void* p, const int64_t* st) { return PackIn{(const uint16_t*)p, st[0], st[1]}; }
+static PackOut pout(void* p, const int64_t* st) { return PackOut{(uint16_t*)p, st[0], st[1]}; }
+
+template <int D, bool FP16>
+static void launch_packed_bwd(const PackArgs& a, int g_q, int g_k, hipStream_t s) {
+  packed_bwd_dq_kernel<D, FP16><<<g_q, kAttnThreads, 0, s>>>(a);  // first: it also writes delta
+  if constexpr (D == 128)
+    packed_bwd_dkdv_x128_kernel<FP16><<<g_k, 2 * kAttnThreads, 0, s>>>(a);
+  else
+    packed_bwd_dkdv_kernel<D, FP16><<<g_k, kAttnThreads, 0, s>>>(a);
+}
+
+extern "C" int eth_packed_attn_fwd(const eth_packed_attn_desc_t* d, const void* q, const void* k, const void* v,
+                                   void* out, float* lse, void* stream) {
+  if (int rc = packed_check(d)) return rc;
+  ETH_CHECK_ARG(q && k && v && out && lse, "eth_packed_attn_fwd: null pointer");
+  ETH_CHECK_ARG(good_strides(q, d->q_strides) && good_strides(k, d->k_strides) && good_strides(v, d->v_strides) &&
+                    good_strides(out, d->o_strides),
+                "eth_packed_attn_fwd: rows must be 16-byte aligned, strides non-negative and rows below 2^24 apart");
+  PackArgs a = packed_args(d);
+  a.q = pin(q, d->q_strides);
+  a.k = pin(k, d->k_strides);
+  a.v = pin(v, d->v_strides);
+  a.out = pout(out, d->o_strides);
+  a.lse = lse;
+  const int grid = d->n_q_tiles * (a.n / a.hp);
+  hipStream_t s = (hipStream_t)stream;
+  const bool fp16 = d->dtype == ETH_F16;
+#define ETH_PACKED_FWD(D)                                          \
+  if (fp16)                                                        \
+    packed_fwd_kernel<D, true><<<grid, kAttnThreads, 0, s>>>(a);   \
+  else                                                             \
+    packed_fwd_kernel<D, false><<<grid, kAttnThreads, 0, s>>>(a);
+  if (a.hd > 96) {
+    ETH_PACKED_FWD(128)
+  } else if (a.hd > 64) {
+    ETH_PACKED_FWD(96)
+  } else {
+    ETH_PACKED_FWD(64)
+  }
+#undef ETH_PACKED_FWD
+  ETH_CHECK_LAUNCH("eth_packed_attn_fwd");
+  return ETH_OK;
+}
+
+extern "C" int eth_packed_attn_bwd(const eth_packed_attn_desc_t* d, const void* q, const void* k, const void* v,
+                                   const void* out, const void* dout, const float* lse, float* delta, void* dq,
+                                   void* dk, void* dv, void* stream) {
+  if (int rc = packed_check(d)) return rc;
+  ETH_CHECK_ARG(q && k && v && out && dout && lse && delta && dq && dk && dv, "eth_packed_attn_bwd: null pointer");
+  ETH_CHECK_ARG(good_strides(q, d->q_strides) && good_strides(k, d->k_strides) && good_strides(v, d->v_strides) &&
+                    good_strides(out, d->o_strides) && good_strides(dout, d->do_strides) &&
+                    good_strides(dq, d->dq_strides) && good_strides(dk, d->dk_strides) &&
+                    good_strides(dv, d->dv_strides),
+                "eth_packed_attn_bwd: rows must be 16-byte aligned, strides non-negative and rows below 2^24 apart");
+  PackArgs a = packed_args(d);
+  a.q = pin(q, d->q_strides);
+  a.k = pin(k, d->k_strides);
+  a.v = pin(v, d->v_strides);
+  a.o = pin(out, d->o_strides);
+  a.dout = pin(dout, d->do_strides);
+  a.dq = pout(dq, d->dq_strides);
+  a.dk = pout(dk, d->dk_strides);
+  a.dv = pout(dv, d->dv_strides);
+  a.lse = const_cast<float*>(lse);
+  a.delta = delta;
+  const int g_q = d->n_q_tiles * (a.n / a.hp), g_k = d->n_k_tiles * a.m;
+  hipStream_t s = (hipStream_t)stream;
+  const bool fp16 = d->dtype == ETH_F16;
+#define ETH_PACKED_BWD(D)                        \
+  if (fp16)                                      \
+    launch_packed_bwd<D, true>(a, g_q, g_k, s);  \
+  else                                           \
+    launch_packed_bwd<D, false>(a, g_q, g_k, s);
+  if (a.hd > 96) {
+    ETH_PACKED_BWD(128)
+  } else if (a.hd > 64) {
+    ETH_PACKED_BWD(96)
+  } else {
+    ETH_PACKED_BWD(64)
+  }
+#undef ETH_PACKED_BWD
+  ETH_CHECK_LAUNCH("eth_packed_attn_bwd");
+  return ETH_OK;
+}

@@ -5,6 +5,7 @@ match what the kernel and its launch grid assume, then enqueues the kernel on
 the current stream.  There is no CPU fallback: CPU tensors raise.
 """
 
+import contextlib
 import ctypes
 import functools
 import itertools
@@ -439,6 +440,116 @@ def attention_bwd(q, k, v, out, dout, lse, dq, dk, dv):
     nat.call("eth_attn_bwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(o4), nat.ptr(do4),
              nat.ptr(lse), nat.ptr(delta), nat.ptr(dq), nat.ptr(dk), nat.ptr(dv), nat.stream_ptr(q.device))
     _observe("attn_bwd", "end", flops)
+
+
+def _device_guard(t):
+    """Launches go to the tensors' device, whichever the current one is."""
+    if t.device.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _check_device(device, *ts):
+    for t in ts:
+        if t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}: one device is needed")
+
+
+def _thd_strides(name, t, written=False):
+    """(row, head) strides of a [rows, heads, hn] view with hn contiguous."""
+    rows, heads, hn = t.shape
+    sr, sh, sd = t.stride()
+    if hn > 1 and sd != 1:
+        raise ValueError(f"{name} must be a [rows, heads, hn] view with hn contiguous")
+    # (the stride of a dimension of size 1 means nothing and may be anything)
+    sr, sh = sr if rows > 1 else heads * hn, sh if heads > 1 else hn
+    if sr % 8 or sh % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: rows must be 16-byte aligned")
+    if written and (sh < hn or sr < hn):
+        raise ValueError(f"{name}: rows that are written may not overlap")
+    return sr, sh
+
+
+def _packed_desc(q, k, v, packed, scale, code):
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("packed attention needs q [rows, heads, hn] and k, v [rows, kv_heads, hn]")
+    rows, n, d = q.shape
+    m = k.shape[1]
+    if k.shape[0] != rows or k.shape[2] != d or rows != packed.total:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and {packed.total} packed rows do not match")
+    if d % 8 or not 8 <= d <= 128:
+        raise ValueError(f"packed attention needs head_dim a multiple of 8 in [8, 128] (got {d})")
+    if m < 1 or n < 1 or n % m:
+        raise ValueError(f"{n} query heads cannot share {m} key and value heads")
+    scale = d**-0.5 if scale is None else float(scale)
+    if not 2.0**-100 <= scale <= 2.0**100:
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    _check_device(packed.device, q, k, v)
+    desc = nat.PackedAttnDesc()
+    desc.rows, desc.heads, desc.kv_heads, desc.head_dim, desc.dtype, desc.scale = rows, n, m, d, code, scale
+    desc.q_tiles, desc.n_q_tiles, desc.k_tiles, desc.n_k_tiles = packed.tiles(
+        nat.value("eth_packed_attn_tile_rows", n, m))
+    desc.q_strides[:] = _thd_strides("q", q)
+    desc.k_strides[:] = _thd_strides("k", k)
+    desc.v_strides[:] = _thd_strides("v", v)
+    return desc
+
+
+def _packed_flops(packed, n, d):
+    return 2.0 * n * d * sum(x * (x + 1) for x in packed.lengths)  # QK^T and PV over the causal half
+
+
+def packed_attention_fwd(q, k, v, packed, scale=None, out=None):
+    """Causal attention over `packed` (PackedSequences) of q [rows, n, hn] and
+    k, v [rows, m, hn] views with any row and head strides; query head h reads
+    key/value head h // (n // m).  Returns (out [rows, n*hn], lse [n, rows],
+    log2 domain); rows of no sequence get zeros (lse -inf)."""
+    code = _check_half(q, k, v)
+    desc = _packed_desc(q, k, v, packed, scale, code)
+    rows, n, d = q.shape
+    if out is None:
+        out = torch.empty(rows, n * d, dtype=q.dtype, device=q.device)
+    elif out.shape != (rows, n * d) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise ValueError("out must be a contiguous [rows, n*hn] tensor like q")
+    desc.o_strides[:] = _thd_strides("out", out.view(rows, n, d), written=True)
+    lse = torch.empty(n, rows, dtype=torch.float32, device=q.device)
+    flops = _packed_flops(packed, n, d) if _observer is not None else 0.0
+    with _device_guard(q):
+        _observe("attn_fwd", "begin", flops)
+        nat.call("eth_packed_attn_fwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(out),
+                 nat.ptr(lse), nat.stream_ptr(q.device))
+        _observe("attn_fwd", "end", flops)
+    return out, lse
+
+
+def packed_attention_bwd(q, k, v, out, dout, lse, packed, dq, dk, dv, scale=None):
+    """Gradients of packed_attention_fwd into dq [rows, n, hn] and dk, dv
+    [rows, m, hn] views; out / dout are contiguous [rows, n*hn].  dk and dv are
+    summed over the query heads that share them, in a fixed order; rows of no
+    sequence get zeros."""
+    code = _check_half(q, k, v, out, dout, dq, dk, dv)
+    desc = _packed_desc(q, k, v, packed, scale, code)
+    rows, n, d = q.shape
+    for name, t in (("out", out), ("dout", dout)):
+        if t.shape != (rows, n * d) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [rows, n*hn]")
+    if lse.shape != (n, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError("lse must be the forward's fp32 [n, rows]")
+    _check_device(q.device, out, dout, lse, dq, dk, dv)
+    desc.o_strides[:] = _thd_strides("out", out.view(rows, n, d))
+    desc.do_strides[:] = _thd_strides("dout", dout.view(rows, n, d))
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if t.shape != like.shape:
+            raise ValueError(f"{name} shape mismatch")
+        getattr(desc, f"{name}_strides")[:] = _thd_strides(name, t, written=True)
+    delta = torch.empty(n, rows, dtype=torch.float32, device=q.device)
+    flops = 2.5 * _packed_flops(packed, n, d) if _observer is not None else 0.0
+    with _device_guard(q):
+        _observe("attn_bwd", "begin", flops)
+        nat.call("eth_packed_attn_bwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(out),
+                 nat.ptr(dout), nat.ptr(lse), nat.ptr(delta), nat.ptr(dq), nat.ptr(dk), nat.ptr(dv),
+                 nat.stream_ptr(q.device))
+        _observe("attn_bwd", "end", flops)
 
 
 # --------------------------------------------------------------- vocabulary --

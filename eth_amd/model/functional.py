@@ -424,6 +424,28 @@ class CausalAttentionFn(torch.autograd.Function):
         return dq, dk, dv
 
 
+class PackedCausalAttentionFn(torch.autograd.Function):
+    """softmax(scale QK^T + causal) V within each sequence of `packed`
+    (eth_amd.packed.PackedSequences) on q [rows, n, hn] and k, v [rows, m, hn]
+    views -> [rows, n*hn]; n / m query heads share each key and value head.
+    Rows of no sequence give zeros and get zero gradients.  scale: 1/sqrt(hn)
+    unless given."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, packed, scale=None):
+        out, lse = K.packed_attention_fwd(q, k, v, packed, scale)
+        ctx.packed, ctx.scale = packed, scale
+        ctx.save_for_backward(q, k, v, out, lse)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        K.packed_attention_bwd(q, k, v, out, dout.contiguous(), lse, ctx.packed, dq, dk, dv, ctx.scale)
+        return dq, dk, dv, None, None
+
+
 class EmbeddingFn(torch.autograd.Function):
     """word[tokens] + pos[positions] -> [s, b, h] (Embedding_v1, dropout p = 0
     handled by the caller)."""

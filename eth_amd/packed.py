@@ -1,0 +1,80 @@
+"""Sequences of different lengths packed into one row dimension.
+
+`PackedSequences` is what the packed attention kernels need to know of a
+batch: which rows form which sequence, as device lists of tiles (blocks of
+queries, blocks of keys, and blocks of rows that no sequence covers), built and
+checked once on the host and shared by every layer of the batch, forward and
+backward.  The lists are ordered by the length of a tile's chain, so that the
+longest start first.
+"""
+
+import numpy as np
+import torch
+
+from . import _native as nat
+
+KEY_TILE_ROWS = 128  # keys per workgroup of the dK/dV kernels
+QUERY_TILE_ROWS = (32, 64, 128)  # queries per workgroup, by the heads that share one
+
+
+def _tile_list(lengths, total, rows, queries):
+    """eth_packed_tile entries of `rows` rows: a query tile's chain grows with
+    its end in the sequence, a key tile's with what is left behind its start."""
+    lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    begins = np.cumsum(lengths) - lengths
+    counts = -(-lengths // rows)
+    seq = np.repeat(np.arange(lengths.size), counts)
+    start = (np.arange(seq.size) - np.repeat(np.cumsum(counts) - counts, counts)) * rows
+    chain = np.minimum(start + rows, lengths[seq]) if queries else lengths[seq] - start
+    order = np.argsort(-chain, kind="stable")
+    covered = int(lengths.sum())
+    spare = np.arange(covered, total, rows)  # rows behind the last sequence
+    tiles = np.zeros(seq.size + spare.size, dtype=nat.PACKED_TILE_DTYPE)
+    tiles["begin"] = np.concatenate([begins[seq][order], spare])
+    tiles["len"] = np.concatenate([lengths[seq][order], -np.minimum(rows, total - spare)])
+    tiles["start"][: seq.size] = start[order]
+    return tiles
+
+
+class PackedSequences:
+    """Rows [0, lengths[0]) are the first sequence, the next lengths[1] rows
+    the second, and so on; rows from sum(lengths) to `total` (default: none)
+    belong to no sequence.  Lengths may be zero.  Device lists are uploaded
+    here, so make it outside of a graph capture, and keep it for as long as a
+    graph that was captured with it is replayed."""
+
+    def __init__(self, lengths, total=None, device="cuda"):
+        if isinstance(lengths, torch.Tensor):
+            if lengths.dim() != 1 or lengths.is_floating_point() or lengths.dtype == torch.bool:
+                raise ValueError("lengths must be a one-dimensional list of whole numbers")
+            lengths = lengths.tolist()
+        lengths = list(lengths)
+        for x in lengths:
+            if isinstance(x, bool) or not isinstance(x, (int, np.integer)) or x < 0:
+                raise ValueError(f"a sequence length must be a whole number of at least 0, got {x!r}")
+        self.lengths = tuple(int(x) for x in lengths)
+        covered = sum(self.lengths)
+        self.total = covered if total is None else int(total)
+        if not covered <= self.total or not 0 < self.total < 2**31:
+            raise ValueError(f"total must be at least 1, at least the {covered} rows of the sequences, and below 2^31 "
+                             f"(got {self.total})")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise ValueError("packed sequences live on the GPU (no CPU fallback)")
+        if self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        lists = {rows: _tile_list(self.lengths, self.total, rows, True) for rows in QUERY_TILE_ROWS}
+        lists["keys"] = _tile_list(self.lengths, self.total, KEY_TILE_ROWS, False)
+        self._table = nat.table_to_device(np.concatenate(list(lists.values())), self.device)
+        self._home = nat.stream_ptr(self.device)
+        self._at, at = {}, self._table.data_ptr()
+        for key, tiles in lists.items():
+            self._at[key] = (at, tiles.size)
+            at += tiles.nbytes
+
+    def tiles(self, query_rows):
+        """(address, count) of the query list of `query_rows` rows a tile and
+        of the key list, for a launch on the current stream."""
+        if nat.stream_ptr(self.device) != self._home and not torch.cuda.is_current_stream_capturing():
+            self._table.record_stream(torch.cuda.current_stream(self.device))
+        return (*self._at[query_rows], *self._at["keys"])

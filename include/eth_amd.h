@@ -396,6 +396,51 @@ int eth_attn_bwd(const eth_attn_desc_t* desc, const void* q, const void* k, cons
                  const void* out, const void* dout, const float* lse, float* delta, void* dq,
                  void* dk, void* dv, void* stream);
 
+/* Causal attention over sequences packed into one row dimension, with query
+ * heads that share key and value heads: q [rows, heads, head_dim], k and v
+ * [rows, kv_heads, head_dim] (strides of row and head in elements, multiples
+ * of 8 and 16-byte aligned bases; head_dim contiguous, a multiple of 8 up to
+ * 128; heads a multiple of kv_heads).  Query head h reads key/value head
+ * h / (heads / kv_heads); a row sees the rows up to itself of its sequence,
+ * out = softmax(scale q k^T) v, scale > 0.  lse [heads, rows] in the log2
+ * domain.
+ *
+ * A tile is `eth_packed_attn_tile_rows(heads, kv_heads)` query rows (128 key
+ * rows in the key list) from `start` on of the sequence [begin, begin + len);
+ * len < 0 marks -len rows from `begin` on that no sequence covers, at most as
+ * many as a tile has: their outputs and gradients are stored as zeros (lse
+ * -inf).  Each list covers every row exactly once, in any order (longest
+ * chains first run fastest); the lists are device memory and are not checked.
+ * Non-finite values of a row of k or v may reach every row of its own
+ * sequence's 64-row block and those behind it, never another sequence.
+ *
+ * The backward reads out and lse of the forward, fills delta [heads, rows] on
+ * the way, and sums dk and dv over the query heads that share them, in a fixed
+ * order (deterministic). */
+typedef struct eth_packed_tile {
+  int32_t begin, len, start, reserved;
+} eth_packed_tile_t;
+
+typedef struct eth_packed_attn_desc {
+  int64_t rows;
+  int64_t q_strides[2], k_strides[2], v_strides[2], o_strides[2];
+  int64_t do_strides[2], dq_strides[2], dk_strides[2], dv_strides[2];
+  const eth_packed_tile_t* q_tiles;
+  const eth_packed_tile_t* k_tiles;
+  int32_t n_q_tiles, n_k_tiles;
+  int32_t heads, kv_heads, head_dim, dtype;
+  float scale;
+  int32_t reserved; /* 0 */
+} eth_packed_attn_desc_t;
+
+/* Query rows of a tile for these head counts (0 if they do not fit). */
+int eth_packed_attn_tile_rows(int heads, int kv_heads);
+int eth_packed_attn_fwd(const eth_packed_attn_desc_t* desc, const void* q, const void* k,
+                        const void* v, void* out, float* lse, void* stream);
+int eth_packed_attn_bwd(const eth_packed_attn_desc_t* desc, const void* q, const void* k,
+                        const void* v, const void* out, const void* dout, const float* lse,
+                        float* delta, void* dq, void* dk, void* dv, void* stream);
+
 /* ------------------------------------------------------------------------
  * Vocabulary side of the first / last stage.
  * eth_embedding_fwd: out[s, b, :] = word[tokens[b, s]] + pos[positions[b, s]]
