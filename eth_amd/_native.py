@@ -107,6 +107,11 @@ SIGNATURES["eth_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["eth_packed_attn_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["eth_packed_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
 
+SIGNATURES["eth_token_logprobs_fwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _P, _I32, _P]
+SIGNATURES["eth_token_logprobs_bwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]
+SIGNATURES["eth_topk_distill_fwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _I64, _I64, _P, _I32, _P]
+SIGNATURES["eth_topk_distill_bwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _P]
+
 
 class AttnDesc(ctypes.Structure):
     """struct eth_attn_desc (include/eth_amd.h)."""
@@ -163,6 +168,7 @@ VALUE_SIGNATURES = {
     "eth_gemm_splitk_workspace": ([_I64, _I64, _I32], _I64),
     "eth_gemm_splitk_pays": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32], _I64),
     "eth_embedding_bwd_workspace": ([_I64, _I64], _I64),
+    "eth_token_logprobs_workspace": ([_I64, _I64, _I32, _I32], _I64),
     "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
 }
 GEMM_ACCUMULATE, GEMM_BIAS = 1, 2

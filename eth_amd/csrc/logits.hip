@@ -1,0 +1,859 @@
+// Row operators over logits [rows, V] (bf16, fp16 or fp32), beside the cross
+// entropy: the log probabilities of given tokens with the row's entropy and
+// its top alternatives, and the distillation loss on a teacher's top logits,
+// forward and backward.
+//
+//   m = max z, s = sum exp(z - m), logp = (z - m) - log s, p = exp(logp)
+//   token log probabilities:  logp[t], H = log s - sum e (z - m) / s, the k
+//     largest logp with their ids (equal ones by the lowest id)
+//     dz_j = g ([j = t] - p_j) - h p_j (logp_j + H)
+//   distillation at temperature tau over the teacher's entries (id, u):
+//     q = softmax(u / tau), p = softmax(z / tau)
+//     loss = tau^2 sum q (log q - log p[id]),  dz_j = g tau (p_j - sum_{id = j} q)
+//
+// All arithmetic is fp32; the row's maximum and log s are kept apart, so that
+// a large common offset of the logits costs no digits.  Rows are read once
+// forward, read and written once backward: HBM bounds them.  Rows may start at
+// any multiple of an element (odd vocabularies): vectors are loaded and stored
+// with the alignment of an element, which the hardware takes.
+#include "common.h"
+
+namespace eth {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLowest = -3.4028234663852886e38f;
+// differences of logits are cut here before they meet a zero probability
+// (0 * -inf); exp of it is 0
+constexpr float kFarBelow = -1e4f;
+
+typedef uint32_t lg_u32x4 __attribute__((ext_vector_type(4)));
+typedef lg_u32x4 lg_u32x4_a2 __attribute__((aligned(2)));
+typedef lg_u32x4 lg_u32x4_a4 __attribute__((aligned(4)));
+
+// one 16-byte vector of E elements of a type
+template <int DT>
+struct Lg {
+  static constexpr int E = 8;
+  typedef uint16_t T;
+  typedef lg_u32x4_a2 V;
+  static __device__ __forceinline__ float one(T v) { return DT == ETH_F16 ? h2f_bits(v) : bf2f(v); }
+  static __device__ __forceinline__ T round(float v) { return DT == ETH_F16 ? f2h_bits(v) : f2bf(v); }
+  static __device__ __forceinline__ void unpack(const lg_u32x4& a, float (&x)[E]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = one((T)(a[j] & 0xffffu));
+      x[2 * j + 1] = one((T)(a[j] >> 16));
+    }
+  }
+  static __device__ __forceinline__ lg_u32x4 pack(const float (&x)[E]) {
+    lg_u32x4 a;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      a[j] = DT == ETH_F16 ? f2h_pair(x[2 * j], x[2 * j + 1]) : f2bf_pair(x[2 * j], x[2 * j + 1]);
+    return a;
+  }
+  static constexpr uint32_t kMinusInf = DT == ETH_F16 ? 0xfc00fc00u : 0xff80ff80u;
+};
+template <>
+struct Lg<ETH_F32> {
+  static constexpr int E = 4;
+  typedef float T;
+  typedef lg_u32x4_a4 V;
+  static __device__ __forceinline__ float one(T v) { return v; }
+  static __device__ __forceinline__ T round(float v) { return v; }
+  static __device__ __forceinline__ void unpack(const lg_u32x4& a, float (&x)[E]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(a[j]);
+  }
+  static __device__ __forceinline__ lg_u32x4 pack(const float (&x)[E]) {
+    lg_u32x4 a;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = __float_as_uint(x[j]);
+    return a;
+  }
+  static constexpr uint32_t kMinusInf = 0xff800000u;
+};
+
+// vectors first, first + STEP, ... of the n elements at z, -inf past them.
+// The partial vector that n % E elements end a row with is one thread's: its
+// elements are loaded one by one, once, and not in every place of the list.
+template <int DT, int NV, int STEP>
+__device__ __forceinline__ void load_vecs(lg_u32x4 (&v)[NV], const typename Lg<DT>::T* z, int64_t first, int64_t n) {
+  constexpr int E = Lg<DT>::E;
+  const int64_t whole = n / E;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int64_t at = first + i * STEP;
+    if (at < whole)
+      v[i] = *reinterpret_cast<const typename Lg<DT>::V*>(z + at * E);
+    else
+      v[i] = lg_u32x4{Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf};
+  }
+  const int64_t rest = n - whole * E, slot = whole - first;
+  if (rest && slot >= 0 && slot % STEP == 0 && slot < NV * STEP) {
+    lg_u32x4 t = lg_u32x4{Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf};
+    float x[E];
+    Lg<DT>::unpack(t, x);
+#pragma unroll
+    for (int j = 0; j < E - 1; ++j)
+      if (j < rest) x[j] = Lg<DT>::one(z[whole * E + j]);
+    t = Lg<DT>::pack(x);  // (values of the type: exact)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (slot == i * STEP) v[i] = t;
+  }
+}
+// A vector's elements for one pass, the vector not known to be what it was:
+// otherwise what was unpacked for one pass is kept for the next, and with it
+// twice the registers or, spilled, much more.
+template <int DT>
+__device__ __forceinline__ void unpack_again(lg_u32x4& v, float (&x)[Lg<DT>::E]) {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" : "+v"(v));
+  Lg<DT>::unpack(v, x);
+}
+// vector i of the n elements at d
+template <int DT>
+__device__ __forceinline__ void store_vec(typename Lg<DT>::T* d, int64_t i, int64_t n, const float (&x)[Lg<DT>::E]) {
+  constexpr int E = Lg<DT>::E;
+  if ((i + 1) * E <= n) {
+    *reinterpret_cast<typename Lg<DT>::V*>(d + i * E) = Lg<DT>::pack(x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (i * E + j < n) d[i * E + j] = Lg<DT>::round(x[j]);
+  }
+}
+
+__device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+
+// max, sum of exponentials and sum of exponentials times their difference from
+// the max, of a part of a row
+struct RowStat {
+  float m, s, a;
+};
+// the same relative to a larger maximum M
+__device__ __forceinline__ RowStat at_max(const RowStat& r, float M) {
+  const float d = fmaxf(r.m - M, kFarBelow), f = exp_f(d);
+  return RowStat{M, r.s * f, (r.a + r.s * d) * f};
+}
+// over the workgroup (NT threads), in every thread; `red` holds 3 * NT / 64 floats
+template <int NT>
+__device__ __forceinline__ RowStat block_stat(RowStat r, float* red) {
+  constexpr int W = NT / 64;
+  r = at_max(r, wave_max(r.m));
+  r.s = wave_sum(r.s);
+  r.a = wave_sum(r.a);
+  if ((threadIdx.x & 63) == 0) {
+    const int w = threadIdx.x >> 6;
+    red[w] = r.m;
+    red[W + w] = r.s;
+    red[2 * W + w] = r.a;
+  }
+  __syncthreads();
+  float M = red[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) M = fmaxf(M, red[w]);
+  RowStat t{M, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    const RowStat x = at_max(RowStat{red[w], red[W + w], red[2 * W + w]}, M);
+    t.s += x.s;
+    t.a += x.a;
+  }
+  return t;
+}
+
+// ---------------------------------------------------- token log probabilities --
+constexpr int kLogpThreads = 512;
+constexpr int kLogpTop = 128;   // most alternatives
+constexpr int kLogpCand = 1024; // candidates that the sort takes
+constexpr int kLogpVecs = 16;   // vectors of a row's part that a thread holds
+
+// floats as whole numbers of the same order: -0 as +0, NaN above everything
+__device__ __forceinline__ uint32_t order_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return v != v ? 0xffffffffu : (b & 0x80000000u ? ~b : b | 0x80000000u);
+}
+__device__ __forceinline__ float of_order(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+// value first, then the lower index: all keys of a row differ
+__device__ __forceinline__ uint64_t key_of(float v, int64_t index) {
+  return (uint64_t)order_of(v) << 32 | (uint32_t)~(uint32_t)index;
+}
+__device__ __forceinline__ int64_t index_of(uint64_t key) { return (int64_t)(uint32_t)~(uint32_t)key; }
+
+struct LogpArgs {
+  const void* z;
+  int64_t ld, V;
+  const int64_t* tokens;
+  int64_t ignore;
+  float* logprob;
+  float* entropy;
+  float2* stats;  // max, log of the sum (-inf: no finite logit)
+  float* top;     // [rows, k]
+  int64_t* ids;
+  int k;
+  int* bad;
+  int parts;          // workgroups per row
+  int64_t part;       // elements of a part (a multiple of a vector's)
+  float4* part_stat;  // [rows, parts]
+  uint64_t* part_key; // [rows, parts, k]
+};
+
+__device__ __forceinline__ bool logp_ignored(const LogpArgs& a, int64_t row) {
+  if (a.tokens[row] != a.ignore) return false;
+  for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
+    a.top[row * a.k + i] = -INFINITY;
+    a.ids[row * a.k + i] = -1;
+  }
+  if (threadIdx.x == 0) {
+    a.logprob[row] = 0.f;
+    a.entropy[row] = 0.f;
+    a.stats[row] = make_float2(0.f, -INFINITY);
+  }
+  return true;
+}
+
+// a row's results from its statistics (one thread)
+template <int DT>
+__device__ __forceinline__ void logp_row(const LogpArgs& a, int64_t row, const RowStat& r) {
+  typedef typename Lg<DT>::T T;
+  int64_t t = a.tokens[row];
+  if (t < 0 || t >= a.V) {
+    *a.bad = 1;
+    t = t < 0 ? 0 : a.V - 1;
+  }
+  const bool none = r.s == 0.f;  // every logit is -inf
+  const float ls = none ? -INFINITY : logf(r.s);
+  const float z = Lg<DT>::one(reinterpret_cast<const T*>(a.z)[row * a.ld + t]);
+  a.stats[row] = make_float2(r.m, ls);
+  a.logprob[row] = none ? -INFINITY : (z - r.m) - ls;
+  a.entropy[row] = none ? 0.f : ls - r.a / r.s;
+}
+__device__ __forceinline__ void logp_top(const LogpArgs& a, int64_t row, const RowStat& r, float ls, int rank,
+                                         uint64_t key) {
+  a.top[row * a.k + rank] = r.s == 0.f ? -INFINITY : (of_order((uint32_t)(key >> 32)) - r.m) - ls;
+  a.ids[row * a.k + rank] = index_of(key);
+}
+
+// The k largest keys of the n elements at z (row indices from `first` on),
+// unsorted, by every thread of a workgroup: the largest key that k keys reach,
+// two bits a pass over the part.
+template <int DT>
+__device__ __noinline__ int logp_exact(const typename Lg<DT>::T* z, int64_t first, int64_t n, int k, uint64_t* cand,
+                                       int* count) {
+  constexpr int W = kLogpThreads / 64;
+  __shared__ int reach_s[3][W];
+  uint64_t f = 0;
+  for (int bit = 62; bit >= 0; bit -= 2) {
+    int reach[3] = {0, 0, 0};
+    for (int64_t i = threadIdx.x; i < n; i += kLogpThreads) {
+      const uint64_t key = key_of(Lg<DT>::one(z[i]), first + i);
+#pragma unroll
+      for (int c = 0; c < 3; ++c) reach[c] += key >= (f | (uint64_t)(c + 1) << bit);
+    }
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+      const int sum = (int)wave_sum((float)reach[c]);  // (below 2^24: exact)
+      if ((threadIdx.x & 63) == 0) reach_s[c][threadIdx.x >> 6] = sum;
+    }
+    __syncthreads();
+    int digit = 0;
+    for (int c = 0; c < 3; ++c) {
+      int total = 0;
+      for (int w = 0; w < W; ++w) total += reach_s[c][w];
+      digit += total >= k;
+    }
+    f |= (uint64_t)digit << bit;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < n; i += kLogpThreads) {
+    const uint64_t key = key_of(Lg<DT>::one(z[i]), first + i);
+    if (key >= f) cand[atomicAdd(count, 1)] = key;  // (exactly k: all keys differ)
+  }
+  __syncthreads();
+  return *count;
+}
+
+// One workgroup per part of a row, the whole row up to 512 * 16 vectors, held
+// in registers: 16 loads in flight per thread, each logit read once.
+//
+// Top alternatives: of the 256 maxima of pairs of threads the k-th largest
+// (to 16 bits, rounded down) is a lower bound of the row's k-th largest, and
+// only about k + k^2 / 512 logits reach it: these are collected in LDS and
+// sorted by counting.  Where more reach it than the sort takes (equal logits, a
+// row of few finite ones) the k-th key is found bit by bit.
+template <int DT, int NV, bool TOP>
+__global__ void __launch_bounds__(kLogpThreads, 4) logp_fwd_kernel(LogpArgs a) {
+  typedef typename Lg<DT>::T T;
+  constexpr int E = Lg<DT>::E, NT = kLogpThreads;
+  __shared__ float red[3 * NT / 64];
+  __shared__ uint64_t cand[TOP ? kLogpCand : 1];
+  __shared__ __attribute__((aligned(16))) uint32_t maxima[TOP ? NT / 2 : 4];
+  __shared__ uint32_t floor_s;
+  __shared__ int count_s;
+
+  const int64_t row = blockIdx.x / a.parts;
+  const int part = blockIdx.x % a.parts;
+  if (a.parts == 1 ? logp_ignored(a, row) : a.tokens[row] == a.ignore) return;
+  const int64_t first = part * a.part;
+  const int64_t n = a.V - first < a.part ? a.V - first : a.part;
+  const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld + first;
+
+  lg_u32x4 v[NV];
+  load_vecs<DT, NV, NT>(v, z, threadIdx.x, n);
+  RowStat r{kLowest, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float x[E];
+    unpack_again<DT>(v[i], x);
+#pragma unroll
+    for (int j = 0; j < E; ++j) r.m = fmaxf(r.m, x[j]);
+  }
+  if constexpr (TOP) {  // (a thread of -inf alone counts as the lowest: a lower bound all the same)
+    const float pm = fmaxf(r.m, __shfl_xor(r.m, 1, 64));
+    if ((threadIdx.x & 1) == 0) maxima[threadIdx.x >> 1] = order_of(pm) >> 16;
+    if (threadIdx.x == 0) count_s = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float x[E];
+    unpack_again<DT>(v[i], x);
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float d = x[j] - r.m, e = exp_f(d);
+      r.s += e;
+      r.a = __builtin_fmaf(e, fmaxf(d, kFarBelow), r.a);
+    }
+  }
+  r = block_stat<NT>(r, red);
+  if (threadIdx.x == 0) {
+    if (a.parts == 1)
+      logp_row<DT>(a, row, r);
+    else
+      a.part_stat[row * a.parts + part] = make_float4(r.m, r.s, r.a, 0.f);
+  }
+  if constexpr (TOP) {
+    if (threadIdx.x < 64) {  // (block_stat's barrier lies behind the maxima)
+      const uint4 k4 = *reinterpret_cast<const uint4*>(&maxima[threadIdx.x * 4]);
+      uint32_t f = 0;
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t c = f | 1u << bit;
+        const int above = __popcll(__ballot(k4.x >= c)) + __popcll(__ballot(k4.y >= c)) +
+                          __popcll(__ballot(k4.z >= c)) + __popcll(__ballot(k4.w >= c));
+        if (above >= a.k) f = c;
+      }
+      if (threadIdx.x == 0) floor_s = f;
+    }
+    __syncthreads();
+    // orders up to that of the lowest finite value: everything, -inf too
+    const uint32_t fo = floor_s << 16;
+    const float floor_v = fo <= 0x00ffffffu ? -INFINITY : of_order(fo);
+      // a bit for every vector with a candidate; the few of them are read again
+    uint32_t hits = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float x[E];
+      unpack_again<DT>(v[i], x);
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < E; ++j) any |= !(x[j] < floor_v);  // NaN too
+      hits |= any ? 1u << i : 0u;
+    }
+    while (hits) {
+      const int64_t at = ((int64_t)(__ffs(hits) - 1) * NT + threadIdx.x) * E;
+      hits &= hits - 1;
+      for (int j = 0; j < E && at + j < n; ++j) {
+        const float x = Lg<DT>::one(z[at + j]);
+        if (x < floor_v) continue;
+        const int slot = atomicAdd(&count_s, 1);
+        if (slot < kLogpCand) cand[slot] = key_of(x, first + at + j);
+      }
+    }
+    __syncthreads();
+    int count = count_s;
+    if (count > kLogpCand) count = logp_exact<DT>(z, first, n, a.k, cand, &count_s);
+    const float ls = logf(r.s);
+    for (int i = threadIdx.x; i < count; i += NT) {
+      const uint64_t key = cand[i];
+      int rank = 0;
+      for (int j = 0; j < count; ++j) rank += cand[j] > key;
+      if (rank >= a.k) continue;
+      if (a.parts == 1)
+        logp_top(a, row, r, ls, rank, key);
+      else
+        a.part_key[(row * a.parts + part) * a.k + rank] = key;
+    }
+  }
+}
+
+// joins the parts of a row: their statistics, and the k largest of their
+// sorted keys (a key's rank is the number of larger ones in every part)
+template <int DT>
+__global__ void __launch_bounds__(256) logp_join_kernel(LogpArgs a) {
+  const int64_t row = blockIdx.x;
+  if (logp_ignored(a, row)) return;
+  const float4* ps = a.part_stat + row * a.parts;
+  float M = kLowest;
+  for (int i = 0; i < a.parts; ++i) M = fmaxf(M, ps[i].x);
+  RowStat r{M, 0.f, 0.f};
+  for (int i = 0; i < a.parts; ++i) {
+    const float4 p = ps[i];
+    const RowStat x = at_max(RowStat{p.x, p.y, p.z}, M);
+    r.s += x.s;
+    r.a += x.a;
+  }
+  if (threadIdx.x == 0) logp_row<DT>(a, row, r);
+  const float ls = logf(r.s);
+  const uint64_t* keys = a.part_key + row * a.parts * a.k;
+  for (int i = threadIdx.x; i < a.parts * a.k; i += blockDim.x) {
+    const uint64_t key = keys[i];
+    int rank = 0;
+    for (int q = 0; q < a.parts && rank < a.k; ++q) {
+      int lo = 0, hi = a.k;  // the first entry of part q that is not larger
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (keys[q * a.k + mid] > key)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      rank += lo;
+    }
+    if (rank < a.k) logp_top(a, row, r, ls, rank, key);
+  }
+}
+
+constexpr int kRowThreads = 256;
+constexpr int kRowVecs = 4;  // vectors of a backward workgroup's thread
+
+// One workgroup per 1024 vectors of a row.  A row without upstream gradient
+// (and one without a finite logit) gets zeros and is not read.
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, int64_t ld, int64_t V,
+                                                               const int64_t* __restrict__ tokens, int64_t ignore,
+                                                               const float2* __restrict__ stats,
+                                                               const float* __restrict__ entropy,
+                                                               const float* __restrict__ dlogprob,
+                                                               const float* __restrict__ dentropy, void* dzv,
+                                                               int64_t ldd, int chunks) {
+  typedef typename Lg<DT>::T T;
+  constexpr int E = Lg<DT>::E;
+  const int64_t row = blockIdx.x / chunks;
+  const int64_t i0 = (int64_t)(blockIdx.x % chunks) * (kRowThreads * kRowVecs) + threadIdx.x;
+  const T* z = reinterpret_cast<const T*>(zv) + row * ld;
+  T* dz = reinterpret_cast<T*>(dzv) + row * ldd;
+  int64_t t = tokens[row];
+  const float2 st = stats[row];
+  const bool out = t == ignore || st.y == -INFINITY;
+  t = t < 0 ? 0 : (t >= V ? V - 1 : t);
+  const float g = out || !dlogprob ? 0.f : dlogprob[row], h = out || !dentropy ? 0.f : dentropy[row];
+  const bool none = g == 0.f && h == 0.f;
+  const float H = entropy[row];
+  lg_u32x4 v[kRowVecs];
+  if (!none) load_vecs<DT, kRowVecs, kRowThreads>(v, z, i0, V);
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    const int64_t i = i0 + u * kRowThreads;
+    if (i * E >= V) break;
+    float x[E];
+    if (none) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) x[j] = 0.f;
+    } else {
+      Lg<DT>::unpack(v[u], x);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float lp = (x[j] - st.x) - st.y, p = exp_f(lp);
+        const float w = g + h * (fmaxf(lp, kFarBelow) + H);
+        x[j] = (i * E + j == t ? g : 0.f) - p * w;
+      }
+    }
+    store_vec<DT>(dz, i, V, x);
+  }
+}
+
+// ----------------------------------------------------------------- distillation --
+constexpr int kDistillTop = 256;  // most teacher entries of a row
+constexpr int kDistillThreads = 512;
+constexpr int kDistillVecs = 8;
+
+struct DistillArgs {
+  const void* z;
+  int64_t ld, V;
+  const int64_t* ids;  // [rows, k]; negative: no entry
+  const void* teacher; // [rows, k] logits
+  int teacher_dtype, k;
+  float tau;
+  float* loss;
+  float2* stats;  // max, log of the sum of exp((z - max) / tau)
+  int* bad;
+  const float* dloss;
+  void* dz;
+  int64_t ldd;
+  int chunks;
+};
+
+// The teacher's distribution over its entries into q_s, absent ones (a
+// negative id, one past the vocabulary, a logit of -inf) with 0; ids into
+// id_s (-1 for absent).  Called by every thread; each row's k entries by the
+// first threads.  Returns whether any entry is there.
+template <int NT>
+__device__ __forceinline__ bool teacher_softmax(const DistillArgs& a, int64_t row, float* q_s, int64_t* id_s,
+                                                float* red) {
+  const int i = threadIdx.x;
+  float u = -INFINITY;
+  int64_t id = -1;
+  if (i < a.k) {
+    id = a.ids[row * a.k + i];
+    if (id >= a.V) {
+      *a.bad = 1;
+      id = -1;
+    }
+    if (id >= 0) u = load_elem(a.teacher, row * a.k + i, a.teacher_dtype);
+  }
+  const float m = wave_max(fmaxf(u, kLowest));
+  if ((i & 63) == 0) red[i >> 6] = m;
+  __syncthreads();
+  float M = red[0];
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) M = fmaxf(M, red[w]);
+  __syncthreads();
+  // (a teacher logit of NaN or +inf makes every q NaN, as the softmax does)
+  const float e = id >= 0 ? exp_f((u - M) / a.tau) : 0.f;
+  const float total = block_sum<NT>(e, red);
+  if (i < a.k) {
+    q_s[i] = total == 0.f ? 0.f : e / total;
+    id_s[i] = q_s[i] == 0.f ? -1 : id;
+  }
+  __syncthreads();
+  return total != 0.f;
+}
+
+// One workgroup per row: the row's statistics at the temperature (each thread
+// over its own vectors, eight in flight, joined once) and the k entries.
+template <int DT>
+__global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArgs a) {
+  typedef typename Lg<DT>::T T;
+  constexpr int E = Lg<DT>::E, NT = kDistillThreads;
+  __shared__ float red[3 * NT / 64];
+  __shared__ float q_s[kDistillTop];
+  __shared__ int64_t id_s[kDistillTop];
+  const int64_t row = blockIdx.x;
+  const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
+  if (!teacher_softmax<NT>(a, row, q_s, id_s, red)) {  // nothing to learn from: the row is not read
+    if (threadIdx.x == 0) {
+      a.loss[row] = 0.f;
+      a.stats[row] = make_float2(0.f, -INFINITY);
+    }
+    return;
+  }
+  const float c = kLog2e / a.tau;
+  float m = kLowest, s = 0.f;
+  const int64_t nv = (a.V + E - 1) / E;
+  for (int64_t i0 = threadIdx.x; i0 < nv; i0 += NT * kDistillVecs) {
+    lg_u32x4 v[kDistillVecs];
+    load_vecs<DT, kDistillVecs, NT>(v, z, i0, a.V);
+    float mx = m;
+#pragma unroll
+    for (int u = 0; u < kDistillVecs; ++u) {
+      float x[E];
+      unpack_again<DT>(v[u], x);
+#pragma unroll
+      for (int j = 0; j < E; ++j) mx = fmaxf(mx, x[j]);
+    }
+    s *= __builtin_amdgcn_exp2f((m - mx) * c);
+    m = mx;
+  #pragma unroll
+    for (int u = 0; u < kDistillVecs; ++u) {
+      float x[E];
+      unpack_again<DT>(v[u], x);
+#pragma unroll
+      for (int j = 0; j < E; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * c);
+    }
+  }
+  const float wm = wave_max(m);
+  const float ws = wave_sum(s * __builtin_amdgcn_exp2f((m - wm) * c));
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = wm;
+    red[NT / 64 + (threadIdx.x >> 6)] = ws;
+  }
+  __syncthreads();
+  float M = red[0], S = 0.f;
+#pragma unroll
+  for (int w = 1; w < NT / 64; ++w) M = fmaxf(M, red[w]);
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) S += red[NT / 64 + w] * __builtin_amdgcn_exp2f((red[w] - M) * c);
+  __syncthreads();
+  const bool none = S == 0.f;  // no finite logit: no probability for any entry
+  const float ls = none ? -INFINITY : logf(S);
+  float part = 0.f;
+  if (threadIdx.x < a.k && id_s[threadIdx.x] >= 0) {
+    const float q = q_s[threadIdx.x];
+    const float lp = none ? -INFINITY : (Lg<DT>::one(z[id_s[threadIdx.x]]) - M) / a.tau - ls;
+    part = q * (logf(q) - lp);
+  }
+  const float loss = block_sum<NT>(part, red);
+  if (threadIdx.x == 0) {
+    a.loss[row] = loss * a.tau * a.tau;
+    a.stats[row] = make_float2(M, ls);
+  }
+}
+
+// One workgroup per 1024 vectors of a row: dz = g tau p, then the entries
+// among them once more with their q (an id that appears more than once by its
+// first entry, with the sum).
+template <int DT>
+__global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(DistillArgs a) {
+  typedef typename Lg<DT>::T T;
+  constexpr int E = Lg<DT>::E;
+  __shared__ float red[kRowThreads / 64];
+  __shared__ float q_s[kDistillTop];
+  __shared__ int64_t id_s[kDistillTop];
+  const int64_t row = blockIdx.x / a.chunks;
+  const int64_t v0 = (int64_t)(blockIdx.x % a.chunks) * (kRowThreads * kRowVecs);
+  const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
+  T* dz = reinterpret_cast<T*>(a.dz) + row * a.ldd;
+  const float2 st = a.stats[row];
+  const float gt = st.y == -INFINITY ? 0.f : a.dloss[row] * a.tau;
+  if (gt == 0.f) {  // (also a row without teacher entries or finite logits)
+    float x[E] = {};
+#pragma unroll
+    for (int u = 0; u < kRowVecs; ++u) store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x);
+    return;
+  }
+  lg_u32x4 v[kRowVecs];
+  load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0 + threadIdx.x, a.V);
+  teacher_softmax<kRowThreads>(a, row, q_s, id_s, red);
+  const float inv = 1.f / a.tau;
+  auto prob = [&](float x) __attribute__((always_inline)) { return exp_f((x - st.x) * inv - st.y); };
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) {
+    float x[E];
+    Lg<DT>::unpack(v[u], x);
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = gt * prob(x[j]);
+    store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x);
+  }
+  __syncthreads();  // the stores below come after those of the same places above
+  const int64_t lo = v0 * E, hi = lo + kRowThreads * kRowVecs * E;
+  if (threadIdx.x < a.k) {
+    const int64_t id = id_s[threadIdx.x];
+    if (id >= lo && id < hi) {
+      float q = 0.f;
+      bool mine = true;
+      for (int i = 0; i < a.k; ++i)
+        if (id_s[i] == id) {
+          mine = mine && i >= (int)threadIdx.x;
+          q += q_s[i];
+        }
+      if (mine) dz[id] = Lg<DT>::round(gt * (prob(Lg<DT>::one(z[id])) - q));
+    }
+  }
+}
+
+}  // namespace eth
+
+using namespace eth;
+
+// (far below what would leave a part of a row empty)
+constexpr int64_t kMostVocab = 1LL << 24;
+static bool logits_shape(int64_t rows, int64_t V, int64_t ld) {
+  return rows > 0 && V > 0 && V <= kMostVocab && ld >= V;
+}
+static int64_t logp_parts(int64_t V, int dtype) {
+  const int64_t most = (int64_t)kLogpThreads * kLogpVecs * (16 / dtype_size(dtype));
+  return (V + most - 1) / most;
+}
+
+extern "C" int64_t eth_token_logprobs_workspace(int64_t rows, int64_t vocab, int top_k, int dtype) {
+  if (!valid_dtype(dtype) || rows <= 0 || vocab <= 0 || vocab > kMostVocab || top_k < 0) return 0;
+  const int64_t parts = logp_parts(vocab, dtype);
+  return parts == 1 ? 0 : rows * parts * (int64_t)(sizeof(float4) + top_k * sizeof(uint64_t));
+}
+
+template <int DT, int NV>
+static void launch_logp(const LogpArgs& a, int grid, hipStream_t s) {
+  if (a.k > 0)
+    logp_fwd_kernel<DT, NV, true><<<grid, kLogpThreads, 0, s>>>(a);
+  else
+    logp_fwd_kernel<DT, NV, false><<<grid, kLogpThreads, 0, s>>>(a);
+}
+template <int DT>
+static void launch_logp_rows(const LogpArgs& a, int64_t rows, hipStream_t s) {
+  const int grid = (int)(rows * a.parts);
+  const int64_t vecs = (a.part / Lg<DT>::E + kLogpThreads - 1) / kLogpThreads;
+  if (vecs <= 4)
+    launch_logp<DT, 4>(a, grid, s);
+  else if (vecs <= 8)
+    launch_logp<DT, 8>(a, grid, s);
+  else
+    launch_logp<DT, kLogpVecs>(a, grid, s);
+  if (a.parts > 1) logp_join_kernel<DT><<<(int)rows, 256, 0, s>>>(a);
+}
+
+extern "C" int eth_token_logprobs_fwd(const void* logits, int64_t ld, const int64_t* tokens, int64_t ignore_index,
+                                      float* logprob, float* entropy, float* stats, float* top_logprobs,
+                                      int64_t* top_ids, int top_k, void* workspace, int64_t rows, int64_t vocab,
+                                      int* bad_index, int dtype, void* stream) {
+  ETH_CHECK_ARG(valid_dtype(dtype), "eth_token_logprobs_fwd: dtype must be bf16/fp16/fp32");
+  ETH_CHECK_ARG(logits_shape(rows, vocab, ld), "eth_token_logprobs_fwd: bad shape");
+  ETH_CHECK_ARG(top_k >= 0 && top_k <= kLogpTop && top_k <= vocab,
+                "eth_token_logprobs_fwd: top_k must be in [0, %d] and within the vocabulary (got %d)", kLogpTop, top_k);
+  ETH_CHECK_ARG(logits && tokens && logprob && entropy && stats && bad_index && (top_k == 0 || (top_logprobs && top_ids)),
+                "eth_token_logprobs_fwd: null pointer");
+  LogpArgs a{};
+  a.parts = (int)logp_parts(vocab, dtype);
+  ETH_CHECK_ARG(a.parts == 1 || (workspace && ((uintptr_t)workspace & 15) == 0),
+                "eth_token_logprobs_fwd: this vocabulary needs a 16-byte aligned workspace");
+  ETH_CHECK_ARG(rows * a.parts < (1LL << 31), "eth_token_logprobs_fwd: too many rows (%lld)", (long long)rows);
+  ETH_CHECK_ARG(((uintptr_t)logits % dtype_size(dtype)) == 0 && ((uintptr_t)stats & 7) == 0,
+                "eth_token_logprobs_fwd: misaligned pointer");
+  a.z = logits;
+  a.ld = ld;
+  a.V = vocab;
+  a.tokens = tokens;
+  a.ignore = ignore_index;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.stats = (float2*)stats;
+  a.top = top_logprobs;
+  a.ids = top_ids;
+  a.k = top_k;
+  a.bad = bad_index;
+  const int64_t E = 16 / dtype_size(dtype), vecs = (vocab + E - 1) / E;
+  a.part = (vecs + a.parts - 1) / a.parts * E;
+  a.part_stat = (float4*)workspace;
+  a.part_key = (uint64_t*)(a.part_stat + rows * a.parts);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == ETH_BF16)
+    launch_logp_rows<ETH_BF16>(a, rows, s);
+  else if (dtype == ETH_F16)
+    launch_logp_rows<ETH_F16>(a, rows, s);
+  else
+    launch_logp_rows<ETH_F32>(a, rows, s);
+  ETH_CHECK_LAUNCH("eth_token_logprobs_fwd");
+  return ETH_OK;
+}
+
+static int row_chunks(int64_t V, int dtype) {
+  const int64_t per = (int64_t)kRowThreads * kRowVecs * (16 / dtype_size(dtype));
+  return (int)((V + per - 1) / per);
+}
+
+extern "C" int eth_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* tokens, int64_t ignore_index,
+                                      const float* stats, const float* entropy, const float* dlogprob,
+                                      const float* dentropy, void* dlogits, int64_t ldd, int64_t rows, int64_t vocab,
+                                      int dtype, void* stream) {
+  ETH_CHECK_ARG(valid_dtype(dtype), "eth_token_logprobs_bwd: dtype must be bf16/fp16/fp32");
+  ETH_CHECK_ARG(logits_shape(rows, vocab, ld) && ldd >= vocab, "eth_token_logprobs_bwd: bad shape");
+  ETH_CHECK_ARG(logits && tokens && stats && entropy && (dlogprob || dentropy) && dlogits,
+                "eth_token_logprobs_bwd: null pointer");
+  ETH_CHECK_ARG(((uintptr_t)logits % dtype_size(dtype)) == 0 && ((uintptr_t)dlogits % dtype_size(dtype)) == 0 &&
+                    ((uintptr_t)stats & 7) == 0,
+                "eth_token_logprobs_bwd: misaligned pointer");
+  const int chunks = row_chunks(vocab, dtype);
+  ETH_CHECK_ARG(rows * chunks < (1LL << 31), "eth_token_logprobs_bwd: too many rows (%lld)", (long long)rows);
+  const int grid = (int)(rows * chunks);
+  hipStream_t s = (hipStream_t)stream;
+#define ETH_LOGP_BWD(DT)                                                                                      \
+  logp_bwd_kernel<DT><<<grid, kRowThreads, 0, s>>>(logits, ld, vocab, tokens, ignore_index, (const float2*)stats, \
+                                                   entropy, dlogprob, dentropy, dlogits, ldd, chunks)
+  if (dtype == ETH_BF16)
+    ETH_LOGP_BWD(ETH_BF16);
+  else if (dtype == ETH_F16)
+    ETH_LOGP_BWD(ETH_F16);
+  else
+    ETH_LOGP_BWD(ETH_F32);
+#undef ETH_LOGP_BWD
+  ETH_CHECK_LAUNCH("eth_token_logprobs_bwd");
+  return ETH_OK;
+}
+
+static int distill_check(const char* who, const void* logits, int64_t ld, const int64_t* ids, const void* teacher,
+                         int teacher_dtype, int k, float tau, const void* stats, int64_t rows, int64_t vocab,
+                         const int* bad, int dtype) {
+  ETH_CHECK_ARG(valid_dtype(dtype) && valid_dtype(teacher_dtype), "%s: dtypes must be bf16/fp16/fp32", who);
+  ETH_CHECK_ARG(logits_shape(rows, vocab, ld) && rows < (1LL << 31), "%s: bad shape", who);
+  ETH_CHECK_ARG(k >= 1 && k <= kDistillTop, "%s: 1 to %d teacher entries a row (got %d)", who, kDistillTop, k);
+  ETH_CHECK_ARG(tau >= 0x1p-20f && tau <= 0x1p20f, "%s: temperature must be positive and finite", who);
+  ETH_CHECK_ARG(logits && ids && teacher && stats && bad, "%s: null pointer", who);
+  ETH_CHECK_ARG(((uintptr_t)logits % dtype_size(dtype)) == 0 && ((uintptr_t)teacher % dtype_size(teacher_dtype)) == 0 &&
+                    ((uintptr_t)stats & 7) == 0,
+                "%s: misaligned pointer", who);
+  return ETH_OK;
+}
+static DistillArgs distill_args(const void* logits, int64_t ld, const int64_t* ids, const void* teacher,
+                                int teacher_dtype, int k, float tau, const float* stats, int64_t vocab, int* bad) {
+  DistillArgs a{};
+  a.z = logits;
+  a.ld = ld;
+  a.V = vocab;
+  a.ids = ids;
+  a.teacher = teacher;
+  a.teacher_dtype = teacher_dtype;
+  a.k = k;
+  a.tau = tau;
+  a.stats = (float2*)stats;
+  a.bad = bad;
+  return a;
+}
+
+extern "C" int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_t* teacher_ids, const void* teacher,
+                                    int teacher_dtype, int k, float temperature, float* loss, float* stats,
+                                    int64_t rows, int64_t vocab, int* bad_index, int dtype, void* stream) {
+  if (int rc = distill_check("eth_topk_distill_fwd", logits, ld, teacher_ids, teacher, teacher_dtype, k, temperature,
+                             stats, rows, vocab, bad_index, dtype))
+    return rc;
+  ETH_CHECK_ARG(loss, "eth_topk_distill_fwd: null pointer");
+  DistillArgs a = distill_args(logits, ld, teacher_ids, teacher, teacher_dtype, k, temperature, stats, vocab,
+                               bad_index);
+  a.loss = loss;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == ETH_BF16)
+    distill_fwd_kernel<ETH_BF16><<<(int)rows, kDistillThreads, 0, s>>>(a);
+  else if (dtype == ETH_F16)
+    distill_fwd_kernel<ETH_F16><<<(int)rows, kDistillThreads, 0, s>>>(a);
+  else
+    distill_fwd_kernel<ETH_F32><<<(int)rows, kDistillThreads, 0, s>>>(a);
+  ETH_CHECK_LAUNCH("eth_topk_distill_fwd");
+  return ETH_OK;
+}
+
+extern "C" int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_ids, const void* teacher,
+                                    int teacher_dtype, int k, float temperature, const float* stats,
+                                    const float* dloss, void* dlogits, int64_t ldd, int64_t rows, int64_t vocab,
+                                    int* bad_index, int dtype, void* stream) {
+  if (int rc = distill_check("eth_topk_distill_bwd", logits, ld, teacher_ids, teacher, teacher_dtype, k, temperature,
+                             stats, rows, vocab, bad_index, dtype))
+    return rc;
+  ETH_CHECK_ARG(dloss && dlogits && ((uintptr_t)dlogits % dtype_size(dtype)) == 0 && ldd >= vocab,
+                "eth_topk_distill_bwd: bad gradient buffers");
+  DistillArgs a = distill_args(logits, ld, teacher_ids, teacher, teacher_dtype, k, temperature, stats, vocab,
+                               bad_index);
+  a.dloss = dloss;
+  a.dz = dlogits;
+  a.ldd = ldd;
+  a.chunks = row_chunks(vocab, dtype);
+  ETH_CHECK_ARG(rows * a.chunks < (1LL << 31), "eth_topk_distill_bwd: too many rows (%lld)", (long long)rows);
+  const int grid = (int)(rows * a.chunks);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == ETH_BF16)
+    distill_bwd_kernel<ETH_BF16><<<grid, kRowThreads, 0, s>>>(a);
+  else if (dtype == ETH_F16)
+    distill_bwd_kernel<ETH_F16><<<grid, kRowThreads, 0, s>>>(a);
+  else
+    distill_bwd_kernel<ETH_F32><<<grid, kRowThreads, 0, s>>>(a);
+  ETH_CHECK_LAUNCH("eth_topk_distill_bwd");
+  return ETH_OK;
+}

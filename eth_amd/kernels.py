@@ -622,6 +622,127 @@ def xent_bwd(logits2d, labels, lse, dloss):
     return dz
 
 
+def _check_logits(logits2d, bad_flag, *ts):
+    """(dtype code, rows, V, row stride) of [rows, V] logits in any of the three types."""
+    if logits2d.dim() != 2 or logits2d.shape[1] < 1:
+        raise ValueError("logits must be [rows, V]")
+    nat.require_cuda(logits2d)
+    code = nat.dtype_code(logits2d.dtype)
+    rows, V = logits2d.shape
+    if V > 1 and logits2d.stride(1) != 1:
+        raise ValueError("logits rows must be contiguous")
+    ld = logits2d.stride(0) if rows > 1 else V
+    if ld < V:
+        raise ValueError("logits rows may not overlap")
+    if bad_flag.dtype != torch.int32 or bad_flag.numel() < 1:
+        raise ValueError("bad_flag must be an int32 tensor")
+    _check_device(logits2d.device, bad_flag, *ts)
+    return code, rows, V, ld
+
+
+def _check_row_values(name, t, rows):
+    if t.dtype != torch.float32 or t.shape != (rows,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous fp32 [rows]")
+
+
+def _check_stats(stats, rows):
+    if stats.dtype != torch.float32 or stats.shape != (rows, 2) or not stats.is_contiguous():
+        raise ValueError("stats must be the forward's fp32 [rows, 2]")
+
+
+def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100):
+    """(logprob [rows], entropy [rows], stats [rows, 2], top_logprobs [rows,
+    top_k] fp32, top_ids [rows, top_k] int64) of logits [rows, V] in bf16, fp16
+    or fp32: the log probability of each row's token, the row's entropy and its
+    top_k largest log probabilities, equal ones by the lowest id.  Rows with
+    token `ignore_index` give 0, 0, -inf and -1; other ids outside the
+    vocabulary are clamped and flagged in `bad_flag`."""
+    code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
+    _check_ids(tokens, (rows,))
+    if not 0 <= top_k <= min(128, V):
+        raise ValueError(f"top_k must be in [0, 128] and within the vocabulary (got {top_k})")
+    new = functools.partial(torch.empty, dtype=torch.float32, device=logits2d.device)
+    logprob, entropy, stats, top = new(rows), new(rows), new(rows, 2), new(rows, top_k)
+    ids = torch.empty(rows, top_k, dtype=torch.int64, device=logits2d.device)
+    if rows:
+        # (the call's own: its two launches may have another thread's between them)
+        ws = nat.value("eth_token_logprobs_workspace", rows, V, top_k, code)
+        ws = torch.empty(ws, dtype=torch.uint8, device=logits2d.device) if ws else None
+        with _device_guard(logits2d):
+            nat.call("eth_token_logprobs_fwd", nat.ptr(logits2d), ld, nat.ptr(tokens), int(ignore_index),
+                     nat.ptr(logprob), nat.ptr(entropy), nat.ptr(stats), nat.ptr(top), nat.ptr(ids), top_k,
+                     nat.ptr(ws), rows, V, nat.ptr(bad_flag), code, nat.stream_ptr(logits2d.device))
+    return logprob, entropy, stats, top, ids
+
+
+def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad_flag, ignore_index=-100):
+    """dlogits [rows, V] for upstream gradients of logprob and entropy (fp32
+    [rows]; one of them may be None)."""
+    given = [t for t in (dlogprob, dentropy) if t is not None]
+    code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens, stats, entropy, *given)
+    _check_ids(tokens, (rows,))
+    _check_stats(stats, rows)
+    for name, t in (("entropy", entropy), ("dlogprob", dlogprob), ("dentropy", dentropy)):
+        if t is not None:
+            _check_row_values(name, t, rows)
+    if not given:
+        raise ValueError("token_logprobs_bwd needs dlogprob or dentropy")
+    dz = torch.empty(rows, V, dtype=logits2d.dtype, device=logits2d.device)
+    if rows:
+        with _device_guard(logits2d):
+            nat.call("eth_token_logprobs_bwd", nat.ptr(logits2d), ld, nat.ptr(tokens), int(ignore_index),
+                     nat.ptr(stats), nat.ptr(entropy), nat.ptr(dlogprob), nat.ptr(dentropy), nat.ptr(dz), V, rows, V,
+                     code, nat.stream_ptr(logits2d.device))
+    return dz
+
+
+def _check_teacher(teacher_ids, teacher_logits, rows, temperature):
+    if teacher_ids.dim() != 2 or teacher_logits.shape != teacher_ids.shape:
+        raise ValueError("teacher ids and logits must both be [rows, k]")
+    k = teacher_ids.shape[1]
+    if not 1 <= k <= 256:
+        raise ValueError(f"1 to 256 teacher entries a row are needed (got {k})")
+    _check_ids(teacher_ids, (rows, k))
+    if not teacher_logits.is_contiguous():
+        raise ValueError("teacher logits must be contiguous")
+    if not 2.0**-20 <= temperature <= 2.0**20:
+        raise ValueError(f"temperature must be positive and finite (got {temperature})")
+    return k, nat.dtype_code(teacher_logits.dtype)
+
+
+def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag):
+    """(loss [rows], stats [rows, 2]): temperature^2 * sum q (log q - log p[id])
+    with q the softmax of a row's k teacher logits (any of the three types) and
+    p that of its V logits, both at the temperature.  Negative ids and teacher
+    logits of -inf are no entries; ids past the vocabulary are none either and
+    are flagged in `bad_flag`."""
+    code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits)
+    k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
+    loss = torch.empty(rows, dtype=torch.float32, device=logits2d.device)
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=logits2d.device)
+    if rows:
+        with _device_guard(logits2d):
+            nat.call("eth_topk_distill_fwd", nat.ptr(logits2d), ld, nat.ptr(teacher_ids), nat.ptr(teacher_logits),
+                     teacher_code, k, float(temperature), nat.ptr(loss), nat.ptr(stats), rows, V, nat.ptr(bad_flag),
+                     code, nat.stream_ptr(logits2d.device))
+    return loss, stats
+
+
+def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag):
+    """dlogits [rows, V] of topk_distill_fwd's loss (dloss fp32 [rows])."""
+    code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits, stats, dloss)
+    k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
+    _check_stats(stats, rows)
+    _check_row_values("dloss", dloss, rows)
+    dz = torch.empty(rows, V, dtype=logits2d.dtype, device=logits2d.device)
+    if rows:
+        with _device_guard(logits2d):
+            nat.call("eth_topk_distill_bwd", nat.ptr(logits2d), ld, nat.ptr(teacher_ids), nat.ptr(teacher_logits),
+                     teacher_code, k, float(temperature), nat.ptr(stats), nat.ptr(dloss), nat.ptr(dz), V, rows, V,
+                     nat.ptr(bad_flag), code, nat.stream_ptr(logits2d.device))
+    return dz
+
+
 def synthetic_batch(sample_ids, seq, vocab, device):
     """tokens [b, s] int64, loss_mask [b, s] fp32, position_ids [b, s] int64
     of the deterministic synthetic batch, computed on the device in one

@@ -496,3 +496,69 @@ class CrossEntropyFn(torch.autograd.Function):
         z, lab, lse = ctx.saved_tensors
         dz = K.xent_bwd(z, lab, lse, dloss.reshape(-1).float().contiguous())
         return dz.view(ctx.shape), None, None
+
+
+def _logit_rows(logits):
+    """[rows, V] of logits [..., V] for the row kernels: the tensor's own
+    memory where its rows are whole and apart, else a copy."""
+    z = logits.reshape(-1, logits.shape[-1])
+    rows, V = z.shape
+    return z if (V == 1 or z.stride(1) == 1) and (rows <= 1 or z.stride(0) >= V) else z.contiguous()
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    """Log probabilities of tokens [...] under logits [..., V] (bf16, fp16 or
+    fp32), the entropy of each row and its top_k largest log probabilities with
+    their ids: (logprob [...], entropy [...], top_logprobs [..., top_k],
+    top_ids [..., top_k]).  Gradients flow from logprob and entropy; the top
+    alternatives are values.  Rows whose token is `ignore_index` give 0, 0,
+    -inf and -1 and get no gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, bad_flag, ignore_index=-100):
+        ctx.set_materialize_grads(False)
+        if tokens.shape != logits.shape[:-1]:
+            raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
+        z, t = _logit_rows(logits), tokens.reshape(-1).contiguous()
+        logprob, entropy, stats, top, ids = K.token_logprobs_fwd(z, t, top_k, bad_flag, ignore_index)
+        ctx.save_for_backward(z, t, stats, entropy)
+        ctx.shape, ctx.ignore_index, ctx.bad_flag = logits.shape, ignore_index, bad_flag
+        shape = logits.shape[:-1]
+        top, ids = top.view(*shape, top_k), ids.view(*shape, top_k)
+        ctx.mark_non_differentiable(top, ids)
+        return logprob.view(shape), entropy.view(shape), top, ids
+
+    @staticmethod
+    def backward(ctx, dlogprob, dentropy, _dtop, _dids):
+        if dlogprob is None and dentropy is None:
+            return None, None, None, None, None
+        z, t, stats, entropy = ctx.saved_tensors
+        dlogprob, dentropy = (None if g is None else g.reshape(-1).float().contiguous() for g in (dlogprob, dentropy))
+        dz = K.token_logprobs_bwd(z, t, stats, entropy, dlogprob, dentropy, ctx.bad_flag, ctx.ignore_index)
+        return dz.view(ctx.shape), None, None, None, None
+
+
+class TopkDistillFn(torch.autograd.Function):
+    """Per-row distillation loss [...] of logits [..., V] on a teacher's top
+    logits teacher_logits [..., k] at teacher_ids [..., k] (int64; negative: no
+    entry): temperature^2 KL(q || p) with q over the row's entries and p over
+    the vocabulary, both at the temperature.  The teacher is a constant."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, temperature, bad_flag):
+        if teacher_ids.shape[:-1] != logits.shape[:-1] or teacher_logits.shape != teacher_ids.shape:
+            raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} and logits {tuple(teacher_logits.shape)} do not "
+                             f"match logits {tuple(logits.shape)}")
+        z = _logit_rows(logits)
+        ids, teacher = (t.reshape(z.shape[0], t.shape[-1]).contiguous() for t in (teacher_ids, teacher_logits))
+        loss, stats = K.topk_distill_fwd(z, ids, teacher, temperature, bad_flag)
+        ctx.save_for_backward(z, ids, teacher, stats)
+        ctx.shape, ctx.temperature, ctx.bad_flag = logits.shape, temperature, bad_flag
+        return loss.view(logits.shape[:-1])
+
+    @staticmethod
+    def backward(ctx, dloss):
+        z, ids, teacher, stats = ctx.saved_tensors
+        dz = K.topk_distill_bwd(z, ids, teacher, ctx.temperature, stats, dloss.reshape(-1).float().contiguous(),
+                                ctx.bad_flag)
+        return dz.view(ctx.shape), None, None, None, None

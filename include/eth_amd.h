@@ -490,6 +490,53 @@ int eth_xent_bwd(const void* logits, int64_t ld, const int64_t* labels, const fl
                  const float* dloss, void* dlogits, int64_t ldd, int64_t rows, int64_t vocab,
                  int dtype, void* stream);
 
+/* Log probabilities of given tokens, the rows' entropies and top alternatives,
+ * of logits [rows, vocab] (row stride `ld` >= vocab; bf16, fp16 or fp32, `dtype`;
+ * aligned to an element; vocab up to 2^24).  Per row, in fp32:
+ *   logprob = z[token] - lse,  entropy = lse - sum p z,  p = exp(z - lse),
+ *   top_logprobs / top_ids [rows, top_k]: the largest z - lse with their ids,
+ *   equal ones by the lowest id (top_k from 0 to 128, at most vocab),
+ *   stats [rows, 2]: the row's maximum and log sum exp(z - max), for the backward.
+ * Logits may be -inf or the type's lowest value.  A row of -inf alone has
+ * logprob and top_logprobs -inf, entropy 0 and no gradient; NaN or +inf in a
+ * row makes its results NaN (NaN sorts first).  Rows whose token is
+ * `ignore_index` are not read: logprob 0, entropy 0, top_logprobs -inf, top_ids
+ * -1.  Other tokens outside [0, vocab) are clamped and set *bad_index to 1.
+ * `workspace`: eth_token_logprobs_workspace bytes, 16-byte aligned (0, NULL, for
+ * vocabularies that one workgroup holds).
+ * The backward writes, for upstream gradients dlogprob and dentropy [rows] (one
+ * may be NULL: zero),
+ *   dlogits_j = dlogprob ([j = token] - p_j) - dentropy p_j (log p_j + entropy);
+ * rows whose upstream gradients are zero get zeros and are not read. */
+int64_t eth_token_logprobs_workspace(int64_t rows, int64_t vocab, int top_k, int dtype);
+int eth_token_logprobs_fwd(const void* logits, int64_t ld, const int64_t* tokens,
+                           int64_t ignore_index, float* logprob, float* entropy, float* stats,
+                           float* top_logprobs, int64_t* top_ids, int top_k, void* workspace,
+                           int64_t rows, int64_t vocab, int* bad_index, int dtype, void* stream);
+int eth_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* tokens,
+                           int64_t ignore_index, const float* stats, const float* entropy,
+                           const float* dlogprob, const float* dentropy, void* dlogits,
+                           int64_t ldd, int64_t rows, int64_t vocab, int dtype, void* stream);
+
+/* Distillation from a teacher's top logits: teacher_ids (int64) and teacher
+ * (logits or log probabilities, `teacher_dtype`) [rows, k], k from 1 to 256.
+ * With q = softmax(teacher / temperature) over a row's entries and
+ * p = softmax(logits / temperature) over its vocabulary,
+ *   loss = temperature^2 sum q (log q - log p[id]).
+ * A negative id is no entry, and so is a teacher logit of -inf; an id at or past
+ * vocab is none and sets *bad_index to 1; an id may appear more than once.  A row
+ * without entries has loss 0, is not read, and gets no gradient.  stats as above, of
+ * logits / temperature.  The backward writes
+ *   dlogits_j = dloss temperature (p_j - sum of q over the entries with id j). */
+int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_t* teacher_ids,
+                         const void* teacher, int teacher_dtype, int k, float temperature,
+                         float* loss, float* stats, int64_t rows, int64_t vocab, int* bad_index,
+                         int dtype, void* stream);
+int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_ids,
+                         const void* teacher, int teacher_dtype, int k, float temperature,
+                         const float* stats, const float* dloss, void* dlogits, int64_t ldd,
+                         int64_t rows, int64_t vocab, int* bad_index, int dtype, void* stream);
+
 /* Tied word-embedding gradients on one rank: root = copy = root + copy (fp32,
  * 16-byte aligned).  Replaces the same-rank branch of
  * synchronize_shared_weights_grads (eth/runtime/megatron/training.py:489-531). */
