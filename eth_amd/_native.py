@@ -104,8 +104,8 @@ SIGNATURES["eth_synthetic_batch"] = [_P, _I64, _I64, _I64, _P, _P, _P, _P]
 SIGNATURES["eth_attn_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["eth_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
 
-SIGNATURES["eth_packed_attn_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
-SIGNATURES["eth_packed_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["eth_packed_attn_fwd"] = [_P, _P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["eth_packed_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
 
 SIGNATURES["eth_token_logprobs_fwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _P, _I32, _P]
 SIGNATURES["eth_token_logprobs_bwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]
@@ -150,6 +150,8 @@ class PackedAttnDesc(ctypes.Structure):
         ("k_tiles", ctypes.c_void_p),
         ("n_q_tiles", ctypes.c_int32),
         ("n_k_tiles", ctypes.c_int32),
+        ("q_split", ctypes.c_int32 * 3),
+        ("k_split", ctypes.c_int32 * 3),
         ("heads", ctypes.c_int32),
         ("kv_heads", ctypes.c_int32),
         ("head_dim", ctypes.c_int32),
@@ -170,6 +172,7 @@ VALUE_SIGNATURES = {
     "eth_embedding_bwd_workspace": ([_I64, _I64], _I64),
     "eth_token_logprobs_workspace": ([_I64, _I64, _I32, _I32], _I64),
     "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
+    "eth_packed_attn_workspace": ([_P, _I32], _I64),
 }
 GEMM_ACCUMULATE, GEMM_BIAS = 1, 2
 

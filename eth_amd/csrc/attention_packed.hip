@@ -43,6 +43,8 @@ struct PackArgs {
   float* delta;  // [n, T] rowsum(dO * O)
   const eth_packed_tile_t* q_tiles;
   const eth_packed_tile_t* k_tiles;
+  eth_packed_split_t q_split, k_split;
+  float4* partial;  // accumulators of split tiles' pieces
   int64_t T;
   int n, m, group;
   int hp;  // query heads per workgroup (1, 2 or 4; divides group)
@@ -56,6 +58,93 @@ __device__ __forceinline__ const uint16_t* row_ptr(const PackIn& t, int64_t row,
 }
 __device__ __forceinline__ uint16_t* row_ptr(const PackOut& t, int64_t row, int h) {
   return t.p + row * t.ss + (int64_t)h * t.sh;
+}
+
+// A tile's chain of steps may be split over several workgroups (`pieces`), whose
+// fp32 accumulators a second kernel joins in order: the first split.tiles
+// tiles of a list, which have the longest chains, take split.pieces workgroups
+// per head each, and those behind them one.
+struct Piece {
+  int tile, head, piece;  // tile of the list, head (or group of heads)
+  int pieces;             // 1: the tile is not split
+};
+__device__ __forceinline__ Piece piece_of(int block, int heads, const eth_packed_split_t& sp) {
+  const int head = block % heads, r = block / heads, cut = sp.tiles * sp.pieces;
+  if (r >= cut) return Piece{sp.tiles + r - cut, head, 0, 1};
+  return Piece{r % sp.tiles, head, r / sp.tiles, sp.pieces};
+}
+// steps of a piece: equal shares, of split.steps or a little less each; the
+// last of a short tile's pieces may be left without any
+struct Steps {
+  int from, to, used;  // used: pieces that have steps
+};
+__device__ __forceinline__ Steps steps_of(int chain, int piece, int pieces, int steps) {
+  if (pieces == 1) return Steps{0, chain, 1};
+  const int want = min((chain + steps - 1) / steps, pieces), share = (chain + want - 1) / want;
+  return Steps{min(piece * share, chain), min((piece + 1) * share, chain), (chain + share - 1) / share};
+}
+// A wave's accumulators of a piece as it holds them, whole float4 vectors side
+// by side: vector i of wave w of a piece's `waves`
+template <int DT>
+__device__ __forceinline__ float4* partial_of(const PackArgs& a, const eth_packed_split_t& sp, int heads,
+                                              const Piece& pc, int piece, int waves, int w, int lane) {
+  return a.partial + ((((int64_t)pc.tile * heads + pc.head) * sp.pieces + piece) * waves + w) * (DT * 4 * 64) + lane;
+}
+template <int DT>
+__device__ __forceinline__ void put_partial(float4* p, const a_f32x16 (&x)[DT]) {
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      p[(t * 4 + g) * 64] = make_float4(x[t][g * 4], x[t][g * 4 + 1], x[t][g * 4 + 2], x[t][g * 4 + 3]);
+}
+template <int DT>
+__device__ __forceinline__ void add_partial(const float4* p, a_f32x16 (&x)[DT], float f) {
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 u = p[(t * 4 + g) * 64];
+      x[t][g * 4 + 0] += u.x * f;
+      x[t][g * 4 + 1] += u.y * f;
+      x[t][g * 4 + 2] += u.z * f;
+      x[t][g * 4 + 3] += u.w * f;
+    }
+}
+// a lane's row of a [D, 32 rows] accumulator, times f, rounded
+template <int DT, bool FP16>
+__device__ __forceinline__ void store_row(uint16_t* p, const a_f32x16 (&x)[DT], float f, int hd, int hl) {
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      if (t * 32 + g * 8 >= hd) continue;  // hd % 8 == 0: whole 8-column groups
+      uint2 v;
+      v.x = pack2<FP16>(x[t][g * 4 + 0] * f, x[t][g * 4 + 1] * f);
+      v.y = pack2<FP16>(x[t][g * 4 + 2] * f, x[t][g * 4 + 3] * f);
+      *reinterpret_cast<uint2*>(p + t * 32 + g * 8 + hl * 4) = v;
+    }
+}
+// A [32 keys, D] accumulator, times f, rounded, by way of the wave's own
+// `stage` (rows SL elements apart) in 16-byte row chunks: lane holds d = t*32 +
+// lane%32 of keys acc_row(r, hl)
+template <int D, int SL, bool FP16>
+__device__ __forceinline__ void store_keys(const PackOut& out, uint16_t* stage, const a_f32x16 (&x)[D / 32], float f,
+                                           int64_t begin, int k0, int len, int kvh, int hd, int lane) {
+  constexpr int CPR = D / 8;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      stage[acc_row(r, lane >> 5) * SL + t * 32 + (lane & 31)] = from_f<FP16>(x[t][r] * f);
+  wave_lds_fence();  // a wave reads back only its own rows
+#pragma unroll
+  for (int i = 0; i < 32 * CPR / 64; ++i) {
+    const int c = i * 64 + lane, kr = c / CPR, col = (c % CPR) * 8;
+    if (k0 + kr >= len || col >= hd) continue;
+    *reinterpret_cast<uint4*>(row_ptr(out, begin + k0 + kr, kvh) + col) =
+        *reinterpret_cast<const uint4*>(stage + kr * SL + col);
+  }
 }
 
 // Direct loads of 64-row blocks of one head of one sequence by four waves:
@@ -125,9 +214,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
 
   // workgroups of one key/value head a multiple of m apart: on one die for
   // m % 8 == 0, whose L2 then serves the shared rows
-  const int hbs = a.n / a.hp, hb = blockIdx.x % hbs;
-  const int kvh = hb % a.m, h0 = kvh * a.group + hb / a.m * a.hp;
-  const eth_packed_tile_t tile = a.q_tiles[blockIdx.x / hbs];
+  const int hbs = a.n / a.hp;
+  const Piece pc = piece_of(blockIdx.x, hbs, a.q_split);
+  const int kvh = pc.head % a.m, h0 = kvh * a.group + pc.head / a.m * a.hp;
+  const eth_packed_tile_t tile = a.q_tiles[pc.tile];
   const int64_t begin = tile.begin;
   if (tile.len < 0) {
     zero_rows(a.out, begin, -tile.len, h0, a.hp, a.hd, kAttnThreads);
@@ -149,9 +239,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
   vc.init(a.v, begin, len, a.hd, w, lane);
   const int64_t kh = kvh * a.k.sh * 2, vh = kvh * a.v.sh * 2;
   const int qend = min(tile.start + bq, len);  // past the tile's last query
-  const int nkv = (qend + kBKV - 1) / kBKV;
-  kc.issue(K0, 0, kh);
-  vc.issue(V0, 0, vh);
+  const Steps st = steps_of((qend + kBKV - 1) / kBKV, pc.piece, pc.pieces, a.q_split.steps);
+  const int nkv = st.to;
+  if (st.from >= nkv) return;
+  kc.issue(K0, st.from * kBKV, kh);
+  vc.issue(V0, st.from * kBKV, vh);
 
   uint4 qf[KS];
   {
@@ -253,27 +345,55 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
     vm_wait_all();  // the next block's rows have landed
     __syncthreads();  // this block's images free, the next block's visible
   };
-  int j = 0;
+  int j = st.from;
   for (; j + 1 < nkv; j += 2) {
     block(j, std::integral_constant<int, 0>{});
     block(j + 1, std::integral_constant<int, 1>{});
   }
   if (j < nkv) block(j, std::integral_constant<int, 0>{});
   l += __shfl_xor(l, 32, 64);
+  if (pc.pieces > 1) {
+    put_partial<DT>(partial_of<DT>(a, a.q_split, hbs, pc, pc.piece, 4, w, lane), o);
+    float2* ml = reinterpret_cast<float2*>(a.partial + (int64_t)a.q_split.tiles * hbs * a.q_split.pieces * (DT * 1024));
+    ml[((((int64_t)pc.tile * hbs + pc.head) * a.q_split.pieces + pc.piece) * 4 + w) * 64 + lane] = make_float2(m, l);
+    return;
+  }
   if (!real) return;  // a row past the sequence
-  const float inv = 1.0f / l;
-  uint16_t* op = row_ptr(a.out, begin + q, h);
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (t * 32 + g * 8 >= a.hd) continue;  // hd % 8 == 0: whole 8-column groups
-      uint2 v;
-      v.x = pack2<FP16>(o[t][g * 4 + 0] * inv, o[t][g * 4 + 1] * inv);
-      v.y = pack2<FP16>(o[t][g * 4 + 2] * inv, o[t][g * 4 + 3] * inv);
-      *reinterpret_cast<uint2*>(op + t * 32 + g * 8 + hl * 4) = v;
-    }
+  store_row<DT, FP16>(row_ptr(a.out, begin + q, h), o, 1.0f / l, a.hd, hl);
   if (hl == 0) a.lse[(int64_t)h * a.T + begin + q] = m + log2f(l);
+}
+
+// joins the pieces of split query tiles, in order
+template <int D, bool FP16>
+__global__ void __launch_bounds__(kAttnThreads) packed_fwd_join_kernel(PackArgs a) {
+  constexpr int DT = D / 32;
+  const int hbs = a.n / a.hp;
+  const Piece pc{(int)(blockIdx.x / hbs), (int)(blockIdx.x % hbs), 0, a.q_split.pieces};
+  const int kvh = pc.head % a.m, h0 = kvh * a.group + pc.head / a.m * a.hp;
+  const eth_packed_tile_t tile = a.q_tiles[pc.tile];
+  if (tile.len < 0) return;  // (stored as zeros by the first launch)
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = h0 + w % a.hp, q = tile.start + w / a.hp * 32 + (lane & 31);
+  const int qend = min(tile.start + kBQ / a.hp, tile.len);
+  const int used = steps_of((qend + kBKV - 1) / kBKV, 0, pc.pieces, a.q_split.steps).used;
+  const float2* ml = reinterpret_cast<const float2*>(a.partial + (int64_t)a.q_split.tiles * hbs * a.q_split.pieces *
+                                                                     (DT * 1024)) +
+                     (((int64_t)pc.tile * hbs + pc.head) * a.q_split.pieces * 4 + w) * 64 + lane;
+  float m = -3.4028234e38f, l = 0.f;
+  for (int i = 0; i < used; ++i) m = fmaxf(m, ml[i * 256].x);
+  a_f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = a_f32x16{};
+  for (int i = 0; i < used; ++i) {
+    const float2 x = ml[i * 256];
+    const float f = fast_exp2(x.x - m);
+    l += x.y * f;
+    add_partial<DT>(partial_of<DT>(a, a.q_split, hbs, pc, i, 4, w, lane), o, f);
+  }
+  if (q >= tile.len) return;
+  store_row<DT, FP16>(row_ptr(a.out, tile.begin + q, h), o, 1.0f / l, a.hd, lane >> 5);
+  if (lane < 32) a.lse[(int64_t)h * a.T + tile.begin + q] = m + log2f(l);
 }
 
 // ------------------------------------------------------------ backward: dQ --
@@ -288,9 +408,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
   __shared__ __attribute__((aligned(16))) uint16_t V0[IMG];
   __shared__ __attribute__((aligned(16))) uint16_t V1[IMG];
 
-  const int hbs = a.n / a.hp, hb = blockIdx.x % hbs;
-  const int kvh = hb % a.m, h0 = kvh * a.group + hb / a.m * a.hp;
-  const eth_packed_tile_t tile = a.q_tiles[blockIdx.x / hbs];
+  const int hbs = a.n / a.hp;
+  const Piece pc = piece_of(blockIdx.x, hbs, a.q_split);
+  const int kvh = pc.head % a.m, h0 = kvh * a.group + pc.head / a.m * a.hp;
+  const eth_packed_tile_t tile = a.q_tiles[pc.tile];
   const int64_t begin = tile.begin;
   if (tile.len < 0) {
     zero_rows(a.dq, begin, -tile.len, h0, a.hp, a.hd, kAttnThreads);
@@ -309,9 +430,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
   vc.init(a.v, begin, len, a.hd, w, lane);
   const int64_t kh = kvh * a.k.sh * 2, vh = kvh * a.v.sh * 2;
   const int qend = min(tile.start + bq, len);
-  const int nkv = (qend + kBKV - 1) / kBKV;
-  kc.issue(K0, 0, kh);
-  vc.issue(V0, 0, vh);
+  const Steps st = steps_of((qend + kBKV - 1) / kBKV, pc.piece, pc.pieces, a.q_split.steps);
+  const int nkv = st.to;
+  if (st.from >= nkv) return;
+  kc.issue(K0, st.from * kBKV, kh);
+  vc.issue(V0, st.from * kBKV, vh);
 
   uint4 qf[KS], of[KS];
   {
@@ -342,7 +465,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
       }
     }
     del += __shfl_xor(del, 32, 64);
-    if (hl == 0 && real) a.delta[srow] = del;
+    if (hl == 0 && real && pc.piece == 0) a.delta[srow] = del;
   }
   a_f32x16 dq[DT];
 #pragma unroll
@@ -406,24 +529,38 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
     vm_wait_all();  // the next block's rows have landed
     __syncthreads();  // this block's images free, the next block's visible
   };
-  int j = 0;
+  int j = st.from;
   for (; j + 1 < nkv; j += 2) {
     block(j, std::integral_constant<int, 0>{});
     block(j + 1, std::integral_constant<int, 1>{});
   }
   if (j < nkv) block(j, std::integral_constant<int, 0>{});
-  if (!real) return;
-  uint16_t* dqp = row_ptr(a.dq, begin + q, h);
+  if (pc.pieces > 1) {
+    put_partial<DT>(partial_of<DT>(a, a.q_split, hbs, pc, pc.piece, 4, w, lane), dq);
+    return;
+  }
+  if (real) store_row<DT, FP16>(row_ptr(a.dq, begin + q, h), dq, a.scale, a.hd, hl);
+}
+
+// joins the pieces of split query tiles, in order
+template <int D, bool FP16>
+__global__ void __launch_bounds__(kAttnThreads) packed_dq_join_kernel(PackArgs a) {
+  constexpr int DT = D / 32;
+  const int hbs = a.n / a.hp;
+  const Piece pc{(int)(blockIdx.x / hbs), (int)(blockIdx.x % hbs), 0, a.q_split.pieces};
+  const int kvh = pc.head % a.m, h0 = kvh * a.group + pc.head / a.m * a.hp;
+  const eth_packed_tile_t tile = a.q_tiles[pc.tile];
+  if (tile.len < 0) return;  // (stored as zeros by the first launch)
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = h0 + w % a.hp, q = tile.start + w / a.hp * 32 + (lane & 31);
+  const int qend = min(tile.start + kBQ / a.hp, tile.len);
+  const int used = steps_of((qend + kBKV - 1) / kBKV, 0, pc.pieces, a.q_split.steps).used;
+  a_f32x16 dq[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (t * 32 + g * 8 >= a.hd) continue;
-      uint2 v;
-      v.x = pack2<FP16>(dq[t][g * 4 + 0] * a.scale, dq[t][g * 4 + 1] * a.scale);
-      v.y = pack2<FP16>(dq[t][g * 4 + 2] * a.scale, dq[t][g * 4 + 3] * a.scale);
-      *reinterpret_cast<uint2*>(dqp + t * 32 + g * 8 + hl * 4) = v;
-    }
+  for (int t = 0; t < DT; ++t) dq[t] = a_f32x16{};
+  for (int i = 0; i < used; ++i) add_partial<DT>(partial_of<DT>(a, a.q_split, hbs, pc, i, 4, w, lane), dq, 1.f);
+  if (q < tile.len) store_row<DT, FP16>(row_ptr(a.dq, tile.begin + q, h), dq, a.scale, a.hd, lane >> 5);
 }
 
 // The steps of a key tile: the 64-query blocks from the tile's first query on,
@@ -436,6 +573,10 @@ struct PackStep {
       block = first;
       ++head;
     }
+  }
+  static __device__ __forceinline__ PackStep at(int i, int first, int nq) {
+    const int head = i / (nq - first);
+    return PackStep{head, first + i - head * (nq - first)};
   }
 };
 
@@ -456,8 +597,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
   __shared__ __attribute__((aligned(16))) float lse_s[2][kBQ2];
   __shared__ __attribute__((aligned(16))) float del_s[2][kBQ2];
 
-  const int kvh = blockIdx.x % a.m;
-  const eth_packed_tile_t tile = a.k_tiles[blockIdx.x / a.m];
+  const Piece pc = piece_of(blockIdx.x, a.m, a.k_split);
+  const int kvh = pc.head;
+  const eth_packed_tile_t tile = a.k_tiles[pc.tile];
   const int64_t begin = tile.begin;
   if (tile.len < 0) {
     zero_rows(a.dk, begin, -tile.len, kvh, 1, a.hd, kAttnThreads);
@@ -497,8 +639,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
     oc.issue(oi, st.block * kBQ2, h * a.dout.sh * 2);
   };
   const int first = tile.start / kBQ2, nq = (len + kBQ2 - 1) / kBQ2;
-  const int steps = (nq - first) * a.group;
-  PackStep cur{0, first}, nxt = cur;
+  const Steps st = steps_of((nq - first) * a.group, pc.piece, pc.pieces, a.k_split.steps);
+  const int steps = st.to - st.from;
+  if (steps <= 0) return;
+  PackStep cur = PackStep::at(st.from, first, nq), nxt = cur;
   nxt.next(first, nq);
   float stat_n = 0.f;
   issue(Q0, O0, cur);
@@ -614,29 +758,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
   }
   if (i < steps) step(i, std::integral_constant<int, 0>{});
 
-  // out through LDS in 16-byte row chunks: lane holds d = t*32 + lane%32 for
-  // keys acc_row(r, hl); dV by way of the dO images, dK of the Q images
-  static_assert(2 * 32 * D <= IMG, "two waves' staging fits an image");
-  uint16_t* sv = (w < 2 ? O0 : O1) + (w & 1) * 32 * D;
-  uint16_t* sk = (w < 2 ? Q0 : Q1) + (w & 1) * 32 * D;
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int o = acc_row(r, hl) * D + t * 32 + (lane & 31);
-      sv[o] = from_f<FP16>(dv[t][r]);
-      sk[o] = from_f<FP16>(dk[t][r] * a.scale);
-    }
-  wave_lds_fence();  // a wave reads back only its own rows
-#pragma unroll
-  for (int i = 0; i < 32 * CPR / 64; ++i) {
-    const int c = i * 64 + lane, kr = c / CPR, col = (c % CPR) * 8;
-    if (k0 + kr >= len || col >= a.hd) continue;
-    *reinterpret_cast<uint4*>(row_ptr(a.dv, begin + k0 + kr, kvh) + col) =
-        *reinterpret_cast<const uint4*>(sv + kr * D + col);
-    *reinterpret_cast<uint4*>(row_ptr(a.dk, begin + k0 + kr, kvh) + col) =
-        *reinterpret_cast<const uint4*>(sk + kr * D + col);
+  if (pc.pieces > 1) {
+    put_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, pc.piece, 8, w, lane), dv);
+    put_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, pc.piece, 8, 4 + w, lane), dk);
+    return;
   }
+  // dV by way of the dO images, dK of the Q images
+  static_assert(2 * 32 * D <= IMG, "two waves' staging fits an image");
+  store_keys<D, D, FP16>(a.dv, (w < 2 ? O0 : O1) + (w & 1) * 32 * D, dv, 1.f, begin, k0, len, kvh, a.hd, lane);
+  store_keys<D, D, FP16>(a.dk, (w < 2 ? Q0 : Q1) + (w & 1) * 32 * D, dk, a.scale, begin, k0, len, kvh, a.hd, lane);
 }
 
 // ------------------------------ backward: dK, dV paired, head dims to 128 --
@@ -657,8 +787,9 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
   __shared__ __attribute__((aligned(16))) float lse_s[2][kBQ2];
   __shared__ __attribute__((aligned(16))) float del_s[2][kBQ2];
 
-  const int kvh = blockIdx.x % a.m;
-  const eth_packed_tile_t tile = a.k_tiles[blockIdx.x / a.m];
+  const Piece pc = piece_of(blockIdx.x, a.m, a.k_split);
+  const int kvh = pc.head;
+  const eth_packed_tile_t tile = a.k_tiles[pc.tile];
   const int64_t begin = tile.begin;
   if (tile.len < 0) {
     zero_rows(a.dk, begin, -tile.len, kvh, 1, a.hd, 2 * kAttnThreads);
@@ -763,7 +894,9 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
   };
 
   const int first = tile.start / kBQ2, nq = (len + kBQ2 - 1) / kBQ2;
-  const int n = (nq - first) * a.group;
+  const Steps st = steps_of((nq - first) * a.group, pc.piece, pc.pieces, a.k_split.steps);
+  const int n = st.to - st.from;
+  if (n <= 0) return;
   auto stat = [&](const PackStep& st) __attribute__((always_inline)) {
     float v = dkw ? 0.f : 1e30f;
     const int qi = st.block * kBQ2 + rt;
@@ -778,7 +911,7 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
     else
       lse_s[p][rt] = v;
   };
-  PackStep cur{0, first}, nxt = cur;
+  PackStep cur = PackStep::at(st.from, first, nq), nxt = cur;
   nxt.next(first, nq);
   float stat_n = 0.f;
   issue(dkw ? O0 : Qx, cur);
@@ -904,27 +1037,37 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
     run(std::true_type{});
   else
     run(std::false_type{});
-  // the 32 x 128 tile of each wave (dV or dK, rounded to 16 bits) through
-  // LDS, then out in 16-byte row chunks: lane holds d = t*32 + lane%32 for
-  // keys acc_row(r, hl); the staging rows are padded by 8 elements
+  if (pc.pieces > 1) {
+    put_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, pc.piece, 8, wv, lane), acc);
+    return;
+  }
+  // the staging rows are padded by 8 elements: 8.5 KB per wave, the dV waves'
+  // in the Q images, the dK waves' in the P buffers
   constexpr int SL = D + 8;
   __syncthreads();  // every image and P buffer read
-  // 8.5 KB per wave: the dV waves' in the Q images, the dK waves' in the P buffers
   uint16_t* stage = (dkw ? reinterpret_cast<uint16_t*>(&Ps[0][0][0][0][0]) : Qx) + w * 32 * SL;
   static_assert(4 * 32 * SL <= 3 * IMG && 4 * 32 * SL * 2 <= (int)sizeof(Ps), "staging fits");
+  store_keys<D, SL, FP16>(dkw ? a.dk : a.dv, stage, acc, dkw ? a.scale : 1.f, begin, k0, len, kvh, a.hd, lane);
+}
+
+// joins the pieces of split key tiles, in order: waves 0 to 3 dV, 4 to 7 dK
+template <int D, bool FP16>
+__global__ void __launch_bounds__(2 * kAttnThreads) packed_dkdv_join_kernel(PackArgs a) {
+  constexpr int DT = D / 32, SL = D + 8;
+  __shared__ __attribute__((aligned(16))) uint16_t stage[8 * 32 * SL];
+  const Piece pc{(int)(blockIdx.x / a.m), (int)(blockIdx.x % a.m), 0, a.k_split.pieces};
+  const eth_packed_tile_t tile = a.k_tiles[pc.tile];
+  if (tile.len < 0) return;  // (stored as zeros by the first launch)
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int first = tile.start / kBQ2, nq = (tile.len + kBQ2 - 1) / kBQ2;
+  const int used = steps_of((nq - first) * a.group, 0, pc.pieces, a.k_split.steps).used;
+  a_f32x16 x[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-      stage[acc_row(r, hl) * SL + t * 32 + (lane & 31)] = from_f<FP16>(dkw ? acc[t][r] * a.scale : acc[t][r]);
-  wave_lds_fence();  // the wave reads back only its own rows
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = i * 64 + lane, kr = c >> 4, col = (c & 15) * 8;  // key row, first column of the chunk
-    if (k0 + kr >= len || col >= a.hd) continue;
-    *reinterpret_cast<uint4*>(row_ptr(dkw ? a.dk : a.dv, begin + k0 + kr, kvh) + col) =
-        *reinterpret_cast<const uint4*>(stage + kr * SL + col);
-  }
+  for (int t = 0; t < DT; ++t) x[t] = a_f32x16{};
+  for (int i = 0; i < used; ++i) add_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, i, 8, wv, lane), x, 1.f);
+  store_keys<D, SL, FP16>(wv < 4 ? a.dv : a.dk, stage + wv * 32 * SL, x, wv < 4 ? 1.f : a.scale, tile.begin,
+                          tile.start + (wv & 3) * 32, tile.len, pc.head, a.hd, lane);
 }
 
 }  // namespace eth
@@ -945,6 +1088,22 @@ static bool good_strides(const void* p, const int64_t* st) {
          st[0] < (1LL << 24);
 }
 
+static bool good_split(const eth_packed_split_t& sp, int n_tiles, int heads) {
+  if (sp.tiles == 0) return true;
+  return sp.tiles > 0 && sp.tiles <= n_tiles && sp.pieces > 1 && sp.steps > 0 &&
+         (int64_t)sp.tiles * sp.pieces * heads < (1LL << 24);
+}
+static int64_t grid_of(const eth_packed_split_t& sp, int n_tiles, int heads) {
+  return (int64_t)heads * (n_tiles - sp.tiles + (sp.tiles ? sp.tiles * sp.pieces : 0));
+}
+// float4 vectors of a piece: 4 waves' accumulators of a query tile (and two
+// statistics a lane, forward), 8 waves' of a key tile
+static int64_t piece_vectors(const eth_packed_split_t& sp, int heads, int width, int waves) {
+  return sp.tiles ? (int64_t)sp.tiles * sp.pieces * heads * waves * (width / 32 * 4 * 64) : 0;
+}
+
+static int width_of(int head_dim) { return head_dim > 96 ? 128 : head_dim > 64 ? 96 : 64; }
+
 static int packed_check(const eth_packed_attn_desc_t* d) {
   ETH_CHECK_ARG(d, "packed attention: null descriptor");
   ETH_CHECK_ARG(d->dtype == ETH_BF16 || d->dtype == ETH_F16, "packed attention: dtype must be bf16/fp16");
@@ -957,6 +1116,8 @@ static int packed_check(const eth_packed_attn_desc_t* d) {
   ETH_CHECK_ARG(d->q_tiles && d->k_tiles && d->n_q_tiles > 0 && d->n_k_tiles > 0, "packed attention: no tiles");
   ETH_CHECK_ARG((int64_t)d->n_q_tiles * d->heads < (1LL << 31) && (int64_t)d->n_k_tiles * d->kv_heads < (1LL << 31),
                 "packed attention: too many tiles");
+  ETH_CHECK_ARG(good_split(d->q_split, d->n_q_tiles, d->heads) && good_split(d->k_split, d->n_k_tiles, d->kv_heads),
+                "packed attention: bad split");
   // (a positive scale keeps the order of the scores, and a product with -inf is -inf)
   ETH_CHECK_ARG(d->scale >= 0x1p-100f && d->scale <= 0x1p100f, "packed attention: scale must be positive and finite");
   return ETH_OK;
@@ -966,6 +1127,8 @@ static PackArgs packed_args(const eth_packed_attn_desc_t* d) {
   PackArgs a{};
   a.q_tiles = d->q_tiles;
   a.k_tiles = d->k_tiles;
+  a.q_split = d->q_split;
+  a.k_split = d->k_split;
   a.T = d->rows;
   a.n = d->heads;
   a.m = d->kv_heads;
@@ -979,17 +1142,33 @@ static PackArgs packed_args(const eth_packed_attn_desc_t* d) {
 static PackIn pin(const void* p, const int64_t* st) { return PackIn{(const uint16_t*)p, st[0], st[1]}; }
 static PackOut pout(void* p, const int64_t* st) { return PackOut{(uint16_t*)p, st[0], st[1]}; }
 
+extern "C" int64_t eth_packed_attn_workspace(const eth_packed_attn_desc_t* d, int backward) {
+  if (packed_check(d)) return 0;
+  const int width = width_of(d->head_dim), hbs = d->heads / heads_per_tile(d->heads / d->kv_heads);
+  const int64_t q = piece_vectors(d->q_split, hbs, width, 4), k = piece_vectors(d->k_split, d->kv_heads, width, 8);
+  // (the backward joins dQ's pieces before dK's and dV's are written)
+  return (backward ? (q > k ? q : k) : q + q / (width / 32 * 4) / 2) * (int64_t)sizeof(float4);
+}
+
+template <int D, bool FP16>
+static void launch_packed_fwd(const PackArgs& a, int grid, hipStream_t s) {
+  packed_fwd_kernel<D, FP16><<<grid, kAttnThreads, 0, s>>>(a);
+  if (a.q_split.tiles) packed_fwd_join_kernel<D, FP16><<<a.q_split.tiles * (a.n / a.hp), kAttnThreads, 0, s>>>(a);
+}
+
 template <int D, bool FP16>
 static void launch_packed_bwd(const PackArgs& a, int g_q, int g_k, hipStream_t s) {
   packed_bwd_dq_kernel<D, FP16><<<g_q, kAttnThreads, 0, s>>>(a);  // first: it also writes delta
+  if (a.q_split.tiles) packed_dq_join_kernel<D, FP16><<<a.q_split.tiles * (a.n / a.hp), kAttnThreads, 0, s>>>(a);
   if constexpr (D == 128)
     packed_bwd_dkdv_x128_kernel<FP16><<<g_k, 2 * kAttnThreads, 0, s>>>(a);
   else
     packed_bwd_dkdv_kernel<D, FP16><<<g_k, kAttnThreads, 0, s>>>(a);
+  if (a.k_split.tiles) packed_dkdv_join_kernel<D, FP16><<<a.k_split.tiles * a.m, 2 * kAttnThreads, 0, s>>>(a);
 }
 
 extern "C" int eth_packed_attn_fwd(const eth_packed_attn_desc_t* d, const void* q, const void* k, const void* v,
-                                   void* out, float* lse, void* stream) {
+                                   void* out, float* lse, void* workspace, void* stream) {
   if (int rc = packed_check(d)) return rc;
   ETH_CHECK_ARG(q && k && v && out && lse, "eth_packed_attn_fwd: null pointer");
   ETH_CHECK_ARG(good_strides(q, d->q_strides) && good_strides(k, d->k_strides) && good_strides(v, d->v_strides) &&
@@ -1001,17 +1180,21 @@ extern "C" int eth_packed_attn_fwd(const eth_packed_attn_desc_t* d, const void* 
   a.v = pin(v, d->v_strides);
   a.out = pout(out, d->o_strides);
   a.lse = lse;
-  const int grid = d->n_q_tiles * (a.n / a.hp);
+  ETH_CHECK_ARG(!a.q_split.tiles || (workspace && ((uintptr_t)workspace & 15) == 0),
+                "eth_packed_attn_fwd: split tiles need a 16-byte aligned workspace");
+  a.partial = (float4*)workspace;
+  const int grid = (int)grid_of(a.q_split, d->n_q_tiles, a.n / a.hp);
   hipStream_t s = (hipStream_t)stream;
   const bool fp16 = d->dtype == ETH_F16;
-#define ETH_PACKED_FWD(D)                                          \
-  if (fp16)                                                        \
-    packed_fwd_kernel<D, true><<<grid, kAttnThreads, 0, s>>>(a);   \
-  else                                                             \
-    packed_fwd_kernel<D, false><<<grid, kAttnThreads, 0, s>>>(a);
-  if (a.hd > 96) {
+#define ETH_PACKED_FWD(D)                        \
+  if (fp16)                                      \
+    launch_packed_fwd<D, true>(a, grid, s);      \
+  else                                           \
+    launch_packed_fwd<D, false>(a, grid, s);
+  const int width = width_of(a.hd);
+  if (width == 128) {
     ETH_PACKED_FWD(128)
-  } else if (a.hd > 64) {
+  } else if (width == 96) {
     ETH_PACKED_FWD(96)
   } else {
     ETH_PACKED_FWD(64)
@@ -1023,7 +1206,7 @@ extern "C" int eth_packed_attn_fwd(const eth_packed_attn_desc_t* d, const void* 
 
 extern "C" int eth_packed_attn_bwd(const eth_packed_attn_desc_t* d, const void* q, const void* k, const void* v,
                                    const void* out, const void* dout, const float* lse, float* delta, void* dq,
-                                   void* dk, void* dv, void* stream) {
+                                   void* dk, void* dv, void* workspace, void* stream) {
   if (int rc = packed_check(d)) return rc;
   ETH_CHECK_ARG(q && k && v && out && dout && lse && delta && dq && dk && dv, "eth_packed_attn_bwd: null pointer");
   ETH_CHECK_ARG(good_strides(q, d->q_strides) && good_strides(k, d->k_strides) && good_strides(v, d->v_strides) &&
@@ -1042,7 +1225,10 @@ extern "C" int eth_packed_attn_bwd(const eth_packed_attn_desc_t* d, const void* 
   a.dv = pout(dv, d->dv_strides);
   a.lse = const_cast<float*>(lse);
   a.delta = delta;
-  const int g_q = d->n_q_tiles * (a.n / a.hp), g_k = d->n_k_tiles * a.m;
+  ETH_CHECK_ARG((!a.q_split.tiles && !a.k_split.tiles) || (workspace && ((uintptr_t)workspace & 15) == 0),
+                "eth_packed_attn_bwd: split tiles need a 16-byte aligned workspace");
+  a.partial = (float4*)workspace;
+  const int g_q = (int)grid_of(a.q_split, d->n_q_tiles, a.n / a.hp), g_k = (int)grid_of(a.k_split, d->n_k_tiles, a.m);
   hipStream_t s = (hipStream_t)stream;
   const bool fp16 = d->dtype == ETH_F16;
 #define ETH_PACKED_BWD(D)                        \
@@ -1050,9 +1236,10 @@ extern "C" int eth_packed_attn_bwd(const eth_packed_attn_desc_t* d, const void* 
     launch_packed_bwd<D, true>(a, g_q, g_k, s);  \
   else                                           \
     launch_packed_bwd<D, false>(a, g_q, g_k, s);
-  if (a.hd > 96) {
+  const int width = width_of(a.hd);
+  if (width == 128) {
     ETH_PACKED_BWD(128)
-  } else if (a.hd > 64) {
+  } else if (width == 96) {
     ETH_PACKED_BWD(96)
   } else {
     ETH_PACKED_BWD(64)

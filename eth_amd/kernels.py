@@ -487,12 +487,19 @@ def _packed_desc(q, k, v, packed, scale, code):
     _check_device(packed.device, q, k, v)
     desc = nat.PackedAttnDesc()
     desc.rows, desc.heads, desc.kv_heads, desc.head_dim, desc.dtype, desc.scale = rows, n, m, d, code, scale
-    desc.q_tiles, desc.n_q_tiles, desc.k_tiles, desc.n_k_tiles = packed.tiles(
-        nat.value("eth_packed_attn_tile_rows", n, m))
+    (desc.q_tiles, desc.n_q_tiles, desc.k_tiles, desc.n_k_tiles, desc.q_split[:], desc.k_split[:]) = packed.plan(
+        n, m, d)
     desc.q_strides[:] = _thd_strides("q", q)
     desc.k_strides[:] = _thd_strides("k", k)
     desc.v_strides[:] = _thd_strides("v", v)
     return desc
+
+
+def _packed_workspace(desc, backward, device):
+    if not (desc.q_split[0] or backward and desc.k_split[0]):
+        return None
+    size = nat.value("eth_packed_attn_workspace", ctypes.byref(desc), backward)
+    return torch.empty(size, dtype=torch.uint8, device=device)
 
 
 def _packed_flops(packed, n, d):
@@ -513,11 +520,12 @@ def packed_attention_fwd(q, k, v, packed, scale=None, out=None):
         raise ValueError("out must be a contiguous [rows, n*hn] tensor like q")
     desc.o_strides[:] = _thd_strides("out", out.view(rows, n, d), written=True)
     lse = torch.empty(n, rows, dtype=torch.float32, device=q.device)
+    ws = _packed_workspace(desc, 0, q.device)
     flops = _packed_flops(packed, n, d) if _observer is not None else 0.0
     with _device_guard(q):
         _observe("attn_fwd", "begin", flops)
         nat.call("eth_packed_attn_fwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(out),
-                 nat.ptr(lse), nat.stream_ptr(q.device))
+                 nat.ptr(lse), nat.ptr(ws), nat.stream_ptr(q.device))
         _observe("attn_fwd", "end", flops)
     return out, lse
 
@@ -543,12 +551,13 @@ def packed_attention_bwd(q, k, v, out, dout, lse, packed, dq, dk, dv, scale=None
             raise ValueError(f"{name} shape mismatch")
         getattr(desc, f"{name}_strides")[:] = _thd_strides(name, t, written=True)
     delta = torch.empty(n, rows, dtype=torch.float32, device=q.device)
+    ws = _packed_workspace(desc, 1, q.device)
     flops = 2.5 * _packed_flops(packed, n, d) if _observer is not None else 0.0
     with _device_guard(q):
         _observe("attn_bwd", "begin", flops)
         nat.call("eth_packed_attn_bwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(out),
                  nat.ptr(dout), nat.ptr(lse), nat.ptr(delta), nat.ptr(dq), nat.ptr(dk), nat.ptr(dv),
-                 nat.stream_ptr(q.device))
+                 nat.ptr(ws), nat.stream_ptr(q.device))
         _observe("attn_bwd", "end", flops)
 
 

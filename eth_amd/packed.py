@@ -15,17 +15,21 @@ from . import _native as nat
 
 KEY_TILE_ROWS = 128  # keys per workgroup of the dK/dV kernels
 QUERY_TILE_ROWS = (32, 64, 128)  # queries per workgroup, by the heads that share one
+BLOCK_ROWS = 64  # keys (queries) of a step of a query (key) tile
+MIN_PIECE = 8  # steps of a split tile's piece
+WORTH_SPLITTING = 12  # steps that a split has to save
 
 
 def _tile_list(lengths, total, rows, queries):
-    """eth_packed_tile entries of `rows` rows: a query tile's chain grows with
-    its end in the sequence, a key tile's with what is left behind its start."""
+    """(eth_packed_tile entries of `rows` rows, the 64-row blocks of each
+    one's chain): a query tile's chain grows with its end in the sequence, a
+    key tile's with what is left behind its start."""
     lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
     begins = np.cumsum(lengths) - lengths
     counts = -(-lengths // rows)
     seq = np.repeat(np.arange(lengths.size), counts)
     start = (np.arange(seq.size) - np.repeat(np.cumsum(counts) - counts, counts)) * rows
-    chain = np.minimum(start + rows, lengths[seq]) if queries else lengths[seq] - start
+    chain = -(-(np.minimum(start + rows, lengths[seq]) if queries else lengths[seq] - start) // BLOCK_ROWS)
     order = np.argsort(-chain, kind="stable")
     covered = int(lengths.sum())
     spare = np.arange(covered, total, rows)  # rows behind the last sequence
@@ -33,7 +37,24 @@ def _tile_list(lengths, total, rows, queries):
     tiles["begin"] = np.concatenate([begins[seq][order], spare])
     tiles["len"] = np.concatenate([lengths[seq][order], -np.minimum(rows, total - spare)])
     tiles["start"][: seq.size] = start[order]
-    return tiles
+    return tiles, chain[order]
+
+
+def split_chains(chain, heads, slots):
+    """(tiles, pieces, steps) of a list whose `chain` steps (longest first) are
+    run for `heads` heads each on `slots` workgroups at a time: (0, 0, 0) where
+    no tile is worth splitting.
+
+    The list ends no earlier than its longest chain, nor than its steps spread
+    over the slots.  Where the first is well above the second, chains are cut
+    into pieces of about the second."""
+    if not chain.size:
+        return 0, 0, 0
+    steps = max(MIN_PIECE, -(-int(chain.sum()) * heads // slots))
+    longest = int(chain[0])
+    if longest < steps + WORTH_SPLITTING:
+        return 0, 0, 0
+    return int(np.searchsorted(-chain, -steps, side="left")), -(-longest // steps), steps
 
 
 class PackedSequences:
@@ -65,16 +86,26 @@ class PackedSequences:
             self.device = torch.device("cuda", torch.cuda.current_device())
         lists = {rows: _tile_list(self.lengths, self.total, rows, True) for rows in QUERY_TILE_ROWS}
         lists["keys"] = _tile_list(self.lengths, self.total, KEY_TILE_ROWS, False)
-        self._table = nat.table_to_device(np.concatenate(list(lists.values())), self.device)
+        self._table = nat.table_to_device(np.concatenate([tiles for tiles, _ in lists.values()]), self.device)
         self._home = nat.stream_ptr(self.device)
+        self._chains = {key: chain for key, (_, chain) in lists.items()}
         self._at, at = {}, self._table.data_ptr()
-        for key, tiles in lists.items():
+        for key, (tiles, _) in lists.items():
             self._at[key] = (at, tiles.size)
             at += tiles.nbytes
+        self._plans = {}
 
-    def tiles(self, query_rows):
-        """(address, count) of the query list of `query_rows` rows a tile and
-        of the key list, for a launch on the current stream."""
+    def plan(self, heads, kv_heads, head_dim):
+        """(query list address and count, key list address and count, query
+        split, key split) for these heads, for a launch on the current stream."""
         if nat.stream_ptr(self.device) != self._home and not torch.cuda.is_current_stream_capturing():
             self._table.record_stream(torch.cuda.current_stream(self.device))
-        return (*self._at[query_rows], *self._at["keys"])
+        plan = self._plans.get((heads, kv_heads, head_dim))
+        if plan is None:
+            rows = nat.value("eth_packed_attn_tile_rows", heads, kv_heads)
+            cus = torch.cuda.get_device_properties(self.device).multi_processor_count
+            # two query workgroups a compute unit; of dK/dV two up to a head dim of 96, one above
+            q_split = split_chains(self._chains[rows], heads * rows // 128, 2 * cus)
+            k_split = split_chains(self._chains["keys"] * (heads // kv_heads), kv_heads, (1 if head_dim > 96 else 2) * cus)
+            plan = self._plans[heads, kv_heads, head_dim] = (*self._at[rows], *self._at["keys"], q_split, k_split)
+        return plan

@@ -414,12 +414,22 @@ int eth_attn_bwd(const eth_attn_desc_t* desc, const void* q, const void* k, cons
  * Non-finite values of a row of k or v may reach every row of its own
  * sequence's 64-row block and those behind it, never another sequence.
  *
+ * The first q_split.tiles tiles of the query list (k_split, of the key list)
+ * are split: each takes up to `pieces` workgroups of about `steps` steps (64
+ * keys in the query lists; 64 queries of one head in the key list), whose fp32
+ * accumulators a second launch joins in order.  tiles 0: none is.  They need
+ * eth_packed_attn_workspace bytes, 16-byte aligned (NULL where it is 0).
+ *
  * The backward reads out and lse of the forward, fills delta [heads, rows] on
  * the way, and sums dk and dv over the query heads that share them, in a fixed
  * order (deterministic). */
 typedef struct eth_packed_tile {
   int32_t begin, len, start, reserved;
 } eth_packed_tile_t;
+
+typedef struct eth_packed_split {
+  int32_t tiles, pieces, steps;
+} eth_packed_split_t;
 
 typedef struct eth_packed_attn_desc {
   int64_t rows;
@@ -428,6 +438,7 @@ typedef struct eth_packed_attn_desc {
   const eth_packed_tile_t* q_tiles;
   const eth_packed_tile_t* k_tiles;
   int32_t n_q_tiles, n_k_tiles;
+  eth_packed_split_t q_split, k_split;
   int32_t heads, kv_heads, head_dim, dtype;
   float scale;
   int32_t reserved; /* 0 */
@@ -435,11 +446,13 @@ typedef struct eth_packed_attn_desc {
 
 /* Query rows of a tile for these head counts (0 if they do not fit). */
 int eth_packed_attn_tile_rows(int heads, int kv_heads);
+int64_t eth_packed_attn_workspace(const eth_packed_attn_desc_t* desc, int backward);
 int eth_packed_attn_fwd(const eth_packed_attn_desc_t* desc, const void* q, const void* k,
-                        const void* v, void* out, float* lse, void* stream);
+                        const void* v, void* out, float* lse, void* workspace, void* stream);
 int eth_packed_attn_bwd(const eth_packed_attn_desc_t* desc, const void* q, const void* k,
                         const void* v, const void* out, const void* dout, const float* lse,
-                        float* delta, void* dq, void* dk, void* dv, void* stream);
+                        float* delta, void* dq, void* dk, void* dv, void* workspace,
+                        void* stream);
 
 /* ------------------------------------------------------------------------
  * Vocabulary side of the first / last stage.

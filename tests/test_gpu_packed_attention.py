@@ -73,7 +73,19 @@ CASES = [
     ([97] * 7, 0, 12, 12, 16),
     ([1025], 7, 4, 1, 128),
     ([1100, 40], 0, 2, 2, 72),
+    # chains split over several workgroups, in every kernel
+    ([1700, 33], 9, 2, 1, 64),
+    ([5, 1650], 0, 2, 1, 80),
+    ([1500], 0, 3, 1, 128),
+    ([1345, 1281, 0, 600], 0, 4, 4, 128),
 ]
+
+
+def test_cases_split_chains(cuda):
+    """The cases meant to split do, and others do not."""
+    splits = [PackedSequences(lengths, total=sum(lengths) + tail, device=cuda).plan(n, m, hn)[4:]
+              for lengths, tail, n, m, hn in CASES]
+    assert all(q[0] and k[0] for q, k in splits[-4:]) and not any(q[0] or k[0] for q, k in splits[:5])
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

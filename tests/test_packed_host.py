@@ -19,7 +19,7 @@ def test_tile_lists_cover_every_row_once(rows, queries):
     for _ in range(60):
         lengths = [rng.choice((0, 1, rng.randrange(1, 700))) for _ in range(rng.randrange(0, 9))]
         total = max(1, sum(lengths) + rng.choice((0, 0, 1, 40, 300)))
-        tiles = pk._tile_list(lengths, total, rows, queries)
+        tiles, blocks = pk._tile_list(lengths, total, rows, queries)
         seen = np.zeros(total, dtype=int)
         begins = np.cumsum([0, *lengths])
         chains = []
@@ -32,9 +32,30 @@ def test_tile_lists_cover_every_row_once(rows, queries):
             i = [j for j, x in enumerate(lengths) if x and begins[j] == begin]
             assert len(i) == 1 and lengths[i[0]] == length and start % rows == 0 and start < length
             seen[begin + start : begin + min(start + rows, length)] += 1
-            chains.append(min(start + rows, length) if queries else length - start)
+            chains.append(-(-(min(start + rows, length) if queries else length - start) // 64))
         assert (seen == 1).all()
-        assert chains == sorted(chains, reverse=True)
+        assert chains == sorted(chains, reverse=True) == blocks.tolist()
+
+
+def test_split_chains():
+    """Split tiles are the longest, every chain fits its pieces, and no list
+    whose steps fill the slots evenly is split."""
+    assert pk.split_chains(np.array([], dtype=np.int64), 4, 512) == (0, 0, 0)
+    assert pk.split_chains(np.full(512, 40), 1, 512) == (0, 0, 0)
+    assert pk.split_chains(np.array([19]), 1, 512) == (0, 0, 0)
+    assert pk.split_chains(np.array([20, 8, 3]), 1, 512) == (1, 3, 8)
+    rng = random.Random(3)
+    for _ in range(300):
+        chain = np.array(sorted((rng.randrange(1, 300) for _ in range(rng.randrange(1, 80))), reverse=True))
+        heads, slots = rng.choice((1, 2, 8, 32)), rng.choice((256, 512))
+        tiles, pieces, steps = pk.split_chains(chain, heads, slots)
+        if tiles:
+            assert (chain[:tiles] > steps).all() and (chain[tiles:] <= steps).all()
+            assert pieces > 1 and pieces * steps >= chain[0] and chain[0] >= steps + pk.WORTH_SPLITTING
+            assert steps * slots >= chain.sum() * heads or steps == pk.MIN_PIECE
+            assert tiles * heads * steps <= max(chain.sum() * heads, 0)
+        else:
+            assert chain[0] < max(pk.MIN_PIECE, -(-chain.sum() * heads // slots)) + pk.WORTH_SPLITTING
 
 
 @pytest.mark.parametrize("lengths,total", [
@@ -66,7 +87,7 @@ def _desc(**changes):
     d.q_tiles = d.k_tiles = 4096
     d.n_q_tiles = d.n_k_tiles = 1
     for name, value in changes.items():
-        if name.endswith("strides"):
+        if name.endswith(("strides", "split")):
             getattr(d, name)[:] = value
         else:
             setattr(d, name, value)
@@ -77,7 +98,8 @@ def _desc(**changes):
     (dict(dtype=nat.ETH_F32), "bf16/fp16"), (dict(head_dim=60), "head_dim"), (dict(head_dim=136), "head_dim"),
     (dict(heads=3), "multiple of kv_heads"), (dict(kv_heads=0), "multiple of kv_heads"), (dict(rows=0), "rows"),
     (dict(rows=2**31), "rows"), (dict(n_q_tiles=0), "tiles"), (dict(k_tiles=None), "tiles"),
-    (dict(n_q_tiles=2**30), "too many"), (dict(q_strides=(252, 64)), "aligned"), (dict(v_strides=(-256, 64)), "strides"),
+    (dict(n_q_tiles=2**30), "too many"), (dict(q_split=(2, 2, 8)), "split"), (dict(k_split=(1, 1, 8)), "split"),
+    (dict(q_split=(1, 2, 0)), "split"), (dict(k_split=(-1, 2, 8)), "split"), (dict(k_split=(1, 2**24, 8)), "split"), (dict(q_strides=(252, 64)), "aligned"), (dict(v_strides=(-256, 64)), "strides"),
     (dict(k_strides=(2**24, 64)), "strides"), (dict(o_strides=(256, 4)), "aligned"), (dict(scale=0.0), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
 ])
@@ -87,9 +109,10 @@ def test_c_entry_refuses_before_any_launch(changes, match):
     d = _desc(**changes)
     p = 1 << 20
     with pytest.raises(ValueError, match=match):
-        nat.call("eth_packed_attn_fwd", ctypes.byref(d), p, p, p, p, p, None)
+        nat.call("eth_packed_attn_fwd", ctypes.byref(d), p, p, p, p, p, None, None)
+    assert nat.value("eth_packed_attn_workspace", ctypes.byref(d), 0) == 0
     with pytest.raises(ValueError, match=match):
-        nat.call("eth_packed_attn_bwd", ctypes.byref(d), p, p, p, p, p, p, p, p, p, p, None)
+        nat.call("eth_packed_attn_bwd", ctypes.byref(d), p, p, p, p, p, p, p, p, p, p, p, None)
 
 
 def test_c_entry_refuses_null_and_misaligned_pointers():
@@ -101,9 +124,21 @@ def test_c_entry_refuses_null_and_misaligned_pointers():
             args = [p] * 5
             args[i] = bad
             with pytest.raises(ValueError):
-                nat.call("eth_packed_attn_fwd", ctypes.byref(d), *args, None)
+                nat.call("eth_packed_attn_fwd", ctypes.byref(d), *args, None, None)
     with pytest.raises(ValueError, match="null"):
-        nat.call("eth_packed_attn_fwd", None, p, p, p, p, p, None)
+        nat.call("eth_packed_attn_fwd", None, p, p, p, p, p, None, None)
+    d = _desc(q_split=(1, 3, 8), n_q_tiles=2)
+    for ws in (None, p + 8):
+        with pytest.raises(ValueError, match="workspace"):
+            nat.call("eth_packed_attn_fwd", ctypes.byref(d), p, p, p, p, p, ws, None)
+        with pytest.raises(ValueError, match="workspace"):
+            nat.call("eth_packed_attn_bwd", ctypes.byref(d), p, p, p, p, p, p, p, p, p, p, ws, None)
+    # 2 groups of heads x 3 pieces of 4 waves' 32 x 64 accumulators, 64 lanes' statistics
+    assert nat.value("eth_packed_attn_workspace", ctypes.byref(d), 0) == 2 * 3 * 4 * (32 * 64 * 4 + 64 * 8)
+    assert nat.value("eth_packed_attn_workspace", ctypes.byref(d), 1) == 2 * 3 * 4 * 32 * 64 * 4
+    d = _desc(k_split=(1, 3, 8), head_dim=128)
+    assert nat.value("eth_packed_attn_workspace", ctypes.byref(d), 0) == 0
+    assert nat.value("eth_packed_attn_workspace", ctypes.byref(d), 1) == 2 * 3 * 8 * 32 * 128 * 4
 
 
 def test_oracle_gradients_equal_differences():
