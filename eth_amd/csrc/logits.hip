@@ -16,9 +16,26 @@
 // forward, read and written once backward: HBM bounds them.  Rows may start at
 // any multiple of an element (odd vocabularies): vectors are loaded and stored
 // with the alignment of an element, which the hardware takes.
+#include <utility>
+
 #include "common.h"
 
 namespace eth {
+
+// f(0) .. f(N - 1), each call's index a constant
+template <class F, int... I>
+__device__ __forceinline__ void each_place(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each_place(F f) {
+  each_place(std::make_integer_sequence<int, N>{}, f);
+}
+
+// Array length for N vectors of which every access has a constant index: the
+// compiler makes one wide register, copied whole at every access, of an array of
+// up to 32 words before it sees that, and takes a longer one apart.
+constexpr int places_of(int n) { return n < 9 ? 9 : n; }
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.4028234663852886e38f;
@@ -74,34 +91,37 @@ struct Lg<ETH_F32> {
   static constexpr uint32_t kMinusInf = 0xff800000u;
 };
 
-// vectors first, first + STEP, ... of the n elements at z, -inf past them.
-// The partial vector that n % E elements end a row with is one thread's: its
-// elements are loaded one by one, once, and not in every place of the list.
+// Vectors base + threadIdx.x + i * STEP (i < NV) of the n elements at z, -inf
+// past them; returns how many of the NV places hold anything for any thread of
+// the workgroup, the same for all: what the passes over them visit.  Lanes past
+// the row load its last whole vector instead, and only the last place is mended:
+// with a choice at every place the compiler unpacks there and spills.  The
+// partial vector that n % E elements end a row with is loaded one by one.
 template <int DT, int NV, int STEP>
-__device__ __forceinline__ void load_vecs(lg_u32x4 (&v)[NV], const typename Lg<DT>::T* z, int64_t first, int64_t n) {
+__device__ __forceinline__ int load_vecs(lg_u32x4 (&v)[places_of(NV)], const typename Lg<DT>::T* z, int base, int n) {
   constexpr int E = Lg<DT>::E;
-  const int64_t whole = n / E;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int64_t at = first + i * STEP;
-    if (at < whole)
-      v[i] = *reinterpret_cast<const typename Lg<DT>::V*>(z + at * E);
-    else
-      v[i] = lg_u32x4{Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf};
-  }
-  const int64_t rest = n - whole * E, slot = whole - first;
-  if (rest && slot >= 0 && slot % STEP == 0 && slot < NV * STEP) {
-    lg_u32x4 t = lg_u32x4{Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf};
+  const int whole = n / E, rest = n - whole * E, first = base + threadIdx.x;
+  const int places = min((whole + (rest > 0) - base + STEP - 1) / STEP, NV);
+  const int last = max(whole - 1, 0);
+  each_place<NV>([&](auto i) __attribute__((always_inline)) {
+    if (i < places && whole > 0)
+      v[i] = *reinterpret_cast<const typename Lg<DT>::V*>(z + (int64_t)min(first + i * STEP, last) * E);
+  });
+  const int end = first + (places - 1) * STEP;  // the last place's vector
+  lg_u32x4 t = {Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf, Lg<DT>::kMinusInf};
+  if (end == whole && rest) {
     float x[E];
     Lg<DT>::unpack(t, x);
 #pragma unroll
     for (int j = 0; j < E - 1; ++j)
       if (j < rest) x[j] = Lg<DT>::one(z[whole * E + j]);
     t = Lg<DT>::pack(x);  // (values of the type: exact)
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (slot == i * STEP) v[i] = t;
   }
+  asm volatile("" : "+v"(t));  // (whole words: not the elements it was made of)
+  each_place<NV>([&](auto i) __attribute__((always_inline)) {
+    if (i == places - 1 && end >= whole) v[i] = t;
+  });
+  return places;
 }
 // A vector's elements for one pass, the vector not known to be what it was:
 // otherwise what was unpacked for one pass is kept for the next, and with it
@@ -114,10 +134,10 @@ __device__ __forceinline__ void unpack_again(lg_u32x4& v, float (&x)[Lg<DT>::E])
 }
 // vector i of the n elements at d
 template <int DT>
-__device__ __forceinline__ void store_vec(typename Lg<DT>::T* d, int64_t i, int64_t n, const float (&x)[Lg<DT>::E]) {
+__device__ __forceinline__ void store_vec(typename Lg<DT>::T* d, int i, int n, const float (&x)[Lg<DT>::E]) {
   constexpr int E = Lg<DT>::E;
   if ((i + 1) * E <= n) {
-    *reinterpret_cast<typename Lg<DT>::V*>(d + i * E) = Lg<DT>::pack(x);
+    *reinterpret_cast<typename Lg<DT>::V*>(d + (int64_t)i * E) = Lg<DT>::pack(x);
   } else {
 #pragma unroll
     for (int j = 0; j < E; ++j)
@@ -185,14 +205,15 @@ __device__ __forceinline__ float of_order(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 // value first, then the lower index: all keys of a row differ
-__device__ __forceinline__ uint64_t key_of(float v, int64_t index) {
-  return (uint64_t)order_of(v) << 32 | (uint32_t)~(uint32_t)index;
+__device__ __forceinline__ uint64_t key_of(float v, int index) {
+  return (uint64_t)order_of(v) << 32 | ~(uint32_t)index;
 }
 __device__ __forceinline__ int64_t index_of(uint64_t key) { return (int64_t)(uint32_t)~(uint32_t)key; }
 
 struct LogpArgs {
   const void* z;
-  int64_t ld, V;
+  int64_t ld;
+  int V;
   const int64_t* tokens;
   int64_t ignore;
   float* logprob;
@@ -203,7 +224,7 @@ struct LogpArgs {
   int k;
   int* bad;
   int parts;          // workgroups per row
-  int64_t part;       // elements of a part (a multiple of a vector's)
+  int part;           // elements of a part (a multiple of a vector's)
   float4* part_stat;  // [rows, parts]
   uint64_t* part_key; // [rows, parts, k]
 };
@@ -248,14 +269,14 @@ __device__ __forceinline__ void logp_top(const LogpArgs& a, int64_t row, const R
 // unsorted, by every thread of a workgroup: the largest key that k keys reach,
 // two bits a pass over the part.
 template <int DT>
-__device__ __noinline__ int logp_exact(const typename Lg<DT>::T* z, int64_t first, int64_t n, int k, uint64_t* cand,
+__device__ __noinline__ int logp_exact(const typename Lg<DT>::T* z, int first, int n, int k, uint64_t* cand,
                                        int* count) {
   constexpr int W = kLogpThreads / 64;
   __shared__ int reach_s[3][W];
   uint64_t f = 0;
   for (int bit = 62; bit >= 0; bit -= 2) {
     int reach[3] = {0, 0, 0};
-    for (int64_t i = threadIdx.x; i < n; i += kLogpThreads) {
+    for (int i = threadIdx.x; i < n; i += kLogpThreads) {
       const uint64_t key = key_of(Lg<DT>::one(z[i]), first + i);
 #pragma unroll
       for (int c = 0; c < 3; ++c) reach[c] += key >= (f | (uint64_t)(c + 1) << bit);
@@ -277,7 +298,7 @@ __device__ __noinline__ int logp_exact(const typename Lg<DT>::T* z, int64_t firs
   }
   if (threadIdx.x == 0) *count = 0;
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < n; i += kLogpThreads) {
+  for (int i = threadIdx.x; i < n; i += kLogpThreads) {
     const uint64_t key = key_of(Lg<DT>::one(z[i]), first + i);
     if (key >= f) cand[atomicAdd(count, 1)] = key;  // (exactly k: all keys differ)
   }
@@ -306,36 +327,37 @@ __global__ void __launch_bounds__(kLogpThreads, 4) logp_fwd_kernel(LogpArgs a) {
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
   if (a.parts == 1 ? logp_ignored(a, row) : a.tokens[row] == a.ignore) return;
-  const int64_t first = part * a.part;
-  const int64_t n = a.V - first < a.part ? a.V - first : a.part;
+  const int first = part * a.part, n = min(a.V - first, a.part);
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld + first;
 
-  lg_u32x4 v[NV];
-  load_vecs<DT, NV, NT>(v, z, threadIdx.x, n);
+  lg_u32x4 v[places_of(NV)];
+  const int places = load_vecs<DT, NV, NT>(v, z, 0, n);
   RowStat r{kLowest, 0.f, 0.f};
+  each_place<NV>([&](auto i) __attribute__((always_inline)) {
+    if (i < places) {
+      float x[E];
+      unpack_again<DT>(v[i], x);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float x[E];
-    unpack_again<DT>(v[i], x);
-#pragma unroll
-    for (int j = 0; j < E; ++j) r.m = fmaxf(r.m, x[j]);
-  }
+      for (int j = 0; j < E; ++j) r.m = fmaxf(r.m, x[j]);
+    }
+  });
   if constexpr (TOP) {  // (a thread of -inf alone counts as the lowest: a lower bound all the same)
     const float pm = fmaxf(r.m, __shfl_xor(r.m, 1, 64));
     if ((threadIdx.x & 1) == 0) maxima[threadIdx.x >> 1] = order_of(pm) >> 16;
     if (threadIdx.x == 0) count_s = 0;
   }
+  each_place<NV>([&](auto i) __attribute__((always_inline)) {
+    if (i < places) {
+      float x[E];
+      unpack_again<DT>(v[i], x);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float x[E];
-    unpack_again<DT>(v[i], x);
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float d = x[j] - r.m, e = exp_f(d);
-      r.s += e;
-      r.a = __builtin_fmaf(e, fmaxf(d, kFarBelow), r.a);
+      for (int j = 0; j < E; ++j) {
+        const float d = x[j] - r.m, e = exp_f(d);
+        r.s += e;
+        r.a = __builtin_fmaf(e, fmaxf(d, kFarBelow), r.a);
+      }
     }
-  }
+  });
   r = block_stat<NT>(r, red);
   if (threadIdx.x == 0) {
     if (a.parts == 1)
@@ -361,17 +383,18 @@ __global__ void __launch_bounds__(kLogpThreads, 4) logp_fwd_kernel(LogpArgs a) {
     const float floor_v = fo <= 0x00ffffffu ? -INFINITY : of_order(fo);
       // a bit for every vector with a candidate; the few of them are read again
     uint32_t hits = 0;
+    each_place<NV>([&](auto i) __attribute__((always_inline)) {
+      if (i < places) {
+        float x[E];
+        unpack_again<DT>(v[i], x);
+        bool any = false;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float x[E];
-      unpack_again<DT>(v[i], x);
-      bool any = false;
-#pragma unroll
-      for (int j = 0; j < E; ++j) any |= !(x[j] < floor_v);  // NaN too
-      hits |= any ? 1u << i : 0u;
-    }
+        for (int j = 0; j < E; ++j) any |= !(x[j] < floor_v);  // NaN too
+        hits |= any ? 1u << i : 0u;
+      }
+    });
     while (hits) {
-      const int64_t at = ((int64_t)(__ffs(hits) - 1) * NT + threadIdx.x) * E;
+      const int at = ((__ffs(hits) - 1) * NT + threadIdx.x) * E;
       hits &= hits - 1;
       for (int j = 0; j < E && at + j < n; ++j) {
         const float x = Lg<DT>::one(z[at + j]);
@@ -440,7 +463,7 @@ constexpr int kRowVecs = 4;  // vectors of a backward workgroup's thread
 // One workgroup per 1024 vectors of a row.  A row without upstream gradient
 // (and one without a finite logit) gets zeros and is not read.
 template <int DT>
-__global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, int64_t ld, int64_t V,
+__global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, int64_t ld, int V,
                                                                const int64_t* __restrict__ tokens, int64_t ignore,
                                                                const float2* __restrict__ stats,
                                                                const float* __restrict__ entropy,
@@ -450,22 +473,20 @@ __global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, i
   typedef typename Lg<DT>::T T;
   constexpr int E = Lg<DT>::E;
   const int64_t row = blockIdx.x / chunks;
-  const int64_t i0 = (int64_t)(blockIdx.x % chunks) * (kRowThreads * kRowVecs) + threadIdx.x;
+  const int v0 = blockIdx.x % chunks * (kRowThreads * kRowVecs);
   const T* z = reinterpret_cast<const T*>(zv) + row * ld;
   T* dz = reinterpret_cast<T*>(dzv) + row * ldd;
-  int64_t t = tokens[row];
+  const int64_t token = tokens[row];
   const float2 st = stats[row];
-  const bool out = t == ignore || st.y == -INFINITY;
-  t = t < 0 ? 0 : (t >= V ? V - 1 : t);
+  const bool out = token == ignore || st.y == -INFINITY;
+  const int t = token < 0 ? 0 : (token >= V ? V - 1 : (int)token);
   const float g = out || !dlogprob ? 0.f : dlogprob[row], h = out || !dentropy ? 0.f : dentropy[row];
   const bool none = g == 0.f && h == 0.f;
   const float H = entropy[row];
-  lg_u32x4 v[kRowVecs];
-  if (!none) load_vecs<DT, kRowVecs, kRowThreads>(v, z, i0, V);
-#pragma unroll
-  for (int u = 0; u < kRowVecs; ++u) {
-    const int64_t i = i0 + u * kRowThreads;
-    if (i * E >= V) break;
+  lg_u32x4 v[places_of(kRowVecs)];
+  if (!none) load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0, V);
+  each_place<kRowVecs>([&](auto u) __attribute__((always_inline)) {
+    const int i = v0 + u * kRowThreads + threadIdx.x;
     float x[E];
     if (none) {
 #pragma unroll
@@ -480,7 +501,7 @@ __global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, i
       }
     }
     store_vec<DT>(dz, i, V, x);
-  }
+  });
 }
 
 // ----------------------------------------------------------------- distillation --
@@ -490,7 +511,8 @@ constexpr int kDistillVecs = 8;
 
 struct DistillArgs {
   const void* z;
-  int64_t ld, V;
+  int64_t ld;
+  int V;
   const int64_t* ids;  // [rows, k]; negative: no entry
   const void* teacher; // [rows, k] logits
   int teacher_dtype, k;
@@ -560,27 +582,29 @@ __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArg
   }
   const float c = kLog2e / a.tau;
   float m = kLowest, s = 0.f;
-  const int64_t nv = (a.V + E - 1) / E;
-  for (int64_t i0 = threadIdx.x; i0 < nv; i0 += NT * kDistillVecs) {
-    lg_u32x4 v[kDistillVecs];
-    load_vecs<DT, kDistillVecs, NT>(v, z, i0, a.V);
+  const int nv = (a.V + E - 1) / E;
+  for (int v0 = 0; v0 < nv; v0 += NT * kDistillVecs) {
+    lg_u32x4 v[places_of(kDistillVecs)];
+    const int places = load_vecs<DT, kDistillVecs, NT>(v, z, v0, a.V);
     float mx = m;
+    each_place<kDistillVecs>([&](auto u) __attribute__((always_inline)) {
+      if (u < places) {
+        float x[E];
+        unpack_again<DT>(v[u], x);
 #pragma unroll
-    for (int u = 0; u < kDistillVecs; ++u) {
-      float x[E];
-      unpack_again<DT>(v[u], x);
-#pragma unroll
-      for (int j = 0; j < E; ++j) mx = fmaxf(mx, x[j]);
-    }
+        for (int j = 0; j < E; ++j) mx = fmaxf(mx, x[j]);
+      }
+    });
     s *= __builtin_amdgcn_exp2f((m - mx) * c);
     m = mx;
-  #pragma unroll
-    for (int u = 0; u < kDistillVecs; ++u) {
-      float x[E];
-      unpack_again<DT>(v[u], x);
+    each_place<kDistillVecs>([&](auto u) __attribute__((always_inline)) {
+      if (u < places) {
+        float x[E];
+        unpack_again<DT>(v[u], x);
 #pragma unroll
-      for (int j = 0; j < E; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * c);
-    }
+        for (int j = 0; j < E; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * c);
+      }
+    });
   }
   const float wm = wave_max(m);
   const float ws = wave_sum(s * __builtin_amdgcn_exp2f((m - wm) * c));
@@ -621,32 +645,30 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(DistillArgs a)
   __shared__ float q_s[kDistillTop];
   __shared__ int64_t id_s[kDistillTop];
   const int64_t row = blockIdx.x / a.chunks;
-  const int64_t v0 = (int64_t)(blockIdx.x % a.chunks) * (kRowThreads * kRowVecs);
+  const int v0 = blockIdx.x % a.chunks * (kRowThreads * kRowVecs);
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
   T* dz = reinterpret_cast<T*>(a.dz) + row * a.ldd;
   const float2 st = a.stats[row];
   const float gt = st.y == -INFINITY ? 0.f : a.dloss[row] * a.tau;
   if (gt == 0.f) {  // (also a row without teacher entries or finite logits)
     float x[E] = {};
-#pragma unroll
-    for (int u = 0; u < kRowVecs; ++u) store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x);
+    each_place<kRowVecs>([&](auto u) __attribute__((always_inline)) { store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x); });
     return;
   }
-  lg_u32x4 v[kRowVecs];
-  load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0 + threadIdx.x, a.V);
+  lg_u32x4 v[places_of(kRowVecs)];
+  load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0, a.V);
   teacher_softmax<kRowThreads>(a, row, q_s, id_s, red);
   const float inv = 1.f / a.tau;
   auto prob = [&](float x) __attribute__((always_inline)) { return exp_f((x - st.x) * inv - st.y); };
-#pragma unroll
-  for (int u = 0; u < kRowVecs; ++u) {
+  each_place<kRowVecs>([&](auto u) __attribute__((always_inline)) {
     float x[E];
     Lg<DT>::unpack(v[u], x);
 #pragma unroll
     for (int j = 0; j < E; ++j) x[j] = gt * prob(x[j]);
     store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x);
-  }
+  });
   __syncthreads();  // the stores below come after those of the same places above
-  const int64_t lo = v0 * E, hi = lo + kRowThreads * kRowVecs * E;
+  const int lo = v0 * E, hi = lo + kRowThreads * kRowVecs * E;
   if (threadIdx.x < a.k) {
     const int64_t id = id_s[threadIdx.x];
     if (id >= lo && id < hi) {
@@ -721,7 +743,7 @@ extern "C" int eth_token_logprobs_fwd(const void* logits, int64_t ld, const int6
                 "eth_token_logprobs_fwd: misaligned pointer");
   a.z = logits;
   a.ld = ld;
-  a.V = vocab;
+  a.V = (int)vocab;
   a.tokens = tokens;
   a.ignore = ignore_index;
   a.logprob = logprob;
@@ -732,7 +754,7 @@ extern "C" int eth_token_logprobs_fwd(const void* logits, int64_t ld, const int6
   a.k = top_k;
   a.bad = bad_index;
   const int64_t E = 16 / dtype_size(dtype), vecs = (vocab + E - 1) / E;
-  a.part = (vecs + a.parts - 1) / a.parts * E;
+  a.part = (int)((vecs + a.parts - 1) / a.parts * E);
   a.part_stat = (float4*)workspace;
   a.part_key = (uint64_t*)(a.part_stat + rows * a.parts);
   hipStream_t s = (hipStream_t)stream;
@@ -767,7 +789,7 @@ extern "C" int eth_token_logprobs_bwd(const void* logits, int64_t ld, const int6
   const int grid = (int)(rows * chunks);
   hipStream_t s = (hipStream_t)stream;
 #define ETH_LOGP_BWD(DT)                                                                                      \
-  logp_bwd_kernel<DT><<<grid, kRowThreads, 0, s>>>(logits, ld, vocab, tokens, ignore_index, (const float2*)stats, \
+  logp_bwd_kernel<DT><<<grid, kRowThreads, 0, s>>>(logits, ld, (int)vocab, tokens, ignore_index, (const float2*)stats, \
                                                    entropy, dlogprob, dentropy, dlogits, ldd, chunks)
   if (dtype == ETH_BF16)
     ETH_LOGP_BWD(ETH_BF16);
@@ -798,7 +820,7 @@ static DistillArgs distill_args(const void* logits, int64_t ld, const int64_t* i
   DistillArgs a{};
   a.z = logits;
   a.ld = ld;
-  a.V = vocab;
+  a.V = (int)vocab;
   a.ids = ids;
   a.teacher = teacher;
   a.teacher_dtype = teacher_dtype;

@@ -52,8 +52,9 @@ def test_split_chains():
         if tiles:
             assert (chain[:tiles] > steps).all() and (chain[tiles:] <= steps).all()
             assert pieces > 1 and pieces * steps >= chain[0] and chain[0] >= steps + pk.WORTH_SPLITTING
-            assert steps * slots >= chain.sum() * heads or steps == pk.MIN_PIECE
-            assert tiles * heads * steps <= max(chain.sum() * heads, 0)
+            share = -(-chain.sum() * heads // slots)
+            assert pk.MIN_PIECE <= steps <= max(share, pk.MIN_PIECE)
+            assert steps >= min(share, pk.GOOD_PIECE)
         else:
             assert chain[0] < max(pk.MIN_PIECE, -(-chain.sum() * heads // slots)) + pk.WORTH_SPLITTING
 
