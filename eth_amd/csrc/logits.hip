@@ -147,10 +147,21 @@ __device__ __forceinline__ void store_vec(typename Lg<DT>::T* d, int i, int n, c
 
 __device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
+// the largest over the wavefront, in every lane, by the moves of wave_sum
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+  v = dpp_max<0x128>(v);
+  v = dpp_max<0x124>(v);
+  v = dpp_max<0x4e>(v);
+  return dpp_max<0xb1>(v);
 }
 
 // max, sum of exponentials and sum of exponentials times their difference from
@@ -193,8 +204,10 @@ __device__ __forceinline__ RowStat block_stat(RowStat r, float* red) {
 // ---------------------------------------------------- token log probabilities --
 constexpr int kLogpThreads = 512;
 constexpr int kLogpTop = 128;   // most alternatives
-constexpr int kLogpCand = 1024; // candidates that the sort takes
-constexpr int kLogpVecs = 16;   // vectors of a row's part that a thread holds
+constexpr int kLogpCand = 1024; // candidates that the sort takes (a multiple of 16)
+constexpr int kLogpHits = 512;  // vectors with candidates
+constexpr int kLogpVecs = 8;    // vectors that a thread has in flight
+constexpr int kLogpTrips = 2;   // times that, at most, in a part of a row
 
 // floats as whole numbers of the same order: -0 as +0, NaN above everything
 __device__ __forceinline__ uint32_t order_of(float v) {
@@ -302,62 +315,79 @@ __device__ __noinline__ int logp_exact(const typename Lg<DT>::T* z, int first, i
     const uint64_t key = key_of(Lg<DT>::one(z[i]), first + i);
     if (key >= f) cand[atomicAdd(count, 1)] = key;  // (exactly k: all keys differ)
   }
+  if (threadIdx.x < 16) cand[k + threadIdx.x] = 0;
   __syncthreads();
   return *count;
 }
 
-// One workgroup per part of a row, the whole row up to 512 * 16 vectors, held
-// in registers: 16 loads in flight per thread, each logit read once.
+// One workgroup per part of a row, a whole row up to 512 * 16 vectors: eight
+// loads in flight per thread, each logit read once.
 //
-// Top alternatives: of the 256 maxima of pairs of threads the k-th largest
-// (to 16 bits, rounded down) is a lower bound of the row's k-th largest, and
-// only about k + k^2 / 512 logits reach it: these are collected in LDS and
-// sorted by counting.  Where more reach it than the sort takes (equal logits, a
-// row of few finite ones) the k-th key is found bit by bit.
-template <int DT, int NV, bool TOP>
-__global__ void __launch_bounds__(kLogpThreads, 4) logp_fwd_kernel(LogpArgs a) {
+// Top alternatives: every thread keeps the order (16 bits, rounded down) of
+// each of its vectors' maxima.  Of the 256 maxima of pairs of threads the k-th
+// largest is a lower bound of the row's k-th largest, and only about k + k^2 /
+// 512 logits reach it: the few vectors with one are listed in LDS, read again an
+// element per thread, and the candidates among them sorted by counting.  Where
+// more reach it than the sort takes (equal logits, a row of few finite ones) or
+// the row holds a NaN, the k-th key is found bit by bit.
+template <int DT, int TRIPS, bool TOP>
+__global__ void __launch_bounds__(kLogpThreads, 6) logp_fwd_kernel(LogpArgs a) {
   typedef typename Lg<DT>::T T;
-  constexpr int E = Lg<DT>::E, NT = kLogpThreads;
+  constexpr int E = Lg<DT>::E, NT = kLogpThreads, NV = kLogpVecs;
   __shared__ float red[3 * NT / 64];
-  __shared__ uint64_t cand[TOP ? kLogpCand : 1];
+  __shared__ __attribute__((aligned(16))) uint64_t cand[TOP ? kLogpCand : 2];
   __shared__ __attribute__((aligned(16))) uint32_t maxima[TOP ? NT / 2 : 4];
+  __shared__ int hit[TOP ? kLogpHits : 1];
   __shared__ uint32_t floor_s;
-  __shared__ int count_s;
+  __shared__ int count_s, hits_s;
 
   const int64_t row = blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
   if (a.parts == 1 ? logp_ignored(a, row) : a.tokens[row] == a.ignore) return;
   const int first = part * a.part, n = min(a.V - first, a.part);
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld + first;
+  if constexpr (TOP) {
+    for (int i = threadIdx.x; i < kLogpCand; i += NT) cand[i] = 0;
+    if (threadIdx.x == 0) count_s = hits_s = 0;
+  }
 
-  lg_u32x4 v[places_of(NV)];
-  const int places = load_vecs<DT, NV, NT>(v, z, 0, n);
   RowStat r{kLowest, 0.f, 0.f};
-  each_place<NV>([&](auto i) __attribute__((always_inline)) {
-    if (i < places) {
-      float x[E];
-      unpack_again<DT>(v[i], x);
+  uint32_t tops[TRIPS * NV];  // orders of the vectors' maxima
+  each_place<TRIPS * NV>([&](auto i) __attribute__((always_inline)) { tops[i] = 0; });
+  each_place<TRIPS>([&](auto trip) __attribute__((always_inline)) {
+    if (trip * NV * NT * E >= n) return;
+    lg_u32x4 v[places_of(NV)];
+    const int places = load_vecs<DT, NV, NT>(v, z, trip * NV * NT, n);
+    float m = r.m;
+    each_place<NV>([&](auto i) __attribute__((always_inline)) {
+      if (i < places) {
+        float x[E];
+        unpack_again<DT>(v[i], x);
+        float mx = x[0];
 #pragma unroll
-      for (int j = 0; j < E; ++j) r.m = fmaxf(r.m, x[j]);
-    }
+        for (int j = 1; j < E; ++j) mx = fmaxf(mx, x[j]);
+        if constexpr (TOP) tops[trip * NV + i] = order_of(mx) >> 16;
+        m = fmaxf(m, mx);
+      }
+    });
+    r = trip == 0 ? RowStat{m, 0.f, 0.f} : at_max(r, m);
+    each_place<NV>([&](auto i) __attribute__((always_inline)) {
+      if (i < places) {
+        float x[E];
+        unpack_again<DT>(v[i], x);
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float d = x[j] - r.m, e = exp_f(d);
+          r.s += e;
+          r.a = __builtin_fmaf(e, fmaxf(d, kFarBelow), r.a);
+        }
+      }
+    });
   });
   if constexpr (TOP) {  // (a thread of -inf alone counts as the lowest: a lower bound all the same)
     const float pm = fmaxf(r.m, __shfl_xor(r.m, 1, 64));
     if ((threadIdx.x & 1) == 0) maxima[threadIdx.x >> 1] = order_of(pm) >> 16;
-    if (threadIdx.x == 0) count_s = 0;
   }
-  each_place<NV>([&](auto i) __attribute__((always_inline)) {
-    if (i < places) {
-      float x[E];
-      unpack_again<DT>(v[i], x);
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float d = x[j] - r.m, e = exp_f(d);
-        r.s += e;
-        r.a = __builtin_fmaf(e, fmaxf(d, kFarBelow), r.a);
-      }
-    }
-  });
   r = block_stat<NT>(r, red);
   if (threadIdx.x == 0) {
     if (a.parts == 1)
@@ -375,42 +405,46 @@ __global__ void __launch_bounds__(kLogpThreads, 4) logp_fwd_kernel(LogpArgs a) {
                           __popcll(__ballot(k4.z >= c)) + __popcll(__ballot(k4.w >= c));
         if (above >= a.k) f = c;
       }
-      if (threadIdx.x == 0) floor_s = f;
+      // up to the order of the lowest finite value: everything, -inf too
+      if (threadIdx.x == 0) floor_s = f <= (order_of(kLowest) >> 16) ? 0 : f;
     }
     __syncthreads();
-    // orders up to that of the lowest finite value: everything, -inf too
-    const uint32_t fo = floor_s << 16;
-    const float floor_v = fo <= 0x00ffffffu ? -INFINITY : of_order(fo);
-      // a bit for every vector with a candidate; the few of them are read again
+    const uint32_t floor_o = floor_s;
     uint32_t hits = 0;
-    each_place<NV>([&](auto i) __attribute__((always_inline)) {
-      if (i < places) {
-        float x[E];
-        unpack_again<DT>(v[i], x);
-        bool any = false;
-#pragma unroll
-        for (int j = 0; j < E; ++j) any |= !(x[j] < floor_v);  // NaN too
-        hits |= any ? 1u << i : 0u;
-      }
+    each_place<TRIPS * NV>([&](auto i) __attribute__((always_inline)) {
+      hits |= tops[i] >= floor_o && (i * NT + (int)threadIdx.x) * E < n ? 1u << i : 0u;
     });
     while (hits) {
-      const int at = ((__ffs(hits) - 1) * NT + threadIdx.x) * E;
+      const int slot = atomicAdd(&hits_s, 1);
+      if (slot < kLogpHits) hit[slot] = (__ffs(hits) - 1) * NT + threadIdx.x;
       hits &= hits - 1;
-      for (int j = 0; j < E && at + j < n; ++j) {
-        const float x = Lg<DT>::one(z[at + j]);
-        if (x < floor_v) continue;
-        const int slot = atomicAdd(&count_s, 1);
-        if (slot < kLogpCand) cand[slot] = key_of(x, first + at + j);
-      }
+    }
+    __syncthreads();
+    // one element per thread: all loads under way at once
+    const int elems = min(hits_s, kLogpHits) * E;
+    for (int e = threadIdx.x; e < elems; e += NT) {
+      const int at = hit[e / E] * E + e % E;
+      if (at >= n) continue;
+      const uint64_t key = key_of(Lg<DT>::one(z[at]), first + at);
+      if ((uint32_t)(key >> 48) < floor_o) continue;
+      const int slot = atomicAdd(&count_s, 1);
+      if (slot < kLogpCand) cand[slot] = key;
     }
     __syncthreads();
     int count = count_s;
-    if (count > kLogpCand) count = logp_exact<DT>(z, first, n, a.k, cand, &count_s);
+    if (hits_s > kLogpHits || count > kLogpCand || r.s != r.s)
+      count = logp_exact<DT>(z, first, n, a.k, cand, &count_s);
     const float ls = logf(r.s);
     for (int i = threadIdx.x; i < count; i += NT) {
       const uint64_t key = cand[i];
       int rank = 0;
-      for (int j = 0; j < count; ++j) rank += cand[j] > key;
+      for (int j = 0; j < count; j += 16) {  // (zeros behind the last)
+        ulonglong2 c[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) c[u] = *reinterpret_cast<const ulonglong2*>(&cand[j + 2 * u]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) rank += (c[u].x > key) + (c[u].y > key);
+      }
       if (rank >= a.k) continue;
       if (a.parts == 1)
         logp_top(a, row, r, ls, rank, key);
@@ -460,8 +494,18 @@ __global__ void __launch_bounds__(256) logp_join_kernel(LogpArgs a) {
 constexpr int kRowThreads = 256;
 constexpr int kRowVecs = 4;  // vectors of a backward workgroup's thread
 
-// One workgroup per 1024 vectors of a row.  A row without upstream gradient
-// (and one without a finite logit) gets zeros and is not read.
+// zeros in a backward workgroup's vectors
+template <int DT>
+__device__ __forceinline__ void zero_vecs(typename Lg<DT>::T* dz, int v0, int n) {
+  float x[Lg<DT>::E] = {};
+#pragma unroll
+  for (int u = 0; u < kRowVecs; ++u) store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, n, x);
+}
+
+// A workgroup per 1024 vectors of a row: many short ones keep HBM busier than
+// one that walks the row (145 against 170 us for [4096, 50304] bf16).  A row
+// without upstream gradient (and one without a finite logit) gets zeros and is
+// not read.
 template <int DT>
 __global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, int64_t ld, int V,
                                                                const int64_t* __restrict__ tokens, int64_t ignore,
@@ -481,24 +525,22 @@ __global__ void __launch_bounds__(kRowThreads) logp_bwd_kernel(const void* zv, i
   const bool out = token == ignore || st.y == -INFINITY;
   const int t = token < 0 ? 0 : (token >= V ? V - 1 : (int)token);
   const float g = out || !dlogprob ? 0.f : dlogprob[row], h = out || !dentropy ? 0.f : dentropy[row];
-  const bool none = g == 0.f && h == 0.f;
+  if (g == 0.f && h == 0.f) {
+    zero_vecs<DT>(dz, v0, V);
+    return;
+  }
   const float H = entropy[row];
   lg_u32x4 v[places_of(kRowVecs)];
-  if (!none) load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0, V);
+  load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0, V);
   each_place<kRowVecs>([&](auto u) __attribute__((always_inline)) {
     const int i = v0 + u * kRowThreads + threadIdx.x;
     float x[E];
-    if (none) {
+    Lg<DT>::unpack(v[u], x);
 #pragma unroll
-      for (int j = 0; j < E; ++j) x[j] = 0.f;
-    } else {
-      Lg<DT>::unpack(v[u], x);
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float lp = (x[j] - st.x) - st.y, p = exp_f(lp);
-        const float w = g + h * (fmaxf(lp, kFarBelow) + H);
-        x[j] = (i * E + j == t ? g : 0.f) - p * w;
-      }
+    for (int j = 0; j < E; ++j) {
+      const float lp = (x[j] - st.x) - st.y, p = exp_f(lp);
+      const float w = g + h * (fmaxf(lp, kFarBelow) + H);
+      x[j] = (i * E + j == t ? g : 0.f) - p * w;
     }
     store_vec<DT>(dz, i, V, x);
   });
@@ -518,67 +560,60 @@ struct DistillArgs {
   int teacher_dtype, k;
   float tau;
   float* loss;
-  float2* stats;  // max, log of the sum of exp((z - max) / tau)
+  // max, log of the sum of exp((z - max) / tau); the teacher's max, and the sum
+  // of exp((u - max) / tau) over its entries (0: there are none)
+  float4* stats;
   int* bad;
   const float* dloss;
   void* dz;
   int64_t ldd;
-  int chunks;
+  int chunks;  // backward: workgroups per row
 };
 
-// The teacher's distribution over its entries into q_s, absent ones (a
-// negative id, one past the vocabulary, a logit of -inf) with 0; ids into
-// id_s (-1 for absent).  Called by every thread; each row's k entries by the
-// first threads.  Returns whether any entry is there.
-template <int NT>
-__device__ __forceinline__ bool teacher_softmax(const DistillArgs& a, int64_t row, float* q_s, int64_t* id_s,
-                                                float* red) {
-  const int i = threadIdx.x;
-  float u = -INFINITY;
-  int64_t id = -1;
-  if (i < a.k) {
-    id = a.ids[row * a.k + i];
-    if (id >= a.V) {
-      *a.bad = 1;
-      id = -1;
-    }
-    if (id >= 0) u = load_elem(a.teacher, row * a.k + i, a.teacher_dtype);
-  }
-  const float m = wave_max(fmaxf(u, kLowest));
-  if ((i & 63) == 0) red[i >> 6] = m;
-  __syncthreads();
-  float M = red[0];
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) M = fmaxf(M, red[w]);
-  __syncthreads();
-  // (a teacher logit of NaN or +inf makes every q NaN, as the softmax does)
-  const float e = id >= 0 ? exp_f((u - M) / a.tau) : 0.f;
-  const float total = block_sum<NT>(e, red);
-  if (i < a.k) {
-    q_s[i] = total == 0.f ? 0.f : e / total;
-    id_s[i] = q_s[i] == 0.f ? -1 : id;
-  }
-  __syncthreads();
-  return total != 0.f;
+// entry i of a row's teacher: its id, -1 where there is none
+__device__ __forceinline__ int teacher_id(const DistillArgs& a, int64_t row, int i) {
+  if (i >= a.k) return -1;
+  const int64_t id = a.ids[row * a.k + i];
+  if (id >= a.V) *a.bad = 1;
+  return id >= 0 && id < a.V ? (int)id : -1;
+}
+__device__ __forceinline__ float teacher_logit(const DistillArgs& a, int64_t row, int i) {
+  return load_elem(a.teacher, row * a.k + i, a.teacher_dtype);
 }
 
-// One workgroup per row: the row's statistics at the temperature (each thread
-// over its own vectors, eight in flight, joined once) and the k entries.
+// One workgroup per row: the row's statistics at the temperature, each thread
+// over its own vectors, eight in flight.  Every wave looks the ids over (a row
+// without entries is not read); the first one weighs the entries, four a lane,
+// while the others read, and joins it all behind the one barrier.
 template <int DT>
 __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArgs a) {
   typedef typename Lg<DT>::T T;
-  constexpr int E = Lg<DT>::E, NT = kDistillThreads;
-  __shared__ float red[3 * NT / 64];
-  __shared__ float q_s[kDistillTop];
-  __shared__ int64_t id_s[kDistillTop];
+  constexpr int E = Lg<DT>::E, NT = kDistillThreads, PL = kDistillTop / 64;
+  __shared__ float red[2 * NT / 64];
   const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
-  if (!teacher_softmax<NT>(a, row, q_s, id_s, red)) {  // nothing to learn from: the row is not read
+  int id[PL];
+  bool any = false;
+#pragma unroll
+  for (int e = 0; e < PL; ++e) {
+    id[e] = teacher_id(a, row, lane + 64 * e);
+    any |= id[e] >= 0;
+  }
+  if (!__any(any)) {
     if (threadIdx.x == 0) {
       a.loss[row] = 0.f;
-      a.stats[row] = make_float2(0.f, -INFINITY);
+      a.stats[row] = make_float4(0.f, -INFINITY, 0.f, 0.f);
     }
     return;
+  }
+  float u[PL], zu[PL];  // the teacher's logits and the student's for them
+  if (threadIdx.x < 64) {
+#pragma unroll
+    for (int e = 0; e < PL; ++e) {
+      u[e] = id[e] >= 0 ? teacher_logit(a, row, lane + 64 * e) : -INFINITY;
+      zu[e] = id[e] >= 0 ? Lg<DT>::one(z[id[e]]) : 0.f;
+    }
   }
   const float c = kLog2e / a.tau;
   float m = kLowest, s = 0.f;
@@ -608,57 +643,68 @@ __global__ void __launch_bounds__(kDistillThreads) distill_fwd_kernel(DistillArg
   }
   const float wm = wave_max(m);
   const float ws = wave_sum(s * __builtin_amdgcn_exp2f((m - wm) * c));
-  if ((threadIdx.x & 63) == 0) {
+  if (lane == 0) {
     red[threadIdx.x >> 6] = wm;
     red[NT / 64 + (threadIdx.x >> 6)] = ws;
   }
   __syncthreads();
+  if (threadIdx.x >= 64) return;
   float M = red[0], S = 0.f;
 #pragma unroll
   for (int w = 1; w < NT / 64; ++w) M = fmaxf(M, red[w]);
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) S += red[NT / 64 + w] * __builtin_amdgcn_exp2f((red[w] - M) * c);
-  __syncthreads();
   const bool none = S == 0.f;  // no finite logit: no probability for any entry
   const float ls = none ? -INFINITY : logf(S);
-  float part = 0.f;
-  if (threadIdx.x < a.k && id_s[threadIdx.x] >= 0) {
-    const float q = q_s[threadIdx.x];
-    const float lp = none ? -INFINITY : (Lg<DT>::one(z[id_s[threadIdx.x]]) - M) / a.tau - ls;
-    part = q * (logf(q) - lp);
+  float um = kLowest, total = 0.f, loss = 0.f;
+#pragma unroll
+  for (int e = 0; e < PL; ++e) um = fmaxf(um, u[e]);
+  um = wave_max(um);
+  // (a teacher logit of NaN or +inf makes every q NaN, as the softmax does)
+#pragma unroll
+  for (int e = 0; e < PL; ++e) total += id[e] >= 0 ? exp_f((u[e] - um) / a.tau) : 0.f;
+  total = wave_sum(total);
+#pragma unroll
+  for (int e = 0; e < PL; ++e) {
+    const float q = id[e] >= 0 ? exp_f((u[e] - um) / a.tau) / total : 0.f;
+    const float lp = none ? -INFINITY : (zu[e] - M) / a.tau - ls;
+    if (!(q == 0.f)) loss += q * (logf(q) - lp);
   }
-  const float loss = block_sum<NT>(part, red);
-  if (threadIdx.x == 0) {
-    a.loss[row] = loss * a.tau * a.tau;
-    a.stats[row] = make_float2(M, ls);
+  loss = wave_sum(loss);
+  if (lane == 0) {
+    a.loss[row] = total == 0.f ? 0.f : loss * a.tau * a.tau;
+    a.stats[row] = make_float4(M, ls, um, total);
   }
 }
 
-// One workgroup per 1024 vectors of a row: dz = g tau p, then the entries
+// A workgroup per 1024 vectors of a row: dz = g tau p, then the entries
 // among them once more with their q (an id that appears more than once by its
 // first entry, with the sum).
 template <int DT>
 __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(DistillArgs a) {
   typedef typename Lg<DT>::T T;
   constexpr int E = Lg<DT>::E;
-  __shared__ float red[kRowThreads / 64];
   __shared__ float q_s[kDistillTop];
-  __shared__ int64_t id_s[kDistillTop];
+  __shared__ int id_s[kDistillTop];
   const int64_t row = blockIdx.x / a.chunks;
   const int v0 = blockIdx.x % a.chunks * (kRowThreads * kRowVecs);
   const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
   T* dz = reinterpret_cast<T*>(a.dz) + row * a.ldd;
-  const float2 st = a.stats[row];
-  const float gt = st.y == -INFINITY ? 0.f : a.dloss[row] * a.tau;
+  const float4 st = a.stats[row];
+  const float gt = st.y == -INFINITY || st.w == 0.f ? 0.f : a.dloss[row] * a.tau;
   if (gt == 0.f) {  // (also a row without teacher entries or finite logits)
-    float x[E] = {};
-    each_place<kRowVecs>([&](auto u) __attribute__((always_inline)) { store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x); });
+    zero_vecs<DT>(dz, v0, a.V);
     return;
   }
   lg_u32x4 v[places_of(kRowVecs)];
   load_vecs<DT, kRowVecs, kRowThreads>(v, z, v0, a.V);
-  teacher_softmax<kRowThreads>(a, row, q_s, id_s, red);
   const float inv = 1.f / a.tau;
+  if ((int)threadIdx.x < a.k) {
+    const int id = teacher_id(a, row, threadIdx.x);
+    const float q = id >= 0 ? exp_f((teacher_logit(a, row, threadIdx.x) - st.z) / a.tau) / st.w : 0.f;
+    q_s[threadIdx.x] = q;
+    id_s[threadIdx.x] = q == 0.f ? -1 : id;
+  }
   auto prob = [&](float x) __attribute__((always_inline)) { return exp_f((x - st.x) * inv - st.y); };
   each_place<kRowVecs>([&](auto u) __attribute__((always_inline)) {
     float x[E];
@@ -668,10 +714,9 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(DistillArgs a)
     store_vec<DT>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x);
   });
   __syncthreads();  // the stores below come after those of the same places above
-  const int lo = v0 * E, hi = lo + kRowThreads * kRowVecs * E;
-  if (threadIdx.x < a.k) {
-    const int64_t id = id_s[threadIdx.x];
-    if (id >= lo && id < hi) {
+  if ((int)threadIdx.x < a.k) {
+    const int id = id_s[threadIdx.x];
+    if (id >= v0 * E && id < (v0 + kRowThreads * kRowVecs) * E) {
       float q = 0.f;
       bool mine = true;
       for (int i = 0; i < a.k; ++i)
@@ -694,7 +739,7 @@ static bool logits_shape(int64_t rows, int64_t V, int64_t ld) {
   return rows > 0 && V > 0 && V <= kMostVocab && ld >= V;
 }
 static int64_t logp_parts(int64_t V, int dtype) {
-  const int64_t most = (int64_t)kLogpThreads * kLogpVecs * (16 / dtype_size(dtype));
+  const int64_t most = (int64_t)kLogpThreads * kLogpVecs * kLogpTrips * (16 / dtype_size(dtype));
   return (V + most - 1) / most;
 }
 
@@ -704,23 +749,18 @@ extern "C" int64_t eth_token_logprobs_workspace(int64_t rows, int64_t vocab, int
   return parts == 1 ? 0 : rows * parts * (int64_t)(sizeof(float4) + top_k * sizeof(uint64_t));
 }
 
-template <int DT, int NV>
-static void launch_logp(const LogpArgs& a, int grid, hipStream_t s) {
-  if (a.k > 0)
-    logp_fwd_kernel<DT, NV, true><<<grid, kLogpThreads, 0, s>>>(a);
-  else
-    logp_fwd_kernel<DT, NV, false><<<grid, kLogpThreads, 0, s>>>(a);
-}
 template <int DT>
-static void launch_logp_rows(const LogpArgs& a, int64_t rows, hipStream_t s) {
+static void launch_logp(const LogpArgs& a, int64_t rows, hipStream_t s) {
   const int grid = (int)(rows * a.parts);
-  const int64_t vecs = (a.part / Lg<DT>::E + kLogpThreads - 1) / kLogpThreads;
-  if (vecs <= 4)
-    launch_logp<DT, 4>(a, grid, s);
-  else if (vecs <= 8)
-    launch_logp<DT, 8>(a, grid, s);
+  const bool one = a.part <= kLogpThreads * kLogpVecs * Lg<DT>::E;
+  if (a.k > 0 && one)
+    logp_fwd_kernel<DT, 1, true><<<grid, kLogpThreads, 0, s>>>(a);
+  else if (a.k > 0)
+    logp_fwd_kernel<DT, kLogpTrips, true><<<grid, kLogpThreads, 0, s>>>(a);
+  else if (one)
+    logp_fwd_kernel<DT, 1, false><<<grid, kLogpThreads, 0, s>>>(a);
   else
-    launch_logp<DT, kLogpVecs>(a, grid, s);
+    logp_fwd_kernel<DT, kLogpTrips, false><<<grid, kLogpThreads, 0, s>>>(a);
   if (a.parts > 1) logp_join_kernel<DT><<<(int)rows, 256, 0, s>>>(a);
 }
 
@@ -759,11 +799,11 @@ extern "C" int eth_token_logprobs_fwd(const void* logits, int64_t ld, const int6
   a.part_key = (uint64_t*)(a.part_stat + rows * a.parts);
   hipStream_t s = (hipStream_t)stream;
   if (dtype == ETH_BF16)
-    launch_logp_rows<ETH_BF16>(a, rows, s);
+    launch_logp<ETH_BF16>(a, rows, s);
   else if (dtype == ETH_F16)
-    launch_logp_rows<ETH_F16>(a, rows, s);
+    launch_logp<ETH_F16>(a, rows, s);
   else
-    launch_logp_rows<ETH_F32>(a, rows, s);
+    launch_logp<ETH_F32>(a, rows, s);
   ETH_CHECK_LAUNCH("eth_token_logprobs_fwd");
   return ETH_OK;
 }
@@ -811,7 +851,7 @@ static int distill_check(const char* who, const void* logits, int64_t ld, const 
   ETH_CHECK_ARG(tau >= 0x1p-20f && tau <= 0x1p20f, "%s: temperature must be positive and finite", who);
   ETH_CHECK_ARG(logits && ids && teacher && stats && bad, "%s: null pointer", who);
   ETH_CHECK_ARG(((uintptr_t)logits % dtype_size(dtype)) == 0 && ((uintptr_t)teacher % dtype_size(teacher_dtype)) == 0 &&
-                    ((uintptr_t)stats & 7) == 0,
+                    ((uintptr_t)stats & 15) == 0,
                 "%s: misaligned pointer", who);
   return ETH_OK;
 }
@@ -826,7 +866,7 @@ static DistillArgs distill_args(const void* logits, int64_t ld, const int64_t* i
   a.teacher_dtype = teacher_dtype;
   a.k = k;
   a.tau = tau;
-  a.stats = (float2*)stats;
+  a.stats = (float4*)stats;
   a.bad = bad;
   return a;
 }

@@ -654,9 +654,9 @@ def _check_row_values(name, t, rows):
         raise ValueError(f"{name} must be contiguous fp32 [rows]")
 
 
-def _check_stats(stats, rows):
-    if stats.dtype != torch.float32 or stats.shape != (rows, 2) or not stats.is_contiguous():
-        raise ValueError("stats must be the forward's fp32 [rows, 2]")
+def _check_stats(stats, rows, n):
+    if stats.dtype != torch.float32 or stats.shape != (rows, n) or not stats.is_contiguous():
+        raise ValueError(f"stats must be the forward's fp32 [rows, {n}]")
 
 
 def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100):
@@ -690,7 +690,7 @@ def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad
     given = [t for t in (dlogprob, dentropy) if t is not None]
     code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens, stats, entropy, *given)
     _check_ids(tokens, (rows,))
-    _check_stats(stats, rows)
+    _check_stats(stats, rows, 2)
     for name, t in (("entropy", entropy), ("dlogprob", dlogprob), ("dentropy", dentropy)):
         if t is not None:
             _check_row_values(name, t, rows)
@@ -720,7 +720,7 @@ def _check_teacher(teacher_ids, teacher_logits, rows, temperature):
 
 
 def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag):
-    """(loss [rows], stats [rows, 2]): temperature^2 * sum q (log q - log p[id])
+    """(loss [rows], stats [rows, 4]): temperature^2 * sum q (log q - log p[id])
     with q the softmax of a row's k teacher logits (any of the three types) and
     p that of its V logits, both at the temperature.  Negative ids and teacher
     logits of -inf are no entries; ids past the vocabulary are none either and
@@ -728,7 +728,7 @@ def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_fla
     code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits)
     k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
     loss = torch.empty(rows, dtype=torch.float32, device=logits2d.device)
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=logits2d.device)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=logits2d.device)
     if rows:
         with _device_guard(logits2d):
             nat.call("eth_topk_distill_fwd", nat.ptr(logits2d), ld, nat.ptr(teacher_ids), nat.ptr(teacher_logits),
@@ -741,7 +741,7 @@ def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, 
     """dlogits [rows, V] of topk_distill_fwd's loss (dloss fp32 [rows])."""
     code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits, stats, dloss)
     k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
-    _check_stats(stats, rows)
+    _check_stats(stats, rows, 4)
     _check_row_values("dloss", dloss, rows)
     dz = torch.empty(rows, V, dtype=logits2d.dtype, device=logits2d.device)
     if rows:

@@ -538,8 +538,10 @@ int eth_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* tokens
  *   loss = temperature^2 sum q (log q - log p[id]).
  * A negative id is no entry, and so is a teacher logit of -inf; an id at or past
  * vocab is none and sets *bad_index to 1; an id may appear more than once.  A row
- * without entries has loss 0, is not read, and gets no gradient.  stats as above, of
- * logits / temperature.  The backward writes
+ * without entries has loss 0 and gets no gradient.  stats [rows, 4] (16-byte
+ * aligned), for the backward: the row's maximum and log sum exp((z - max) /
+ * temperature), the teacher's maximum and sum exp((u - max) / temperature).  The
+ * backward writes
  *   dlogits_j = dloss temperature (p_j - sum of q over the entries with id j). */
 int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_t* teacher_ids,
                          const void* teacher, int teacher_dtype, int k, float temperature,
