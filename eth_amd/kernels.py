@@ -5,10 +5,10 @@ match what the kernel and its launch grid assume, then enqueues the kernel on
 the current stream.  There is no CPU fallback: CPU tensors raise.
 """
 
-import contextlib
 import ctypes
 import functools
 import itertools
+import math
 
 import numpy as np
 
@@ -442,17 +442,20 @@ def attention_bwd(q, k, v, out, dout, lse, dq, dk, dv):
     _observe("attn_bwd", "end", flops)
 
 
-def _device_guard(t):
-    """Launches go to the tensors' device, whichever the current one is."""
-    if t.device.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(index, name, *args):
+    """nat.call(name, *args, the current stream) on device `index`, whichever
+    the current one is."""
+    if index == torch._C._cuda_getDevice():
+        nat.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            nat.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _check_device(device, *ts):
+def _check_device(index, *ts):
     for t in ts:
-        if t.device != device:
-            raise ValueError(f"tensors on {device} and {t.device}: one device is needed")
+        if t.get_device() != index:
+            raise ValueError(f"tensors on cuda:{index} and {t.device}: one GPU is needed (no CPU fallback)")
 
 
 def _thd_strides(name, t, written=False):
@@ -463,14 +466,25 @@ def _thd_strides(name, t, written=False):
         raise ValueError(f"{name} must be a [rows, heads, hn] view with hn contiguous")
     # (the stride of a dimension of size 1 means nothing and may be anything)
     sr, sh = sr if rows > 1 else heads * hn, sh if heads > 1 else hn
-    if sr % 8 or sh % 8 or t.data_ptr() % 16:
+    if sr % 8 or sh % 8:
         raise ValueError(f"{name}: rows must be 16-byte aligned")
     if written and (sh < hn or sr < hn):
         raise ValueError(f"{name}: rows that are written may not overlap")
     return sr, sh
 
 
-def _packed_desc(q, k, v, packed, scale, code):
+def _packed_desc(packed, scale, q, k, v, *grads):
+    """(descriptor, its reference, workspace bytes) of a packed attention call,
+    built and checked once for these types, shapes and strides and kept with
+    the plan (the addresses are the call's; the entry checks their alignment)."""
+    key = (scale, *[x for t in (q, k, v, *grads) for x in (t.shape, t.stride(), t.dtype)])
+    got = packed.descriptors.get(key)
+    if got is not None:
+        return got
+    code = _HALF_CODES.get(q.dtype)
+    if code is None or any(t.dtype != q.dtype for t in (k, v, *grads)):
+        raise ValueError(f"packed attention needs bf16 or fp16 tensors of one type, got "
+                         f"{', '.join(str(t.dtype) for t in (q, k, v, *grads))}")
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape:
         raise ValueError("packed attention needs q [rows, heads, hn] and k, v [rows, kv_heads, hn]")
     rows, n, d = q.shape
@@ -481,25 +495,26 @@ def _packed_desc(q, k, v, packed, scale, code):
         raise ValueError(f"packed attention needs head_dim a multiple of 8 in [8, 128] (got {d})")
     if m < 1 or n < 1 or n % m:
         raise ValueError(f"{n} query heads cannot share {m} key and value heads")
-    scale = d**-0.5 if scale is None else float(scale)
-    if not 2.0**-100 <= scale <= 2.0**100:
+    c = d**-0.5 if scale is None else float(scale)
+    if not 2.0**-100 <= c <= 2.0**100:
         raise ValueError(f"scale must be positive and finite (got {scale})")
-    _check_device(packed.device, q, k, v)
     desc = nat.PackedAttnDesc()
-    desc.rows, desc.heads, desc.kv_heads, desc.head_dim, desc.dtype, desc.scale = rows, n, m, d, code, scale
+    desc.rows, desc.heads, desc.kv_heads, desc.head_dim, desc.dtype, desc.scale = rows, n, m, d, code, c
     (desc.q_tiles, desc.n_q_tiles, desc.k_tiles, desc.n_k_tiles, desc.q_split[:], desc.k_split[:]) = packed.plan(
         n, m, d)
-    desc.q_strides[:] = _thd_strides("q", q)
-    desc.k_strides[:] = _thd_strides("k", k)
-    desc.v_strides[:] = _thd_strides("v", v)
-    return desc
-
-
-def _packed_workspace(desc, backward, device):
-    if not (desc.q_split[0] or backward and desc.k_split[0]):
-        return None
-    size = nat.value("eth_packed_attn_workspace", ctypes.byref(desc), backward)
-    return torch.empty(size, dtype=torch.uint8, device=device)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        getattr(desc, f"{name}_strides")[:] = _thd_strides(name, t)
+    desc.o_strides[:] = desc.do_strides[:] = (n * d, d)  # (contiguous [rows, n*hn])
+    for name, t, like in zip(("dq", "dk", "dv"), grads, (q, k, v)):
+        if t.shape != like.shape:
+            raise ValueError(f"{name} shape mismatch")
+        getattr(desc, f"{name}_strides")[:] = _thd_strides(name, t, written=True)
+    ref = ctypes.byref(desc)
+    size = 0
+    if desc.q_split[0] or grads and desc.k_split[0]:
+        size = nat.value("eth_packed_attn_workspace", ref, 1 if grads else 0)
+    got = packed.descriptors[key] = desc, ref, size
+    return got
 
 
 def _packed_flops(packed, n, d):
@@ -511,21 +526,24 @@ def packed_attention_fwd(q, k, v, packed, scale=None, out=None):
     k, v [rows, m, hn] views with any row and head strides; query head h reads
     key/value head h // (n // m).  Returns (out [rows, n*hn], lse [n, rows],
     log2 domain); rows of no sequence get zeros (lse -inf)."""
-    code = _check_half(q, k, v)
-    desc = _packed_desc(q, k, v, packed, scale, code)
+    index = packed.device.index
+    _check_device(index, q, k, v)
+    _, ref, size = _packed_desc(packed, scale, q, k, v)
+    packed.in_use()
     rows, n, d = q.shape
     if out is None:
         out = torch.empty(rows, n * d, dtype=q.dtype, device=q.device)
     elif out.shape != (rows, n * d) or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
         raise ValueError("out must be a contiguous [rows, n*hn] tensor like q")
-    desc.o_strides[:] = _thd_strides("out", out.view(rows, n, d), written=True)
     lse = torch.empty(n, rows, dtype=torch.float32, device=q.device)
-    ws = _packed_workspace(desc, 0, q.device)
-    flops = _packed_flops(packed, n, d) if _observer is not None else 0.0
-    with _device_guard(q):
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    args = (ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), nat.ptr(ws))
+    if _observer is None:
+        _launch(index, "eth_packed_attn_fwd", *args)
+    else:
+        flops = _packed_flops(packed, n, d)
         _observe("attn_fwd", "begin", flops)
-        nat.call("eth_packed_attn_fwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(out),
-                 nat.ptr(lse), nat.ptr(ws), nat.stream_ptr(q.device))
+        _launch(index, "eth_packed_attn_fwd", *args)
         _observe("attn_fwd", "end", flops)
     return out, lse
 
@@ -535,29 +553,26 @@ def packed_attention_bwd(q, k, v, out, dout, lse, packed, dq, dk, dv, scale=None
     [rows, m, hn] views; out / dout are contiguous [rows, n*hn].  dk and dv are
     summed over the query heads that share them, in a fixed order; rows of no
     sequence get zeros."""
-    code = _check_half(q, k, v, out, dout, dq, dk, dv)
-    desc = _packed_desc(q, k, v, packed, scale, code)
+    index = packed.device.index
+    _check_device(index, q, k, v, out, dout, lse, dq, dk, dv)
+    _, ref, size = _packed_desc(packed, scale, q, k, v, dq, dk, dv)
+    packed.in_use()
     rows, n, d = q.shape
     for name, t in (("out", out), ("dout", dout)):
-        if t.shape != (rows, n * d) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous [rows, n*hn]")
+        if t.shape != (rows, n * d) or t.dtype != q.dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous [rows, n*hn] like q")
     if lse.shape != (n, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be the forward's fp32 [n, rows]")
-    _check_device(q.device, out, dout, lse, dq, dk, dv)
-    desc.o_strides[:] = _thd_strides("out", out.view(rows, n, d))
-    desc.do_strides[:] = _thd_strides("dout", dout.view(rows, n, d))
-    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
-        if t.shape != like.shape:
-            raise ValueError(f"{name} shape mismatch")
-        getattr(desc, f"{name}_strides")[:] = _thd_strides(name, t, written=True)
     delta = torch.empty(n, rows, dtype=torch.float32, device=q.device)
-    ws = _packed_workspace(desc, 1, q.device)
-    flops = 2.5 * _packed_flops(packed, n, d) if _observer is not None else 0.0
-    with _device_guard(q):
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    args = (ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
+            delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), nat.ptr(ws))
+    if _observer is None:
+        _launch(index, "eth_packed_attn_bwd", *args)
+    else:
+        flops = 2.5 * _packed_flops(packed, n, d)
         _observe("attn_bwd", "begin", flops)
-        nat.call("eth_packed_attn_bwd", ctypes.byref(desc), nat.ptr(q), nat.ptr(k), nat.ptr(v), nat.ptr(out),
-                 nat.ptr(dout), nat.ptr(lse), nat.ptr(delta), nat.ptr(dq), nat.ptr(dk), nat.ptr(dv),
-                 nat.ptr(ws), nat.stream_ptr(q.device))
+        _launch(index, "eth_packed_attn_bwd", *args)
         _observe("attn_bwd", "end", flops)
 
 
@@ -632,21 +647,26 @@ def xent_bwd(logits2d, labels, lse, dloss):
 
 
 def _check_logits(logits2d, bad_flag, *ts):
-    """(dtype code, rows, V, row stride) of [rows, V] logits in any of the three types."""
+    """(device index, dtype code, rows, V, row stride) of [rows, V] logits in
+    any of the three types."""
     if logits2d.dim() != 2 or logits2d.shape[1] < 1:
         raise ValueError("logits must be [rows, V]")
-    nat.require_cuda(logits2d)
+    index = logits2d.get_device()
+    if index < 0:
+        raise ValueError("eth_amd kernels run on the GPU only (no CPU fallback)")
     code = nat.dtype_code(logits2d.dtype)
     rows, V = logits2d.shape
-    if V > 1 and logits2d.stride(1) != 1:
+    ld, s1 = logits2d.stride()
+    if V > 1 and s1 != 1:
         raise ValueError("logits rows must be contiguous")
-    ld = logits2d.stride(0) if rows > 1 else V
+    if rows <= 1:
+        ld = V
     if ld < V:
         raise ValueError("logits rows may not overlap")
     if bad_flag.dtype != torch.int32 or bad_flag.numel() < 1:
         raise ValueError("bad_flag must be an int32 tensor")
-    _check_device(logits2d.device, bad_flag, *ts)
-    return code, rows, V, ld
+    _check_device(index, bad_flag, *ts)
+    return index, code, rows, V, ld
 
 
 def _check_row_values(name, t, rows):
@@ -659,36 +679,39 @@ def _check_stats(stats, rows, n):
         raise ValueError(f"stats must be the forward's fp32 [rows, {n}]")
 
 
-def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100):
+def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100, shape=None):
     """(logprob [rows], entropy [rows], stats [rows, 2], top_logprobs [rows,
     top_k] fp32, top_ids [rows, top_k] int64) of logits [rows, V] in bf16, fp16
     or fp32: the log probability of each row's token, the row's entropy and its
     top_k largest log probabilities, equal ones by the lowest id.  Rows with
     token `ignore_index` give 0, 0, -inf and -1; other ids outside the
-    vocabulary are clamped and flagged in `bad_flag`."""
-    code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
+    vocabulary are clamped and flagged in `bad_flag`.  `shape`: the rows' shape
+    in the results (default [rows])."""
+    index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
     _check_ids(tokens, (rows,))
     if not 0 <= top_k <= min(128, V):
         raise ValueError(f"top_k must be in [0, 128] and within the vocabulary (got {top_k})")
+    shape = (rows,) if shape is None else tuple(shape)
+    if math.prod(shape) != rows:
+        raise ValueError(f"shape {shape} does not hold {rows} rows")
     new = functools.partial(torch.empty, dtype=torch.float32, device=logits2d.device)
-    logprob, entropy, stats, top = new(rows), new(rows), new(rows, 2), new(rows, top_k)
-    ids = torch.empty(rows, top_k, dtype=torch.int64, device=logits2d.device)
+    logprob, entropy, stats, top = new(shape), new(shape), new(rows, 2), new(*shape, top_k)
+    ids = torch.empty(*shape, top_k, dtype=torch.int64, device=logits2d.device)
     if rows:
         # (the call's own: its two launches may have another thread's between them)
         ws = nat.value("eth_token_logprobs_workspace", rows, V, top_k, code)
         ws = torch.empty(ws, dtype=torch.uint8, device=logits2d.device) if ws else None
-        with _device_guard(logits2d):
-            nat.call("eth_token_logprobs_fwd", nat.ptr(logits2d), ld, nat.ptr(tokens), int(ignore_index),
-                     nat.ptr(logprob), nat.ptr(entropy), nat.ptr(stats), nat.ptr(top), nat.ptr(ids), top_k,
-                     nat.ptr(ws), rows, V, nat.ptr(bad_flag), code, nat.stream_ptr(logits2d.device))
+        _launch(index, "eth_token_logprobs_fwd", logits2d.data_ptr(), ld, tokens.data_ptr(), ignore_index,
+                logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top.data_ptr(), ids.data_ptr(), top_k,
+                nat.ptr(ws), rows, V, bad_flag.data_ptr(), code)
     return logprob, entropy, stats, top, ids
 
 
-def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad_flag, ignore_index=-100):
-    """dlogits [rows, V] for upstream gradients of logprob and entropy (fp32
-    [rows]; one of them may be None)."""
+def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad_flag, ignore_index=-100, shape=None):
+    """dlogits [rows, V] (as `shape`, if given) for upstream gradients of
+    logprob and entropy (fp32 [rows]; one of them may be None)."""
     given = [t for t in (dlogprob, dentropy) if t is not None]
-    code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens, stats, entropy, *given)
+    index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens, stats, entropy, *given)
     _check_ids(tokens, (rows,))
     _check_stats(stats, rows, 2)
     for name, t in (("entropy", entropy), ("dlogprob", dlogprob), ("dentropy", dentropy)):
@@ -696,13 +719,19 @@ def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad
             _check_row_values(name, t, rows)
     if not given:
         raise ValueError("token_logprobs_bwd needs dlogprob or dentropy")
-    dz = torch.empty(rows, V, dtype=logits2d.dtype, device=logits2d.device)
+    dz = _new_dlogits(logits2d, shape)
     if rows:
-        with _device_guard(logits2d):
-            nat.call("eth_token_logprobs_bwd", nat.ptr(logits2d), ld, nat.ptr(tokens), int(ignore_index),
-                     nat.ptr(stats), nat.ptr(entropy), nat.ptr(dlogprob), nat.ptr(dentropy), nat.ptr(dz), V, rows, V,
-                     code, nat.stream_ptr(logits2d.device))
+        _launch(index, "eth_token_logprobs_bwd", logits2d.data_ptr(), ld, tokens.data_ptr(), ignore_index,
+                stats.data_ptr(), entropy.data_ptr(), nat.ptr(dlogprob), nat.ptr(dentropy), dz.data_ptr(), V, rows, V,
+                code)
     return dz
+
+
+def _new_dlogits(logits2d, shape):
+    shape = logits2d.shape if shape is None else tuple(shape)
+    if math.prod(shape) != logits2d.numel():
+        raise ValueError(f"shape {shape} does not hold {tuple(logits2d.shape)} logits")
+    return torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
 
 
 def _check_teacher(teacher_ids, teacher_logits, rows, temperature):
@@ -719,36 +748,39 @@ def _check_teacher(teacher_ids, teacher_logits, rows, temperature):
     return k, nat.dtype_code(teacher_logits.dtype)
 
 
-def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag):
+def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag, shape=None):
     """(loss [rows], stats [rows, 4]): temperature^2 * sum q (log q - log p[id])
     with q the softmax of a row's k teacher logits (any of the three types) and
     p that of its V logits, both at the temperature.  Negative ids and teacher
     logits of -inf are no entries; ids past the vocabulary are none either and
-    are flagged in `bad_flag`."""
-    code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits)
+    are flagged in `bad_flag`.  `shape`: the rows' shape in the loss (default
+    [rows])."""
+    index, code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits)
     k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
-    loss = torch.empty(rows, dtype=torch.float32, device=logits2d.device)
+    shape = (rows,) if shape is None else tuple(shape)
+    if math.prod(shape) != rows:
+        raise ValueError(f"shape {shape} does not hold {rows} rows")
+    loss = torch.empty(shape, dtype=torch.float32, device=logits2d.device)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=logits2d.device)
     if rows:
-        with _device_guard(logits2d):
-            nat.call("eth_topk_distill_fwd", nat.ptr(logits2d), ld, nat.ptr(teacher_ids), nat.ptr(teacher_logits),
-                     teacher_code, k, float(temperature), nat.ptr(loss), nat.ptr(stats), rows, V, nat.ptr(bad_flag),
-                     code, nat.stream_ptr(logits2d.device))
+        _launch(index, "eth_topk_distill_fwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
+                teacher_logits.data_ptr(), teacher_code, k, temperature, loss.data_ptr(), stats.data_ptr(), rows, V,
+                bad_flag.data_ptr(), code)
     return loss, stats
 
 
-def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag):
-    """dlogits [rows, V] of topk_distill_fwd's loss (dloss fp32 [rows])."""
-    code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits, stats, dloss)
+def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag, shape=None):
+    """dlogits [rows, V] (as `shape`, if given) of topk_distill_fwd's loss
+    (dloss fp32 [rows])."""
+    index, code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits, stats, dloss)
     k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
     _check_stats(stats, rows, 4)
     _check_row_values("dloss", dloss, rows)
-    dz = torch.empty(rows, V, dtype=logits2d.dtype, device=logits2d.device)
+    dz = _new_dlogits(logits2d, shape)
     if rows:
-        with _device_guard(logits2d):
-            nat.call("eth_topk_distill_bwd", nat.ptr(logits2d), ld, nat.ptr(teacher_ids), nat.ptr(teacher_logits),
-                     teacher_code, k, float(temperature), nat.ptr(stats), nat.ptr(dloss), nat.ptr(dz), V, rows, V,
-                     nat.ptr(bad_flag), code, nat.stream_ptr(logits2d.device))
+        _launch(index, "eth_topk_distill_bwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
+                teacher_logits.data_ptr(), teacher_code, k, temperature, stats.data_ptr(), dloss.data_ptr(),
+                dz.data_ptr(), V, rows, V, bad_flag.data_ptr(), code)
     return dz
 
 

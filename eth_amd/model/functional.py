@@ -441,7 +441,9 @@ class PackedCausalAttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
         K.packed_attention_bwd(q, k, v, out, dout.contiguous(), lse, ctx.packed, dq, dk, dv, ctx.scale)
         return dq, dk, dv, None, None
 
@@ -501,9 +503,17 @@ class CrossEntropyFn(torch.autograd.Function):
 def _logit_rows(logits):
     """[rows, V] of logits [..., V] for the row kernels: the tensor's own
     memory where its rows are whole and apart, else a copy."""
-    z = logits.reshape(-1, logits.shape[-1])
+    z = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     rows, V = z.shape
-    return z if (V == 1 or z.stride(1) == 1) and (rows <= 1 or z.stride(0) >= V) else z.contiguous()
+    s0, s1 = z.stride()
+    return z if (V == 1 or s1 == 1) and (rows <= 1 or s0 >= V) else z.contiguous()
+
+
+def _row_values(t, rows):
+    """An upstream gradient as contiguous fp32 [rows]."""
+    if t is None or t.dtype == torch.float32 and t.dim() == 1 and t.is_contiguous():
+        return t
+    return t.reshape(rows).float().contiguous()
 
 
 class TokenLogprobsFn(torch.autograd.Function):
@@ -517,25 +527,25 @@ class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, bad_flag, ignore_index=-100):
         ctx.set_materialize_grads(False)
-        if tokens.shape != logits.shape[:-1]:
-            raise ValueError(f"tokens {tuple(tokens.shape)} do not match logits {tuple(logits.shape)}")
+        shape = tokens.shape
+        if shape != logits.shape[:-1]:
+            raise ValueError(f"tokens {tuple(shape)} do not match logits {tuple(logits.shape)}")
         z, t = _logit_rows(logits), tokens.reshape(-1).contiguous()
-        logprob, entropy, stats, top, ids = K.token_logprobs_fwd(z, t, top_k, bad_flag, ignore_index)
+        logprob, entropy, stats, top, ids = K.token_logprobs_fwd(z, t, top_k, bad_flag, ignore_index, shape)
         ctx.save_for_backward(z, t, stats, entropy)
         ctx.shape, ctx.ignore_index, ctx.bad_flag = logits.shape, ignore_index, bad_flag
-        shape = logits.shape[:-1]
-        top, ids = top.view(*shape, top_k), ids.view(*shape, top_k)
         ctx.mark_non_differentiable(top, ids)
-        return logprob.view(shape), entropy.view(shape), top, ids
+        return logprob, entropy, top, ids
 
     @staticmethod
     def backward(ctx, dlogprob, dentropy, _dtop, _dids):
         if dlogprob is None and dentropy is None:
             return None, None, None, None, None
         z, t, stats, entropy = ctx.saved_tensors
-        dlogprob, dentropy = (None if g is None else g.reshape(-1).float().contiguous() for g in (dlogprob, dentropy))
-        dz = K.token_logprobs_bwd(z, t, stats, entropy, dlogprob, dentropy, ctx.bad_flag, ctx.ignore_index)
-        return dz.view(ctx.shape), None, None, None, None
+        rows = z.shape[0]
+        dz = K.token_logprobs_bwd(z, t, stats, entropy.reshape(rows), _row_values(dlogprob, rows),
+                                  _row_values(dentropy, rows), ctx.bad_flag, ctx.ignore_index, ctx.shape)
+        return dz, None, None, None, None
 
 
 class TopkDistillFn(torch.autograd.Function):
@@ -546,19 +556,22 @@ class TopkDistillFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, teacher_ids, teacher_logits, temperature, bad_flag):
-        if teacher_ids.shape[:-1] != logits.shape[:-1] or teacher_logits.shape != teacher_ids.shape:
+        shape = logits.shape[:-1]
+        if teacher_ids.shape[:-1] != shape or teacher_logits.shape != teacher_ids.shape:
             raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} and logits {tuple(teacher_logits.shape)} do not "
                              f"match logits {tuple(logits.shape)}")
         z = _logit_rows(logits)
-        ids, teacher = (t.reshape(z.shape[0], t.shape[-1]).contiguous() for t in (teacher_ids, teacher_logits))
-        loss, stats = K.topk_distill_fwd(z, ids, teacher, temperature, bad_flag)
+        if len(shape) != 1:
+            teacher_ids, teacher_logits = (t.reshape(z.shape[0], t.shape[-1]) for t in (teacher_ids, teacher_logits))
+        ids, teacher = teacher_ids.contiguous(), teacher_logits.contiguous()
+        loss, stats = K.topk_distill_fwd(z, ids, teacher, temperature, bad_flag, shape)
         ctx.save_for_backward(z, ids, teacher, stats)
         ctx.shape, ctx.temperature, ctx.bad_flag = logits.shape, temperature, bad_flag
-        return loss.view(logits.shape[:-1])
+        return loss
 
     @staticmethod
     def backward(ctx, dloss):
         z, ids, teacher, stats = ctx.saved_tensors
-        dz = K.topk_distill_bwd(z, ids, teacher, ctx.temperature, stats, dloss.reshape(-1).float().contiguous(),
-                                ctx.bad_flag)
-        return dz.view(ctx.shape), None, None, None, None
+        dz = K.topk_distill_bwd(z, ids, teacher, ctx.temperature, stats, _row_values(dloss, z.shape[0]), ctx.bad_flag,
+                                ctx.shape)
+        return dz, None, None, None, None

@@ -101,12 +101,17 @@ class PackedSequences:
             self._at[key] = (at, tiles.size)
             at += tiles.nbytes
         self._plans = {}
+        self.descriptors = {}  # of calls with this plan, by shapes and strides
+
+    def in_use(self):
+        """A launch on the current stream is about to read the lists."""
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._home:
+            if not torch.cuda.is_current_stream_capturing():
+                self._table.record_stream(torch.cuda.current_stream(self.device))
 
     def plan(self, heads, kv_heads, head_dim):
         """(query list address and count, key list address and count, query
-        split, key split) for these heads, for a launch on the current stream."""
-        if nat.stream_ptr(self.device) != self._home and not torch.cuda.is_current_stream_capturing():
-            self._table.record_stream(torch.cuda.current_stream(self.device))
+        split, key split) for these heads."""
         plan = self._plans.get((heads, kv_heads, head_dim))
         if plan is None:
             rows = nat.value("eth_packed_attn_tile_rows", heads, kv_heads)
