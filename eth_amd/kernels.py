@@ -8,7 +8,6 @@ the current stream.  There is no CPU fallback: CPU tensors raise.
 import ctypes
 import functools
 import itertools
-import math
 
 import numpy as np
 
@@ -521,15 +520,23 @@ def _packed_flops(packed, n, d):
     return 2.0 * n * d * sum(x * (x + 1) for x in packed.lengths)  # QK^T and PV over the causal half
 
 
+def _packed_launch(name, kind, work, q, packed, *args):
+    packed.in_use()
+    if _observer is None:
+        return _launch(packed.device.index, name, *args)
+    flops = work * _packed_flops(packed, q.shape[1], q.shape[2])
+    _observe(kind, "begin", flops)
+    _launch(packed.device.index, name, *args)
+    _observe(kind, "end", flops)
+
+
 def packed_attention_fwd(q, k, v, packed, scale=None, out=None):
     """Causal attention over `packed` (PackedSequences) of q [rows, n, hn] and
     k, v [rows, m, hn] views with any row and head strides; query head h reads
     key/value head h // (n // m).  Returns (out [rows, n*hn], lse [n, rows],
     log2 domain); rows of no sequence get zeros (lse -inf)."""
-    index = packed.device.index
-    _check_device(index, q, k, v)
+    _check_device(packed.device.index, q, k, v)
     _, ref, size = _packed_desc(packed, scale, q, k, v)
-    packed.in_use()
     rows, n, d = q.shape
     if out is None:
         out = torch.empty(rows, n * d, dtype=q.dtype, device=q.device)
@@ -537,14 +544,8 @@ def packed_attention_fwd(q, k, v, packed, scale=None, out=None):
         raise ValueError("out must be a contiguous [rows, n*hn] tensor like q")
     lse = torch.empty(n, rows, dtype=torch.float32, device=q.device)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    args = (ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), nat.ptr(ws))
-    if _observer is None:
-        _launch(index, "eth_packed_attn_fwd", *args)
-    else:
-        flops = _packed_flops(packed, n, d)
-        _observe("attn_fwd", "begin", flops)
-        _launch(index, "eth_packed_attn_fwd", *args)
-        _observe("attn_fwd", "end", flops)
+    _packed_launch("eth_packed_attn_fwd", "attn_fwd", 1.0, q, packed, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                   out.data_ptr(), lse.data_ptr(), nat.ptr(ws))
     return out, lse
 
 
@@ -553,27 +554,41 @@ def packed_attention_bwd(q, k, v, out, dout, lse, packed, dq, dk, dv, scale=None
     [rows, m, hn] views; out / dout are contiguous [rows, n*hn].  dk and dv are
     summed over the query heads that share them, in a fixed order; rows of no
     sequence get zeros."""
-    index = packed.device.index
-    _check_device(index, q, k, v, out, dout, lse, dq, dk, dv)
-    _, ref, size = _packed_desc(packed, scale, q, k, v, dq, dk, dv)
-    packed.in_use()
+    _check_device(packed.device.index, q, k, v, out, dout, lse, dq, dk, dv)
+    desc = _packed_desc(packed, scale, q, k, v, dq, dk, dv)
     rows, n, d = q.shape
     for name, t in (("out", out), ("dout", dout)):
         if t.shape != (rows, n * d) or t.dtype != q.dtype or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous [rows, n*hn] like q")
     if lse.shape != (n, rows) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise ValueError("lse must be the forward's fp32 [n, rows]")
-    delta = torch.empty(n, rows, dtype=torch.float32, device=q.device)
+    _packed_bwd(desc, q, k, v, out, dout, lse, packed, dq, dk, dv)
+
+
+def _packed_bwd(desc, q, k, v, out, dout, lse, packed, dq, dk, dv):
+    _, ref, size = desc
+    delta = torch.empty(lse.shape, dtype=torch.float32, device=q.device)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    args = (ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr(),
-            delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), nat.ptr(ws))
-    if _observer is None:
-        _launch(index, "eth_packed_attn_bwd", *args)
-    else:
-        flops = 2.5 * _packed_flops(packed, n, d)
-        _observe("attn_bwd", "begin", flops)
-        _launch(index, "eth_packed_attn_bwd", *args)
-        _observe("attn_bwd", "end", flops)
+    _packed_launch("eth_packed_attn_bwd", "attn_bwd", 2.5, q, packed, ref, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                   out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                   dv.data_ptr(), nat.ptr(ws))
+
+
+def _packed_attention_grads(q, k, v, out, dout, lse, packed, scale=None):
+    """(dq, dk, dv) of packed_attention_bwd in new tensors, for the very q, k,
+    v, out, lse and scale of a packed_attention_fwd call, which are not checked
+    again; dout is like out."""
+    key = "grads", scale, q.shape, q.stride(), k.shape, k.stride(), v.stride(), q.dtype
+    desc = packed.descriptors.get(key)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    if desc is None:
+        desc = packed.descriptors[key] = _packed_desc(packed, scale, q, k, v, dq, dk, dv)
+    if dout.shape != out.shape or dout.dtype != out.dtype or dout.get_device() != out.get_device():
+        raise ValueError("dout must be like out")
+    _packed_bwd(desc, q, k, v, out, dout.contiguous(), lse, packed, dq, dk, dv)
+    return dq, dk, dv
 
 
 # --------------------------------------------------------------- vocabulary --
@@ -679,21 +694,23 @@ def _check_stats(stats, rows, n):
         raise ValueError(f"stats must be the forward's fp32 [rows, {n}]")
 
 
-def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100, shape=None):
+def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100):
     """(logprob [rows], entropy [rows], stats [rows, 2], top_logprobs [rows,
     top_k] fp32, top_ids [rows, top_k] int64) of logits [rows, V] in bf16, fp16
     or fp32: the log probability of each row's token, the row's entropy and its
     top_k largest log probabilities, equal ones by the lowest id.  Rows with
     token `ignore_index` give 0, 0, -inf and -1; other ids outside the
-    vocabulary are clamped and flagged in `bad_flag`.  `shape`: the rows' shape
-    in the results (default [rows])."""
-    index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
+    vocabulary are clamped and flagged in `bad_flag`."""
+    return _token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index, (logits2d.shape[0],))[:5]
+
+
+def _token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index, shape):
+    """token_logprobs_fwd with the rows in `shape` in its results, and behind
+    them the operands' layout for the backward."""
+    layout = index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
     _check_ids(tokens, (rows,))
     if not 0 <= top_k <= min(128, V):
         raise ValueError(f"top_k must be in [0, 128] and within the vocabulary (got {top_k})")
-    shape = (rows,) if shape is None else tuple(shape)
-    if math.prod(shape) != rows:
-        raise ValueError(f"shape {shape} does not hold {rows} rows")
     new = functools.partial(torch.empty, dtype=torch.float32, device=logits2d.device)
     logprob, entropy, stats, top = new(shape), new(shape), new(rows, 2), new(*shape, top_k)
     ids = torch.empty(*shape, top_k, dtype=torch.int64, device=logits2d.device)
@@ -704,12 +721,12 @@ def token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index=-100, sha
         _launch(index, "eth_token_logprobs_fwd", logits2d.data_ptr(), ld, tokens.data_ptr(), ignore_index,
                 logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top.data_ptr(), ids.data_ptr(), top_k,
                 nat.ptr(ws), rows, V, bad_flag.data_ptr(), code)
-    return logprob, entropy, stats, top, ids
+    return logprob, entropy, stats, top, ids, layout
 
 
-def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad_flag, ignore_index=-100, shape=None):
-    """dlogits [rows, V] (as `shape`, if given) for upstream gradients of
-    logprob and entropy (fp32 [rows]; one of them may be None)."""
+def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad_flag, ignore_index=-100):
+    """dlogits [rows, V] for upstream gradients of logprob and entropy (fp32
+    [rows]; one of them may be None)."""
     given = [t for t in (dlogprob, dentropy) if t is not None]
     index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens, stats, entropy, *given)
     _check_ids(tokens, (rows,))
@@ -719,19 +736,20 @@ def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad
             _check_row_values(name, t, rows)
     if not given:
         raise ValueError("token_logprobs_bwd needs dlogprob or dentropy")
-    dz = _new_dlogits(logits2d, shape)
+    return _token_logprobs_bwd((index, code, rows, V, ld), logits2d, tokens, stats, entropy, dlogprob, dentropy,
+                               ignore_index, logits2d.shape)
+
+
+def _token_logprobs_bwd(layout, logits2d, tokens, stats, entropy, dlogprob, dentropy, ignore_index, shape):
+    """token_logprobs_bwd of operands that a forward checked (`layout`:
+    _check_logits' result; upstream gradients as contiguous fp32 [rows])."""
+    index, code, rows, V, ld = layout
+    dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
     if rows:
         _launch(index, "eth_token_logprobs_bwd", logits2d.data_ptr(), ld, tokens.data_ptr(), ignore_index,
                 stats.data_ptr(), entropy.data_ptr(), nat.ptr(dlogprob), nat.ptr(dentropy), dz.data_ptr(), V, rows, V,
                 code)
     return dz
-
-
-def _new_dlogits(logits2d, shape):
-    shape = logits2d.shape if shape is None else tuple(shape)
-    if math.prod(shape) != logits2d.numel():
-        raise ValueError(f"shape {shape} does not hold {tuple(logits2d.shape)} logits")
-    return torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
 
 
 def _check_teacher(teacher_ids, teacher_logits, rows, temperature):
@@ -748,35 +766,45 @@ def _check_teacher(teacher_ids, teacher_logits, rows, temperature):
     return k, nat.dtype_code(teacher_logits.dtype)
 
 
-def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag, shape=None):
+def topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag):
     """(loss [rows], stats [rows, 4]): temperature^2 * sum q (log q - log p[id])
     with q the softmax of a row's k teacher logits (any of the three types) and
     p that of its V logits, both at the temperature.  Negative ids and teacher
     logits of -inf are no entries; ids past the vocabulary are none either and
-    are flagged in `bad_flag`.  `shape`: the rows' shape in the loss (default
-    [rows])."""
-    index, code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits)
+    are flagged in `bad_flag`."""
+    return _topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag, (logits2d.shape[0],))[:2]
+
+
+def _topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_flag, shape):
+    """topk_distill_fwd with the rows in `shape` in its loss, and behind its
+    results the operands' layout for the backward."""
+    layout = index, code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits)
     k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
-    shape = (rows,) if shape is None else tuple(shape)
-    if math.prod(shape) != rows:
-        raise ValueError(f"shape {shape} does not hold {rows} rows")
     loss = torch.empty(shape, dtype=torch.float32, device=logits2d.device)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=logits2d.device)
     if rows:
         _launch(index, "eth_topk_distill_fwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
                 teacher_logits.data_ptr(), teacher_code, k, temperature, loss.data_ptr(), stats.data_ptr(), rows, V,
                 bad_flag.data_ptr(), code)
-    return loss, stats
+    return loss, stats, layout
 
 
-def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag, shape=None):
-    """dlogits [rows, V] (as `shape`, if given) of topk_distill_fwd's loss
-    (dloss fp32 [rows])."""
+def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag):
+    """dlogits [rows, V] of topk_distill_fwd's loss (dloss fp32 [rows])."""
     index, code, rows, V, ld = _check_logits(logits2d, bad_flag, teacher_ids, teacher_logits, stats, dloss)
-    k, teacher_code = _check_teacher(teacher_ids, teacher_logits, rows, temperature)
+    _check_teacher(teacher_ids, teacher_logits, rows, temperature)
     _check_stats(stats, rows, 4)
     _check_row_values("dloss", dloss, rows)
-    dz = _new_dlogits(logits2d, shape)
+    return _topk_distill_bwd((index, code, rows, V, ld), logits2d, teacher_ids, teacher_logits, temperature, stats,
+                             dloss, bad_flag, logits2d.shape)
+
+
+def _topk_distill_bwd(layout, logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag, shape):
+    """topk_distill_bwd of operands that a forward checked (`layout`:
+    _check_logits' result; dloss as contiguous fp32 [rows])."""
+    index, code, rows, V, ld = layout
+    k, teacher_code = teacher_ids.shape[1], nat.dtype_code(teacher_logits.dtype)
+    dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
     if rows:
         _launch(index, "eth_topk_distill_bwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
                 teacher_logits.data_ptr(), teacher_code, k, temperature, stats.data_ptr(), dloss.data_ptr(),

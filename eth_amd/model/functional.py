@@ -441,11 +441,7 @@ class PackedCausalAttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        K.packed_attention_bwd(q, k, v, out, dout.contiguous(), lse, ctx.packed, dq, dk, dv, ctx.scale)
-        return dq, dk, dv, None, None
+        return (*K._packed_attention_grads(q, k, v, out, dout, lse, ctx.packed, ctx.scale), None, None)
 
 
 class EmbeddingFn(torch.autograd.Function):
@@ -509,11 +505,12 @@ def _logit_rows(logits):
     return z if (V == 1 or s1 == 1) and (rows <= 1 or s0 >= V) else z.contiguous()
 
 
-def _row_values(t, rows):
-    """An upstream gradient as contiguous fp32 [rows]."""
-    if t is None or t.dtype == torch.float32 and t.dim() == 1 and t.is_contiguous():
+def _row_values(t):
+    """An upstream gradient of row values as contiguous fp32, in any shape
+    (autograd gives it the values' own shape and device)."""
+    if t is None or t.dtype == torch.float32 and t.is_contiguous():
         return t
-    return t.reshape(rows).float().contiguous()
+    return t.float().contiguous()
 
 
 class TokenLogprobsFn(torch.autograd.Function):
@@ -531,9 +528,9 @@ class TokenLogprobsFn(torch.autograd.Function):
         if shape != logits.shape[:-1]:
             raise ValueError(f"tokens {tuple(shape)} do not match logits {tuple(logits.shape)}")
         z, t = _logit_rows(logits), tokens.reshape(-1).contiguous()
-        logprob, entropy, stats, top, ids = K.token_logprobs_fwd(z, t, top_k, bad_flag, ignore_index, shape)
+        logprob, entropy, stats, top, ids, ctx.layout = K._token_logprobs_fwd(z, t, top_k, bad_flag, ignore_index, shape)
         ctx.save_for_backward(z, t, stats, entropy)
-        ctx.shape, ctx.ignore_index, ctx.bad_flag = logits.shape, ignore_index, bad_flag
+        ctx.shape, ctx.ignore_index = logits.shape, ignore_index
         ctx.mark_non_differentiable(top, ids)
         return logprob, entropy, top, ids
 
@@ -542,9 +539,8 @@ class TokenLogprobsFn(torch.autograd.Function):
         if dlogprob is None and dentropy is None:
             return None, None, None, None, None
         z, t, stats, entropy = ctx.saved_tensors
-        rows = z.shape[0]
-        dz = K.token_logprobs_bwd(z, t, stats, entropy.reshape(rows), _row_values(dlogprob, rows),
-                                  _row_values(dentropy, rows), ctx.bad_flag, ctx.ignore_index, ctx.shape)
+        dz = K._token_logprobs_bwd(ctx.layout, z, t, stats, entropy, _row_values(dlogprob), _row_values(dentropy),
+                                   ctx.ignore_index, ctx.shape)
         return dz, None, None, None, None
 
 
@@ -564,7 +560,7 @@ class TopkDistillFn(torch.autograd.Function):
         if len(shape) != 1:
             teacher_ids, teacher_logits = (t.reshape(z.shape[0], t.shape[-1]) for t in (teacher_ids, teacher_logits))
         ids, teacher = teacher_ids.contiguous(), teacher_logits.contiguous()
-        loss, stats = K.topk_distill_fwd(z, ids, teacher, temperature, bad_flag, shape)
+        loss, stats, ctx.layout = K._topk_distill_fwd(z, ids, teacher, temperature, bad_flag, shape)
         ctx.save_for_backward(z, ids, teacher, stats)
         ctx.shape, ctx.temperature, ctx.bad_flag = logits.shape, temperature, bad_flag
         return loss
@@ -572,6 +568,6 @@ class TopkDistillFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dloss):
         z, ids, teacher, stats = ctx.saved_tensors
-        dz = K.topk_distill_bwd(z, ids, teacher, ctx.temperature, stats, _row_values(dloss, z.shape[0]), ctx.bad_flag,
-                                ctx.shape)
+        dz = K._topk_distill_bwd(ctx.layout, z, ids, teacher, ctx.temperature, stats, _row_values(dloss), ctx.bad_flag,
+                                 ctx.shape)
         return dz, None, None, None, None
