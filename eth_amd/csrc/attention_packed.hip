@@ -363,17 +363,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
   if (hl == 0) a.lse[(int64_t)h * a.T + begin + q] = m + log2f(l);
 }
 
-// joins the pieces of split query tiles, in order
+// joins the pieces of split query tiles, in order, a wave's rows per workgroup
 template <int D, bool FP16>
-__global__ void __launch_bounds__(kAttnThreads) packed_fwd_join_kernel(PackArgs a) {
+__global__ void __launch_bounds__(64) packed_fwd_join_kernel(PackArgs a) {
   constexpr int DT = D / 32;
   const int hbs = a.n / a.hp;
-  const Piece pc{(int)(blockIdx.x / hbs), (int)(blockIdx.x % hbs), 0, a.q_split.pieces};
+  const int w = blockIdx.x % 4, r = blockIdx.x / 4;
+  const Piece pc{r / hbs, r % hbs, 0, a.q_split.pieces};
   const int kvh = pc.head % a.m, h0 = kvh * a.group + pc.head / a.m * a.hp;
   const eth_packed_tile_t tile = a.q_tiles[pc.tile];
   if (tile.len < 0) return;  // (stored as zeros by the first launch)
-  const int lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x;
   const int h = h0 + w % a.hp, q = tile.start + w / a.hp * 32 + (lane & 31);
   const int qend = min(tile.start + kBQ / a.hp, tile.len);
   const int used = steps_of((qend + kBKV - 1) / kBKV, 0, pc.pieces, a.q_split.steps).used;
@@ -542,17 +542,17 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
   if (real) store_row<DT, FP16>(row_ptr(a.dq, begin + q, h), dq, a.scale, a.hd, hl);
 }
 
-// joins the pieces of split query tiles, in order
+// joins the pieces of split query tiles, in order, a wave's rows per workgroup
 template <int D, bool FP16>
-__global__ void __launch_bounds__(kAttnThreads) packed_dq_join_kernel(PackArgs a) {
+__global__ void __launch_bounds__(64) packed_dq_join_kernel(PackArgs a) {
   constexpr int DT = D / 32;
   const int hbs = a.n / a.hp;
-  const Piece pc{(int)(blockIdx.x / hbs), (int)(blockIdx.x % hbs), 0, a.q_split.pieces};
+  const int w = blockIdx.x % 4, r = blockIdx.x / 4;
+  const Piece pc{r / hbs, r % hbs, 0, a.q_split.pieces};
   const int kvh = pc.head % a.m, h0 = kvh * a.group + pc.head / a.m * a.hp;
   const eth_packed_tile_t tile = a.q_tiles[pc.tile];
   if (tile.len < 0) return;  // (stored as zeros by the first launch)
-  const int lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x;
   const int h = h0 + w % a.hp, q = tile.start + w / a.hp * 32 + (lane & 31);
   const int qend = min(tile.start + kBQ / a.hp, tile.len);
   const int used = steps_of((qend + kBKV - 1) / kBKV, 0, pc.pieces, a.q_split.steps).used;
@@ -1050,12 +1050,15 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
   store_keys<D, SL, FP16>(dkw ? a.dk : a.dv, stage, acc, dkw ? a.scale : 1.f, begin, k0, len, kvh, a.hd, lane);
 }
 
-// joins the pieces of split key tiles, in order: waves 0 to 3 dV, 4 to 7 dK
+// joins the pieces of split key tiles, in order, 32 keys per workgroup: wave 0
+// dV, wave 1 dK (two waves rather than eight: the reads of 124 split tiles of
+// 128 x 64 spread over four times the workgroups, 27 -> 25 us)
 template <int D, bool FP16>
-__global__ void __launch_bounds__(2 * kAttnThreads) packed_dkdv_join_kernel(PackArgs a) {
+__global__ void __launch_bounds__(128) packed_dkdv_join_kernel(PackArgs a) {
   constexpr int DT = D / 32, SL = D + 8;
-  __shared__ __attribute__((aligned(16))) uint16_t stage[8 * 32 * SL];
-  const Piece pc{(int)(blockIdx.x / a.m), (int)(blockIdx.x % a.m), 0, a.k_split.pieces};
+  __shared__ __attribute__((aligned(16))) uint16_t stage[2 * 32 * SL];
+  const int w = blockIdx.x % 4, b = blockIdx.x / 4;
+  const Piece pc{b / a.m, b % a.m, 0, a.k_split.pieces};
   const eth_packed_tile_t tile = a.k_tiles[pc.tile];
   if (tile.len < 0) return;  // (stored as zeros by the first launch)
   const int lane = threadIdx.x & 63;
@@ -1065,9 +1068,10 @@ __global__ void __launch_bounds__(2 * kAttnThreads) packed_dkdv_join_kernel(Pack
   a_f32x16 x[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) x[t] = a_f32x16{};
-  for (int i = 0; i < used; ++i) add_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, i, 8, wv, lane), x, 1.f);
-  store_keys<D, SL, FP16>(wv < 4 ? a.dv : a.dk, stage + wv * 32 * SL, x, wv < 4 ? 1.f : a.scale, tile.begin,
-                          tile.start + (wv & 3) * 32, tile.len, pc.head, a.hd, lane);
+  for (int i = 0; i < used; ++i)
+    add_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, i, 8, wv * 4 + w, lane), x, 1.f);
+  store_keys<D, SL, FP16>(wv == 0 ? a.dv : a.dk, stage + wv * 32 * SL, x, wv == 0 ? 1.f : a.scale, tile.begin,
+                          tile.start + w * 32, tile.len, pc.head, a.hd, lane);
 }
 
 }  // namespace eth
@@ -1153,18 +1157,18 @@ extern "C" int64_t eth_packed_attn_workspace(const eth_packed_attn_desc_t* d, in
 template <int D, bool FP16>
 static void launch_packed_fwd(const PackArgs& a, int grid, hipStream_t s) {
   packed_fwd_kernel<D, FP16><<<grid, kAttnThreads, 0, s>>>(a);
-  if (a.q_split.tiles) packed_fwd_join_kernel<D, FP16><<<a.q_split.tiles * (a.n / a.hp), kAttnThreads, 0, s>>>(a);
+  if (a.q_split.tiles) packed_fwd_join_kernel<D, FP16><<<4 * a.q_split.tiles * (a.n / a.hp), 64, 0, s>>>(a);
 }
 
 template <int D, bool FP16>
 static void launch_packed_bwd(const PackArgs& a, int g_q, int g_k, hipStream_t s) {
   packed_bwd_dq_kernel<D, FP16><<<g_q, kAttnThreads, 0, s>>>(a);  // first: it also writes delta
-  if (a.q_split.tiles) packed_dq_join_kernel<D, FP16><<<a.q_split.tiles * (a.n / a.hp), kAttnThreads, 0, s>>>(a);
+  if (a.q_split.tiles) packed_dq_join_kernel<D, FP16><<<4 * a.q_split.tiles * (a.n / a.hp), 64, 0, s>>>(a);
   if constexpr (D == 128)
     packed_bwd_dkdv_x128_kernel<FP16><<<g_k, 2 * kAttnThreads, 0, s>>>(a);
   else
     packed_bwd_dkdv_kernel<D, FP16><<<g_k, kAttnThreads, 0, s>>>(a);
-  if (a.k_split.tiles) packed_dkdv_join_kernel<D, FP16><<<a.k_split.tiles * a.m, 2 * kAttnThreads, 0, s>>>(a);
+  if (a.k_split.tiles) packed_dkdv_join_kernel<D, FP16><<<4 * a.k_split.tiles * a.m, 128, 0, s>>>(a);
 }
 
 extern "C" int eth_packed_attn_fwd(const eth_packed_attn_desc_t* d, const void* q, const void* k, const void* v,
