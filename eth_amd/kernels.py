@@ -476,6 +476,7 @@ def _packed_desc(packed, scale, q, k, v, *grads):
     """(descriptor, its reference, workspace bytes) of a packed attention call,
     built and checked once for these types, shapes and strides and kept with
     the plan (the addresses are the call's; the entry checks their alignment)."""
+    scale = None if scale is None else float(scale)
     key = (scale, *[x for t in (q, k, v, *grads) for x in (t.shape, t.stride(), t.dtype)])
     got = packed.descriptors.get(key)
     if got is not None:
@@ -494,7 +495,7 @@ def _packed_desc(packed, scale, q, k, v, *grads):
         raise ValueError(f"packed attention needs head_dim a multiple of 8 in [8, 128] (got {d})")
     if m < 1 or n < 1 or n % m:
         raise ValueError(f"{n} query heads cannot share {m} key and value heads")
-    c = d**-0.5 if scale is None else float(scale)
+    c = d**-0.5 if scale is None else scale
     if not 2.0**-100 <= c <= 2.0**100:
         raise ValueError(f"scale must be positive and finite (got {scale})")
     desc = nat.PackedAttnDesc()
@@ -708,6 +709,7 @@ def _token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index, shape):
     """token_logprobs_fwd with the rows in `shape` in its results, and behind
     them the operands' layout for the backward."""
     layout = index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
+    top_k, ignore_index = int(top_k), int(ignore_index)
     _check_ids(tokens, (rows,))
     if not 0 <= top_k <= min(128, V):
         raise ValueError(f"top_k must be in [0, 128] and within the vocabulary (got {top_k})")
@@ -746,7 +748,7 @@ def _token_logprobs_bwd(layout, logits2d, tokens, stats, entropy, dlogprob, dent
     index, code, rows, V, ld = layout
     dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
     if rows:
-        _launch(index, "eth_token_logprobs_bwd", logits2d.data_ptr(), ld, tokens.data_ptr(), ignore_index,
+        _launch(index, "eth_token_logprobs_bwd", logits2d.data_ptr(), ld, tokens.data_ptr(), int(ignore_index),
                 stats.data_ptr(), entropy.data_ptr(), nat.ptr(dlogprob), nat.ptr(dentropy), dz.data_ptr(), V, rows, V,
                 code)
     return dz
@@ -784,7 +786,7 @@ def _topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_fl
     stats = torch.empty(rows, 4, dtype=torch.float32, device=logits2d.device)
     if rows:
         _launch(index, "eth_topk_distill_fwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
-                teacher_logits.data_ptr(), teacher_code, k, temperature, loss.data_ptr(), stats.data_ptr(), rows, V,
+                teacher_logits.data_ptr(), teacher_code, k, float(temperature), loss.data_ptr(), stats.data_ptr(), rows, V,
                 bad_flag.data_ptr(), code)
     return loss, stats, layout
 
@@ -807,7 +809,7 @@ def _topk_distill_bwd(layout, logits2d, teacher_ids, teacher_logits, temperature
     dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
     if rows:
         _launch(index, "eth_topk_distill_bwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
-                teacher_logits.data_ptr(), teacher_code, k, temperature, stats.data_ptr(), dloss.data_ptr(),
+                teacher_logits.data_ptr(), teacher_code, k, float(temperature), stats.data_ptr(), dloss.data_ptr(),
                 dz.data_ptr(), V, rows, V, bad_flag.data_ptr(), code)
     return dz
 

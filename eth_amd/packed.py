@@ -78,7 +78,7 @@ class PackedSequences:
             lengths = lengths.tolist()
         lengths = list(lengths)
         for x in lengths:
-            if isinstance(x, bool) or not isinstance(x, (int, np.integer)) or x < 0:
+            if type(x) is not int and not isinstance(x, np.integer) or x < 0:
                 raise ValueError(f"a sequence length must be a whole number of at least 0, got {x!r}")
         self.lengths = tuple(int(x) for x in lengths)
         covered = sum(self.lengths)

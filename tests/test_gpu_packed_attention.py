@@ -70,6 +70,8 @@ CASES = [
     ([640, 70], 0, 2, 1, 128),
     ([257, 19], 3, 8, 1, 8),
     ([0, 0, 5, 0], 200, 12, 6, 120),
+    ([0, 0], 70, 4, 2, 128),  # no sequence at all
+    ([], 3, 2, 2, 64),
     ([97] * 7, 0, 12, 12, 16),
     ([1025], 7, 4, 1, 128),
     ([1100, 40], 0, 2, 2, 72),
@@ -152,6 +154,29 @@ def test_layouts_and_broadcast_heads(cuda):
     for name, g in (("out", out.view(q.shape)), ("lse", lse), ("dq", dq), ("dk", dk), ("dv", dv)):
         assert torch.equal(g, want[name]), name
     assert (grads[:, 1::2] == 7.0).all()
+
+
+def test_gradients_of_broadcast_inputs(cuda):
+    """One key/value head broadcast to all by expand, and one row of queries to
+    all rows: autograd adds up the copies' gradients."""
+    announce("packed attention broadcast inputs")
+    lengths, n, hn = [40, 33], 4, 64
+    gen = torch.Generator().manual_seed(12)
+    q, k, v = (torch.randn(*s, generator=gen).half().to(cuda).requires_grad_(True)
+               for s in ((1, n, hn), (73, 1, hn), (73, 1, hn)))
+    dout = torch.randn(73, n * hn, generator=gen).half().to(cuda)
+    packed = PackedSequences(lengths, device=cuda)
+    out = PackedCausalAttentionFn.apply(q.expand(73, n, hn), k.expand(73, n, hn), v.expand(73, n, hn), packed)
+    got = torch.autograd.grad(out, (q, k, v), dout)
+    full = [t.detach().expand(73, n, hn).contiguous() for t in (q, k, v)]
+    each = _run(*full, packed, dout)
+    assert torch.equal(out.view(73, n, hn), each["out"])
+    for g, name, dim in zip(got, ("dq", "dk", "dv"), (0, 1, 1)):
+        want = each[name].double().sum(dim, keepdim=True)
+        # (each copy's gradient is the kernel's; their sum may round in fp16 at every addition)
+        assert g.shape == want.shape
+        bound = each[name].double().abs().sum(dim, keepdim=True) * 2.0**-10 + 2.0**-20
+        assert ((g.double() - want).abs() <= bound).all(), name
 
 
 def test_given_output_and_rows_of_no_sequence(cuda):
