@@ -116,7 +116,9 @@ class PackedSequences:
         if plan is None:
             rows = nat.value("eth_packed_attn_tile_rows", heads, kv_heads)
             cus = torch.cuda.get_device_properties(self.device).multi_processor_count
-            # two query workgroups a compute unit; of dK/dV two up to a head dim of 96, one above
+            # query workgroups a compute unit: two (where a third fits, at a head dim of 64, it
+            # shares the same pipes: filling its slots too by splitting took 333 us, not 308, of
+            # 16384 rows of 8 heads on one); of dK/dV two up to a head dim of 96, one above
             q_split = split_chains(self._chains[rows], heads * rows // 128, 2 * cus)
             k_split = split_chains(self._chains["keys"] * (heads // kv_heads), kv_heads, (1 if head_dim > 96 else 2) * cus)
             plan = self._plans[heads, kv_heads, head_dim] = (*self._at[rows], *self._at["keys"], q_split, k_split)
