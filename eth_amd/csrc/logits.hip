@@ -727,7 +727,9 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(DistillArgs a)
     for (int j = 0; j < E; ++j) x[j] = gt * prob(x[j]);
     store_vec<DT, STREAM>(dz, v0 + u * kRowThreads + threadIdx.x, a.V, x);
   });
-  __syncthreads();  // the stores below come after those of the same places above
+  // the stores below come after those of the same places above, other waves' too
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __syncthreads();
   if (here) {
     int before = 0, all = 0;  // entries with this id
     for (int i = 0; i < a.k; i += 16) {  // (-1 behind the last)
