@@ -8,6 +8,7 @@ the current stream.  There is no CPU fallback: CPU tensors raise.
 import ctypes
 import functools
 import itertools
+import operator
 
 import numpy as np
 
@@ -467,7 +468,7 @@ def _thd_strides(name, t, written=False):
     sr, sh = sr if rows > 1 else heads * hn, sh if heads > 1 else hn
     if sr % 8 or sh % 8:
         raise ValueError(f"{name}: rows must be 16-byte aligned")
-    if written and (sh < hn or sr < hn):
+    if written and not (sh >= hn and sr >= (heads - 1) * sh + hn or sr >= hn and sh >= (rows - 1) * sr + hn):
         raise ValueError(f"{name}: rows that are written may not overlap")
     return sr, sh
 
@@ -709,7 +710,7 @@ def _token_logprobs_fwd(logits2d, tokens, top_k, bad_flag, ignore_index, shape):
     """token_logprobs_fwd with the rows in `shape` in its results, and behind
     them the operands' layout for the backward."""
     layout = index, code, rows, V, ld = _check_logits(logits2d, bad_flag, tokens)
-    top_k, ignore_index = int(top_k), int(ignore_index)
+    top_k, ignore_index = operator.index(top_k), operator.index(ignore_index)
     _check_ids(tokens, (rows,))
     if not 0 <= top_k <= min(128, V):
         raise ValueError(f"top_k must be in [0, 128] and within the vocabulary (got {top_k})")
@@ -748,7 +749,7 @@ def _token_logprobs_bwd(layout, logits2d, tokens, stats, entropy, dlogprob, dent
     index, code, rows, V, ld = layout
     dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
     if rows:
-        _launch(index, "eth_token_logprobs_bwd", logits2d.data_ptr(), ld, tokens.data_ptr(), int(ignore_index),
+        _launch(index, "eth_token_logprobs_bwd", logits2d.data_ptr(), ld, tokens.data_ptr(), operator.index(ignore_index),
                 stats.data_ptr(), entropy.data_ptr(), nat.ptr(dlogprob), nat.ptr(dentropy), dz.data_ptr(), V, rows, V,
                 code)
     return dz

@@ -429,10 +429,14 @@ class PackedCausalAttentionFn(torch.autograd.Function):
     (eth_amd.packed.PackedSequences) on q [rows, n, hn] and k, v [rows, m, hn]
     views -> [rows, n*hn]; n / m query heads share each key and value head.
     Rows of no sequence give zeros and get zero gradients.  scale: 1/sqrt(hn)
-    unless given."""
+    unless given.  A value that is not finite reaches the outputs of its own
+    sequence only, of the rows behind it and of those before it in the same
+    64-row block (a product of a masked zero with it is NaN); gradients of any
+    row of the sequence."""
 
     @staticmethod
     def forward(ctx, q, k, v, packed, scale=None):
+        scale = None if scale is None else float(scale)  # (a tensor's value of now)
         out, lse = K.packed_attention_fwd(q, k, v, packed, scale)
         ctx.packed, ctx.scale = packed, scale
         ctx.save_for_backward(q, k, v, out, lse)
@@ -552,7 +556,7 @@ class TopkDistillFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, teacher_ids, teacher_logits, temperature, bad_flag):
-        shape = logits.shape[:-1]
+        shape, temperature = logits.shape[:-1], float(temperature)
         if teacher_ids.shape[:-1] != shape or teacher_logits.shape != teacher_ids.shape:
             raise ValueError(f"teacher ids {tuple(teacher_ids.shape)} and logits {tuple(teacher_logits.shape)} do not "
                              f"match logits {tuple(logits.shape)}")

@@ -8,6 +8,8 @@ backward.  The lists are ordered by the length of a tile's chain, so that the
 longest start first.
 """
 
+import operator
+
 import numpy as np
 import torch
 
@@ -82,7 +84,9 @@ class PackedSequences:
                 raise ValueError(f"a sequence length must be a whole number of at least 0, got {x!r}")
         self.lengths = tuple(int(x) for x in lengths)
         covered = sum(self.lengths)
-        self.total = covered if total is None else int(total)
+        if isinstance(total, (bool, float)):
+            raise ValueError(f"total must be a whole number, got {total!r}")
+        self.total = covered if total is None else operator.index(total)
         if not covered <= self.total or not 0 < self.total < 2**31:
             raise ValueError(f"total must be at least 1, at least the {covered} rows of the sequences, and below 2^31 "
                              f"(got {self.total})")

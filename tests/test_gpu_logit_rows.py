@@ -389,3 +389,22 @@ def test_refusals(cuda):
         TokenLogprobsFn.apply(z, t[:2], 0, bad)
     with pytest.raises(ValueError):
         TopkDistillFn.apply(z, ids[:2], u[:2], 1.0, bad)
+
+
+def test_whole_numbers_and_a_temperature_tensor(cuda):
+    announce("logit rows arguments")
+    bad = _bad(cuda)
+    z = torch.randn(4, 100, device=cuda)
+    t = torch.zeros(4, dtype=torch.int64, device=cuda)
+    for changes in (dict(top_k=2.5), dict(ignore_index=0.5)):
+        with pytest.raises(TypeError):
+            K.token_logprobs_fwd(z, t, **(dict(top_k=2, bad_flag=bad) | changes))
+    ids, u = torch.arange(12, device=cuda).view(4, 3), torch.randn(4, 3, device=cuda)
+    grads = []
+    for temperature in (2.0, torch.tensor(2.0), torch.tensor(2.0, device=cuda)):
+        leaf = z.clone().requires_grad_(True)
+        loss = TopkDistillFn.apply(leaf, ids, u, temperature, bad)
+        if isinstance(temperature, torch.Tensor):
+            temperature.fill_(5.0)
+        grads.append(torch.autograd.grad(loss.sum(), leaf)[0])
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])

@@ -320,3 +320,17 @@ def test_refusals(cuda):
                     dict(dout=torch.zeros(256, 8, **bf16).t())):
         with pytest.raises(ValueError):
             bwd(**changes)
+
+
+def test_scale_of_a_tensor_is_its_value_of_the_call(cuda):
+    announce("packed attention scale from a tensor")
+    mixed, dout = _inputs(40, 4, 2, 64, torch.bfloat16, 31)
+    packed = PackedSequences([25, 15], device=cuda)
+    grads = []
+    for scale in (0.25, torch.tensor(0.25), torch.tensor(0.25, device=cuda)):
+        leaf = mixed.to(cuda).requires_grad_(True)
+        out = PackedCausalAttentionFn.apply(*_split(leaf, 4, 2), packed, scale)
+        if isinstance(scale, torch.Tensor):
+            scale.fill_(3.0)
+        grads.append(torch.autograd.grad(out, leaf, dout.to(cuda))[0])
+    assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from eth_amd import _native as nat
+from eth_amd import kernels as K
 from eth_amd import packed as pk
 from oracle.packed import packed_attention
 
@@ -173,3 +174,24 @@ def test_oracle_is_attention_of_each_sequence_alone():
         x = [t[a:b].transpose(0, 1).repeat_interleave(n // t.shape[1], 0) for t in (q, k, v)]
         want = F.scaled_dot_product_attention(*x, is_causal=True).transpose(0, 1)
         assert torch.allclose(out[a:b], want, atol=1e-12)
+
+
+@pytest.mark.parametrize("total", [7.5, 8.0, True])
+def test_total_is_a_whole_number(total):
+    with pytest.raises(ValueError, match="whole"):
+        pk.PackedSequences([1], total=total)
+
+
+@pytest.mark.parametrize("strides,fits", [
+    ((256, 64), True), ((64, 512), True), ((512, 128), True), ((64, 64), False), ((128, 64), False), ((64, 256), False),
+    ((248, 64), False), ((64, 504), False), ((64, 0), False), ((0, 64), False),
+])
+def test_written_rows_may_not_overlap(strides, fits):
+    """8 rows of 4 heads of 64: apart by rows or by heads, or refused."""
+    t = torch.zeros(8192).as_strided((8, 4, 64), (*strides, 1))
+    if fits:
+        assert K._thd_strides("dq", t, written=True) == strides
+    else:
+        with pytest.raises(ValueError, match="overlap"):
+            K._thd_strides("dq", t, written=True)
+    assert K._thd_strides("q", t) == strides
