@@ -214,6 +214,10 @@ __device__ __forceinline__ void matrix_phase(bool on) {
 }
 
 // ------------------------------------------------------------------ forward --
+// Largest sum of a lane's 32 P of a block before the maximum is taken again:
+// within fp16, whose P is rounded relative to its own size all the same
+constexpr float kMostSum = 1024.f;
+
 // 4 waves x 32 rows; a row is a (query, head) pair: hp heads of a group share
 // the workgroup's K and V blocks, 128 / hp queries each, so that a short
 // sequence wastes less of a tile and the waves' chains are of equal length.
@@ -269,8 +273,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
   a_f32x16 o[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) o[t] = a_f32x16{};
-  // running max (log2 units) and sum for query q; the lowest finite start
-  // keeps exp2(-inf - m) at 0 for masked keys
+  // exponent offset (log2 units; the running max when last taken) and sum for
+  // query q; the lowest finite start keeps exp2(-inf - m) at 0 for masked keys
   float m = -3.4028234e38f, l = 0.f;
 
   int aoff[KS], toff[DT][2];
@@ -320,41 +324,53 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
           for (int r = 0; r < 16; ++r)
             if (kv0 + t * 32 + swz_row(r, hl) > q) sc[t][r] = -INFINITY;
       }
-      float mx = sc[0][0];
+      // P at the exponent offset m of the blocks before (O / l and lse do not
+      // depend on it): only where a lane's sum says that m has fallen too far
+      // below the scores, or that there was none yet, is the maximum taken.  The
+      // softmax, not the products, fills the pipes here (at a head dim of 64 VALU
+      // 81 % busy, matrix cores 53 %): 16 of its 200 issue slots a block and the
+      // exchange between half-waves less, 16384 rows of 8 heads on one 299.4 -> 294.5
+      // us, 24 heads on three of 3000, 100 and 5000 rows 124.8 -> 117.3, 8192 rows of
+      // 16 heads of 128 81.4 -> 79.3.
+      uint32_t pk[2][8];
+      float rs = 0.f;
+      auto probs = [&]() __attribute__((always_inline)) {
+        rs = 0.f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mnew = fmaxf(m, mx * sl2);
-      // m is the exponent offset, kept within kRescaleLog2 below the running
-      // max (most blocks then skip the rescale); O / l and lse do not depend on it
-      if (__any(mnew > m + kRescaleLog2)) {
-        const float alpha = fast_exp2(m - mnew);
+          for (int i = 0; i < 8; ++i) {
+            const float p0 = fast_exp2(__builtin_fmaf(sc[t][2 * i], sl2, -m));
+            const float p1 = fast_exp2(__builtin_fmaf(sc[t][2 * i + 1], sl2, -m));
+            rs += p0;
+            rs += p1;
+            pk[t][i] = pack2<FP16>(p0, p1);
+          }
+      };
+      probs();
+      if (__any(!(rs <= kMostSum))) {
+        float mx = sc[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[t][r]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float mnew = fmaxf(m, mx * sl2), alpha = fast_exp2(m - mnew);
         l *= alpha;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[t][r] *= alpha;
         m = mnew;
+        probs();
       }
-      float rs = 0.f;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = fast_exp2(__builtin_fmaf(sc[t][r], sl2, -m));
-          sc[t][r] = p;
-          rs += p;
-        }
       l += rs;
       matrix_phase<D>(true);
       // O^T += V^T P^T over the 64 keys (4 k-steps of 16)
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
-        const int t = kk >> 1, e0 = (kk & 1) * 8;
-        const uint4 pb = make_uint4(pack2<FP16>(sc[t][e0 + 0], sc[t][e0 + 1]), pack2<FP16>(sc[t][e0 + 2], sc[t][e0 + 3]),
-                                    pack2<FP16>(sc[t][e0 + 4], sc[t][e0 + 5]), pack2<FP16>(sc[t][e0 + 6], sc[t][e0 + 7]));
+        const int t = kk >> 1, i0 = (kk & 1) * 4;
+        const uint4 pb = make_uint4(pk[t][i0], pk[t][i0 + 1], pk[t][i0 + 2], pk[t][i0 + 3]);
         const uint16_t* vp = vi + kk * 16 * D;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = mma<FP16>(img_tr(vp, toff[dt][0], toff[dt][1]), pb, o[dt]);

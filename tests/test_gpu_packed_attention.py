@@ -334,3 +334,46 @@ def test_scale_of_a_tensor_is_its_value_of_the_call(cuda):
             scale.fill_(3.0)
         grads.append(torch.autograd.grad(out, leaf, dout.to(cuda))[0])
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+@pytest.mark.parametrize("dtype", U)
+@pytest.mark.parametrize("hn", [64, 96, 128])
+def test_scores_that_rise_and_fall_along_a_sequence(cuda, dtype, hn):
+    """Whole numbers, whose products are exact: the scores of even queries rise
+    by 46 (log2 units) every 64 keys, up to 370, and those of odd ones fall, so
+    that the running maximum is taken again at every block or never.  An exponent
+    is off by one rounding, 2^-24 * 2^9, and P by 2^-15 of itself."""
+    announce(f"packed attention rising scores {dtype} hn={hn}")
+    lengths, n, m = [520, 1, 40], 4, 2
+    rows = sum(lengths)
+    gen = torch.Generator().manual_seed(hn)
+    mixed = torch.randint(-1, 2, (rows, n + 2 * m, hn), generator=gen).to(dtype)
+    at = torch.arange(rows)
+    mixed[:, :n, 0] = torch.where(at % 2 == 0, 8, -8).to(dtype)[:, None]
+    mixed[:, n : n + m, 0] = (at // 2 % 256).to(dtype)[:, None]
+    _, dout = _inputs(rows, n, m, hn, dtype, 3)
+    scale = 0.125
+    ref = packed_attention(*(t.double() for t in _split(mixed, n, m)), lengths, scale,
+                           dout.double().view(rows, n, hn), u=U[dtype])
+    got = _run(*_split(mixed.to(cuda), n, m), PackedSequences(lengths, device=cuda), dout.to(cuda), scale)
+    _check(got, ref, dtype)
+
+
+def test_a_query_of_nan_leaves_the_others(cuda):
+    """NaN scores of one query make its wave take its maxima anew each block: the
+    other rows are the clean call's but for their exponents' offsets (P rounded
+    at another power of two: a step of bf16; lse, of at most 2^4, by 2^-20 a
+    rounding)."""
+    announce("packed attention NaN query")
+    lengths, n, m, dtype = [200, 30], 4, 2, torch.bfloat16
+    mixed, _ = _inputs(230, n, m, 64, dtype, 41)
+    packed = PackedSequences(lengths, device=cuda)
+    want, want_lse = K.packed_attention_fwd(*_split(mixed.to(cuda), n, m), packed)
+    mixed[150, 1] = math.nan
+    got, lse = K.packed_attention_fwd(*_split(mixed.to(cuda), n, m), packed)
+    got, want = (t.view(230, n, 64) for t in (got, want))
+    assert got[150, 1].isnan().all() and lse[1, 150].isnan()
+    keep = torch.ones(230, n, dtype=torch.bool, device=cuda)
+    keep[150, 1] = False
+    assert torch.allclose(got[keep].float(), want[keep].float(), rtol=2.0**-7, atol=2.0**-9)
+    assert torch.allclose(lse.t()[keep], want_lse.t()[keep], rtol=0, atol=2.0**-18)
