@@ -408,3 +408,35 @@ def test_whole_numbers_and_a_temperature_tensor(cuda):
             temperature.fill_(5.0)
         grads.append(torch.autograd.grad(loss.sum(), leaf)[0])
     assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
+@pytest.mark.parametrize("top_k", [128, 127, 20, 1])
+@pytest.mark.parametrize("V", [262144, 2**21 + 3, 2**24])
+def test_alternatives_joined_from_many_parts(cuda, V, top_k):
+    """The largest logits spread over the parts of a long row in shares of every
+    size (1, 2, 4, .. of a part, all in one, one in each), among equal ones and
+    among random ones: the ids of a stable sort, and its log probabilities."""
+    announce(f"token logprobs joined V={V} k={top_k}")
+    gen = torch.Generator().manual_seed(V % 1000 + top_k)
+    z = torch.zeros(5, V)
+    z[1] = torch.randn(V, generator=gen)
+    z[2, V // 2 : V // 2 + 300] = 4.0 + torch.randn(300, generator=gen).abs()
+    z[3, :: max(1, V // 200)] += 3.0
+    at, share = 0, 64
+    while share:
+        for _ in range(max(1, 64 // share)):  # 64 in all of every share
+            z[4, at : at + share] = 5.0 + torch.randn(share, generator=gen).abs()
+            at += 32768
+            if at + 64 > V:
+                break
+        if at + 64 > V:
+            break
+        share //= 2
+    tokens, bad = torch.zeros(5, dtype=torch.int64), _bad(cuda)
+    got = K.token_logprobs_fwd(z.to(cuda), tokens.to(cuda), top_k, bad)
+    for row in range(5):
+        order = torch.sort(z[row], descending=True, stable=True).indices[:top_k]
+        assert torch.equal(got[4][row].cpu(), order), row
+        want = (z[row].double() - z[row].double().logsumexp(0))[order]
+        # fp32 sums and logs of values below 2^5
+        assert (got[3][row].cpu().double() - want).abs().max() < 2.0**-16, row
