@@ -17,7 +17,20 @@
 // read in swizzled order, so that P^T stays in registers as the operand of
 // O^T = V^T P^T; 64-row blocks go global->LDS by direct loads into XOR-swizzled
 // images a block ahead; fp32 base-2 softmax.  P and dS are rounded to the
-// inputs' type for the second product, as the matrix cores take it.
+// inputs' type for the second product, as the matrix cores take it, and delta is
+// formed of the stored output: dQ and dK are 0.0025 of their norm from 64 bits in
+// bf16 (8192 rows, heads of 128) where the rounding of the results alone is
+// 0.0017.  A further product with what the rounding of dS leaves would bring
+// about 0.0020, and take a quarter more time backward (16384 rows, 8 heads of 64 on
+// one: 982 -> 1223 us), which buys less than one bit of a gradient that is
+// rounded to 8.
+//
+// What bounds it: the exponentials and the products, which share a SIMD's issue
+// and the card's power (the clock falls to 1.6-1.8 GHz under them, where waiting
+// costs little and instructions count).  Of all SIMDs' cycles the matrix cores
+// and the VALU are busy: forward 0.54 and 0.71 at a head dim of 64, 0.48 and 0.43 at
+// 128; dQ 0.61 and 0.66, 0.50 and 0.36; dK/dV 0.50 and 0.40, 0.47 and 0.30.  LDS is at
+// 0.24-0.38 throughout, without bank conflicts; HBM is idle.
 //
 // A block's buffer resource starts at its first row and ends with its
 // sequence's last element, so that rows past the sequence read zeros without a
@@ -221,6 +234,8 @@ constexpr float kMostSum = 1024.f;
 // 4 waves x 32 rows; a row is a (query, head) pair: hp heads of a group share
 // the workgroup's K and V blocks, 128 / hp queries each, so that a short
 // sequence wastes less of a tile and the waves' chains are of equal length.
+// 16384 rows, 8 heads of 64 on one: 300 us, 0.92 PFLOP/s; 4 x 2048 rows, 16 heads of
+// 128: 80 us, 0.86; a row's 96 in three sequences 6 us.
 template <int D, bool FP16>
 __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a) {
   constexpr int KS = D / 16;  // k-steps over the head dim
@@ -327,9 +342,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
       // P at the exponent offset m of the blocks before (O / l and lse do not
       // depend on it): only where a lane's sum says that m has fallen too far
       // below the scores, or that there was none yet, is the maximum taken.  The
-      // softmax, not the products, fills the pipes here (at a head dim of 64 VALU
-      // 81 % busy, matrix cores 53 %): 16 of its 200 issue slots a block and the
-      // exchange between half-waves less, 16384 rows of 8 heads on one 299.4 -> 294.5
+      // VALU has the most to do here (at a head dim of 64 it was busy 0.81 of the
+      // cycles with the maximum, 0.71 without): 16384 rows of 8 heads on one 299.4 -> 294.5
       // us, 24 heads on three of 3000, 100 and 5000 rows 124.8 -> 117.3, 8192 rows of
       // 16 heads of 128 81.4 -> 79.3.
       uint32_t pk[2][8];
@@ -433,7 +447,10 @@ __global__ void __launch_bounds__(64) packed_fwd_join_kernel(PackArgs a) {
 
 // ------------------------------------------------------------ backward: dQ --
 // Workgroups as in the forward.  Runs first: it also writes delta, which the
-// dK/dV kernels read.
+// dK/dV kernels read.  S is formed again here and there: seven products for the
+// five that a single pass would take, whose dQ however would be summed by atomics
+// in no fixed order.  410 us at 16384 rows, 8 heads of 64 on one; 98 us at 8192
+// packed rows, 16 heads of 128 on four.
 template <int D, bool FP16>
 __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs a) {
   constexpr int KS = D / 16, DT = D / 32;
@@ -617,7 +634,10 @@ struct PackStep {
 
 // ------------------------------------- backward: dK, dV, head dims to 96 --
 // dK and dV of 32 keys in one wave, four waves per 128 keys, one barrier per
-// 64 queries (see attn_bwd_dkdv_kernel).
+// 64 queries (see attn_bwd_dkdv_kernel).  600 us at 16384 rows, 8 heads of 64 on
+// one.  Slower here: three workgroups a compute unit, at 29 spilled registers
+// (982 -> 1129 us backward); both 32-query tiles of a step in one straight line
+// (982 -> 981, 254 -> 256).
 template <int D, bool FP16>
 __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackArgs a) {
   static_assert(D == 64 || D == 96, "wider heads run on the paired kernel");
@@ -810,7 +830,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
 // attn_bwd_dkdv_x128_kernel): in step j the dV wave computes S(j) and P(j),
 // hands P (fp32) over through LDS and adds P(j)^T dO(j) into dV, while the dK
 // wave first finishes step j-1 and then computes dP(j) - delta.  Three Q
-// images, two dO images and two P buffers (145 KB of LDS).
+// images, two dO images and two P buffers (145 KB of LDS).  165 us at 8192 packed
+// rows, 16 heads of 128 on four.
 template <bool FP16>
 __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kernel(PackArgs a) {
   constexpr int D = 128, KS = D / 16, DT = D / 32;
