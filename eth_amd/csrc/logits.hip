@@ -346,10 +346,10 @@ __device__ __forceinline__ int logp_rank(const uint64_t* cand, int count, uint64
 // loads in flight per thread, each logit read once.
 //
 // Top alternatives: every thread keeps the order (16 bits, rounded down) of
-// each of its vectors' maxima.  Of 256 maxima of the threads' (of a thread or a pair of them) the k-th
-// largest is a lower bound of the row's k-th largest, and only about k + k^2 /
-// 512 logits reach it: the few vectors with one are listed in LDS, read again an
-// element per thread, and the candidates among them sorted by counting.  Where
+// each of its vectors' maxima.  Of 256 maxima, each of a thread or of a pair of
+// them, the k-th largest is a lower bound of the row's k-th largest, and only
+// about k + k^2 / 512 logits reach it: the few vectors with one are listed in LDS,
+// read again an element per thread, and the candidates sorted by counting.  Where
 // more reach it than the sort takes (equal logits, a row of few finite ones) or
 // the row holds a NaN, the k-th key is found bit by bit.  HBM bounds it without
 // alternatives ([4096, 50304] bf16 77 us, 5.3 TB/s); listing and sorting them, for

@@ -11,6 +11,7 @@ by L + |logp| 2^-22, the entropy by L + a (2^-15 + ...) < L + (1 + a) 2^-14.
 Gradients add one rounding of half a step of the logits' type."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -440,3 +441,32 @@ def test_alternatives_joined_from_many_parts(cuda, V, top_k):
         want = (z[row].double() - z[row].double().logsumexp(0))[order]
         # fp32 sums and logs of values below 2^5
         assert (got[3][row].cpu().double() - want).abs().max() < 2.0**-16, row
+
+
+def test_threads_do_not_share_workspaces(cuda):
+    """Three threads with a stream each on rows of several parts."""
+    announce("logit rows threads")
+    bad = _bad(cuda)
+    zs = [torch.randn(6, 140000, generator=torch.Generator().manual_seed(i)).half().to(cuda) for i in range(3)]
+    t = torch.arange(6, device=cuda)
+    want = [K.token_logprobs_fwd(z, t, 40, bad) for z in zs]
+    torch.cuda.synchronize()
+    got, errors = [None] * 3, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(cuda)):
+                for _ in range(10):
+                    got[i] = K.token_logprobs_fwd(zs[i], t, 40, bad)
+                torch.cuda.current_stream(cuda).synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not errors, errors
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(g, w))

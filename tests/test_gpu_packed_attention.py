@@ -9,6 +9,7 @@ most, which changes P, and all that follows, by the same share: an eighth of u
 in bf16, and as much as half of u in fp16, whose bound is doubled for it."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -377,3 +378,92 @@ def test_a_query_of_nan_leaves_the_others(cuda):
     keep[150, 1] = False
     assert torch.allclose(got[keep].float(), want[keep].float(), rtol=2.0**-7, atol=2.0**-9)
     assert torch.allclose(lse.t()[keep], want_lse.t()[keep], rtol=0, atol=2.0**-18)
+
+
+@pytest.mark.parametrize("n,m,hn", [(4, 1, 64), (2, 2, 128)])
+def test_very_many_sequences_of_one_row(cuda, n, m, hn):
+    """A sequence of one row has P = 1: out is v, dq and dk are zero but for
+    delta's rounding (dP - delta: the same products, summed in another order),
+    dv the sum of dout over the group."""
+    announce(f"packed attention 70000 sequences n={n} m={m} hn={hn}")
+    rows, dtype = 70000, torch.bfloat16
+    mixed, dout = _inputs(rows, n, m, hn, dtype, 51)
+    # small whole numbers: every sum is exact
+    dout = torch.randint(-2, 3, dout.shape, generator=torch.Generator().manual_seed(1)).to(dtype)
+    mixed[:, n + m :] = torch.randint(-2, 3, (rows, m, hn), generator=torch.Generator().manual_seed(2)).to(dtype)
+    q, k, v = (t.contiguous().to(cuda) for t in _split(mixed, n, m))
+    got = _run(q, k, v, PackedSequences([1] * rows, device=cuda), dout.to(cuda))
+    do = dout.to(cuda).view(rows, n, hn)
+    assert torch.equal(got["out"], v.repeat_interleave(n // m, 1))
+    assert torch.equal(got["dv"], do.view(rows, m, n // m, hn).sum(2))
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+
+
+def test_threads_share_a_plan(cuda):
+    """Four threads with a stream each, forward and backward through one plan,
+    its descriptors and splits made by whichever comes first."""
+    announce("packed attention threads")
+    lengths, n, m, hn, dtype = [1700, 33], 2, 1, 64, torch.bfloat16
+    mixed, dout = _inputs(1733, n, m, hn, dtype, 61)
+    args = [t.contiguous().to(cuda) for t in _split(mixed, n, m)]
+    dout = dout.to(cuda)
+    want = _run(*args, PackedSequences(lengths, device=cuda), dout)
+    packed = PackedSequences(lengths, device=cuda)
+    torch.cuda.synchronize()
+    results, errors = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(cuda)):
+                for _ in range(5):
+                    leaves = [t.clone().requires_grad_(True) for t in args]
+                    out = PackedCausalAttentionFn.apply(*leaves, packed)
+                    grads = torch.autograd.grad(out, leaves, dout)
+                torch.cuda.current_stream(cuda).synchronize()
+                results[i] = out.detach(), *grads
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for r in results:
+        for g, name in zip(r, ("out", "dq", "dk", "dv")):
+            assert torch.equal(g.view_as(want[name]), want[name]), name
+
+
+def test_two_graphs_of_split_chains_replayed_in_turn(cuda):
+    """Two captured training steps whose chains are split, their workspaces in
+    one memory pool, replayed in turn on new inputs with eager calls between."""
+    announce("packed attention two graphs, split chains")
+    n, m, hn, dtype = 2, 1, 64, torch.bfloat16
+    rows = 1733
+    plans = [PackedSequences(x, device=cuda) for x in ([1700, 33], [20, 1713])]
+    sets = [tuple(t.to(cuda) for t in _inputs(rows, n, m, hn, dtype, seed)) for seed in (71, 72, 73)]
+    want = [[_run(*_split(x, n, m), p, do) for x, do in sets] for p in plans]
+    buffers = [tuple(t.clone() for t in sets[0]) for _ in plans]
+    graphs, held, pool = [], [], None
+    for p, (x, do) in zip(plans, buffers):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _run(*_split(x, n, m), p, do)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            held.append(_run(*_split(x, n, m), p, do))
+        pool = g.pool()
+        graphs.append(g)
+    for i in (0, 1, 2, 0):
+        for g, h, w, (x, do), p in zip(graphs, held, want, buffers, plans):
+            x.copy_(sets[i][0])
+            do.copy_(sets[i][1])
+            g.replay()
+            eager = _run(*_split(sets[i - 1][0], n, m), p, sets[i - 1][1])
+            torch.cuda.synchronize()
+            for name in ("out", "lse", "dq", "dk", "dv"):
+                assert torch.equal(h[name], w[i][name]), name
+                assert torch.equal(eager[name], w[i - 1][name]), name
