@@ -19,7 +19,7 @@ KEY_TILE_ROWS = 128  # keys per workgroup of the dK/dV kernels
 QUERY_TILE_ROWS = (32, 64, 128)  # queries per workgroup, by the heads that share one
 BLOCK_ROWS = 64  # keys (queries) of a step of a query (key) tile
 MIN_PIECE = 8  # steps of a split tile's piece, at least
-GOOD_PIECE = 28  # and where the work is enough to fill the slots
+GOOD_PIECE = 28  # and where the work fills the slots several times over
 WORTH_SPLITTING = 12  # steps that a split has to save
 
 
@@ -50,19 +50,21 @@ def split_chains(chain, heads, slots):
 
     The list ends no earlier than its longest chain, nor than its steps spread
     over the slots.  Where the first is well above the second, chains are cut:
-    into pieces of the second, or where that is long into smaller ones, which
-    fill the slots more evenly until their partial sums cost more.  Backward of
-    16384 rows, 8 heads of 64 on one, 258 steps a slot (us): uncut 3006, pieces
-    of 258 1198, 129 1072, 86 1018, 65 1012, 43 1021; of 8192 packed rows, 16
-    heads of 128 on four, 53 steps a slot: 295, 53 254, 27 248, 18 268; of 8
-    sequences of 1024, the same heads, 36 steps: 185, 36 183, 18 188."""
+    into pieces of half as much again as the second, whose partial sums cost less
+    than its own would, or where that is long into smaller ones, which fill the
+    slots more evenly until their partial sums cost more.  Backward of 16384 rows,
+    8 heads of 64 on one, 258 steps a slot (us): uncut 3006, pieces of 258 1198, 129
+    1072, 86 1018, 65 1012, 43 1021; of 8192 packed rows, 16 heads of 128 on four, 53
+    steps a slot: 295, 53 254, 27 248, 18 268; of 8192 rows of one head of 128, 9 and
+    17 steps a slot, pieces of 9 and 17 145, of 13 and 25 112; of 3 x 1311 rows, 32
+    heads of 80 on eight, 23 steps, pieces of 23 195, of 28 170."""
     if not chain.size:
         return 0, 0, 0
-    share = max(MIN_PIECE, -(-int(chain.sum()) * heads // slots))
+    share = -(-int(chain.sum()) * heads // slots)
+    steps = max(MIN_PIECE, min(share * 3 // 2, max(GOOD_PIECE, share * 2 // 7)))
     longest = int(chain[0])
-    if longest < share + WORTH_SPLITTING:
+    if longest < max(share, steps) + WORTH_SPLITTING:
         return 0, 0, 0
-    steps = min(share, max(GOOD_PIECE, share * 2 // 7))
     return int(np.searchsorted(-chain, -steps, side="left")), -(-longest // steps), steps
 
 

@@ -52,12 +52,14 @@ def test_split_chains():
         tiles, pieces, steps = pk.split_chains(chain, heads, slots)
         if tiles:
             assert (chain[:tiles] > steps).all() and (chain[tiles:] <= steps).all()
-            assert pieces > 1 and pieces * steps >= chain[0] and chain[0] >= steps + pk.WORTH_SPLITTING
             share = -(-chain.sum() * heads // slots)
-            assert pk.MIN_PIECE <= steps <= max(share, pk.MIN_PIECE)
+            assert pieces > 1 and pieces * steps >= chain[0]
+            assert chain[0] >= max(steps, share) + pk.WORTH_SPLITTING
+            assert pk.MIN_PIECE <= steps <= max(share * 1.5, pk.MIN_PIECE)
             assert steps >= min(share, pk.GOOD_PIECE)
         else:
-            assert chain[0] < max(pk.MIN_PIECE, -(-chain.sum() * heads // slots)) + pk.WORTH_SPLITTING
+            share = -(-chain.sum() * heads // slots)
+            assert chain[0] < max(pk.MIN_PIECE, share, min(share * 1.5, pk.GOOD_PIECE)) + pk.WORTH_SPLITTING
 
 
 @pytest.mark.parametrize("lengths,total", [
