@@ -245,7 +245,7 @@ constexpr float kMostSum = 1024.f;
 // the workgroup's K and V blocks, 128 / hp queries each, so that a short
 // sequence wastes less of a tile and the waves' chains are of equal length.
 // 16384 rows, 8 heads of 64 on one: 300 us, 0.92 PFLOP/s; 4 x 2048 rows, 16 heads of
-// 128: 80 us, 0.86; a row's 96 in three sequences 6 us.
+// 128: 77.6 us, 0.89; 96 rows in three sequences 6 us.
 template <int D, bool FP16>
 __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a) {
   constexpr int KS = D / 16;  // k-steps over the head dim
@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(64) packed_fwd_join_kernel(PackArgs a) {
 // Workgroups as in the forward.  Runs first: it also writes delta, which the
 // dK/dV kernels read.  S is formed again here and there: seven products for the
 // five that a single pass would take, whose dQ however would be summed by atomics
-// in no fixed order.  410 us at 16384 rows, 8 heads of 64 on one; 98 us at 8192
+// in no fixed order.  410 us at 16384 rows, 8 heads of 64 on one; 94 us at 8192
 // packed rows, 16 heads of 128 on four.
 template <int D, bool FP16>
 __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs a) {
