@@ -536,7 +536,8 @@ def packed_attention_fwd(q, k, v, packed, scale=None, out=None):
     """Causal attention over `packed` (PackedSequences) of q [rows, n, hn] and
     k, v [rows, m, hn] views with any row and head strides; query head h reads
     key/value head h // (n // m).  Returns (out [rows, n*hn], lse [n, rows],
-    log2 domain); rows of no sequence get zeros (lse -inf)."""
+    log2 domain); rows of no sequence get zeros (lse -inf).  A given `out` shares
+    no memory with q, k and v."""
     _check_device(packed.device.index, q, k, v)
     _, ref, size = _packed_desc(packed, scale, q, k, v)
     rows, n, d = q.shape
