@@ -109,7 +109,7 @@ SIGNATURES["eth_packed_attn_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
 
 SIGNATURES["eth_token_logprobs_fwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I32, _P, _I64, _I64, _P, _I32, _P]
 SIGNATURES["eth_token_logprobs_bwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _P]
-SIGNATURES["eth_topk_distill_fwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _I64, _I64, _P, _I32, _P]
+SIGNATURES["eth_topk_distill_fwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _I64, _P, _I32, _P]
 SIGNATURES["eth_topk_distill_bwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _P]
 
 
@@ -171,6 +171,7 @@ VALUE_SIGNATURES = {
     "eth_gemm_splitk_pays": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32], _I64),
     "eth_embedding_bwd_workspace": ([_I64, _I64], _I64),
     "eth_token_logprobs_workspace": ([_I64, _I64, _I32, _I32], _I64),
+    "eth_topk_distill_workspace": ([_I64, _I64, _I32], _I64),
     "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
     "eth_packed_attn_workspace": ([_P, _I32], _I64),
 }

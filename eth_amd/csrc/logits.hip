@@ -618,6 +618,8 @@ struct DistillArgs {
   void* dz;
   int64_t ldd;
   int chunks;  // backward: workgroups per row
+  int parts, part;    // forward: workgroups per row, elements of each
+  float2* part_stat;  // [rows, parts]: max, sum of exp((z - max) / tau)
 };
 
 // entry i of a row's teacher: its id, -1 where there is none
@@ -631,48 +633,89 @@ __device__ __forceinline__ float teacher_logit(const DistillArgs& a, int64_t row
   return load_elem(a.teacher, row * a.k + i, a.teacher_dtype);
 }
 
-// One workgroup per row: the row's statistics at the temperature, each thread
-// over its own vectors, eight in flight.  Every wave looks the ids over (a row
-// without entries is not read); the first one weighs the entries, four a lane,
-// while the others read, and joins it all behind the one barrier.  HBM bounds it
-// ([4096, 50304] bf16, 64 entries: 73 us, 5.6 TB/s), and for few rows the time that
-// one workgroup takes to read one (20 us for 262144 logits).
-template <int DT, int NT>
-__global__ void __launch_bounds__(NT) distill_fwd_kernel(DistillArgs a) {
-  typedef typename Lg<DT>::T T;
-  constexpr int E = Lg<DT>::E, PL = kDistillTop / 64;
-  __shared__ float red[2 * NT / 64];
-  const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x & 63;
-  const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
-  int id[PL];
+// A lane's entries of a row: entry lane + 64 e of its teacher, for one wave (id),
+// and the teacher's logits and the student's for them (u, zu).
+constexpr int kDistillLane = kDistillTop / 64;
+struct DistillEntries {
+  int id[kDistillLane];
+  float u[kDistillLane], zu[kDistillLane];
+};
+// whether the row has entries; a row without gets its results here
+__device__ __forceinline__ bool distill_ids(const DistillArgs& a, int64_t row, int lane, DistillEntries& t) {
   bool any = false;
 #pragma unroll
-  for (int e = 0; e < PL; ++e) {
-    id[e] = teacher_id(a, row, lane + 64 * e);
-    any |= id[e] >= 0;
+  for (int e = 0; e < kDistillLane; ++e) {
+    t.id[e] = teacher_id(a, row, lane + 64 * e);
+    any |= t.id[e] >= 0;
   }
-  if (!__any(any)) {
-    if (threadIdx.x == 0) {
-      a.loss[row] = 0.f;
-      a.stats[row] = make_float4(0.f, -INFINITY, 0.f, 0.f);
-    }
-    return;
+  if (__any(any)) return true;
+  if (threadIdx.x == 0) {  // (every part of it stores the same)
+    a.loss[row] = 0.f;
+    a.stats[row] = make_float4(0.f, -INFINITY, 0.f, 0.f);
   }
-  float u[PL], zu[PL];  // the teacher's logits and the student's for them
-  if (threadIdx.x < 64) {
+  return false;
+}
+template <int DT>
+__device__ __forceinline__ void distill_logits(const DistillArgs& a, int64_t row, int lane, DistillEntries& t) {
+  const typename Lg<DT>::T* z = reinterpret_cast<const typename Lg<DT>::T*>(a.z) + row * a.ld;
 #pragma unroll
-    for (int e = 0; e < PL; ++e) {
-      u[e] = id[e] >= 0 ? teacher_logit(a, row, lane + 64 * e) : -INFINITY;
-      zu[e] = id[e] >= 0 ? Lg<DT>::one(z[id[e]]) : 0.f;
-    }
+  for (int e = 0; e < kDistillLane; ++e) {
+    t.u[e] = t.id[e] >= 0 ? teacher_logit(a, row, lane + 64 * e) : -INFINITY;
+    t.zu[e] = t.id[e] >= 0 ? Lg<DT>::one(z[t.id[e]]) : 0.f;
   }
+}
+// a row's results from its maximum M and sum S of exp((z - M) / tau) (one wave)
+__device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, int lane, const DistillEntries& t, float M,
+                                            float S) {
+  const bool none = S == 0.f;  // no finite logit: no probability for any entry
+  const float ls = none ? -INFINITY : logf(S);
+  float um = kLowest, total = 0.f, loss = 0.f;
+#pragma unroll
+  for (int e = 0; e < kDistillLane; ++e) um = fmaxf(um, t.u[e]);
+  um = wave_max(um);
+  // (a teacher logit of NaN or +inf makes every q NaN, as the softmax does)
+#pragma unroll
+  for (int e = 0; e < kDistillLane; ++e) total += t.id[e] >= 0 ? exp_f((t.u[e] - um) / a.tau) : 0.f;
+  total = wave_sum(total);
+#pragma unroll
+  for (int e = 0; e < kDistillLane; ++e) {
+    const float q = t.id[e] >= 0 ? exp_f((t.u[e] - um) / a.tau) / total : 0.f;
+    const float lp = none ? -INFINITY : (t.zu[e] - M) / a.tau - ls;
+    if (!(q == 0.f)) loss += q * (logf(q) - lp);
+  }
+  loss = wave_sum(loss);
+  if (lane == 0) {
+    a.loss[row] = total == 0.f ? 0.f : loss * a.tau * a.tau;
+    a.stats[row] = make_float4(M, ls, um, total);
+  }
+}
+
+// One workgroup per row, or where rows are few and long per part of one: its
+// statistics at the temperature, each thread over its own vectors, eight in
+// flight.  Every wave looks the ids over (a row without entries is not read); of a
+// whole row the first one weighs the entries, four a lane, while the others read,
+// and joins it all behind the one barrier.  HBM bounds it ([4096, 50304] bf16, 64
+// entries: 73 us, 5.6 TB/s), and for few rows the time that one workgroup takes to
+// read its share.
+template <int DT, int NT, bool PARTS>
+__global__ void __launch_bounds__(NT) distill_fwd_kernel(DistillArgs a) {
+  typedef typename Lg<DT>::T T;
+  constexpr int E = Lg<DT>::E;
+  __shared__ float red[2 * NT / 64];
+  const int64_t row = PARTS ? blockIdx.x / a.parts : blockIdx.x;
+  const int first = PARTS ? blockIdx.x % a.parts * a.part : 0, n = PARTS ? min(a.V - first, a.part) : a.V;
+  const int lane = threadIdx.x & 63;
+  const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld + first;
+  DistillEntries t;
+  if (!distill_ids(a, row, lane, t)) return;
+  if constexpr (!PARTS)
+    if (threadIdx.x < 64) distill_logits<DT>(a, row, lane, t);
   const float c = kLog2e / a.tau;
   float m = kLowest, s = 0.f;
-  const int nv = (a.V + E - 1) / E;
+  const int nv = (n + E - 1) / E;
   for (int v0 = 0; v0 < nv; v0 += NT * kDistillVecs) {
     lg_u32x4 v[places_of(kDistillVecs)];
-    const int places = load_vecs<DT, kDistillVecs, NT>(v, z, v0, a.V);
+    const int places = load_vecs<DT, kDistillVecs, NT>(v, z, v0, n);
     float mx = m;
     each_place<kDistillVecs>([&](auto u) __attribute__((always_inline)) {
       if (u < places) {
@@ -706,27 +749,32 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(DistillArgs a) {
   for (int w = 1; w < NT / 64; ++w) M = fmaxf(M, red[w]);
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) S += red[NT / 64 + w] * __builtin_amdgcn_exp2f((red[w] - M) * c);
-  const bool none = S == 0.f;  // no finite logit: no probability for any entry
-  const float ls = none ? -INFINITY : logf(S);
-  float um = kLowest, total = 0.f, loss = 0.f;
-#pragma unroll
-  for (int e = 0; e < PL; ++e) um = fmaxf(um, u[e]);
-  um = wave_max(um);
-  // (a teacher logit of NaN or +inf makes every q NaN, as the softmax does)
-#pragma unroll
-  for (int e = 0; e < PL; ++e) total += id[e] >= 0 ? exp_f((u[e] - um) / a.tau) : 0.f;
-  total = wave_sum(total);
-#pragma unroll
-  for (int e = 0; e < PL; ++e) {
-    const float q = id[e] >= 0 ? exp_f((u[e] - um) / a.tau) / total : 0.f;
-    const float lp = none ? -INFINITY : (zu[e] - M) / a.tau - ls;
-    if (!(q == 0.f)) loss += q * (logf(q) - lp);
+  if constexpr (PARTS) {
+    if (lane == 0) a.part_stat[blockIdx.x] = make_float2(M, S);
+  } else {
+    distill_row(a, row, lane, t, M, S);
   }
-  loss = wave_sum(loss);
-  if (lane == 0) {
-    a.loss[row] = total == 0.f ? 0.f : loss * a.tau * a.tau;
-    a.stats[row] = make_float4(M, ls, um, total);
+}
+
+// joins the parts of a row, one wave
+template <int DT>
+__global__ void __launch_bounds__(64) distill_join_kernel(DistillArgs a) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  DistillEntries t;
+  if (!distill_ids(a, row, lane, t)) return;
+  distill_logits<DT>(a, row, lane, t);
+  const float c = kLog2e / a.tau;
+  const float2* ps = a.part_stat + row * a.parts;
+  float m = kLowest, s = 0.f;
+  for (int i = lane; i < a.parts; i += 64) {
+    const float2 p = ps[i];
+    const float mx = fmaxf(m, p.x);
+    s = s * __builtin_amdgcn_exp2f((m - mx) * c) + p.y * __builtin_amdgcn_exp2f((p.x - mx) * c);
+    m = mx;
   }
+  const float M = wave_max(m);
+  distill_row(a, row, lane, t, M, wave_sum(s * __builtin_amdgcn_exp2f((m - M) * c)));
 }
 
 // A workgroup per 1024 vectors of a row: dz = g tau p, then the entries
@@ -955,19 +1003,40 @@ static DistillArgs distill_args(const void* logits, int64_t ld, const int64_t* i
   return a;
 }
 
+// Parts that a row's forward is cut into: rows of four trips of a workgroup and
+// more, into four parts and more, up to the two workgroups a compute unit that many
+// rows fill by themselves ([4, 262144] fp16 20.4 us in one part each, 5.3 + 3.2 in
+// eight with the join; [64, 262144] bf16 21.9, 7.2 + 4.0; [1, 2^24] fp32 1261, 13.4 +
+// 5.0; [200, 262144] in two 24.0 + 4.0, which is no gain).
+static int64_t distill_parts(int64_t rows, int64_t V, int dtype) {
+  const int64_t trip = (int64_t)kDistillThreads * kDistillVecs * (16 / dtype_size(dtype));
+  const int64_t trips = (V + trip - 1) / trip, most = 512 / rows;
+  return trips < 4 || most < 4 ? 1 : trips < most ? trips : most;
+}
+extern "C" int64_t eth_topk_distill_workspace(int64_t rows, int64_t vocab, int dtype) {
+  if (!valid_dtype(dtype) || rows <= 0 || vocab <= 0 || vocab > kMostVocab) return 0;
+  const int64_t parts = distill_parts(rows, vocab, dtype);
+  return parts == 1 ? 0 : rows * parts * (int64_t)sizeof(float2);
+}
+
 // (256 threads for short rows as above: [8192, 8000] bf16 40 -> 27 us; [4096,
 // 32000] 46.4 us with 512, 48.9 with 256)
 template <int DT>
-static void launch_distill_fwd(const DistillArgs& a, int rows, hipStream_t s) {
-  if (a.V <= 256 * kDistillVecs * Lg<DT>::E)
-    distill_fwd_kernel<DT, 256><<<rows, 256, 0, s>>>(a);
-  else
-    distill_fwd_kernel<DT, kDistillThreads><<<rows, kDistillThreads, 0, s>>>(a);
+static void launch_distill_fwd(DistillArgs a, int rows, hipStream_t s) {
+  if (a.parts > 1) {
+    distill_fwd_kernel<DT, kDistillThreads, true><<<rows * a.parts, kDistillThreads, 0, s>>>(a);
+    distill_join_kernel<DT><<<rows, 64, 0, s>>>(a);
+  } else if (a.V <= 256 * kDistillVecs * Lg<DT>::E) {
+    distill_fwd_kernel<DT, 256, false><<<rows, 256, 0, s>>>(a);
+  } else {
+    distill_fwd_kernel<DT, kDistillThreads, false><<<rows, kDistillThreads, 0, s>>>(a);
+  }
 }
 
 extern "C" int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_t* teacher_ids, const void* teacher,
                                     int teacher_dtype, int k, float temperature, float* loss, float* stats,
-                                    int64_t rows, int64_t vocab, int* bad_index, int dtype, void* stream) {
+                                    void* workspace, int64_t rows, int64_t vocab, int* bad_index, int dtype,
+                                    void* stream) {
   if (int rc = distill_check("eth_topk_distill_fwd", logits, ld, teacher_ids, teacher, teacher_dtype, k, temperature,
                              stats, rows, vocab, bad_index, dtype))
     return rc;
@@ -975,6 +1044,12 @@ extern "C" int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_
   DistillArgs a = distill_args(logits, ld, teacher_ids, teacher, teacher_dtype, k, temperature, stats, vocab,
                                bad_index);
   a.loss = loss;
+  a.parts = (int)distill_parts(rows, vocab, dtype);
+  ETH_CHECK_ARG(a.parts == 1 || (workspace && ((uintptr_t)workspace & 7) == 0),
+                "eth_topk_distill_fwd: so few rows of this vocabulary need an 8-byte aligned workspace");
+  const int64_t E = 16 / dtype_size(dtype), vecs = (vocab + E - 1) / E;
+  a.part = (int)((vecs + a.parts - 1) / a.parts * E);
+  a.part_stat = (float2*)workspace;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == ETH_BF16)
     launch_distill_fwd<ETH_BF16>(a, (int)rows, s);

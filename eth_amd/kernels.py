@@ -787,9 +787,11 @@ def _topk_distill_fwd(logits2d, teacher_ids, teacher_logits, temperature, bad_fl
     loss = torch.empty(shape, dtype=torch.float32, device=logits2d.device)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=logits2d.device)
     if rows:
+        ws = nat.value("eth_topk_distill_workspace", rows, V, code)
+        ws = torch.empty(ws, dtype=torch.uint8, device=logits2d.device) if ws else None
         _launch(index, "eth_topk_distill_fwd", logits2d.data_ptr(), ld, teacher_ids.data_ptr(),
-                teacher_logits.data_ptr(), teacher_code, k, float(temperature), loss.data_ptr(), stats.data_ptr(), rows, V,
-                bad_flag.data_ptr(), code)
+                teacher_logits.data_ptr(), teacher_code, k, float(temperature), loss.data_ptr(), stats.data_ptr(),
+                nat.ptr(ws), rows, V, bad_flag.data_ptr(), code)
     return loss, stats, layout
 
 

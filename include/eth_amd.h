@@ -540,13 +540,15 @@ int eth_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* tokens
  * vocab is none and sets *bad_index to 1; an id may appear more than once.  A row
  * without entries has loss 0 and gets no gradient.  stats [rows, 4] (16-byte
  * aligned), for the backward: the row's maximum and log sum exp((z - max) /
- * temperature), the teacher's maximum and sum exp((u - max) / temperature).  The
- * backward writes
+ * temperature), the teacher's maximum and sum exp((u - max) / temperature).
+ * `workspace`: eth_topk_distill_workspace bytes, 8-byte aligned (0, NULL, but for
+ * few rows of a large vocabulary).  The backward writes
  *   dlogits_j = dloss temperature (p_j - sum of q over the entries with id j). */
+int64_t eth_topk_distill_workspace(int64_t rows, int64_t vocab, int dtype);
 int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_t* teacher_ids,
                          const void* teacher, int teacher_dtype, int k, float temperature,
-                         float* loss, float* stats, int64_t rows, int64_t vocab, int* bad_index,
-                         int dtype, void* stream);
+                         float* loss, float* stats, void* workspace, int64_t rows, int64_t vocab,
+                         int* bad_index, int dtype, void* stream);
 int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_ids,
                          const void* teacher, int teacher_dtype, int k, float temperature,
                          const float* stats, const float* dloss, void* dlogits, int64_t ldd,

@@ -175,7 +175,7 @@ def test_token_logprobs_ignored_and_out_of_range(cuda):
 @pytest.mark.parametrize("rows,V,k,tau,teacher,pad", [
     (1, 1, 1, 1.0, torch.float32, 0), (3, 7, 7, 0.5, torch.float32, 1), (2, 130, 20, 2.0, torch.bfloat16, 0),
     (3, 4099, 64, 1.0, torch.float16, 5), (2, 50257, 256, 4.0, torch.float32, 47), (1, 50304, 8, 1.0, torch.float32, 0),
-    (2, 70001, 100, 0.7, torch.float32, 0),
+    (2, 70001, 100, 0.7, torch.float32, 0), (3, 98305, 20, 1.0, torch.float32, 3), (1, 2**20 + 5, 256, 2.0, torch.bfloat16, 0),
 ])
 def test_topk_distill(cuda, dtype, rows, V, k, tau, teacher, pad):
     announce(f"distill {dtype} rows={rows} V={V} k={k} tau={tau} {teacher}")
@@ -204,7 +204,7 @@ def _distill_case(cuda, zd, z, ids, u, tau, dloss, bad_expected=0):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("V", [50, 9001])
+@pytest.mark.parametrize("V", [50, 9001, 100003])
 def test_topk_distill_special_rows(cuda, dtype, V):
     """Rows without entries, with absent, repeated and masked ones, masked
     students, equal logits, a mask of the lowest value."""

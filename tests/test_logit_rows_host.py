@@ -14,8 +14,8 @@ LOGP = dict(logits=P, ld=100, tokens=P, ignore=-100, logprob=P, entropy=P, stats
             vocab=100, bad=P, dtype=nat.ETH_BF16, stream=None)
 LOGP_BWD = dict(logits=P, ld=100, tokens=P, ignore=-100, stats=P, entropy=P, dlogprob=P, dentropy=P, dz=P, ldd=100,
                 rows=4, vocab=100, dtype=nat.ETH_BF16, stream=None)
-DISTILL = dict(logits=P, ld=100, ids=P, teacher=P, teacher_dtype=nat.ETH_F32, k=8, tau=1.0, loss=P, stats=P, rows=4,
-               vocab=100, bad=P, dtype=nat.ETH_BF16, stream=None)
+DISTILL = dict(logits=P, ld=100, ids=P, teacher=P, teacher_dtype=nat.ETH_F32, k=8, tau=1.0, loss=P, stats=P, ws=None,
+               rows=4, vocab=100, bad=P, dtype=nat.ETH_BF16, stream=None)
 DISTILL_BWD = dict(logits=P, ld=100, ids=P, teacher=P, teacher_dtype=nat.ETH_F32, k=8, tau=1.0, stats=P, dloss=P, dz=P,
                    ldd=100, rows=4, vocab=100, bad=P, dtype=nat.ETH_BF16, stream=None)
 
@@ -32,7 +32,8 @@ DISTILL_BWD = dict(logits=P, ld=100, ids=P, teacher=P, teacher_dtype=nat.ETH_F32
     ("eth_topk_distill_fwd", DISTILL, [
         dict(dtype=3), dict(teacher_dtype=3), dict(ld=99), dict(rows=0), dict(k=0), dict(k=257), dict(tau=0.0),
         dict(tau=-1.0), dict(tau=math.nan), dict(tau=math.inf), dict(ids=None), dict(teacher=None), dict(loss=None),
-        dict(stats=None), dict(bad=None), dict(teacher=P + 2), dict(rows=2**31)]),
+        dict(stats=None), dict(bad=None), dict(teacher=P + 2), dict(rows=2**31), dict(vocab=2**18, ld=2**18),
+        dict(vocab=2**18, ld=2**18, ws=P + 4)]),
     ("eth_topk_distill_bwd", DISTILL_BWD, [
         dict(dtype=3), dict(ldd=99), dict(k=0), dict(tau=0.0), dict(dloss=None), dict(dz=None), dict(dz=P + 1),
         dict(stats=P + 4), dict(rows=2**31)]),
@@ -49,6 +50,14 @@ def test_workspace_only_for_rows_of_several_parts():
     assert ws(7, 65537, 20, nat.ETH_F16) == 7 * 2 * (16 + 160)
     assert ws(7, 32769, 0, nat.ETH_F32) == 7 * 2 * 16
     assert ws(0, 65537, 20, nat.ETH_F16) == 0 and ws(7, 65537, 20, 5) == 0
+
+
+def test_distillation_workspace_only_for_few_long_rows():
+    ws = lambda *a: nat.value("eth_topk_distill_workspace", *a)  # noqa: E731
+    assert ws(1, 98304, nat.ETH_BF16) == 0 and ws(129, 2**18, nat.ETH_BF16) == 0
+    assert ws(1, 98305, nat.ETH_F16) == 4 * 8 and ws(1, 98304, nat.ETH_F32) == 6 * 8
+    assert ws(64, 2**18, nat.ETH_BF16) == 64 * 8 * 8 and ws(128, 2**18, nat.ETH_BF16) == 128 * 4 * 8
+    assert ws(1, 2**24, nat.ETH_F32) == 512 * 8 and ws(0, 2**18, nat.ETH_F32) == 0 and ws(1, 2**18, 7) == 0
 
 
 def _slope(f, x, d):
