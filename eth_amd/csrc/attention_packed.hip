@@ -221,21 +221,6 @@ __device__ __forceinline__ void zero_rows(const PackOut& t, int64_t row0, int ro
   }
 }
 
-// A wave between its softmax and its matrix instructions: at a head dim of 64,
-// where three workgroups share a compute unit and the softmax takes longer than
-// the products, waves in their products go first (16384 rows, 8 heads on one
-// 333.6 -> 320.8 us, 2 x 4096 rows of 16 heads 90.3 -> 88.4; at 128 the other way,
-// 69.2 -> 71.4 us for 8192 packed rows; no difference in the backward kernels).
-template <int D>
-__device__ __forceinline__ void matrix_phase(bool on) {
-  if constexpr (D == 64) {
-    if (on)
-      __builtin_amdgcn_s_setprio(1);
-    else
-      __builtin_amdgcn_s_setprio(0);
-  }
-}
-
 // ------------------------------------------------------------------ forward --
 // Largest sum of a lane's 32 P of a block before the maximum is taken again:
 // within fp16, whose P is rounded relative to its own size all the same
@@ -326,7 +311,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
       // fragment order pinned as in the equal-length kernel
       a_f32x16 sc[2];
       {
-        matrix_phase<D>(true);
         uint4 kr[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kr[ks] = *reinterpret_cast<const uint4*>(ki + aoff[ks]);
@@ -340,7 +324,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) sc[1] = mma<FP16>(kr[ks], qf[ks], ks == 0 ? a_f32x16{} : sc[1]);
-        matrix_phase<D>(false);
       }
       if (kv0 + kBKV - 1 > q0) {  // diagonal block: mask keys after the query
 #pragma unroll
@@ -389,7 +372,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
         probs();
       }
       l += rs;
-      matrix_phase<D>(true);
       // O^T += V^T P^T over the 64 keys (4 k-steps of 16)
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
@@ -399,7 +381,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) o[dt] = mma<FP16>(img_tr(vp, toff[dt][0], toff[dt][1]), pb, o[dt]);
       }
-      matrix_phase<D>(false);
     }
     vm_wait_all();  // the next block's rows have landed
     __syncthreads();  // this block's images free, the next block's visible
