@@ -580,8 +580,12 @@ def _packed_bwd(desc, q, k, v, out, dout, lse, packed, dq, dk, dv):
 def _packed_attention_grads(q, k, v, out, dout, lse, packed, scale=None):
     """(dq, dk, dv) of packed_attention_bwd in new tensors, for the very q, k,
     v, out, lse and scale of a packed_attention_fwd call, which are not checked
-    again; dout is like out."""
-    key = "grads", scale, q.shape, q.stride(), k.shape, k.stride(), v.stride(), q.dtype
+    again but for where and how they lie now (hooks on saved tensors may have
+    moved them); dout is like out."""
+    _check_device(packed.device.index, q, k, v, out, lse)
+    if out.dtype != q.dtype or lse.dtype != torch.float32 or not out.is_contiguous() or not lse.is_contiguous():
+        raise ValueError("saved tensors came back in another type or layout")
+    key = "grads", scale, q.shape, q.stride(), k.shape, k.stride(), v.stride(), q.dtype, k.dtype, v.dtype
     desc = packed.descriptors.get(key)
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
@@ -687,6 +691,25 @@ def _check_logits(logits2d, bad_flag, *ts):
     return index, code, rows, V, ld
 
 
+def _saved_layout(layout, logits2d, *ts):
+    """The layout of logits that a forward checked (`layout`: _check_logits'
+    result), as autograd gives them back to its backward: hooks on saved tensors
+    may have moved them, and rows that were apart then lie side by side.  `ts`:
+    (tensor, type) of what was contiguous beside them."""
+    index, code, rows, V, _ = layout
+    ld, s1 = logits2d.stride()
+    if rows <= 1:
+        ld = V
+    if logits2d.shape != (rows, V) or nat.dtype_code(logits2d.dtype) != code or V > 1 and s1 != 1 or ld < V:
+        raise ValueError("saved logits came back in another shape, type or layout")
+    for t, dtype in ts:
+        if t.dtype != dtype or not t.is_contiguous():
+            raise ValueError("saved tensors came back in another type or layout")
+        _check_device(index, t)
+    _check_device(index, logits2d)
+    return index, code, rows, V, ld
+
+
 def _check_row_values(name, t, rows):
     if t.dtype != torch.float32 or t.shape != (rows,) or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous fp32 [rows]")
@@ -745,8 +768,8 @@ def token_logprobs_bwd(logits2d, tokens, stats, entropy, dlogprob, dentropy, bad
 
 
 def _token_logprobs_bwd(layout, logits2d, tokens, stats, entropy, dlogprob, dentropy, ignore_index, shape):
-    """token_logprobs_bwd of operands that a forward checked (`layout`:
-    _check_logits' result; upstream gradients as contiguous fp32 [rows])."""
+    """token_logprobs_bwd of operands that a forward checked (`layout`: their
+    layout now; upstream gradients as contiguous fp32 [rows])."""
     index, code, rows, V, ld = layout
     dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)
     if rows:
@@ -806,8 +829,8 @@ def topk_distill_bwd(logits2d, teacher_ids, teacher_logits, temperature, stats, 
 
 
 def _topk_distill_bwd(layout, logits2d, teacher_ids, teacher_logits, temperature, stats, dloss, bad_flag, shape):
-    """topk_distill_bwd of operands that a forward checked (`layout`:
-    _check_logits' result; dloss as contiguous fp32 [rows])."""
+    """topk_distill_bwd of operands that a forward checked (`layout`: their
+    layout now; dloss as contiguous fp32 [rows])."""
     index, code, rows, V, ld = layout
     k, teacher_code = teacher_ids.shape[1], nat.dtype_code(teacher_logits.dtype)
     dz = torch.empty(shape, dtype=logits2d.dtype, device=logits2d.device)

@@ -543,7 +543,9 @@ class TokenLogprobsFn(torch.autograd.Function):
         if dlogprob is None and dentropy is None:
             return None, None, None, None, None
         z, t, stats, entropy = ctx.saved_tensors
-        dz = K._token_logprobs_bwd(ctx.layout, z, t, stats, entropy, _row_values(dlogprob), _row_values(dentropy),
+        f32 = torch.float32
+        layout = K._saved_layout(ctx.layout, z, (t, torch.int64), (stats, f32), (entropy, f32))
+        dz = K._token_logprobs_bwd(layout, z, t, stats, entropy, _row_values(dlogprob), _row_values(dentropy),
                                    ctx.ignore_index, ctx.shape)
         return dz, None, None, None, None
 
@@ -566,12 +568,13 @@ class TopkDistillFn(torch.autograd.Function):
         ids, teacher = teacher_ids.contiguous(), teacher_logits.contiguous()
         loss, stats, ctx.layout = K._topk_distill_fwd(z, ids, teacher, temperature, bad_flag, shape)
         ctx.save_for_backward(z, ids, teacher, stats)
-        ctx.shape, ctx.temperature, ctx.bad_flag = logits.shape, temperature, bad_flag
+        ctx.shape, ctx.temperature, ctx.bad_flag, ctx.teacher = logits.shape, temperature, bad_flag, teacher.dtype
         return loss
 
     @staticmethod
     def backward(ctx, dloss):
         z, ids, teacher, stats = ctx.saved_tensors
-        dz = K._topk_distill_bwd(ctx.layout, z, ids, teacher, ctx.temperature, stats, _row_values(dloss), ctx.bad_flag,
+        layout = K._saved_layout(ctx.layout, z, (ids, torch.int64), (teacher, ctx.teacher), (stats, torch.float32))
+        dz = K._topk_distill_bwd(layout, z, ids, teacher, ctx.temperature, stats, _row_values(dloss), ctx.bad_flag,
                                  ctx.shape)
         return dz, None, None, None, None
