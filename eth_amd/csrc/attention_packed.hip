@@ -23,7 +23,8 @@
 // 0.0017.  A further product with what the rounding of dS leaves would bring
 // about 0.0020, and take a quarter more time backward (16384 rows, 8 heads of 64 on
 // one: 982 -> 1223 us), which buys less than one bit of a gradient that is
-// rounded to 8.
+// rounded to 8.  In fp16 (11 bits) they are 0.0003 where the rounding of the results
+// alone is 0.0002, for gradients of any size (see kGradShift).
 //
 // What bounds it: the exponentials and the products, which share a SIMD's issue
 // and the card's power (the clock falls to 1.6-1.8 GHz under them, where waiting
@@ -123,6 +124,49 @@ __device__ __forceinline__ void add_partial(const float4* p, a_f32x16 (&x)[DT], 
       x[t][g * 4 + 2] += u.z * f;
       x[t][g * 4 + 3] += u.w * f;
     }
+}
+// fp16 gradients: P is about 1/L along L keys, and dS = P (dP - delta) is smaller or
+// larger by the upstream gradient's size: rounded as they are, both leave fp16's
+// normal numbers (4000 rows, gradients of 1e-4: dQ 0.0126 of its norm off, where its
+// own rounding is 0.0023; with dP of 2^18 dS is infinite).  The second products take
+// them times powers of two, which the results lose again: P times 2^kProbShift (the
+// largest P is 1, but for scores so far out that it is not exact any more), dS times
+// 2^shift, which starts above any use and falls, for the wave, where a |dS| passes
+// kMostGrad.  Backward of 8192 packed rows, 16 heads of 128 on four: 281 -> 284 us;
+// 16384, 8 of 64 on one: 1153 -> 1173; 16 x 512 rows, 16 heads of 64: 70 -> 73.
+constexpr int kProbShift = 12;
+constexpr int kGradShift = 64;
+constexpr float kMostGrad = 32768.f;
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// dS (times 2^shift) and the sums of it so far made smaller where dS asks for it;
+// returns by how much shift fell.  A lane with a value that is not finite has
+// no finite sum to keep and does not count.
+template <int DT>
+__device__ __forceinline__ int fit_grads(a_f32x16& ds, a_f32x16 (&sum)[DT], int& shift) {
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(ds[r]));
+  if (__builtin_expect(!__any(most > kMostGrad), 1)) return 0;
+  most = most < INFINITY ? most : 0.f;
+  most = wave_max(most);
+  if (!(most > kMostGrad)) return 0;
+  const int down = (int)(__builtin_amdgcn_readfirstlane(__float_as_uint(most)) >> 23) - (127 + 9);  // to 2^9 ..
+  const float f = pow2(-down);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ds[r] *= f;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[t][r] *= f;
+  shift -= down;
+  return down;
+}
+template <int DT>
+__device__ __forceinline__ void times(a_f32x16 (&x)[DT], float f) {
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[t][r] *= f;
 }
 // 32 rows of [rows, D] 16-bit values in the wave's own `stage` (rows SL elements
 // apart) to rows r0 .. of a head, those below len, in 16-byte row chunks
@@ -491,7 +535,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
     }
   }
   const int64_t srow = (int64_t)h * a.T + begin + q;
-  const float lse = real ? a.lse[srow] : 1e30f;
+  int shift = FP16 ? kGradShift : 0;  // of dS and of the sums of it
+  float lse = real ? a.lse[srow] - (float)shift : 1e30f;
   // delta = rowsum(dO * O) for this query, from the dO fragments already in
   // registers (the two half-waves hold alternate 8-element chunks of the row)
   float del = 0.f;
@@ -560,6 +605,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
         dsoft(std::true_type{});
       else
         dsoft(std::false_type{});
+      if constexpr (FP16) lse += (float)fit_grads<DT>(dp, dq, shift);
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
         const int kk = t * 2 + k2, e0 = k2 * 8;
@@ -579,13 +625,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dq_kernel(PackArgs
     block(j + 1, std::integral_constant<int, 1>{});
   }
   if (j < nkv) block(j, std::integral_constant<int, 0>{});
+  const float unit = FP16 ? pow2(-shift) : 1.f;  // (a power of two)
   if (pc.pieces > 1) {
+    if constexpr (FP16) times<DT>(dq, unit);
     put_partial<DT>(partial_of<DT>(a, a.q_split, hbs, pc, pc.piece, 4, w, lane), dq);
     return;
   }
   if (q0 >= len) return;
   uint16_t* stage = w == 0 ? K0 : w == 1 ? K1 : w == 2 ? V0 : V1;
-  store_rows<D, D + 8, FP16>(a.dq, stage, dq, a.scale, begin, q0, len, h, a.hd, lane);
+  store_rows<D, D + 8, FP16>(a.dq, stage, dq, a.scale * unit, begin, q0, len, h, a.hd, lane);
 }
 
 // joins the pieces of split query tiles, in order, a wave's rows per workgroup
@@ -679,7 +727,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
   };
   auto stat_store = [&](int p, float v) __attribute__((always_inline)) {
     if (rt < 64)
-      lse_s[p][rt] = v;
+      lse_s[p][rt] = FP16 ? v - (float)kProbShift : v;
     else if (rt < 128)
       del_s[p][rt - 64] = -v;
   };
@@ -711,6 +759,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
   a_f32x16 dk[DT], dv[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) dk[t] = dv[t] = a_f32x16{};
+  int shift = kGradShift;  // fp16: of dS and dK
 
   int aoff[KS], toff[DT][2];
 #pragma unroll
@@ -784,8 +833,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
 #pragma unroll
         for (int d2 = 0; d2 < DT; ++d2) dv[d2] = mma<FP16>(pa, bfrag(oi, kk, d2), dv[d2]);
       }
+      if constexpr (FP16) {
+        const float f = pow2(shift - kProbShift);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = s[r] * dp[r];
+        for (int r = 0; r < 16; ++r) dp[r] = s[r] * f * dp[r];
+        fit_grads<DT>(dp, dk, shift);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = s[r] * dp[r];
+      }
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
         const int kk = t * 2 + k2, e0 = k2 * 8;
@@ -808,15 +864,20 @@ __global__ void __launch_bounds__(kAttnThreads, 2) packed_bwd_dkdv_kernel(PackAr
   }
   if (i < steps) step(i, std::integral_constant<int, 0>{});
 
+  const float dv_unit = FP16 ? pow2(-kProbShift) : 1.f, dk_unit = FP16 ? pow2(-shift) : 1.f;
   if (pc.pieces > 1) {
+    if constexpr (FP16) {
+      times<DT>(dv, dv_unit);
+      times<DT>(dk, dk_unit);
+    }
     put_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, pc.piece, 8, w, lane), dv);
     put_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, pc.piece, 8, 4 + w, lane), dk);
     return;
   }
   // dV by way of the dO images, dK of the Q images
   static_assert(2 * 32 * D <= IMG, "two waves' staging fits an image");
-  store_keys<D, D, FP16>(a.dv, (w < 2 ? O0 : O1) + (w & 1) * 32 * D, dv, 1.f, begin, k0, len, kvh, a.hd, lane);
-  store_keys<D, D, FP16>(a.dk, (w < 2 ? Q0 : Q1) + (w & 1) * 32 * D, dk, a.scale, begin, k0, len, kvh, a.hd, lane);
+  store_keys<D, D, FP16>(a.dv, (w < 2 ? O0 : O1) + (w & 1) * 32 * D, dv, dv_unit, begin, k0, len, kvh, a.hd, lane);
+  store_keys<D, D, FP16>(a.dk, (w < 2 ? Q0 : Q1) + (w & 1) * 32 * D, dk, a.scale * dk_unit, begin, k0, len, kvh, a.hd, lane);
 }
 
 // ------------------------------ backward: dK, dV paired, head dims to 128 --
@@ -864,6 +925,7 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) kf[ks] = load_row16<true>(kp, key < len, ks * 16 + hl * 8, a.hd);
   }
+  int shift = kGradShift;  // fp16: of dS and dK (the dK wave)
   a_f32x16 acc[DT];  // dV in the dV wave, dK in the dK wave
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = a_f32x16{};
@@ -898,12 +960,15 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if (pbuf) {
+        const float f = pow2(shift - kProbShift);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const a_u32x4 pv = pbuf[w][t][g][lane];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[t][4 * g + e] = __uint_as_float(pv[e]) * x[t][4 * g + e];
+          for (int e = 0; e < 4; ++e)
+            x[t][4 * g + e] = (FP16 ? __uint_as_float(pv[e]) * f : __uint_as_float(pv[e])) * x[t][4 * g + e];
         }
+        if constexpr (FP16) fit_grads<DT>(x[t], acc, shift);
       }
 #pragma unroll
       for (int k2 = 0; k2 < 2; ++k2) {
@@ -960,7 +1025,7 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
     if (dkw)
       del_s[p][rt] = -v;
     else
-      lse_s[p][rt] = v;
+      lse_s[p][rt] = FP16 ? v - (float)kProbShift : v;
   };
   PackStep cur = PackStep::at(st.from, first, nq), nxt = cur;
   nxt.next(first, nq);
@@ -1088,7 +1153,9 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
     run(std::true_type{});
   else
     run(std::false_type{});
+  const float unit = FP16 ? pow2(dkw ? -shift : -kProbShift) : 1.f;
   if (pc.pieces > 1) {
+    if constexpr (FP16) times<DT>(acc, unit);
     put_partial<DT>(partial_of<DT>(a, a.k_split, a.m, pc, pc.piece, 8, wv, lane), acc);
     return;
   }
@@ -1098,7 +1165,7 @@ __global__ void __launch_bounds__(2 * kAttnThreads, 1) packed_bwd_dkdv_x128_kern
   __syncthreads();  // every image and P buffer read
   uint16_t* stage = (dkw ? reinterpret_cast<uint16_t*>(&Ps[0][0][0][0][0]) : Qx) + w * 32 * SL;
   static_assert(4 * 32 * SL <= 3 * IMG && 4 * 32 * SL * 2 <= (int)sizeof(Ps), "staging fits");
-  store_keys<D, SL, FP16>(dkw ? a.dk : a.dv, stage, acc, dkw ? a.scale : 1.f, begin, k0, len, kvh, a.hd, lane);
+  store_keys<D, SL, FP16>(dkw ? a.dk : a.dv, stage, acc, dkw ? a.scale * unit : unit, begin, k0, len, kvh, a.hd, lane);
 }
 
 // joins the pieces of split key tiles, in order, 32 keys per workgroup: wave 0

@@ -35,7 +35,7 @@ __device__ __forceinline__ uint16_t from_f(float v) {
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (FP16)
-    return (uint32_t)f2h_bits(a) | ((uint32_t)f2h_bits(b) << 16);
+    return f2h_pair(a, b);
   else
     return f2bf_pair(a, b);
 }

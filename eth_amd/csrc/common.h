@@ -118,6 +118,23 @@ __device__ __forceinline__ float wave_sum(float v) {
   return dpp_add<0xb1>(v);   // quad_perm:[1,0,3,2]
 }
 
+// the largest over the wavefront, in every lane, by the moves of wave_sum
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+  v = dpp_max<0x128>(v);
+  v = dpp_max<0x124>(v);
+  v = dpp_max<0x4e>(v);
+  return dpp_max<0xb1>(v);
+}
+
 // Block-wide sum for blockDim.x == NT (multiple of 64).  `red` must hold
 // NT/64 floats of shared memory.  Every thread receives the total.
 template <int NT>

@@ -155,23 +155,6 @@ __device__ __forceinline__ void store_vec(typename Lg<DT>::T* d, int i, int n, c
 
 __device__ __forceinline__ float exp_f(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// the largest over the wavefront, in every lane, by the moves of wave_sum
-template <int CTRL>
-__device__ __forceinline__ float dpp_max(float v) {
-  return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true)));
-}
-__device__ __forceinline__ float wave_max(float v) {
-  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-  u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
-  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
-  v = dpp_max<0x128>(v);
-  v = dpp_max<0x124>(v);
-  v = dpp_max<0x4e>(v);
-  return dpp_max<0xb1>(v);
-}
-
 // max, sum of exponentials and sum of exponentials times their difference from
 // the max, of a part of a row
 struct RowStat {
