@@ -710,14 +710,16 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(DistillArgs a) {
     });
     s *= __builtin_amdgcn_exp2f((m - mx) * c);
     m = mx;
+    float trip = 0.f;  // closed by itself: a sum of V / 512 terms one after the other would lose digits
     each_place<kDistillVecs>([&](auto u) __attribute__((always_inline)) {
       if (u < places) {
         float x[E];
         unpack_again<DT>(v[u], x);
 #pragma unroll
-        for (int j = 0; j < E; ++j) s += __builtin_amdgcn_exp2f((x[j] - m) * c);
+        for (int j = 0; j < E; ++j) trip += __builtin_amdgcn_exp2f((x[j] - m) * c);
       }
     });
+    s += trip;
   }
   const float wm = wave_max(m);
   const float ws = wave_sum(s * __builtin_amdgcn_exp2f((m - wm) * c));
