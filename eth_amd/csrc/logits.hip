@@ -842,6 +842,16 @@ static_assert(kMostVocab * 4 <= (int64_t)kLogpParts * kLogpThreads * kLogpVecs *
 static bool logits_shape(int64_t rows, int64_t V, int64_t ld) {
   return rows > 0 && V > 0 && V <= kMostVocab && ld >= V;
 }
+// Rows of `per` workgroups of at most `threads` threads that one launch takes:
+// a grid has fewer than 2^32 threads, and more rows go in several launches.
+static int64_t launch_rows(int64_t per, int threads) { return ((1LL << 32) - 1) / (per * threads); }
+template <class T>
+static void advance(T*& p, int64_t elements) {
+  if (p) p += elements;
+}
+static void advance(const void*& p, int64_t elements, int dtype) {
+  p = (const char*)p + elements * dtype_size(dtype);
+}
 static int64_t logp_parts(int64_t V, int dtype) {
   const int64_t most = (int64_t)kLogpThreads * kLogpVecs * kLogpTrips * (16 / dtype_size(dtype));
   return (V + most - 1) / most;
@@ -913,13 +923,26 @@ extern "C" int eth_token_logprobs_fwd(const void* logits, int64_t ld, const int6
   a.part_stat = (float4*)workspace;
   a.part_key = (uint64_t*)(a.part_stat + rows * a.parts);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == ETH_BF16)
-    launch_logp<ETH_BF16>(a, rows, s);
-  else if (dtype == ETH_F16)
-    launch_logp<ETH_F16>(a, rows, s);
-  else
-    launch_logp<ETH_F32>(a, rows, s);
-  ETH_CHECK_LAUNCH("eth_token_logprobs_fwd");
+  const int64_t most = launch_rows(a.parts, kLogpThreads);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    if (dtype == ETH_BF16)
+      launch_logp<ETH_BF16>(a, n, s);
+    else if (dtype == ETH_F16)
+      launch_logp<ETH_F16>(a, n, s);
+    else
+      launch_logp<ETH_F32>(a, n, s);
+    ETH_CHECK_LAUNCH("eth_token_logprobs_fwd");
+    advance(a.z, n * ld, dtype);
+    advance(a.tokens, n);
+    advance(a.logprob, n);
+    advance(a.entropy, n);
+    advance(a.stats, n);
+    advance(a.top, n * top_k);
+    advance(a.ids, n * top_k);
+    advance(a.part_stat, n * a.parts);
+    advance(a.part_key, n * a.parts * top_k);
+  }
   return ETH_OK;
 }
 
@@ -941,21 +964,34 @@ extern "C" int eth_token_logprobs_bwd(const void* logits, int64_t ld, const int6
                 "eth_token_logprobs_bwd: misaligned pointer");
   const int chunks = row_chunks(vocab, dtype);
   ETH_CHECK_ARG(rows * chunks < (1LL << 31), "eth_token_logprobs_bwd: too many rows (%lld)", (long long)rows);
-  const int grid = (int)(rows * chunks);
   hipStream_t s = (hipStream_t)stream;
   const bool stream_out = rows * vocab * dtype_size(dtype) > kStreamBytes;
-#define ETH_LOGP_BWD(DT)                                                                                         \
-  (stream_out ? logp_bwd_kernel<DT, true> : logp_bwd_kernel<DT, false>)<<<grid, kRowThreads, 0, s>>>(            \
-      logits, ld, (int)vocab, tokens, ignore_index, (const float2*)stats, entropy, dlogprob, dentropy, dlogits, \
-      ldd, chunks)
-  if (dtype == ETH_BF16)
-    ETH_LOGP_BWD(ETH_BF16);
-  else if (dtype == ETH_F16)
-    ETH_LOGP_BWD(ETH_F16);
-  else
-    ETH_LOGP_BWD(ETH_F32);
+  const float2* row_stats = (const float2*)stats;
+  const void* dz = dlogits;
+  const int64_t most = launch_rows(chunks, kRowThreads);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    const int grid = (int)(n * chunks);
+#define ETH_LOGP_BWD(DT)                                                                              \
+  (stream_out ? logp_bwd_kernel<DT, true> : logp_bwd_kernel<DT, false>)<<<grid, kRowThreads, 0, s>>>( \
+      logits, ld, (int)vocab, tokens, ignore_index, row_stats, entropy, dlogprob, dentropy,           \
+      const_cast<void*>(dz), ldd, chunks)
+    if (dtype == ETH_BF16)
+      ETH_LOGP_BWD(ETH_BF16);
+    else if (dtype == ETH_F16)
+      ETH_LOGP_BWD(ETH_F16);
+    else
+      ETH_LOGP_BWD(ETH_F32);
 #undef ETH_LOGP_BWD
-  ETH_CHECK_LAUNCH("eth_token_logprobs_bwd");
+    ETH_CHECK_LAUNCH("eth_token_logprobs_bwd");
+    advance(logits, n * ld, dtype);
+    advance(dz, n * ldd, dtype);
+    advance(tokens, n);
+    advance(row_stats, n);
+    advance(entropy, n);
+    advance(dlogprob, n);
+    advance(dentropy, n);
+  }
   return ETH_OK;
 }
 
@@ -1004,6 +1040,20 @@ extern "C" int64_t eth_topk_distill_workspace(int64_t rows, int64_t vocab, int d
   return parts == 1 ? 0 : rows * parts * (int64_t)sizeof(float2);
 }
 
+// the rows behind the first n
+static void distill_advance(DistillArgs& a, int64_t n, int dtype) {
+  advance(a.z, n * a.ld, dtype);
+  const void* dz = a.dz;
+  if (dz) advance(dz, n * a.ldd, dtype);
+  a.dz = const_cast<void*>(dz);
+  advance(a.ids, n * a.k);
+  advance(a.teacher, n * a.k, a.teacher_dtype);
+  advance(a.loss, n);
+  advance(a.stats, n);
+  advance(a.dloss, n);
+  advance(a.part_stat, n * a.parts);
+}
+
 // (256 threads for short rows as above: [8192, 8000] bf16 40 -> 27 us; [4096,
 // 32000] 46.4 us with 512, 48.9 with 256)
 template <int DT>
@@ -1036,13 +1086,18 @@ extern "C" int eth_topk_distill_fwd(const void* logits, int64_t ld, const int64_
   a.part = (int)((vecs + a.parts - 1) / a.parts * E);
   a.part_stat = (float2*)workspace;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == ETH_BF16)
-    launch_distill_fwd<ETH_BF16>(a, (int)rows, s);
-  else if (dtype == ETH_F16)
-    launch_distill_fwd<ETH_F16>(a, (int)rows, s);
-  else
-    launch_distill_fwd<ETH_F32>(a, (int)rows, s);
-  ETH_CHECK_LAUNCH("eth_topk_distill_fwd");
+  const int64_t most = launch_rows(a.parts, kDistillThreads);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    if (dtype == ETH_BF16)
+      launch_distill_fwd<ETH_BF16>(a, (int)n, s);
+    else if (dtype == ETH_F16)
+      launch_distill_fwd<ETH_F16>(a, (int)n, s);
+    else
+      launch_distill_fwd<ETH_F32>(a, (int)n, s);
+    ETH_CHECK_LAUNCH("eth_topk_distill_fwd");
+    distill_advance(a, n, dtype);
+  }
   return ETH_OK;
 }
 
@@ -1062,18 +1117,23 @@ extern "C" int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_
   a.ldd = ldd;
   a.chunks = row_chunks(vocab, dtype);
   ETH_CHECK_ARG(rows * a.chunks < (1LL << 31), "eth_topk_distill_bwd: too many rows (%lld)", (long long)rows);
-  const int grid = (int)(rows * a.chunks);
   hipStream_t s = (hipStream_t)stream;
   const bool stream_out = rows * vocab * dtype_size(dtype) > kStreamBytes;
+  const int64_t most = launch_rows(a.chunks, kRowThreads);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = rows - r < most ? rows - r : most;
+    const int grid = (int)(n * a.chunks);
 #define ETH_DISTILL_BWD(DT) \
   (stream_out ? distill_bwd_kernel<DT, true> : distill_bwd_kernel<DT, false>)<<<grid, kRowThreads, 0, s>>>(a)
-  if (dtype == ETH_BF16)
-    ETH_DISTILL_BWD(ETH_BF16);
-  else if (dtype == ETH_F16)
-    ETH_DISTILL_BWD(ETH_F16);
-  else
-    ETH_DISTILL_BWD(ETH_F32);
+    if (dtype == ETH_BF16)
+      ETH_DISTILL_BWD(ETH_BF16);
+    else if (dtype == ETH_F16)
+      ETH_DISTILL_BWD(ETH_F16);
+    else
+      ETH_DISTILL_BWD(ETH_F32);
 #undef ETH_DISTILL_BWD
-  ETH_CHECK_LAUNCH("eth_topk_distill_bwd");
+    ETH_CHECK_LAUNCH("eth_topk_distill_bwd");
+    distill_advance(a, n, dtype);
+  }
   return ETH_OK;
 }
