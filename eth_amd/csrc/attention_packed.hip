@@ -1240,6 +1240,11 @@ static int packed_check(const eth_packed_attn_desc_t* d) {
                 "packed attention: too many tiles");
   ETH_CHECK_ARG(good_split(d->q_split, d->n_q_tiles, d->heads) && good_split(d->k_split, d->n_k_tiles, d->kv_heads),
                 "packed attention: bad split");
+  // (a grid of 2^32 threads or more would be launched modulo 2^32, without an error)
+  const int64_t g_q = grid_of(d->q_split, d->n_q_tiles, d->heads / heads_per_tile(d->heads / d->kv_heads)),
+                g_k = grid_of(d->k_split, d->n_k_tiles, d->kv_heads);
+  ETH_CHECK_ARG(g_q * kAttnThreads < (1LL << 32) && g_k * (d->head_dim > 96 ? 2 : 1) * kAttnThreads < (1LL << 32),
+                "packed attention: too many tiles (%lld and %lld workgroups)", (long long)g_q, (long long)g_k);
   // (a positive scale keeps the order of the scores, and a product with -inf is -inf)
   ETH_CHECK_ARG(d->scale >= 0x1p-100f && d->scale <= 0x1p100f, "packed attention: scale must be positive and finite");
   return ETH_OK;

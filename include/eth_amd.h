@@ -419,6 +419,9 @@ int eth_attn_bwd(const eth_attn_desc_t* desc, const void* q, const void* k, cons
  * keys in the query lists; 64 queries of one head in the key list), whose fp32
  * accumulators a second launch joins in order.  tiles 0: none is.  They need
  * eth_packed_attn_workspace bytes, 16-byte aligned (NULL where it is 0).
+ * A launch has fewer than 2^24 workgroups (one a tile or piece and head, or 2 or
+ * 4 query heads that share one; key lists fewer than 2^23 above a head dim of 96):
+ * more tiles are refused.
  *
  * The backward reads out and lse of the forward, fills delta [heads, rows] on
  * the way, and sums dk and dv over the query heads that share them, in a fixed
