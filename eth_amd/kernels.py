@@ -703,13 +703,12 @@ def _saved_layout(layout, logits2d, *ts):
     ld, s1 = logits2d.stride()
     if rows <= 1:
         ld = V
-    if logits2d.shape != (rows, V) or nat.dtype_code(logits2d.dtype) != code or V > 1 and s1 != 1 or ld < V:
-        raise ValueError("saved logits came back in another shape, type or layout")
+    if (logits2d.shape != (rows, V) or nat.dtype_code(logits2d.dtype) != code or V > 1 and s1 != 1 or ld < V
+            or logits2d.get_device() != index):
+        raise ValueError("saved logits came back in another shape, type or layout, or elsewhere")
     for t, dtype in ts:
-        if t.dtype != dtype or not t.is_contiguous():
-            raise ValueError("saved tensors came back in another type or layout")
-        _check_device(index, t)
-    _check_device(index, logits2d)
+        if t.dtype != dtype or not t.is_contiguous() or t.get_device() != index:
+            raise ValueError("saved tensors came back in another type or layout, or elsewhere")
     return index, code, rows, V, ld
 
 
