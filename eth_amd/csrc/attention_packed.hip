@@ -19,19 +19,28 @@
 // images a block ahead; fp32 base-2 softmax.  P and dS are rounded to the
 // inputs' type for the second product, as the matrix cores take it, and delta is
 // formed of the stored output: dQ and dK are 0.0025 of their norm from 64 bits in
-// bf16 (8192 rows, heads of 128) where the rounding of the results alone is
-// 0.0017.  A further product with what the rounding of dS leaves would bring
-// about 0.0020, and take a quarter more time backward (16384 rows, 8 heads of 64 on
-// one: 982 -> 1223 us), which buys less than one bit of a gradient that is
-// rounded to 8.  In fp16 (11 bits) they are 0.0003 where the rounding of the results
-// alone is 0.0002, for gradients of any size (see kGradShift).
+// bf16 (8192 rows, heads of 128): 0.0017 by the rounding of the results, 0.0017 by that
+// of dS and 0.0007 by that of the output in delta (0.0016 to 0.002 in sequences of 30 rows,
+// whose dQ and dK are 0.003 off).  A further product with what the rounding of dS
+// leaves would bring about 0.0020, and take a quarter more time backward (16384 rows,
+// 8 heads of 64 on one: 982 -> 1223 us), which buys less than one bit of a gradient
+// that is rounded to 8.  In fp16 (11 bits) all of it is an eighth: 0.0003 to 0.0004
+// where the rounding of the results alone is 0.0002, for gradients of any size (see
+// kGradShift).
+//
+// The same call gives the same bits every time.  A row's bits do depend on what
+// else is in the call, within these roundings: one query's scores can move the
+// exponent offset of the 31 beside it in its wave (fp16: its dS that of theirs), and
+// the whole batch decides which chains are cut where.
 //
 // What bounds it: the exponentials and the products, which share a SIMD's issue
 // and the card's power (the clock falls to 1.6-1.8 GHz under them, where waiting
 // costs little and instructions count).  Of all SIMDs' cycles the matrix cores
-// and the VALU are busy: forward 0.54 and 0.71 at a head dim of 64, 0.48 and 0.43 at
-// 128; dQ 0.61 and 0.66, 0.50 and 0.36; dK/dV 0.50 and 0.40, 0.47 and 0.30.  LDS is at
-// 0.24-0.38 throughout, without bank conflicts; HBM is idle.
+// and the VALU are busy: forward 0.53 and 0.71 at a head dim of 64, 0.51 and 0.48 at
+// 128; dQ 0.61 and 0.67, 0.52 and 0.39; dK/dV 0.50 and 0.40, 0.47 and 0.30.  LDS is at
+// 0.27-0.38 throughout, with bank conflicts in at most 0.012; HBM is idle.  dK/dV at
+// 128 fills none of them: its waves wait 0.28 of their time for loads and at the
+// barrier of every 64 queries, and nothing else is on the CU.
 //
 // A block's buffer resource starts at its first row and ends with its
 // sequence's last element, so that rows past the sequence read zeros without a
@@ -274,7 +283,7 @@ constexpr float kMostSum = 1024.f;
 // the workgroup's K and V blocks, 128 / hp queries each, so that a short
 // sequence wastes less of a tile and the waves' chains are of equal length.
 // 16384 rows, 8 heads of 64 on one: 300 us, 0.92 PFLOP/s; 4 x 2048 rows, 16 heads of
-// 128: 77.6 us, 0.89; 96 rows in three sequences 6 us.
+// 128: 79.9 us, 0.86; 96 rows in three sequences 4.9 us (launches of one graph).
 template <int D, bool FP16>
 __global__ void __launch_bounds__(kAttnThreads, 2) packed_fwd_kernel(PackArgs a) {
   constexpr int KS = D / 16;  // k-steps over the head dim

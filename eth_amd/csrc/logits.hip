@@ -13,7 +13,8 @@
 //
 // All arithmetic is fp32; the row's maximum and log s are kept apart, so that
 // a large common offset of the logits costs no digits.  Rows are read once
-// forward, read and written once backward: HBM bounds them.  Rows may start at
+// forward, read and written once backward: HBM bounds them (a large copy moves 5.15
+// TB/s here; reads alone have reached 7.2).  Rows may start at
 // any multiple of an element (odd vocabularies): vectors are loaded and stored
 // with the alignment of an element, which the hardware takes.
 #include <utility>
@@ -334,9 +335,11 @@ __device__ __forceinline__ int logp_rank(const uint64_t* cand, int count, uint64
 // about k + k^2 / 512 logits reach it: the few vectors with one are listed in LDS,
 // read again an element per thread, and the candidates sorted by counting.  Where
 // more reach it than the sort takes (equal logits, a row of few finite ones) or
-// the row holds a NaN, the k-th key is found bit by bit.  HBM bounds it without
-// alternatives ([4096, 50304] bf16 77 us, 5.3 TB/s); listing and sorting them, for
-// which a workgroup has nothing else to do, adds to it (20: 92 us, 128: 108).
+// the row holds a NaN, the k-th key is found bit by bit: right, but 32 passes over
+// the part ([2048, 50304] bf16, 20 alternatives: 48 us; of 10 allowed tokens, of equal
+// logits or with a NaN in every row 3340).  HBM bounds it without alternatives
+// ([4096, 50304] bf16 80 us alone, 5.2 TB/s); listing and sorting them, for which a
+// workgroup has nothing else to do, adds to it (20: 92 us, 128: 108).
 template <int DT, int NT, int TRIPS, bool TOP>
 __global__ void __launch_bounds__(NT, 6) logp_fwd_kernel(LogpArgs a) {
   typedef typename Lg<DT>::T T;
@@ -678,8 +681,9 @@ __device__ __forceinline__ void distill_row(const DistillArgs& a, int64_t row, i
 // flight.  Every wave looks the ids over (a row without entries is not read); of a
 // whole row the first one weighs the entries, four a lane, while the others read,
 // and joins it all behind the one barrier.  HBM bounds it ([4096, 50304] bf16, 64
-// entries: 73 us, 5.6 TB/s), and for few rows the time that one workgroup takes to
-// read its share.
+// entries: 75 us alone, 5.5 TB/s; 90 behind a backward pass, whose lines are written
+// back meanwhile), and for few rows the time that one workgroup takes to read its
+// share.
 template <int DT, int NT, bool PARTS>
 __global__ void __launch_bounds__(NT) distill_fwd_kernel(DistillArgs a) {
   typedef typename Lg<DT>::T T;

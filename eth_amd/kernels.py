@@ -556,7 +556,8 @@ def packed_attention_bwd(q, k, v, out, dout, lse, packed, dq, dk, dv, scale=None
     """Gradients of packed_attention_fwd into dq [rows, n, hn] and dk, dv
     [rows, m, hn] views; out / dout are contiguous [rows, n*hn].  dk and dv are
     summed over the query heads that share them, in a fixed order; rows of no
-    sequence get zeros."""
+    sequence get zeros.  dq, dk and dv share no memory with each other or with the
+    other operands."""
     _check_device(packed.device.index, q, k, v, out, dout, lse, dq, dk, dv)
     desc = _packed_desc(packed, scale, q, k, v, dq, dk, dv)
     rows, n, d = q.shape

@@ -425,7 +425,8 @@ int eth_attn_bwd(const eth_attn_desc_t* desc, const void* q, const void* k, cons
  *
  * The backward reads out and lse of the forward, fills delta [heads, rows] on
  * the way, and sums dk and dv over the query heads that share them, in a fixed
- * order (deterministic). */
+ * order (deterministic).  What is written (out, lse, delta, dq, dk, dv, workspace)
+ * shares no memory with anything else of the call. */
 typedef struct eth_packed_tile {
   int32_t begin, len, start, reserved;
 } eth_packed_tile_t;
