@@ -112,6 +112,10 @@ SIGNATURES["eth_token_logprobs_bwd"] = [_P, _I64, _P, _I64, _P, _P, _P, _P, _P, 
 SIGNATURES["eth_topk_distill_fwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _I64, _P, _I32, _P]
 SIGNATURES["eth_topk_distill_bwd"] = [_P, _I64, _P, _P, _I32, _I32, _F32, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _P]
 
+SIGNATURES["eth_linear_xent_fwd"] = [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I32, _P]
+SIGNATURES["eth_linear_xent_bwd"] = [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I32, _I32, _P, _I64, _I64, _I64,
+                                     _I32, _P]
+
 
 class AttnDesc(ctypes.Structure):
     """struct eth_attn_desc (include/eth_amd.h)."""
@@ -172,6 +176,7 @@ VALUE_SIGNATURES = {
     "eth_embedding_bwd_workspace": ([_I64, _I64], _I64),
     "eth_token_logprobs_workspace": ([_I64, _I64, _I32, _I32], _I64),
     "eth_topk_distill_workspace": ([_I64, _I64, _I32], _I64),
+    "eth_linear_xent_workspace": ([_I64, _I64, _I64, _I64, _I32], _I64),
     "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
     "eth_packed_attn_workspace": ([_P, _I32], _I64),
 }

@@ -1,0 +1,646 @@
+// Cross entropy of a linear head, loss_r = log sum_v exp z_rv - z_r,label with
+// z = h W^T, whose logits z never reach memory, forward and backward.
+//
+//   forward   every tile of z is reduced where its product ends, in its
+//             accumulators: per row the maximum and sum of exponentials of the
+//             tile's columns, and the label's logit; a second kernel joins a
+//             row's parts.
+//   backward  piece by piece of the vocabulary: the piece's tiles of z once
+//             more, dz = dloss (exp(z - lse) - [v = label]) stored in 16 bits
+//             (the matrix cores' operand) where z would have been, and with it
+//             dh += dz W (fp32, over the pieces) and dW = dz^T h.
+//
+// Rows whose label is ignored, and backward rows without upstream gradient,
+// take no part: the others' indices are listed on the device first, the
+// products gather their rows of h and end with the list, and what such rows
+// hold (infinities, NaN) reaches nothing.
+//
+// Powers of two.  A row's dloss is split as 2^e m, 1 <= |m| < 2; dz carries m
+// (in fp16 times 2^14, as exponentials down to 2^-28 then keep all digits), dh
+// gets the row's 2^e back in fp32, and the rows of h that dW is formed of carry
+// 2^(e - the largest e), so that gradients of any size keep their digits in
+// fp16 as in bf16.  (A row's share of dW loses digits where its dloss is 2^-14
+// of the largest and nothing else reaches the same row of dW.)
+//
+// No counterpart in the reference, whose head keeps the logits
+// (model/flex_ops.py:1976-1981 after language_model.py:24-38).
+#include <algorithm>
+
+#include "gemm_tiles.h"
+
+namespace eth {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// How a call's rows are listed: `count` rows take part, row r of the list
+// being row rows[r] of h with label[r] (clamped); `alpha` is dW's factor.
+struct XentHead {
+  int count;
+  float alpha;
+};
+
+// over the four lanes that hold a row of the accumulators (lane % 16)
+__device__ __forceinline__ float row_max(float v) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(p.x) + __uint_as_float(p.y);
+  p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p.x) + __uint_as_float(p.y);
+}
+
+// Parts of 16 rows lie together, [row / 16][part][row % 16], so a tile writes
+// and the join reads whole lines.
+struct XentPart {
+  float m2, s;  // maximum of z log2(e), sum of 2^(z log2(e) - m2)
+};
+
+struct XentStats {
+  static constexpr bool kSized = true, kGathers = true, kStarts = false, kMaps = false, kReduces = true;
+  const XentHead* head;
+  const int* rows;
+  const int* label;
+  XentPart* part;
+  float* picked;
+  int v0;      // the launch's first column in the vocabulary
+  int part0;   // and its first part
+  int parts;   // of a row, in all
+
+  __device__ __forceinline__ void size(GemmArgs& g) const { g.M = min(g.M, head->count); }
+
+  template <int TI, int TJ>
+  __device__ __forceinline__ void reduce(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int N) const {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+    const int p = part0 + col0 / (TJ * 16);
+    const bool edge = col0 + TJ * 16 > N;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int row = row0 + i * 16 + l16;
+      const bool live = row < M;
+      float z[TJ * 4];
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[j * 4 + e] = acc[i][j][e];
+      const int t = (live ? label[row] : -1) - v0 - col0;
+      if (__ballot(live && t >= 0 && t < TJ * 16)) {
+        // (one of a row's four lanes holds its label's logit; a column past N
+        // is no label)
+        float mine = 0.f;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t == j * 16 + lg * 4 + e) mine = z[j * 4 + e];
+        if (live && t >= 0 && t < TJ * 16 && ((t >> 2) & 3) == lg) picked[row] = mine;
+      }
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col0 + j * 16 + lg * 4 + e >= N) z[j * 4 + e] = -INFINITY;
+      }
+      float m = z[0];
+#pragma unroll
+      for (int k = 1; k < TJ * 4; ++k) m = fmaxf(m, z[k]);
+      const float m2 = row_max(m) * kLog2e;
+      const float at = m2 == -INFINITY ? 0.f : m2;  // (columns past N alone)
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < TJ * 4; ++k) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[k], kLog2e, -at));
+      s = row_sum(s);
+      if (lg == 0 && live) part[((int64_t)(row >> 4) * parts + p) * 16 + l16] = XentPart{m2, s};
+    }
+  }
+};
+
+// dz in place of z: mult (2^(z log2 e - lse2) - [v = label]), zero past the
+// vocabulary.
+struct XentGrad {
+  static constexpr bool kSized = true, kGathers = true, kStarts = false, kMaps = true, kReduces = false;
+  const XentHead* head;
+  const int* rows;
+  const int* label;
+  const float* lse2;
+  const float* mult;
+  int v0;      // the piece's first column in the vocabulary
+  int n_real;  // columns of the vocabulary in it
+
+  __device__ __forceinline__ void size(GemmArgs& g) const {
+    g.M = min(g.M, head->count);
+    g.c_bytes = g.M > 0 ? (uint32_t)(((int64_t)(g.M - 1) * g.ldc + g.N) * 2) : 0;
+  }
+
+  template <int TI, int TJ>
+  __device__ __forceinline__ void map(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int) const {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+    const bool edge = col0 + TJ * 16 > n_real;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int row = row0 + i * 16 + l16;
+      const bool live = row < M;
+      const float at = live ? lse2[row] : 0.f, f = live ? mult[row] : 0.f;
+      const int t = (live ? label[row] : -1) - v0 - col0;
+      const bool here = __ballot(live && t >= 0 && t < TJ * 16) != 0;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float d = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -at));
+          if (here && t == j * 16 + lg * 4 + e) d -= 1.f;
+          d *= f;
+          if (edge && col0 + j * 16 + lg * 4 + e >= n_real) d = 0.f;
+          acc[i][j][e] = d;
+        }
+    }
+  }
+};
+
+// dh of a piece: the list's rows of dz
+struct XentRows {
+  static constexpr bool kSized = true, kGathers = false, kStarts = false, kMaps = false, kReduces = false;
+  const XentHead* head;
+
+  __device__ __forceinline__ void size(GemmArgs& g) const {
+    g.M = min(g.M, head->count);
+    g.a_bytes = g.M > 0 ? (uint32_t)(((int64_t)(g.M - 1) * g.lda + g.K) * 2) : 0;
+    g.c_bytes = g.c_bytes && g.M > 0 ? (uint32_t)(((int64_t)(g.M - 1) * g.ldc + g.N) * 4) : 0;
+  }
+};
+
+// dW of a piece: the list's rows are its depth
+struct XentDepth {
+  static constexpr bool kSized = true, kGathers = false, kStarts = false, kMaps = false, kReduces = false;
+  const XentHead* head;
+
+  __device__ __forceinline__ void size(GemmArgs& g) const {
+    g.K = min(g.K, head->count);
+    g.alpha = head->alpha;
+    // (dz has whole 16-byte units behind its last column)
+    g.a_bytes = g.K > 0 ? (uint32_t)(((int64_t)(g.K - 1) * g.lda + (g.M + 7) / 8 * 8) * 2) : 0;
+    g.b_bytes = g.K > 0 ? (uint32_t)(((int64_t)(g.K - 1) * g.ldb + g.N) * 2) : 0;
+  }
+};
+
+// ------------------------------------------------------------- row lists --
+// One workgroup lists the rows that take part, in order.  Forward (dloss
+// NULL): ignored rows get loss 0 here.  Backward: also each listed row's
+// statistics and powers of two, and where each row went (`at`, -1: nowhere).
+struct XentList {
+  const int64_t* labels;
+  int64_t ignore;
+  int64_t n;
+  int64_t vocab;
+  XentHead* head;
+  int* rows;
+  int* label;
+  float* loss;  // forward
+  int* bad;
+  const float* dloss;  // backward
+  const float* lse;
+  int* at;
+  int* exps;
+  float* lse2;
+  float* mult;
+  float* back;
+  int shift;  // dz's power of two
+};
+constexpr int kListThreads = 1024;
+
+// e with 1 <= |v| 2^-e < 2 (0 of what is not finite)
+__device__ __forceinline__ int exponent_of(float v) {
+  return __builtin_isfinite(v) && v != 0.f ? ilogbf(v) : 0;
+}
+
+__global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
+  __shared__ int sums[kListThreads / 64];
+  __shared__ int highs[kListThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int64_t per = (g.n + kListThreads - 1) / kListThreads, a = tid * per, b = min(g.n, a + per);
+  const bool back = g.dloss != nullptr;
+  int mine = 0, high = -1000;
+  for (int64_t r = a; r < b; ++r) {
+    if (g.labels[r] == g.ignore) continue;
+    if (back) {
+      const float d = g.dloss[r];
+      if (d == 0.f) continue;
+      if (__builtin_isfinite(d)) high = max(high, ilogbf(d));
+    }
+    ++mine;
+  }
+  // exclusive sum over the workgroup, and the largest exponent
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(incl, o);
+    if (lane >= o) incl += v;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) high = max(high, __shfl_xor(high, o));
+  if (lane == 63) sums[wid] = incl;
+  if (lane == 0) highs[wid] = high;
+  __syncthreads();
+  int before = incl - mine, total = 0;
+  for (int w = 0; w < kListThreads / 64; ++w) {
+    if (w < wid) before += sums[w];
+    total += sums[w];
+    high = max(high, highs[w]);
+  }
+  if (high == -1000) high = 0;
+  if (tid == 0) *g.head = XentHead{total, ldexpf(1.f, high - g.shift)};
+  bool wild = false;
+  for (int64_t r = a; r < b; ++r) {
+    const int64_t t = g.labels[r];
+    const float d = back ? g.dloss[r] : 1.f;
+    if (t == g.ignore || d == 0.f) {
+      if (back)
+        g.at[r] = -1;
+      else
+        g.loss[r] = 0.f;
+      continue;
+    }
+    wild |= t < 0 || t >= g.vocab;
+    g.rows[before] = (int)r;
+    g.label[before] = (int)(t < 0 ? 0 : t >= g.vocab ? g.vocab - 1 : t);
+    if (back) {
+      const int e = exponent_of(d);
+      g.at[r] = before;
+      g.exps[before] = e - high;
+      g.lse2[before] = g.lse[r];
+      g.mult[before] = ldexpf(d, g.shift - e);
+      g.back[before] = ldexpf(1.f, e - g.shift);
+    }
+    ++before;
+  }
+  if (wild && !back) *g.bad = 1;
+}
+
+// ------------------------------------------------------------------ join --
+// A workgroup joins 16 rows: 64 threads a row, each every 64th part, then a
+// tree.  `lse` in the log2 domain.
+constexpr int kJoinThreads = 1024;
+__device__ __forceinline__ XentPart join(XentPart a, XentPart b) {
+  const float m = fmaxf(a.m2, b.m2), at = m == -INFINITY ? 0.f : m;
+  return XentPart{m, a.s * __builtin_amdgcn_exp2f(a.m2 - at) + b.s * __builtin_amdgcn_exp2f(b.m2 - at)};
+}
+__global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead* head, const int* rows,
+                                                                 const XentPart* part, const float* picked, int parts,
+                                                                 float* loss, float* lse) {
+  __shared__ XentPart red[kJoinThreads / 16][16];
+  const int r = threadIdx.x & 15, k = threadIdx.x >> 4, row = blockIdx.x * 16 + r, n = head->count;
+  if ((int)blockIdx.x * 16 >= n) return;
+  XentPart v{-INFINITY, 0.f};
+  if (row < n) {
+    const XentPart* mine = part + (int64_t)blockIdx.x * parts * 16 + r;
+    for (int p = k; p < parts; p += kJoinThreads / 16) v = join(v, mine[(int64_t)p * 16]);
+  }
+  red[k][r] = v;
+  for (int half = kJoinThreads / 32; half; half >>= 1) {
+    __syncthreads();
+    if (k < half) red[k][r] = join(red[k][r], red[k + half][r]);
+  }
+  if (k == 0 && row < n) {
+    const XentPart t = red[0][r];
+    const float l = __builtin_amdgcn_logf(t.s);
+    // (apart from each other the large terms cancel exactly first)
+    const int64_t o = rows[row];
+    loss[o] = kLn2 * (__builtin_fmaf(-picked[row], kLog2e, t.m2) + l);
+    lse[o] = t.m2 + l;
+  }
+}
+
+// ---------------------------------------------------------------- gather --
+// The list's rows of h, each times its power of two: dW's second operand.
+template <bool FP16>
+__global__ void __launch_bounds__(256) xent_gather_kernel(const XentHead* head, const int* rows, const int* exps,
+                                                          const uint16_t* h, int64_t ldh, uint16_t* out, int hidden) {
+  const int row = blockIdx.x;
+  if (row >= head->count) return;
+  const uint16_t* src = h + (int64_t)rows[row] * ldh;
+  const float f = ldexpf(1.f, exps[row]);
+  for (int c = threadIdx.x * 8; c < hidden; c += 256 * 8) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(src + c);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint16_t lo = (uint16_t)w[k], hi = (uint16_t)(w[k] >> 16);
+      o[k] = FP16 ? f2h_pair(h2f_bits(lo) * f, h2f_bits(hi) * f) : f2bf_pair(bf2f(lo) * f, bf2f(hi) * f);
+    }
+    *reinterpret_cast<uint4*>(out + (int64_t)row * hidden + c) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// dh of every row: the sum of its slices times its power of two, rounded once;
+// zeros where it took no part.
+template <bool FP16>
+__global__ void __launch_bounds__(256) xent_finish_kernel(const int* at, const float* back, const float* slices,
+                                                          int n_slices, int64_t stride, uint16_t* dh, int hidden) {
+  const int64_t row = blockIdx.x;
+  const int p = at[row];
+  const float f = p < 0 ? 0.f : back[p];
+  for (int c = threadIdx.x * 8; c < hidden; c += 256 * 8) {
+    uint32_t o[4] = {0, 0, 0, 0};
+    if (p >= 0) {
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < n_slices; ++s) {
+        const float4* src = reinterpret_cast<const float4*>(slices + s * stride + (int64_t)p * hidden + c);
+        const float4 x = src[0], y = src[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        o[k] = FP16 ? f2h_pair(v[2 * k] * f, v[2 * k + 1] * f) : f2bf_pair(v[2 * k] * f, v[2 * k + 1] * f);
+    }
+    *reinterpret_cast<uint4*>(dh + row * hidden + c) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// ------------------------------------------------------------------ host --
+template <bool A_K, bool B_K, bool FP16, bool SHORT, class X>
+static int launch_product(int tile, const GemmArgs& a, const X& x, hipStream_t s, int splits = 1) {
+  const int64_t tiles = (int64_t)((a.M + tile - 1) / tile) * ((a.N + tile - 1) / tile) * splits;
+  const dim3 grid((unsigned)tiles);
+  if (tile == 256) {
+    if (SHORT || a.K % 64)  // (SHORT: the depth is the device's, its last k-tile of any length)
+      gemm256_m16_kernel<A_K, B_K, FP16, true, X><<<grid, 256, 0, s>>>(a, x);
+    else if constexpr (!SHORT)
+      gemm256_m16_kernel<A_K, B_K, FP16, false, X><<<grid, 256, 0, s>>>(a, x);
+  } else if (tile == 128) {
+    gemm_ring_kernel<128, A_K, B_K, FP16, X><<<grid, 256, 0, s>>>(a, x);
+  } else {
+    gemm_ring_kernel<64, A_K, B_K, FP16, X><<<grid, 256, 0, s>>>(a, x);
+  }
+  ETH_CHECK_LAUNCH("eth_linear_xent");
+  return ETH_OK;
+}
+
+constexpr int64_t kMaxBytes = (1LL << 31) - 1;
+// Workspace for a piece of dz, at most (a piece is 256 columns at least).
+constexpr int64_t kPieceBytes = 256LL << 20;
+
+static int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+static int64_t room(int64_t bytes) { return up(bytes, 256); }
+
+// Columns of W that a launch's 32-bit offsets reach, whole 256s.
+static int64_t reach(int64_t ldw) { return std::max<int64_t>(256, kMaxBytes / (2 * ldw) / 256 * 256); }
+
+struct XentForward {
+  int tile;
+  int64_t chunk;  // columns of a launch
+  int64_t parts;  // of a row
+  int64_t rows, label, picked, part, bytes;  // workspace offsets
+};
+static XentForward plan_forward(int64_t n, int64_t hidden, int64_t vocab, int64_t ldw) {
+  XentForward p;
+  p.chunk = std::min(vocab, reach(ldw));
+  p.tile = plan_tile(n, p.chunk, hidden, true, GemmForm{false, hidden % 64 != 0, 0});
+  const int64_t wide = p.tile / 2;  // columns of a wave
+  p.parts = 0;
+  for (int64_t v = 0; v < vocab; v += p.chunk) p.parts += up(std::min(p.chunk, vocab - v), p.tile) / wide;
+  int64_t o = room(sizeof(XentHead));
+  p.rows = o, o += room(n * 4);
+  p.label = o, o += room(n * 4);
+  p.picked = o, o += room(n * 4);
+  p.part = o, o += room(up(n, 16) * p.parts * (int64_t)sizeof(XentPart));
+  p.bytes = o;
+  return p;
+}
+
+struct XentBackward {
+  int z_tile, w_tile;
+  int splits;           // of dh's depth
+  int64_t piece, ldz;   // columns of a piece, of its rows
+  int64_t rows, label, at, exps, lse2, mult, back, gathered, dz, dh, bytes;
+};
+static XentBackward plan_backward(int64_t n, int64_t hidden, int64_t vocab, int64_t ldw, bool need_dh, bool need_dw) {
+  XentBackward p;
+  int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
+  most = std::min(most, reach(std::max(ldw, hidden)));
+  const int64_t pieces = (vocab + most - 1) / most;
+  p.piece = std::min(up(vocab, 8), up((vocab + pieces - 1) / pieces, 256));
+  p.ldz = up(p.piece, 8);
+  p.z_tile = plan_tile(n, p.piece, hidden, true, GemmForm{false, hidden % 64 != 0, 0});
+  p.w_tile = plan_tile(p.piece, hidden, n, true, GemmForm{false, false, 0});
+  // dh has few tiles and a deep product: split until the chip is full
+  const int64_t tiles = (n + 255) / 256 * ((hidden + 255) / 256);
+  p.splits = 1;
+  while (p.splits < 16 && tiles * p.splits * 2 <= 256 && p.piece / (p.splits * 2) >= 512) p.splits *= 2;
+  int64_t o = room(sizeof(XentHead));
+  for (int64_t* at : {&p.rows, &p.label, &p.at, &p.exps, &p.lse2, &p.mult, &p.back}) *at = o, o += room(n * 4);
+  p.gathered = o, o += need_dw ? room(n * hidden * 2) : 0;
+  p.dz = o, o += room(n * p.ldz * 2);
+  p.dh = o, o += need_dh ? room(p.splits * n * hidden * 4) : 0;
+  p.bytes = o;
+  return p;
+}
+
+static int check_xent(const char* name, const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                      const void* workspace, int64_t n, int64_t hidden, int64_t vocab, int dtype) {
+  ETH_CHECK_ARG(dtype == ETH_BF16 || dtype == ETH_F16, "%s: h and W must be bf16 or fp16", name);
+  // (256 columns of dz, a piece's least, stay within 32-bit offsets)
+  ETH_CHECK_ARG(n > 0 && hidden > 0 && vocab > 0 && n < (1LL << 21) && vocab <= (1LL << 24) && hidden < (1LL << 20),
+                "%s: bad shape: %lld rows, hidden %lld, vocabulary %lld", name, (long long)n, (long long)hidden,
+                (long long)vocab);
+  ETH_CHECK_ARG(h && w && labels && workspace, "%s: null operand", name);
+  ETH_CHECK_ARG(hidden % 8 == 0 && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= hidden && ldw >= hidden,
+                "%s: hidden (%lld) and row strides (%lld, %lld) must be multiples of 8", name, (long long)hidden,
+                (long long)ldh, (long long)ldw);
+  ETH_CHECK_ARG(((uintptr_t)h & 15) == 0 && ((uintptr_t)w & 15) == 0 && ((uintptr_t)workspace & 255) == 0,
+                "%s: h and W must be 16-byte, the workspace 256-byte aligned", name);
+  ETH_CHECK_ARG(((n - 1) * ldh + hidden) * 2 <= kMaxBytes, "%s: rows above 2 GiB are not supported", name);
+  ETH_CHECK_ARG((n + 63) / 64 * ((vocab + 63) / 64) < (1LL << 24), "%s: %lld rows of %lld logits are too many", name,
+                (long long)n, (long long)vocab);
+  return ETH_OK;
+}
+
+static GemmArgs product_args(const void* A, int64_t a_elems, int64_t lda, const void* B, int64_t b_elems, int64_t ldb,
+                             int64_t M, int64_t N, int64_t K) {
+  GemmArgs a{};
+  a.A = (const uint16_t*)A;
+  a.B = (const uint16_t*)B;
+  a.a_bytes = (uint32_t)(a_elems * 2);
+  a.b_bytes = (uint32_t)(b_elems * 2);
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.lda = lda;
+  a.ldb = ldb;
+  a.alpha = 1.f;
+  return a;
+}
+
+template <bool FP16>
+static int xent_forward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const XentForward& p, char* ws,
+                        int64_t n, int64_t hidden, int64_t vocab, hipStream_t s) {
+  int part0 = 0;
+  for (int64_t v0 = 0; v0 < vocab; v0 += p.chunk) {
+    const int64_t cols = std::min(p.chunk, vocab - v0);
+    const GemmArgs a = product_args(h, (n - 1) * ldh + hidden, ldh, w + v0 * ldw, (cols - 1) * ldw + hidden, ldw, n,
+                                    cols, hidden);
+    const XentStats x{(const XentHead*)ws, (const int*)(ws + p.rows), (const int*)(ws + p.label),
+                      (XentPart*)(ws + p.part), (float*)(ws + p.picked), (int)v0, part0, (int)p.parts};
+    const int rc = launch_product<true, true, FP16, false>(p.tile, a, x, s);
+    if (rc != ETH_OK) return rc;
+    part0 += (int)(up(cols, p.tile) / (p.tile / 2));
+  }
+  return ETH_OK;
+}
+
+template <bool FP16>
+static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const XentBackward& p,
+                         char* ws, int64_t n, int64_t hidden, int64_t vocab, uint16_t* dh, void* dw, int dw_dtype,
+                         int accumulate, hipStream_t s) {
+  const XentHead* head = (const XentHead*)ws;
+  const int* rows = (const int*)(ws + p.rows);
+  uint16_t* gathered = (uint16_t*)(ws + p.gathered);
+  uint16_t* dz = (uint16_t*)(ws + p.dz);
+  float* slices = (float*)(ws + p.dh);
+  if (dw) {
+    xent_gather_kernel<FP16><<<(unsigned)n, 256, 0, s>>>(head, rows, (const int*)(ws + p.exps), h, ldh, gathered,
+                                                         (int)hidden);
+    ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
+  }
+  const int esz = dw_dtype == ETH_F32 ? 4 : 2;
+  for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
+    const int64_t real = std::min(p.piece, vocab - v0), cols = up(real, 8);
+    const uint16_t* wp = w + v0 * ldw;
+    const int64_t w_elems = (real - 1) * ldw + hidden;
+    GemmArgs a = product_args(h, (n - 1) * ldh + hidden, ldh, wp, w_elems, ldw, n, cols, hidden);
+    a.C = dz;
+    a.ldc = p.ldz;
+    a.c_dtype = FP16 ? ETH_F16 : ETH_BF16;
+    a.c_vec = true;
+    const XentGrad grad{head, rows, (const int*)(ws + p.label), (const float*)(ws + p.lse2),
+                        (const float*)(ws + p.mult), (int)v0, (int)real};
+    int rc = launch_product<true, true, FP16, false>(p.z_tile, a, grad, s);
+    if (rc != ETH_OK) return rc;
+    if (dh) {
+      GemmArgs d = product_args(dz, (n - 1) * p.ldz + cols, p.ldz, wp, w_elems, ldw, n, hidden, cols);
+      d.C = slices;
+      d.ldc = hidden;
+      d.c_dtype = ETH_F32;
+      d.c_vec = true;
+      d.flags = v0 ? ETH_GEMM_ACCUMULATE : 0;
+      const bool wide = wide_takes(n, hidden, hidden, 4, true);
+      d.c_bytes = wide ? 1 : 0;
+      // the same split of the depth in every piece (the last may need fewer)
+      d.k_split = (int)up((p.piece + p.splits - 1) / p.splits, 64);
+      d.c_split_stride = n * hidden;
+      const int splits = (int)((cols + d.k_split - 1) / d.k_split);
+      if (!wide) d.k_split = 0;
+      rc = launch_product<true, false, FP16, false>(wide ? 256 : 128, d, XentRows{head}, s, wide ? splits : 1);
+      if (rc != ETH_OK) return rc;
+    }
+    if (dw) {
+      GemmArgs d = product_args(dz, 0, p.ldz, gathered, 0, hidden, real, hidden, n);
+      d.C = (char*)dw + v0 * hidden * esz;
+      d.ldc = hidden;
+      d.c_dtype = dw_dtype;
+      d.flags = accumulate ? ETH_GEMM_ACCUMULATE : 0;
+      d.c_vec = true;
+      const bool wide = wide_takes(real, hidden, hidden, esz, true);
+      d.c_bytes = wide ? (uint32_t)(real * hidden * esz) : 0;
+      rc = launch_product<false, false, FP16, true>(wide || p.w_tile != 256 ? p.w_tile : 128, d, XentDepth{head}, s);
+      if (rc != ETH_OK) return rc;
+    }
+  }
+  if (dh) {
+    const bool wide = wide_takes(n, hidden, hidden, 4, true);
+    // slices that the first, deepest piece filled
+    const int64_t k_split = up((p.piece + p.splits - 1) / p.splits, 64), first = up(std::min(p.piece, vocab), 8);
+    const int filled = wide ? (int)((first + k_split - 1) / k_split) : 1;
+    xent_finish_kernel<FP16><<<(unsigned)n, 256, 0, s>>>((const int*)(ws + p.at), (const float*)(ws + p.back), slices,
+                                                         filled, n * hidden, dh, (int)hidden);
+    ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
+  }
+  return ETH_OK;
+}
+
+}  // namespace eth
+
+using namespace eth;
+
+extern "C" int64_t eth_linear_xent_workspace(int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw, int grads) {
+  if (rows <= 0 || hidden <= 0 || vocab <= 0 || ldw < hidden) return 0;
+  if (!grads) return plan_forward(rows, hidden, vocab, ldw).bytes;
+  return plan_backward(rows, hidden, vocab, ldw, grads & 1, grads & 2).bytes;
+}
+
+extern "C" int eth_linear_xent_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                                   int64_t ignore_index, float* loss, float* lse, void* workspace, int64_t rows,
+                                   int64_t hidden, int64_t vocab, int* bad_index, int dtype, void* stream) {
+  const int rc = check_xent("eth_linear_xent_fwd", h, ldh, w, ldw, labels, workspace, rows, hidden, vocab, dtype);
+  if (rc != ETH_OK) return rc;
+  ETH_CHECK_ARG(loss && lse && bad_index, "eth_linear_xent_fwd: null operand");
+  const XentForward p = plan_forward(rows, hidden, vocab, ldw);
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  XentList list{};
+  list.labels = labels;
+  list.ignore = ignore_index;
+  list.n = rows;
+  list.vocab = vocab;
+  list.head = (XentHead*)ws;
+  list.rows = (int*)(ws + p.rows);
+  list.label = (int*)(ws + p.label);
+  list.loss = loss;
+  list.bad = bad_index;
+  xent_list_kernel<<<1, kListThreads, 0, s>>>(list);
+  ETH_CHECK_LAUNCH("eth_linear_xent_fwd");
+  const int done = dtype == ETH_F16
+                       ? xent_forward<true>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden, vocab, s)
+                       : xent_forward<false>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden, vocab, s);
+  if (done != ETH_OK) return done;
+  xent_join_kernel<<<(unsigned)((rows + 15) / 16), kJoinThreads, 0, s>>>(
+      (const XentHead*)ws, (const int*)(ws + p.rows), (const XentPart*)(ws + p.part), (const float*)(ws + p.picked),
+      (int)p.parts, loss, lse);
+  ETH_CHECK_LAUNCH("eth_linear_xent_fwd");
+  return ETH_OK;
+}
+
+extern "C" int eth_linear_xent_bwd(const void* h, int64_t ldh, const void* w, int64_t ldw, const int64_t* labels,
+                                   int64_t ignore_index, const float* lse, const float* dloss, void* dh, void* dw,
+                                   int dw_dtype, int accumulate, void* workspace, int64_t rows, int64_t hidden,
+                                   int64_t vocab, int dtype, void* stream) {
+  const int rc = check_xent("eth_linear_xent_bwd", h, ldh, w, ldw, labels, workspace, rows, hidden, vocab, dtype);
+  if (rc != ETH_OK) return rc;
+  ETH_CHECK_ARG(lse && dloss && (dh || dw), "eth_linear_xent_bwd: null operand");
+  ETH_CHECK_ARG(((uintptr_t)dh & 15) == 0 && ((uintptr_t)dw & 15) == 0,
+                "eth_linear_xent_bwd: dh and dW must be 16-byte aligned");
+  ETH_CHECK_ARG(!dw || dw_dtype == dtype || dw_dtype == ETH_F32, "eth_linear_xent_bwd: bad dW type %d", dw_dtype);
+  ETH_CHECK_ARG(!accumulate || !dw || dw_dtype == ETH_F32, "eth_linear_xent_bwd: accumulate needs fp32 dW");
+  const XentBackward p = plan_backward(rows, hidden, vocab, ldw, dh != nullptr, dw != nullptr);
+  char* ws = (char*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  XentList list{};
+  list.labels = labels;
+  list.ignore = ignore_index;
+  list.n = rows;
+  list.vocab = vocab;
+  list.head = (XentHead*)ws;
+  list.rows = (int*)(ws + p.rows);
+  list.label = (int*)(ws + p.label);
+  list.dloss = dloss;
+  list.lse = lse;
+  list.at = (int*)(ws + p.at);
+  list.exps = (int*)(ws + p.exps);
+  list.lse2 = (float*)(ws + p.lse2);
+  list.mult = (float*)(ws + p.mult);
+  list.back = (float*)(ws + p.back);
+  list.shift = dtype == ETH_F16 ? 14 : 0;
+  xent_list_kernel<<<1, kListThreads, 0, s>>>(list);
+  ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
+  return dtype == ETH_F16 ? xent_backward<true>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden,
+                                                vocab, (uint16_t*)dh, dw, dw_dtype, accumulate, s)
+                          : xent_backward<false>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden,
+                                                 vocab, (uint16_t*)dh, dw, dw_dtype, accumulate, s);
+}

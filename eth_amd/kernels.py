@@ -844,6 +844,86 @@ def _topk_distill_bwd(layout, logits2d, teacher_ids, teacher_logits, temperature
     return dz
 
 
+def _check_head(hidden2d, weight, labels, *ts):
+    """(device index, dtype code, rows, H, V, row strides) of a linear head's
+    operands: hidden [rows, H], weight [V, H], labels [rows]."""
+    if hidden2d.dim() != 2 or weight.dim() != 2 or hidden2d.shape[1] != weight.shape[1] or weight.shape[0] < 1:
+        raise ValueError(f"hidden {tuple(hidden2d.shape)} and weight {tuple(weight.shape)} must be [rows, H] and [V, H]")
+    code = _HALF_CODES.get(hidden2d.dtype)
+    if code is None or weight.dtype != hidden2d.dtype:
+        raise ValueError(f"hidden and weight must be bf16 or fp16 and of one type, got {hidden2d.dtype}, {weight.dtype}")
+    index = hidden2d.get_device()
+    if index < 0:
+        raise ValueError("eth_amd kernels run on the GPU only (no CPU fallback)")
+    _check_device(index, weight, labels, *ts)
+    rows, H = hidden2d.shape
+    V = weight.shape[0]
+    if H < 1 or H % 8:
+        raise ValueError(f"the hidden size must be a multiple of 8 (got {H})")
+    _check_ids(labels, (rows,))
+    strides = []
+    for name, t in (("hidden", hidden2d), ("weight", weight)):
+        ld, s1 = t.stride()
+        if s1 != 1:
+            raise ValueError(f"{name} rows must be contiguous")
+        ld = H if t.shape[0] <= 1 else ld
+        if ld < H or ld % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name}: rows must be 16-byte aligned and may not overlap")
+        strides.append(ld)
+    return index, code, rows, H, V, *strides
+
+
+def linear_xent_fwd(hidden2d, weight, labels, bad_flag, ignore_index=-100):
+    """(loss [rows], lse [rows]) in fp32 of the cross entropy of logits hidden2d
+    [rows, H] @ weight[V, H]^T, which are not kept, against int64 labels [rows].
+    Rows with label `ignore_index` have loss 0 and are not read; other labels
+    outside the vocabulary are clamped and flagged in `bad_flag`."""
+    index, code, rows, H, V, ldh, ldw = _check_head(hidden2d, weight, labels, bad_flag)
+    if bad_flag.dtype != torch.int32 or bad_flag.numel() < 1:
+        raise ValueError("bad_flag must be an int32 tensor")
+    loss, lse = torch.empty(2, rows, dtype=torch.float32, device=hidden2d.device)
+    if rows:
+        ws = nat.value("eth_linear_xent_workspace", rows, H, V, ldw, 0)
+        ws = torch.empty(ws, dtype=torch.uint8, device=hidden2d.device)
+        _launch(index, "eth_linear_xent_fwd", hidden2d.data_ptr(), ldh, weight.data_ptr(), ldw, labels.data_ptr(),
+                operator.index(ignore_index), loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), rows, H, V,
+                bad_flag.data_ptr(), code)
+    return loss, lse
+
+
+def linear_xent_bwd(hidden2d, weight, labels, lse, dloss, ignore_index=-100, need_dhidden=True, need_dweight=True,
+                    dweight=None, accumulate=False):
+    """(dhidden [rows, H], dweight [V, H]) for dloss fp32 [rows], None where not
+    needed: in the operands' type, or dweight into a given fp32 tensor, stored or
+    added."""
+    index, code, rows, H, V, ldh, ldw = _check_head(hidden2d, weight, labels, lse, dloss)
+    _check_row_values("lse", lse, rows)
+    _check_row_values("dloss", dloss, rows)
+    if dweight is not None:
+        _check_device(index, dweight)
+        if dweight.dtype != torch.float32 or dweight.shape != (V, H) or not dweight.is_contiguous():
+            raise ValueError("dweight must be contiguous fp32 [V, H]")
+        if dweight.data_ptr() % 16:
+            raise ValueError("dweight must be 16-byte aligned")
+        need_dweight = True
+    elif accumulate:
+        raise ValueError("accumulate needs a given dweight")
+    elif need_dweight:
+        dweight = torch.empty(V, H, dtype=weight.dtype, device=weight.device)
+    dhidden = torch.empty(rows, H, dtype=hidden2d.dtype, device=hidden2d.device) if need_dhidden else None
+    if not rows:
+        if need_dweight and not accumulate:
+            dweight.zero_()
+    elif need_dhidden or need_dweight:
+        ws = nat.value("eth_linear_xent_workspace", rows, H, V, ldw, (1 if need_dhidden else 0) + (2 if need_dweight else 0))
+        ws = torch.empty(ws, dtype=torch.uint8, device=hidden2d.device)
+        _launch(index, "eth_linear_xent_bwd", hidden2d.data_ptr(), ldh, weight.data_ptr(), ldw, labels.data_ptr(),
+                operator.index(ignore_index), lse.data_ptr(), dloss.data_ptr(), nat.ptr(dhidden), nat.ptr(dweight),
+                nat.dtype_code(dweight.dtype) if need_dweight else code, 1 if accumulate else 0, ws.data_ptr(), rows, H,
+                V, code)
+    return dhidden, dweight
+
+
 def synthetic_batch(sample_ids, seq, vocab, device):
     """tokens [b, s] int64, loss_mask [b, s] fp32, position_ids [b, s] int64
     of the deterministic synthetic batch, computed on the device in one

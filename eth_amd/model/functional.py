@@ -139,6 +139,29 @@ def _wgrad(weight, dy2, x2, mg, accumulate):
     x2.record_stream(side)
 
 
+def _chained(weight, device):
+    """Orders a contribution to weight's main grad on the current stream into the
+    chain that _wgrad forms: waits for the last one, and returns what is called
+    behind the new one."""
+    if not _overlap["wgrad"]:
+        return lambda: None
+    home, here = _overlap["home"], _here(device.index)
+    side, current = K.side_stream(device), torch.cuda.current_stream(device)
+    last = getattr(weight, "_eth_side_grad", None)
+    if last:
+        current.wait_stream(side)
+    elif last is False and home is not None and here != home:
+        current.wait_stream(_stream(home))
+
+    def after():
+        weight._eth_side_grad = here != home
+        if here != home:
+            K.mark_side_launch()
+            side.wait_stream(current)
+
+    return after
+
+
 class LinearFn(torch.autograd.Function):
     """y = x @ W^T (+ b): ColumnParallelLinear / RowParallelLinear at TP=1."""
 
@@ -578,3 +601,45 @@ class TopkDistillFn(torch.autograd.Function):
         dz = K._topk_distill_bwd(layout, z, ids, teacher, ctx.temperature, stats, _row_values(dloss), ctx.bad_flag,
                                  ctx.shape)
         return dz, None, None, None, None
+
+
+def _aligned_rows(x):
+    """x [..., H] as [rows, H] whose rows the kernels can read in place: its own
+    memory where they are whole, apart and 16-byte aligned, else a copy."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    rows, cols = x2.shape
+    s0, s1 = x2.stride()
+    if (cols > 1 and s1 != 1) or (rows > 1 and (s0 < cols or s0 % 8)):
+        return x2.clone(memory_format=torch.contiguous_format)
+    return x2.clone() if x2.data_ptr() % 16 else x2
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """Per-token loss [...] (fp32) of the head's logits hidden [..., H] @
+    weight[V, H]^T against int64 labels [...]: LinearFn and CrossEntropyFn in
+    one, without the logits in memory.  Rows whose label is `ignore_index` have
+    loss 0, are not read and get no gradient."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, bad_flag, ignore_index=-100):
+        if labels.shape != hidden.shape[:-1]:
+            raise ValueError(f"labels {tuple(labels.shape)} do not match hidden {tuple(hidden.shape)}")
+        h, lab = _aligned_rows(hidden), labels.reshape(-1).contiguous()
+        loss, lse = K.linear_xent_fwd(h, weight, lab, bad_flag, ignore_index)
+        ctx.save_for_backward(h, weight, lab, lse)
+        ctx.shape, ctx.ignore_index = hidden.shape, ignore_index
+        return loss.view(labels.shape)
+
+    @staticmethod
+    def backward(ctx, dloss):
+        h, weight, lab, lse = ctx.saved_tensors
+        need_h, need_w = ctx.needs_input_grad[:2]
+        mg, accumulate = _fp32_accum_target(weight) if need_w else (None, False)
+        after = _chained(weight, h.device) if mg is not None else None
+        dh, dw = K.linear_xent_bwd(_aligned_rows(h), weight, lab, lse, _row_values(dloss.reshape(-1)), ctx.ignore_index,
+                                   need_h, need_w, mg, accumulate)
+        if mg is not None:
+            after()
+            grad_written(weight)
+            dw = None
+        return None if dh is None else dh.view(ctx.shape), dw, None, None, None

@@ -558,6 +558,36 @@ int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_
                          const float* stats, const float* dloss, void* dlogits, int64_t ldd,
                          int64_t rows, int64_t vocab, int* bad_index, int dtype, void* stream);
 
+/* Cross entropy of a linear head whose logits z = h w^T are never kept:
+ * h [rows, hidden] (row stride ldh), w [vocab, hidden] (row stride ldw), both bf16
+ * or fp16 (`dtype`), 16-byte aligned, hidden and strides multiples of 8; rows below
+ * 2^21 and 2 GiB, vocab up to 2^24 (w of any size).  Per row, in fp32:
+ *   loss = log sum exp z - z[label],   lse for the backward (log2 domain).
+ * Rows whose label is `ignore_index` are not read and have loss 0 (their lse is
+ * not written); other labels outside [0, vocab) are clamped and set *bad_index to
+ * 1.  NaN or an infinity in a row of h reaches its own loss; in w, every row's.
+ * The backward gives, for upstream gradients dloss [rows] and the forward's lse,
+ *   dz = dloss (exp(z - lse) - [v = label]),   dh = dz w,   dw = dz^T h,
+ * dh [rows, hidden] and dw [vocab, hidden] contiguous, either of them NULL where it
+ * is not wanted; dw in `dtype`, or fp32 (then stored, or added to with `accumulate`).
+ * Rows that are ignored or whose dloss is zero get dh 0 and take no part in dw.
+ * dz is rounded to 16 bits for the products (a row's dloss enters as a mantissa, so
+ * gradients of any size keep their digits); sums are fp32, in a fixed order.
+ * `workspace`: eth_linear_xent_workspace bytes, 256-byte aligned (grads: 0 for the
+ * forward, or 1 for dh + 2 for dw; at most about 256 MiB for a piece of dz, or 512
+ * bytes a row, beside a row of fp32 dh for up to 16 splits and a copy of h). */
+int64_t eth_linear_xent_workspace(int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw,
+                                  int grads);
+int eth_linear_xent_fwd(const void* h, int64_t ldh, const void* w, int64_t ldw,
+                        const int64_t* labels, int64_t ignore_index, float* loss, float* lse,
+                        void* workspace, int64_t rows, int64_t hidden, int64_t vocab,
+                        int* bad_index, int dtype, void* stream);
+int eth_linear_xent_bwd(const void* h, int64_t ldh, const void* w, int64_t ldw,
+                        const int64_t* labels, int64_t ignore_index, const float* lse,
+                        const float* dloss, void* dh, void* dw, int dw_dtype, int accumulate,
+                        void* workspace, int64_t rows, int64_t hidden, int64_t vocab, int dtype,
+                        void* stream);
+
 /* Tied word-embedding gradients on one rank: root = copy = root + copy (fp32,
  * 16-byte aligned).  Replaces the same-rank branch of
  * synchronize_shared_weights_grads (eth/runtime/megatron/training.py:489-531). */
