@@ -116,6 +116,9 @@ SIGNATURES["eth_linear_xent_fwd"] = [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _
 SIGNATURES["eth_linear_xent_bwd"] = [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I32, _I32, _P, _I64, _I64, _I64,
                                      _I32, _P]
 
+SIGNATURES["eth_residual_norm_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["eth_residual_norm_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+
 
 class AttnDesc(ctypes.Structure):
     """struct eth_attn_desc (include/eth_amd.h)."""
@@ -165,6 +168,30 @@ class PackedAttnDesc(ctypes.Structure):
     ]
 
 
+class ResidualNormDesc(ctypes.Structure):
+    """struct eth_residual_norm_desc (include/eth_amd.h)."""
+
+    _fields_ = [
+        ("post_gamma", ctypes.c_void_p),
+        ("post_beta", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("gamma", ctypes.c_void_p),
+        ("beta", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("residual_scale", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("rms", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
+class ResidualNormGrad(ctypes.Structure):
+    """struct eth_residual_norm_grad (include/eth_amd.h)."""
+
+    _fields_ = [("grad", ctypes.c_void_p), ("fp32", ctypes.c_int32), ("accumulate", ctypes.c_int32)]
+
+
 # functions returning a value instead of a status
 VALUE_SIGNATURES = {
     "eth_ln_bwd_workspace": ([_I64, _I64], _I64),
@@ -176,6 +203,7 @@ VALUE_SIGNATURES = {
     "eth_embedding_bwd_workspace": ([_I64, _I64], _I64),
     "eth_token_logprobs_workspace": ([_I64, _I64, _I32, _I32], _I64),
     "eth_topk_distill_workspace": ([_I64, _I64, _I32], _I64),
+    "eth_residual_norm_workspace": ([_I64, _I64], _I64),
     "eth_linear_xent_workspace": ([_I64, _I64, _I64, _I64, _I32], _I64),
     "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
     "eth_packed_attn_workspace": ([_P, _I32], _I64),

@@ -294,6 +294,101 @@ def reduce_partials(part, out, accumulate):
     return out
 
 
+def _norm_desc(x, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms):
+    """(device index, descriptor) of residual norm operands: contiguous x
+    [..., cols] and parameters [cols] of its type."""
+    code = _HALF_CODES.get(x.dtype)
+    if code is None:
+        raise ValueError(f"expected bf16/fp16 tensors, got {x.dtype}")
+    index = x.get_device()
+    if index < 0:
+        raise ValueError("eth_amd kernels run on the GPU only (no CPU fallback)")
+    rows, cols = _rows_cols(x)
+    if cols < 1 or cols % 8 or cols > 8192:
+        raise ValueError(f"the normalized size must be a multiple of 8 up to 8192 (got {cols})")
+    if rms and (post_beta is not None or beta is not None):
+        raise ValueError("root-mean-square norms have no betas")
+    if not rms and (post_beta is None or beta is None):
+        raise ValueError("betas are needed (but for root-mean-square norms)")
+    desc = nat.ResidualNormDesc()
+    for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("gate", gate), ("gamma", gamma),
+                    ("beta", beta)):
+        if t is None and name in ("post_gamma", "gamma"):
+            raise ValueError(f"{name} is needed")
+        if t is not None:
+            if t.dtype != x.dtype or t.shape != (cols,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [{cols}] tensor of the input type")
+            if t.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned")
+            _check_device(index, t)
+            setattr(desc, name, t.data_ptr())
+    desc.rows, desc.cols, desc.rms, desc.dtype = rows, cols, 1 if rms else 0, code
+    desc.residual_scale, desc.eps = float(residual_scale), float(eps)
+    return index, desc
+
+
+def _check_like(name, t, x):
+    if t.shape != x.shape or t.dtype != x.dtype or not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be a contiguous, 16-byte aligned tensor like x")
+
+
+def residual_norm_fwd(x, residual, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps=1e-5, rms=False):
+    """(h, y, stats): h = residual_scale * residual + gate * norm(x), y = norm(h)
+    of the stored h, each norm with its gamma and beta; gate None: one.  With
+    `rms` the norms are root-mean-square ones and have no betas (None).  stats
+    [4, rows] fp32, for the backward."""
+    index, desc = _norm_desc(x, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms)
+    _check_device(index, residual)
+    _check_like("x", x, x)
+    _check_like("residual", residual, x)
+    h, y = torch.empty_like(x), torch.empty_like(x)
+    stats = torch.empty(4, desc.rows, dtype=torch.float32, device=x.device)
+    _launch(index, "eth_residual_norm_fwd", ctypes.byref(desc), x.data_ptr(), residual.data_ptr(), h.data_ptr(),
+            y.data_ptr(), stats.data_ptr())
+    return h, y, stats
+
+
+def residual_norm_bwd(x, h, stats, dh, dy, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms, grads,
+                      need_dx=True, need_dresidual=True):
+    """(dx, dresidual) of residual_norm_fwd for the gradients dh of h and dy of y
+    (one of them may be None), None where not needed.  `grads`: for post_gamma,
+    post_beta, gate, gamma and beta a pair (tensor [cols] that the parameter's
+    gradient is written to, whether it is added), or None; of the parameters'
+    type, or fp32 (which alone can be added to); no two of them the same."""
+    index, desc = _norm_desc(x, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms)
+    given = [t for t in (dh, dy) if t is not None]
+    if not given:
+        raise ValueError("residual_norm_bwd needs dh or dy")
+    _check_device(index, h, stats, *given)
+    for name, t in (("x", x), ("h", h), ("dh", dh), ("dy", dy)):
+        if t is not None:
+            _check_like(name, t, x)
+    if stats.dtype != torch.float32 or stats.shape != (4, desc.rows) or not stats.is_contiguous():
+        raise ValueError("stats must be the forward's fp32 [4, rows]")
+    table = (nat.ResidualNormGrad * 5)()
+    for entry, pair, param in zip(table, grads, (post_gamma, post_beta, gate, gamma, beta)):
+        if pair is None:
+            continue
+        t, accumulate = pair
+        _check_device(index, t)
+        if param is None or t.dtype not in (x.dtype, torch.float32) or t.numel() != desc.cols or not t.is_contiguous():
+            raise ValueError("a parameter's gradient must be a contiguous [cols] tensor of its type or fp32")
+        if accumulate and t.dtype != torch.float32:
+            raise ValueError("accumulate needs an fp32 gradient")
+        entry.grad, entry.fp32, entry.accumulate = t.data_ptr(), t.dtype == torch.float32, bool(accumulate)
+    dx = torch.empty_like(x) if need_dx else None
+    dresidual = torch.empty_like(x) if need_dresidual else None
+    if not desc.rows:
+        for pair in grads:
+            if pair is not None and not pair[1]:
+                pair[0].zero_()
+        return dx, dresidual
+    ws = torch.empty(nat.value("eth_residual_norm_workspace", desc.rows, desc.cols), dtype=torch.float32, device=x.device)
+    _launch(index, "eth_residual_norm_bwd", ctypes.byref(desc), x.data_ptr(), h.data_ptr(), stats.data_ptr(), nat.ptr(dh),
+            nat.ptr(dy), nat.ptr(dx), nat.ptr(dresidual), table, ws.data_ptr())
+    return dx, dresidual
+
+
 # -------------------------------------------------------------- elementwise --
 def bias_gelu_fwd(x, bias):
     code = _check_half(x, bias)

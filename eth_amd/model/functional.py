@@ -309,6 +309,66 @@ class LayerNormResidualFn(torch.autograd.Function):
         return dx, dg.to(gamma.dtype), db.to(beta.dtype), None
 
 
+def _whole(t):
+    """t contiguous and 16-byte aligned (its own memory where it is)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+class GatedResidualNormFn(torch.autograd.Function):
+    """(h, y): h = residual_scale * residual + gate * norm(x), the residual
+    stream behind a block whose output x is normed (post_gamma, post_beta) and
+    gated (gate [cols], None: one), and y = norm(h) (gamma, beta) for the next
+    block, in one pass.  The norms are LayerNorms, or with `rms` root-mean-square
+    norms without betas (None)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps=1e-5, rms=False):
+        ctx.set_materialize_grads(False)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+        xc, scale = _whole(x), float(residual_scale)
+        h, y, stats = K.residual_norm_fwd(xc, _whole(residual), post_gamma, post_beta, gate, scale, gamma, beta, eps, rms)
+        ctx.save_for_backward(xc, h, stats, post_gamma, post_beta, gate, gamma, beta)
+        ctx.scale, ctx.eps, ctx.rms = scale, eps, rms
+        return h, y
+
+    @staticmethod
+    def backward(ctx, dh, dy):
+        if dh is None and dy is None:
+            return (None,) * 10
+        x, h, stats, *params = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        targets, returned, places, added = [], [], set(), []
+        for p, need in zip(params, (needs[2], needs[3], needs[4], needs[6], needs[7])):
+            target = result = None
+            if need:
+                mg, accumulate = _fp32_accum_target(p)
+                if mg is None:
+                    result = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+                    target = result, False
+                elif mg.data_ptr() in places:
+                    # (one parameter in two places of the call: its second gradient is added behind it)
+                    target = torch.empty(p.shape, dtype=torch.float32, device=p.device), False
+                    added.append((mg, target[0]))
+                else:
+                    target = mg, accumulate
+                    places.add(mg.data_ptr())
+            targets.append(target)
+            returned.append(result)
+        pg, pb, gate, gamma, beta = params
+        dx, dres = K.residual_norm_bwd(_whole(x), _whole(h), stats, None if dh is None else _whole(dh),
+                                       None if dy is None else _whole(dy), pg, pb, gate, ctx.scale, gamma, beta, ctx.eps,
+                                       ctx.rms, targets, needs[0], needs[1])
+        for mg, extra in added:
+            mg.view(-1).add_(extra.view(-1))
+        for p, t, r in zip(params, targets, returned):
+            if t is not None and r is None:
+                grad_written(p)
+        dpg, dpb, dgate, dg, db = returned
+        return dx, dres, dpg, dpb, dgate, None, dg, db, None, None
+
+
 class BiasGeluFn(torch.autograd.Function):
     """gelu_tanh(x + b) (flex_ops.py:1882-1906)."""
 

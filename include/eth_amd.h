@@ -458,6 +458,41 @@ int eth_packed_attn_bwd(const eth_packed_attn_desc_t* desc, const void* q, const
                         float* delta, void* dq, void* dk, void* dv, void* workspace,
                         void* stream);
 
+/* The norm behind a block, its gate, the scaled residual and the norm before the
+ * next block, on contiguous [rows, cols] tensors of bf16 or fp16 (`dtype`; cols a
+ * multiple of 8 up to 8192, rows below 2^26; 16-byte aligned):
+ *   n = norm(x) post_gamma + post_beta,  h = residual_scale residual + gate n,
+ *   y = norm(h) gamma + beta  (of the stored h),
+ * norm(v) = (v - mean) / sqrt(variance + eps), or with `rms` v / sqrt(mean of
+ * squares + eps), then without betas (NULL).  gate [cols] NULL: one.
+ * stats [4, rows] fp32: mean and inverse deviation of x, then of h, for the
+ * backward (means 0 with rms).
+ * The backward takes dh (the gradient of h from its other consumers) and dy, one
+ * of which may be NULL (zero), writes dx and dresidual (either may be NULL), and
+ * the gradients of the five parameters, grads[0..4] in the descriptor's order:
+ * each NULL, in `dtype`, or in fp32 (stored, or added to with `accumulate`), no two
+ * of them in one place.  Column sums are fp32, in a fixed order.  `workspace`:
+ * eth_residual_norm_workspace fp32 elements.  rows 0: nothing is done. */
+typedef struct eth_residual_norm_desc {
+  const void *post_gamma, *post_beta, *gate, *gamma, *beta;
+  int64_t rows, cols;
+  float residual_scale, eps;
+  int32_t rms, dtype;
+} eth_residual_norm_desc_t;
+
+typedef struct eth_residual_norm_grad {
+  void* grad;
+  int32_t fp32, accumulate;
+} eth_residual_norm_grad_t;
+
+int eth_residual_norm_fwd(const eth_residual_norm_desc_t* desc, const void* x, const void* residual,
+                          void* h, void* y, float* stats, void* stream);
+int64_t eth_residual_norm_workspace(int64_t rows, int64_t cols);
+int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const void* x, const void* h,
+                          const float* stats, const void* dh, const void* dy, void* dx,
+                          void* dresidual, const eth_residual_norm_grad_t* grads,
+                          float* workspace, void* stream);
+
 /* ------------------------------------------------------------------------
  * Vocabulary side of the first / last stage.
  * eth_embedding_fwd: out[s, b, :] = word[tokens[b, s]] + pos[positions[b, s]]
