@@ -43,6 +43,10 @@ BUCKET_DTYPE = np.dtype(
 )
 # struct eth_packed_tile (16 bytes)
 PACKED_TILE_DTYPE = np.dtype([("begin", "<i4"), ("len", "<i4"), ("start", "<i4"), ("reserved", "<i4")])
+# struct eth_adapter_tile (16 bytes), struct eth_adapter_chunk (8 bytes)
+ADAPTER_TILE_DTYPE = np.dtype([("row", "<i4"), ("rows", "<i4"), ("adapter", "<i4"), ("scale", "<f4")])
+ADAPTER_CHUNK_DTYPE = np.dtype([("first", "<i4"), ("tiles", "<i4")])
+ADAPTER_TILE_ROWS = 32
 # struct eth_adam_tensor (64 bytes)
 ADAM_TENSOR_DTYPE = np.dtype(
     {
@@ -119,6 +123,9 @@ SIGNATURES["eth_linear_xent_bwd"] = [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _
 SIGNATURES["eth_residual_norm_fwd"] = [_P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["eth_residual_norm_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
 
+SIGNATURES["eth_adapter_linear_fwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["eth_adapter_linear_bwd"] = [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]
+
 
 class AttnDesc(ctypes.Structure):
     """struct eth_attn_desc (include/eth_amd.h)."""
@@ -168,6 +175,37 @@ class PackedAttnDesc(ctypes.Structure):
     ]
 
 
+class AdapterDesc(ctypes.Structure):
+    """struct eth_adapter_desc (include/eth_amd.h)."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("in_", ctypes.c_int64),
+        ("out", ctypes.c_int64),
+        ("ldx", ctypes.c_int64),
+        ("ldw", ctypes.c_int64),
+        ("tiles", ctypes.c_void_p),
+        ("chunks", ctypes.c_void_p),
+        ("first_chunk", ctypes.c_void_p),
+        ("used", ctypes.c_void_p),
+        ("of_row", ctypes.c_void_p),
+        ("n_tiles", ctypes.c_int32),
+        ("n_chunks", ctypes.c_int32),
+        ("n_used", ctypes.c_int32),
+        ("n_listed", ctypes.c_int32),
+        ("adapters", ctypes.c_int32),
+        ("rank", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class AdapterGrad(ctypes.Structure):
+    """struct eth_adapter_grad (include/eth_amd.h)."""
+
+    _fields_ = [("grad", ctypes.c_void_p), ("fp32", ctypes.c_int32), ("accumulate", ctypes.c_int32)]
+
+
 class ResidualNormDesc(ctypes.Structure):
     """struct eth_residual_norm_desc (include/eth_amd.h)."""
 
@@ -204,6 +242,7 @@ VALUE_SIGNATURES = {
     "eth_token_logprobs_workspace": ([_I64, _I64, _I32, _I32], _I64),
     "eth_topk_distill_workspace": ([_I64, _I64, _I32], _I64),
     "eth_residual_norm_workspace": ([_I64, _I64], _I64),
+    "eth_adapter_linear_workspace": ([_P, _I32], _I64),
     "eth_linear_xent_workspace": ([_I64, _I64, _I64, _I64, _I32], _I64),
     "eth_packed_attn_tile_rows": ([_I32, _I32], _I32),
     "eth_packed_attn_workspace": ([_P, _I32], _I64),

@@ -1,0 +1,752 @@
+// Low-rank adapters of many tasks beside a shared projection:
+//
+//   y = x W^T + bias + s (x A_a^T) B_a^T     a: the row's adapter, s its scale
+//
+// and with dy:  dx = dy W + s (dy B_a) A_a,  dA_a = sum over a's rows of
+// (s dy B_a)^T x,  dB_a = sum of dy^T (s x A_a^T).
+//
+//   shrink    u = s x A_a^T (backward: s dy B_a) of 32-row tiles of one adapter
+//             each, memory-bound on x: the waves of a workgroup share the depth,
+//             fragments go from memory to the matrix cores without LDS
+//   product   the shared projection's tiles (gemm_tiles.h), whose accumulators
+//             start at u B_a^T (backward: u A_a) instead of zero, so y and dx
+//             are written once
+//   outer     dA and dB: u^T x and dy^T u over chunks of an adapter's tiles, the
+//             16-bit values transposed 8 x 8 in registers, memory-bound on x and dy
+//   join      an adapter's chunks added in order, rounded once
+//
+// u is rounded to 16 bits, the matrix cores' operand.  In fp16 a tile's u carries
+// a power of two that puts its largest value at 2^13 to 2^14, so that it keeps its
+// digits whatever the size of gradients and adapters.
+//
+// No counterpart in the reference, whose linear layers (mpu/layers.py:357-370,
+// 452-470) have one weight for all rows.
+#include <algorithm>
+
+#include "gemm_tiles.h"
+
+namespace eth {
+
+constexpr int kTileRows = ETH_ADAPTER_TILE_ROWS;
+
+// 16 bytes of 8 values, zeros past `r`'s end (offset kOob and beyond)
+__device__ __forceinline__ uint4 load8(rsrc_t r, int32_t off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+
+// ---------------------------------------------------------------- shrink --
+struct ShrinkArgs {
+  const eth_adapter_tile_t* tiles;
+  const uint16_t* x;  // [rows][ldx], K of it
+  const uint16_t* a;  // [adapters][r][K]
+  int64_t ldx;
+  int K, r, rp;
+  uint16_t* u;       // [rows][rp]: rp the rank rounded up to 32, zeros behind it
+  float* row_scale;  // [rows] (fp16)
+  uint16_t* ut;      // [tile][rp][32], zeros behind the tile's rows; or NULL
+  float* tile_scale; // [tile] (fp16)
+};
+
+// RB: blocks of 16 ranks; W waves, each with a range of the depth.
+template <int RB, int W, bool FP16>
+__global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
+  constexpr int RS = RB * 16 + 4;  // padded row of the partial sums
+  __shared__ __attribute__((aligned(16))) float red[W][kTileRows][RS];
+  __shared__ float high[W];
+  const eth_adapter_tile_t t = g.tiles[blockIdx.x];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const rsrc_t xs = make_rsrc(g.x + (int64_t)t.row * g.ldx, (uint32_t)(((t.rows - 1) * g.ldx + g.K) * 2));
+  const rsrc_t as = make_rsrc(g.a + (int64_t)t.adapter * g.r * g.K, (uint32_t)(g.r * g.K * 2));
+  const bool second = t.rows > 16;
+  f32x4_t acc[2][RB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < RB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int steps = (g.K + 31) / 32, per = (steps + W - 1) / W;
+  const int s0 = wid * per, s1 = min(steps, s0 + per);
+  int32_t xo[2], ao[RB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) xo[i] = i * 16 + l16 < t.rows ? (int32_t)(((i * 16 + l16) * g.ldx + lg * 8) * 2) : kOob;
+#pragma unroll
+  for (int j = 0; j < RB; ++j) ao[j] = j * 16 + l16 < g.r ? ((j * 16 + l16) * g.K + lg * 8) * 2 : kOob;
+  constexpr int UN = RB >= 4 ? 2 : 4;  // steps whose loads are in flight together
+  for (int s = s0; s < s1; s += UN) {
+    uint4 fx[UN][2], fa[UN][RB];
+#pragma unroll
+    for (int n = 0; n < UN; ++n) {
+      // (past this wave's range, or the depth: zeros)
+      const bool in = s + n < s1 && (s + n) * 32 + lg * 8 < g.K;
+      const int32_t at = (s + n) * 64;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) fx[n][i] = load8(xs, in && xo[i] != kOob && (i == 0 || second) ? xo[i] + at : kOob);
+#pragma unroll
+      for (int j = 0; j < RB; ++j) fa[n][j] = load8(as, in && ao[j] != kOob ? ao[j] + at : kOob);
+    }
+#pragma unroll
+    for (int n = 0; n < UN; ++n)
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        acc[0][j] = mfma16<FP16>(fa[n][j], fx[n][0], acc[0][j]);
+        if (second) acc[1][j] = mfma16<FP16>(fa[n][j], fx[n][1], acc[1][j]);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < RB; ++j)
+      *reinterpret_cast<f32x4_t*>(&red[wid][i * 16 + l16][j * 16 + lg * 4]) = acc[i][j];
+  __syncthreads();
+  // the waves' sums in order, the scale, and the largest value
+  constexpr int CELLS = kTileRows * RB * 4, PER = (CELLS + 64 * W - 1) / (64 * W);  // of four ranks
+  f32x4_t v[PER];
+  float top = 0.f;
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int cell = c * 64 * W + (int)threadIdx.x, row = cell / (RB * 4), j = cell % (RB * 4) * 4;
+    if (cell >= CELLS) break;
+    f32x4_t s = *reinterpret_cast<const f32x4_t*>(&red[0][row][j]);
+#pragma unroll
+    for (int w = 1; w < W; ++w) s += *reinterpret_cast<const f32x4_t*>(&red[w][row][j]);
+    s *= t.scale;
+    v[c] = s;
+    if (FP16)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = __builtin_isfinite(s[e]) ? fmaxf(top, fabsf(s[e])) : top;
+  }
+  float down = 1.f, up = 1.f;  // what the stored u is times, and what brings it back
+  if (FP16) {
+    top = wave_max(top);
+    if (lane == 0) high[wid] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, high[w]);
+    if (top > 0.f) {
+      const int e = max(-100, min(100, ilogbf(top) - 13));
+      down = ldexpf(1.f, -e);
+      up = ldexpf(1.f, e);
+    }
+    if (threadIdx.x == 0 && g.ut) g.tile_scale[blockIdx.x] = up;
+    if ((int)threadIdx.x < t.rows) g.row_scale[t.row + threadIdx.x] = up;
+  }
+  __syncthreads();  // (red is read no more: its first rows take u^T)
+  uint16_t* turned = reinterpret_cast<uint16_t*>(&red[0][0][0]);  // [RB * 16][32 + 8]
+  constexpr int TS = kTileRows + 8;
+#pragma unroll
+  for (int c = 0; c < PER; ++c) {
+    const int cell = c * 64 * W + (int)threadIdx.x, row = cell / (RB * 4), j = cell % (RB * 4) * 4;
+    if (cell >= CELLS) break;
+    uint32_t lo, hi;
+    if (FP16) {
+      lo = f2h_pair(v[c][0] * down, v[c][1] * down);
+      hi = f2h_pair(v[c][2] * down, v[c][3] * down);
+    } else {
+      lo = f2bf_pair(v[c][0], v[c][1]);
+      hi = f2bf_pair(v[c][2], v[c][3]);
+    }
+    if (g.u && row < t.rows && j < g.rp) {
+      u32x2_t o = {lo, hi};
+      *reinterpret_cast<u32x2_t*>(g.u + (int64_t)(t.row + row) * g.rp + j) = o;
+    }
+    turned[(j + 0) * TS + row] = (uint16_t)lo;
+    turned[(j + 1) * TS + row] = (uint16_t)(lo >> 16);
+    turned[(j + 2) * TS + row] = (uint16_t)hi;
+    turned[(j + 3) * TS + row] = (uint16_t)(hi >> 16);
+  }
+  if (RB == 1 && g.u) {  // (rp 32: the second half of a row of 16 ranks)
+    for (int c = threadIdx.x; c < kTileRows * 2; c += 64 * W)
+      if (c / 2 < t.rows)
+        *reinterpret_cast<uint4*>(g.u + (int64_t)(t.row + c / 2) * g.rp + 16 + c % 2 * 8) = make_uint4(0, 0, 0, 0);
+  }
+  if (!g.ut) return;
+  __syncthreads();
+  uint16_t* out = g.ut + (int64_t)blockIdx.x * g.rp * kTileRows;
+  for (int c = threadIdx.x; c < g.rp * 4; c += 64 * W) {
+    const int j = c / 4, row = c % 4 * 8;
+    const uint4 o = j < RB * 16 ? *reinterpret_cast<const uint4*>(turned + j * TS + row) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(out + j * kTileRows + row) = o;
+  }
+}
+
+// --------------------------------------------------------------- product --
+// The accumulators start at u e^T, e [adapters][cols][r] (forward B, backward
+// A transposed): for each adapter of the wave's rows (mostly one) the product of
+// all its rows, zeros in the place of the others', by fragments from memory.
+struct AdapterStart {
+  static constexpr bool kSized = false, kGathers = false, kStarts = true, kMaps = false, kReduces = false;
+  const int* of_row;
+  const uint16_t* u;
+  const float* row_scale;
+  const uint16_t* e;
+  int r, rp;
+
+  __device__ __forceinline__ uint4 u_frag(int row, int k, bool there) const {
+    return there ? *reinterpret_cast<const uint4*>(u + (int64_t)row * rp + k) : make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ uint4 e_frag(int adapter, int col, int k, int N) const {
+    return col < N && k < r ? *reinterpret_cast<const uint4*>(e + ((int64_t)adapter * N + col) * r + k)
+                            : make_uint4(0, 0, 0, 0);
+  }
+
+  // The products are the kernel's own kind, on accumulators that stay where they
+  // are: through the builtin the wide kernel spills 130 to 380 registers, and the
+  // ring kernel's accumulators move between its products and the start's.
+  template <bool FP16, bool PINNED>
+  __device__ __forceinline__ static void mul(f32x4_t& c, const uint4& a, const uint4& b) {
+    if constexpr (PINNED)
+      mfma16_asm<FP16>(c, a, b);
+    else
+      mfma16_tied<FP16>(c, a, b);
+  }
+
+  // bits 15 and 31: whether one of eight values is an infinity or NaN (one more
+  // carries out of an exponent of all ones)
+  template <bool FP16>
+  __device__ __forceinline__ static uint32_t not_finite(const uint4& v) {
+    constexpr uint32_t top = FP16 ? 0x7c007c00u : 0x7f807f80u, one = FP16 ? 0x04000400u : 0x00800080u;
+    return ((v.x & top) + one) | ((v.y & top) + one) | ((v.z & top) + one) | ((v.w & top) + one);
+  }
+
+  template <bool FP16, bool PINNED, int TI, int TJ>
+  __device__ __forceinline__ void start(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int N) const {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+    constexpr int NONE = 0x7fffffff;
+    int mine[TI];
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int row = row0 + i * 16 + l16;
+      mine[i] = row < M ? of_row[row] : -2;
+    }
+    // whether all rows (but those past M) have one adapter
+    const int first = __builtin_amdgcn_readfirstlane(mine[0]);
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) same &= mine[i] == first || mine[i] == -2;
+    const bool one = __ballot(!same) == 0;
+    // the least adapter of the wave's rows above `last`
+    auto next = [&](int last) __attribute__((always_inline)) {
+      int v = NONE;
+#pragma unroll
+      for (int i = 0; i < TI; ++i) v = mine[i] > last ? min(v, mine[i]) : v;
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) v = min(v, __shfl_xor(v, o));
+      return __builtin_amdgcn_readfirstlane(v);
+    };
+    int a = next(-1), k = 0;
+    while (a != NONE) {
+      uint4 fe[TJ], fu[TI];
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) fe[j] = e_frag(a, col0 + j * 16 + l16, k + lg * 8, N);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) fu[i] = u_frag(row0 + i * 16 + l16, k + lg * 8, mine[i] == a);
+      if (!one) {
+        // zero times another adapter's infinity or NaN is NaN: where its fragments
+        // hold one, zeros take their place, and its own rows become NaN
+        uint32_t wild = 0;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wild |= not_finite<FP16>(fe[j]);
+        if (__ballot((wild & 0x80008000u) != 0)) {
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) fe[j] = make_uint4(0, 0, 0, 0);
+          const uint32_t nan = FP16 ? 0x7e007e00u : 0x7fc07fc0u;
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+            if (mine[i] == a) fu[i] = make_uint4(nan, nan, nan, nan);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) mul<FP16, PINNED>(acc[i][j], fe[j], fu[i]);
+      k += 32;
+      if (k >= rp) {
+        k = 0;
+        a = next(a);
+      }
+    }
+    // asm MFMAs: wait states before anything reads their accumulators
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+    if (FP16) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        const float f = mine[i] >= 0 ? row_scale[row0 + i * 16 + l16] : 0.f;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] *= f;
+        if (PINNED) __builtin_amdgcn_sched_barrier(0);  // (a row block at a time: 26 registers spilled else)
+      }
+    }
+  }
+};
+
+// ------------------------------------------------------------- transpose --
+// [adapters][rows][cols] -> [adapters][cols][rows], 64 x 64 a workgroup, of the
+// adapters that are in use.
+struct TurnArgs {
+  const uint16_t* from;
+  uint16_t* to;
+  int rows, cols;
+};
+__global__ void __launch_bounds__(256) adapter_turn_kernel(TurnArgs a, TurnArgs b, const int* used, int a_tiles) {
+  __shared__ uint16_t tile[64][66];
+  const bool second = (int)blockIdx.x >= a_tiles;
+  const TurnArgs t = second ? b : a;
+  const int at = second ? blockIdx.x - a_tiles : blockIdx.x, wide = (t.cols + 63) / 64;
+  const int r0 = at / wide * 64, c0 = at % wide * 64;
+  const int64_t base = (int64_t)used[blockIdx.y] * t.rows * t.cols;
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int r = r0 + i / 64, c = c0 + i % 64;
+    if (r < t.rows && c < t.cols) tile[i / 64][i % 64] = t.from[base + (int64_t)r * t.cols + c];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int c = c0 + i / 64, r = r0 + i % 64;
+    if (r < t.rows && c < t.cols) t.to[base + (int64_t)c * t.rows + r] = tile[i % 64][i / 64];
+  }
+}
+
+// ----------------------------------------------------------------- outer --
+// part[chunk][r][C] = sum over the chunk's tiles of u^T q: 128 columns a
+// workgroup, its four waves taking tiles in turn.
+struct OuterArgs {
+  const eth_adapter_tile_t* tiles;
+  const eth_adapter_chunk_t* chunks;
+  const uint16_t* ut;
+  const float* tile_scale;  // (fp16)
+  const uint16_t* q;        // [rows][ldq], C of it
+  int64_t ldq;
+  int C, r, rp;
+  float* part;
+};
+
+// rows a (low) and b (high) of column 2 w + h from the packed pairs
+__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, int h) {
+  return __builtin_amdgcn_perm(b, a, h ? 0x07060302u : 0x05040100u);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
+
+template <int RB, bool FP16>
+__global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs g) {
+  __shared__ __attribute__((aligned(16))) float sum[RB * 16][128 + 4];
+  const eth_adapter_chunk_t c = g.chunks[blockIdx.y];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = blockIdx.x * 128 + l16 * 8;
+  // acc[j][f]: ranks 16 j + 4 (lane / 16) + 0..3, column col + f
+  f32x4_t acc[RB][8];
+#pragma unroll
+  for (int j = 0; j < RB; ++j)
+#pragma unroll
+    for (int f = 0; f < 8; ++f) acc[j][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // (fp16) the chunk's largest power of two: its sums are without it, and tiles of
+  // smaller ones are taken down to it (losing what the sums would not hold)
+  float have = 0.f;
+  if (FP16)
+    for (int k = 0; k < c.tiles; ++k) have = fmaxf(have, g.tile_scale[c.first + k]);
+  for (int k = wid; k < c.tiles; k += 4) {
+    const int at = c.first + k;
+    const eth_adapter_tile_t t = g.tiles[at];
+    const rsrc_t qs = make_rsrc(g.q + (int64_t)t.row * g.ldq, (uint32_t)(((t.rows - 1) * g.ldq + g.C) * 2));
+    uint4 row[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      row[i] = load8(qs, lg * 8 + i < t.rows && col < g.C ? (int32_t)(((lg * 8 + i) * g.ldq + col) * 2) : kOob);
+    uint4 fu[RB];
+    const uint16_t* ut = g.ut + (int64_t)at * g.rp * kTileRows + lg * 8;
+#pragma unroll
+    for (int j = 0; j < RB; ++j) fu[j] = *reinterpret_cast<const uint4*>(ut + (j * 16 + l16) * kTileRows);
+    if (FP16) {
+      typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+      const _Float16 f = (_Float16)(g.tile_scale[at] / have);
+#pragma unroll
+      for (int j = 0; j < RB; ++j) fu[j] = __builtin_bit_cast(uint4, __builtin_bit_cast(half8, fu[j]) * f);
+    }
+    // eight rows of eight columns -> a column's eight rows
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+      const int w = f >> 1, h = f & 1;
+      const uint4 fq = make_uint4(pair_of(word_of(row[0], w), word_of(row[1], w), h),
+                                  pair_of(word_of(row[2], w), word_of(row[3], w), h),
+                                  pair_of(word_of(row[4], w), word_of(row[5], w), h),
+                                  pair_of(word_of(row[6], w), word_of(row[7], w), h));
+#pragma unroll
+      for (int j = 0; j < RB; ++j) acc[j][f] = mfma16<FP16>(fu[j], fq, acc[j][f]);
+    }
+  }
+  // the waves' sums, one wave after the other
+  const float back = FP16 ? have : 1.f;
+  for (int w = 0; w < 4; ++w) {
+    if (w == wid) {
+#pragma unroll
+      for (int j = 0; j < RB; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f32x4_t* s = reinterpret_cast<f32x4_t*>(&sum[j * 16 + lg * 4 + e][l16 * 8]);
+          f32x4_t lo = {acc[j][0][e], acc[j][1][e], acc[j][2][e], acc[j][3][e]};
+          f32x4_t hi = {acc[j][4][e], acc[j][5][e], acc[j][6][e], acc[j][7][e]};
+          lo *= back;
+          hi *= back;
+          if (w) {
+            lo += s[0];
+            hi += s[1];
+          }
+          s[0] = lo;
+          s[1] = hi;
+        }
+    }
+    __syncthreads();
+  }
+  float* out = g.part + (int64_t)blockIdx.y * g.r * g.C;
+  for (int i = threadIdx.x; i < g.r * 32; i += 256) {
+    const int j = i / 32, q = i % 32 * 4, at = blockIdx.x * 128 + q;
+    if (at < g.C)
+      *reinterpret_cast<f32x4_t*>(out + (int64_t)j * g.C + at) = *reinterpret_cast<const f32x4_t*>(&sum[j][q]);
+  }
+}
+
+// ------------------------------------------------------------------ join --
+// An adapter's gradient: its chunks added in order; zeros where it has none.
+// dA [adapters][r][K] is stored as summed, dB [adapters][N][r] turned: a thread
+// has eight ranks of a column.
+struct JoinArgs {
+  const float* part;
+  const int* first_chunk;  // [listed + 1]
+  int listed;              // adapters from there on have none
+  int C, r;
+  void* out;
+  int fp32, accumulate, turned;
+};
+__device__ __forceinline__ void put8(void* out, int64_t at, int fp32, int accumulate, int dtype, const float (&v)[8]) {
+  if (fp32) {
+    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at);
+    float4 a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
+    if (accumulate) {
+      const float4 p = o[0], q = o[1];
+      a.x += p.x; a.y += p.y; a.z += p.z; a.w += p.w;
+      b.x += q.x; b.y += q.y; b.z += q.z; b.w += q.w;
+    }
+    o[0] = a;
+    o[1] = b;
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    w[k] = dtype == ETH_F16 ? f2h_pair(v[2 * k], v[2 * k + 1]) : f2bf_pair(v[2 * k], v[2 * k + 1]);
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__global__ void __launch_bounds__(256) adapter_join_kernel(JoinArgs g, int dtype) {
+  const int a = blockIdx.y, eights = g.r / 8 * g.C, i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= eights) return;
+  const int c0 = a < g.listed ? g.first_chunk[a] : 0, c1 = a < g.listed ? g.first_chunk[a + 1] : 0;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int64_t chunk = (int64_t)g.r * g.C;
+  if (g.turned) {
+    const int j = i / g.C * 8, col = i % g.C;
+    for (int c = c0; c < c1; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] += g.part[c * chunk + (int64_t)(j + e) * g.C + col];
+    put8(g.out, (int64_t)a * chunk + (int64_t)col * g.r + j, g.fp32, g.accumulate, dtype, v);
+  } else {
+    for (int c = c0; c < c1; ++c) {
+      const float4* p = reinterpret_cast<const float4*>(g.part + c * chunk + (int64_t)i * 8);
+      const float4 x = p[0], y = p[1];
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+    }
+    put8(g.out, (int64_t)a * chunk + (int64_t)i * 8, g.fp32, g.accumulate, dtype, v);
+  }
+}
+
+// ------------------------------------------------------------------ host --
+static int64_t room(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+static int padded_rank(int64_t r) { return (int)((r + 31) / 32 * 32); }
+
+// How the product [M, N] x K deep runs: its tile, or 256x256 tiles in several
+// splits of K joined by a second kernel, by the rules of the plain products.
+struct ProductPlan {
+  int tile, splits;
+  int64_t workspace;
+};
+static ProductPlan plan_product(int64_t M, int64_t N, int64_t K, int b_kcontig) {
+  ProductPlan p{0, 1, 0};
+  const GemmForm form = gemm_form(M, N, K, 1, b_kcontig, false);
+  p.tile = plan_tile(M, N, K, wide_takes(M, N, N, 2, true), form);
+  const int64_t tiles = (M + 255) / 256 * ((N + 255) / 256);
+  int splits = 1;
+  while (tiles <= 128 && splits < 16 && tiles * splits * 2 <= 256 && K / (splits * 2) >= 1024) splits *= 2;
+  if (splits > 1 && 4 * (M + 256) * N < (1LL << 31) &&
+      eth_gemm_splitk_pays(M, N, K, splits, 1, b_kcontig, ETH_BF16)) {
+    p.tile = 256;
+    p.splits = splits;
+    p.workspace = eth_gemm_splitk_workspace(M, N, splits);
+  }
+  return p;
+}
+
+template <bool B_K, bool FP16, class X>
+static int launch_adapted(const ProductPlan& p, GemmArgs a, const X& x, float* partials, hipStream_t s) {
+  if (p.splits > 1) {
+    GemmArgs d = a;
+    d.C = partials;
+    d.bias = nullptr;
+    d.flags = 0;
+    d.ldc = a.N;
+    d.c_dtype = ETH_F32;
+    d.c_bytes = (uint32_t)((int64_t)a.M * a.N * 4);
+    d.k_split = (int)(((a.K + p.splits - 1) / p.splits + 63) / 64 * 64);
+    d.c_split_stride = (int64_t)a.M * a.N;
+    const int splits = (a.K + d.k_split - 1) / d.k_split;
+    const int tiles = ((a.M + 255) / 256) * ((a.N + 255) / 256) * splits;
+    if (a.K % 64)
+      gemm256_m16_kernel<true, B_K, FP16, true, X><<<tiles, 256, 0, s>>>(d, x);
+    else
+      gemm256_m16_kernel<true, B_K, FP16, false, X><<<tiles, 256, 0, s>>>(d, x);
+    ETH_CHECK_LAUNCH("eth_adapter_linear");
+    const SplitSum sum{partials, splits, d.c_split_stride, a.C, a.ldc, a.bias, a.M, a.N, a.c_dtype, 0, 1.f};
+    const int64_t quads = (int64_t)a.M * (a.N / 4);
+    splitk_sum_kernel<FP16><<<(int)std::min<int64_t>((quads + 255) / 256, 2048), 256, 0, s>>>(sum);
+    ETH_CHECK_LAUNCH("eth_adapter_linear");
+    return ETH_OK;
+  }
+  const int tiles = ((a.M + p.tile - 1) / p.tile) * ((a.N + p.tile - 1) / p.tile);
+  if (p.tile == 256) {
+    if (a.K % 64)
+      gemm256_m16_kernel<true, B_K, FP16, true, X><<<tiles, 256, 0, s>>>(a, x);
+    else
+      gemm256_m16_kernel<true, B_K, FP16, false, X><<<tiles, 256, 0, s>>>(a, x);
+  } else if (p.tile == 128) {
+    gemm_ring_kernel<128, true, B_K, FP16, X><<<tiles, 256, 0, s>>>(a, x);
+  } else {
+    gemm_ring_kernel<64, true, B_K, FP16, X><<<tiles, 256, 0, s>>>(a, x);
+  }
+  ETH_CHECK_LAUNCH("eth_adapter_linear");
+  return ETH_OK;
+}
+
+template <bool FP16>
+static int launch_shrink(const ShrinkArgs& g, int n_tiles, hipStream_t s) {
+#define ETH_SHRINK(RB, W) adapter_shrink_kernel<RB, W, FP16><<<n_tiles, 64 * W, 0, s>>>(g)
+  if (g.r <= 16) ETH_SHRINK(1, 8);
+  else if (g.r <= 32) ETH_SHRINK(2, 8);
+  else if (g.r <= 64) ETH_SHRINK(4, 8);
+  else ETH_SHRINK(8, 4);
+#undef ETH_SHRINK
+  ETH_CHECK_LAUNCH("eth_adapter_linear");
+  return ETH_OK;
+}
+
+template <bool FP16>
+static int launch_outer(const OuterArgs& g, int n_chunks, hipStream_t s) {
+  const dim3 grid((unsigned)((g.C + 127) / 128), (unsigned)n_chunks);
+#define ETH_OUTER(RB) adapter_outer_kernel<RB, FP16><<<grid, 256, 0, s>>>(g)
+  if (g.r <= 16) ETH_OUTER(1);
+  else if (g.r <= 32) ETH_OUTER(2);
+  else if (g.r <= 64) ETH_OUTER(4);
+  else ETH_OUTER(8);
+#undef ETH_OUTER
+  ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
+  return ETH_OK;
+}
+
+static int check_adapter(const char* name, const eth_adapter_desc_t* d) {
+  ETH_CHECK_ARG(d, "%s: null descriptor", name);
+  ETH_CHECK_ARG(d->dtype == ETH_BF16 || d->dtype == ETH_F16, "%s: dtype must be bf16 or fp16", name);
+  const int64_t M = d->rows, N = d->out, K = d->in;
+  ETH_CHECK_ARG(M > 0 && N > 0 && K > 0 && N % 8 == 0 && K % 8 == 0 && M < (1LL << 31) && N < (1LL << 31) &&
+                    K < (1LL << 31),
+                "%s: bad shape: %lld rows, %lld in, %lld out (multiples of 8)", name, (long long)M, (long long)K,
+                (long long)N);
+  ETH_CHECK_ARG(d->rank >= 8 && d->rank <= 128 && d->rank % 8 == 0, "%s: the rank must be a multiple of 8 up to 128 (got %d)",
+                name, d->rank);
+  ETH_CHECK_ARG(d->ldx >= K && d->ldw >= K && d->ldx % 8 == 0 && d->ldw % 8 == 0,
+                "%s: row strides must be multiples of 8", name);
+  ETH_CHECK_ARG(d->adapters > 0 && d->n_tiles >= 0 && d->n_chunks >= 0 && d->n_chunks < 65536 && d->n_used >= 0 &&
+                    d->n_used <= d->n_listed && d->n_listed <= d->adapters && d->adapters < 65536 && d->n_tiles < (1 << 23) &&
+                    (d->n_tiles > 0) == (d->n_chunks > 0) && (d->n_tiles > 0) == (d->n_used > 0),
+                "%s: bad lists", name);
+  ETH_CHECK_ARG(!d->n_tiles || (d->tiles && d->chunks && d->of_row && d->used && d->first_chunk), "%s: null list", name);
+  ETH_CHECK_ARG(((M - 1) * d->ldx + K) * 2 < (1LL << 31) && ((N - 1) * d->ldw + K) * 2 < (1LL << 31) &&
+                    M * N * 2 < (1LL << 31) && M * K * 2 < (1LL << 31) && (int64_t)d->rank * std::max(K, N) * 2 < (1LL << 31),
+                "%s: operands above 2 GiB are not supported", name);
+  return ETH_OK;
+}
+
+struct AdapterForward {
+  int64_t u, row_scale, product, bytes;
+  ProductPlan plan;
+};
+static AdapterForward plan_adapter_fwd(const eth_adapter_desc_t* d) {
+  AdapterForward p;
+  p.plan = plan_product(d->rows, d->out, d->in, 1);
+  int64_t o = 0;
+  p.u = o, o += room(d->rows * padded_rank(d->rank) * 2);
+  p.row_scale = o, o += room(d->rows * 4);
+  p.product = o, o += room(p.plan.workspace);
+  p.bytes = o;
+  return p;
+}
+struct AdapterBackward {
+  int64_t u, row_scale, ut, tile_scale, at, bt, part, product, bytes;
+  ProductPlan plan;
+};
+static AdapterBackward plan_adapter_bwd(const eth_adapter_desc_t* d) {
+  AdapterBackward p;
+  p.plan = plan_product(d->rows, d->in, d->out, 0);
+  const int rp = padded_rank(d->rank);
+  int64_t o = 0;
+  p.u = o, o += room(d->rows * rp * 2);
+  p.row_scale = o, o += room(d->rows * 4);
+  p.ut = o, o += room((int64_t)d->n_tiles * rp * kTileRows * 2);
+  p.tile_scale = o, o += room((int64_t)d->n_tiles * 4);
+  p.at = o, o += room((int64_t)d->adapters * d->rank * d->in * 2);
+  p.bt = o, o += room((int64_t)d->adapters * d->rank * d->out * 2);
+  // dA's and dB's chunks, one after the other, and the product's partial sums
+  // (its stream order lets all three share)
+  p.part = o;
+  p.product = o;
+  o += room(std::max((int64_t)d->n_chunks * d->rank * std::max(d->in, d->out) * 4, p.plan.workspace));
+  p.bytes = o;
+  return p;
+}
+
+static GemmArgs adapter_product(const eth_adapter_desc_t* d, const void* A, int64_t lda, int64_t a_cols, const void* B,
+                                void* C, int64_t N, const void* bias) {
+  GemmArgs a{};
+  a.A = (const uint16_t*)A;
+  a.B = (const uint16_t*)B;
+  a.a_bytes = (uint32_t)(((d->rows - 1) * lda + a_cols) * 2);
+  a.b_bytes = (uint32_t)(((d->out - 1) * d->ldw + d->in) * 2);
+  a.C = C;
+  a.bias = (const uint16_t*)bias;
+  a.M = (int)d->rows;
+  a.N = (int)N;
+  a.K = (int)a_cols;
+  a.lda = lda;
+  a.ldb = d->ldw;
+  a.ldc = N;
+  a.c_dtype = d->dtype;
+  a.flags = bias ? ETH_GEMM_BIAS : 0;
+  a.alpha = 1.f;
+  a.c_vec = true;
+  a.c_bytes = (uint32_t)(d->rows * N * 2);
+  return a;
+}
+
+template <bool FP16>
+static int adapter_forward(const eth_adapter_desc_t* d, const void* x, const void* w, const void* bias,
+                           const void* lora_a, const void* lora_b, void* y, void* ut, float* tile_scale, char* ws,
+                           hipStream_t s) {
+  const AdapterForward p = plan_adapter_fwd(d);
+  const int rp = padded_rank(d->rank);
+  const GemmArgs a = adapter_product(d, x, d->ldx, d->in, w, y, d->out, bias);
+  if (!d->n_tiles) return launch_adapted<true, FP16>(p.plan, a, PlainProduct{}, (float*)(ws + p.product), s);
+  const ShrinkArgs g{d->tiles, (const uint16_t*)x, (const uint16_t*)lora_a, d->ldx, (int)d->in, d->rank, rp,
+                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale};
+  const int rc = launch_shrink<FP16>(g, d->n_tiles, s);
+  if (rc != ETH_OK) return rc;
+  const AdapterStart start{d->of_row, g.u, g.row_scale, (const uint16_t*)lora_b, d->rank, rp};
+  return launch_adapted<true, FP16>(p.plan, a, start, (float*)(ws + p.product), s);
+}
+
+template <bool FP16>
+static int adapter_backward(const eth_adapter_desc_t* d, const void* x, const void* w, const void* lora_a,
+                            const void* lora_b, const void* dy, const void* ut, const float* tile_scale, void* dx,
+                            const eth_adapter_grad_t* da, const eth_adapter_grad_t* db, char* ws, hipStream_t s) {
+  const AdapterBackward p = plan_adapter_bwd(d);
+  const int rp = padded_rank(d->rank);
+  int rc = ETH_OK;
+  GemmArgs a = adapter_product(d, dy, d->out, d->out, w, dx, d->in, nullptr);
+  if (!d->n_tiles) {
+    if (dx) rc = launch_adapted<false, FP16>(p.plan, a, PlainProduct{}, (float*)(ws + p.product), s);
+    if (rc != ETH_OK) return rc;
+  }
+  if (d->n_tiles && (dx || da->grad)) {
+    // A^T for the start of dx, B^T for u
+    const TurnArgs turn_a{(const uint16_t*)lora_a, (uint16_t*)(ws + p.at), d->rank, (int)d->in};
+    const TurnArgs turn_b{(const uint16_t*)lora_b, (uint16_t*)(ws + p.bt), (int)d->out, d->rank};
+    const int high = (d->rank + 63) / 64;
+    const int a_tiles = dx ? high * (int)((d->in + 63) / 64) : 0, b_tiles = high * (int)((d->out + 63) / 64);
+    adapter_turn_kernel<<<dim3((unsigned)(a_tiles + b_tiles), (unsigned)d->n_used), 256, 0, s>>>(turn_a, turn_b, d->used,
+                                                                                                a_tiles);
+    ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
+    const ShrinkArgs g{d->tiles, (const uint16_t*)dy, turn_b.to, d->out, (int)d->out, d->rank, rp,
+                       (uint16_t*)(dx ? ws + p.u : nullptr), (float*)(ws + p.row_scale),
+                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale)};
+    rc = launch_shrink<FP16>(g, d->n_tiles, s);
+    if (rc != ETH_OK) return rc;
+    if (dx) {
+      const AdapterStart start{d->of_row, g.u, g.row_scale, turn_a.to, d->rank, rp};
+      rc = launch_adapted<false, FP16>(p.plan, a, start, (float*)(ws + p.product), s);
+      if (rc != ETH_OK) return rc;
+    }
+  }
+  for (int which = 0; which < 2; ++which) {
+    const eth_adapter_grad_t* t = which ? db : da;
+    if (!t->grad) continue;
+    const int C = (int)(which ? d->out : d->in);
+    if (d->n_tiles) {
+      const OuterArgs g{d->tiles, d->chunks, which ? (const uint16_t*)ut : (const uint16_t*)(ws + p.ut),
+                        which ? tile_scale : (const float*)(ws + p.tile_scale),
+                        which ? (const uint16_t*)dy : (const uint16_t*)x, which ? d->out : d->ldx, C, d->rank, rp,
+                        (float*)(ws + p.part)};
+      rc = launch_outer<FP16>(g, d->n_chunks, s);
+      if (rc != ETH_OK) return rc;
+    }
+    if (!d->n_tiles && t->accumulate) continue;
+    const JoinArgs j{(const float*)(ws + p.part), d->first_chunk, d->n_tiles ? d->n_listed : 0, C, d->rank, t->grad, t->fp32, t->accumulate, which};
+    adapter_join_kernel<<<dim3((unsigned)((d->rank / 8 * (int64_t)C + 255) / 256), (unsigned)d->adapters), 256, 0, s>>>(
+        j, d->dtype);
+    ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
+  }
+  return ETH_OK;
+}
+
+}  // namespace eth
+
+using namespace eth;
+
+extern "C" int64_t eth_adapter_linear_workspace(const eth_adapter_desc_t* desc, int backward) {
+  if (check_adapter("eth_adapter_linear_workspace", desc) != ETH_OK) return -1;
+  return backward ? plan_adapter_bwd(desc).bytes : plan_adapter_fwd(desc).bytes;
+}
+
+extern "C" int eth_adapter_linear_fwd(const eth_adapter_desc_t* desc, const void* x, const void* w, const void* bias,
+                                      const void* lora_a, const void* lora_b, void* y, void* ut, float* tile_scale,
+                                      void* workspace, void* stream) {
+  const int rc = check_adapter("eth_adapter_linear_fwd", desc);
+  if (rc != ETH_OK) return rc;
+  ETH_CHECK_ARG(x && w && lora_a && lora_b && y && workspace && (!ut || desc->dtype != ETH_F16 || tile_scale),
+                "eth_adapter_linear_fwd: null operand");
+  ETH_CHECK_ARG((((uintptr_t)x | (uintptr_t)w | (uintptr_t)lora_a | (uintptr_t)lora_b | (uintptr_t)y | (uintptr_t)ut) &
+                 15u) == 0 && ((uintptr_t)workspace & 255) == 0,
+                "eth_adapter_linear_fwd: operands must be 16-byte, the workspace 256-byte aligned");
+  return desc->dtype == ETH_F16
+             ? adapter_forward<true>(desc, x, w, bias, lora_a, lora_b, y, ut, tile_scale, (char*)workspace,
+                                     (hipStream_t)stream)
+             : adapter_forward<false>(desc, x, w, bias, lora_a, lora_b, y, ut, tile_scale, (char*)workspace,
+                                      (hipStream_t)stream);
+}
+
+extern "C" int eth_adapter_linear_bwd(const eth_adapter_desc_t* desc, const void* x, const void* w, const void* lora_a,
+                                      const void* lora_b, const void* dy, const void* ut, const float* tile_scale,
+                                      void* dx, const eth_adapter_grad_t* da, const eth_adapter_grad_t* db,
+                                      void* workspace, void* stream) {
+  const int rc = check_adapter("eth_adapter_linear_bwd", desc);
+  if (rc != ETH_OK) return rc;
+  ETH_CHECK_ARG(x && w && lora_a && lora_b && dy && da && db && workspace, "eth_adapter_linear_bwd: null operand");
+  ETH_CHECK_ARG(dx || da->grad || db->grad, "eth_adapter_linear_bwd: nothing to compute");
+  ETH_CHECK_ARG(!db->grad || !desc->n_tiles || (ut && (desc->dtype != ETH_F16 || tile_scale)),
+                "eth_adapter_linear_bwd: dB needs what the forward saved");
+  ETH_CHECK_ARG((((uintptr_t)x | (uintptr_t)w | (uintptr_t)lora_a | (uintptr_t)lora_b | (uintptr_t)dy | (uintptr_t)ut |
+                  (uintptr_t)dx | (uintptr_t)da->grad | (uintptr_t)db->grad) & 15u) == 0 &&
+                    ((uintptr_t)workspace & 255) == 0,
+                "eth_adapter_linear_bwd: operands must be 16-byte, the workspace 256-byte aligned");
+  for (const eth_adapter_grad_t* t : {da, db})
+    ETH_CHECK_ARG(!t->accumulate || t->fp32, "eth_adapter_linear_bwd: accumulate needs an fp32 gradient");
+  return desc->dtype == ETH_F16
+             ? adapter_backward<true>(desc, x, w, lora_a, lora_b, dy, ut, tile_scale, dx, da, db, (char*)workspace,
+                                      (hipStream_t)stream)
+             : adapter_backward<false>(desc, x, w, lora_a, lora_b, dy, ut, tile_scale, dx, da, db, (char*)workspace,
+                                       (hipStream_t)stream);
+}

@@ -112,64 +112,6 @@ extern "C" int eth_gemm_plan(int64_t M, int64_t N, int64_t K, int a_kcontig, int
   return ETH_OK;
 }
 
-namespace eth {
-struct SplitSum {
-  const float* W;   // [splits][M][N] partial products
-  int splits;
-  int64_t stride;   // elements between splits
-  void* C;
-  int64_t ldc;
-  const uint16_t* bias;
-  int M, N;
-  int c_dtype, flags;
-  float alpha;
-};
-// C[m, n] (+)= alpha * sum_s W[s][m*N + n] (+ bias[n]), splits added in order
-// (deterministic) and rounded once.  Four columns a thread; the splits' loads
-// go out four at a time.
-template <bool FP16>
-__global__ void __launch_bounds__(256) splitk_sum_kernel(SplitSum g) {
-  const int nq = g.N / 4;
-  const int64_t total = (int64_t)g.M * nq;
-  for (int64_t q = blockIdx.x * 256LL + threadIdx.x; q < total; q += gridDim.x * 256LL) {
-    const int m = (int)(q / nq), n = (int)(q - (int64_t)m * nq) * 4;
-    const float* w = g.W + (int64_t)m * g.N + n;
-    f32x4_t v = *reinterpret_cast<const f32x4_t*>(w);
-    int s = 1;
-    for (; s + 3 < g.splits; s += 4) {
-      f32x4_t u[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) u[e] = *reinterpret_cast<const f32x4_t*>(w + (s + e) * g.stride);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v += u[e];
-    }
-    for (; s < g.splits; ++s) v += *reinterpret_cast<const f32x4_t*>(w + s * g.stride);
-    float bn[4] = {0.f, 0.f, 0.f, 0.f};
-    if (g.bias) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bn[e] = FP16 ? h2f_bits(g.bias[n + e]) : bf2f(g.bias[n + e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = v[e] * g.alpha + bn[e];
-    const int64_t o = (int64_t)m * g.ldc + n;
-    if (g.c_dtype == ETH_F32) {
-      f32x4_t* c = reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(g.C) + o);
-      *c = (g.flags & ETH_GEMM_ACCUMULATE) ? *c + v : v;
-    } else {
-      u32x2_t r;
-      if (g.c_dtype == ETH_BF16) {
-        r.x = f2bf_pair(v[0], v[1]);
-        r.y = f2bf_pair(v[2], v[3]);
-      } else {
-        r.x = f2h_bits(v[0]) | ((uint32_t)f2h_bits(v[1]) << 16);
-        r.y = f2h_bits(v[2]) | ((uint32_t)f2h_bits(v[3]) << 16);
-      }
-      *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint16_t*>(g.C) + o) = r;
-    }
-  }
-}
-}  // namespace eth
-
 extern "C" int64_t eth_gemm_splitk_workspace(int64_t M, int64_t N, int splits) {
   return splits > 0 && M > 0 && N > 0 ? (int64_t)splits * M * N * 4 : 0;
 }

@@ -227,8 +227,8 @@ struct GemmArgs {
 //  * kSized: size(g) puts sizes that only the device knows into g (at most
 //    those of the launch; row tiles past g.M leave at once);
 //  * kGathers: row r of A lies at row rows[r];
-//  * kStarts: start(acc, row0, col0, M, N) puts the accumulators' first values
-//    in place of zeros (split-K: in the first split);
+//  * kStarts: start<FP16, PINNED>(acc, row0, col0, M, N) adds to the zeros that
+//    the accumulators start at (split-K: in the first split);
 //  * kMaps: map(acc, row0, col0, M, N) changes the accumulators before C is
 //    stored;
 //  * kReduces: reduce(acc, row0, col0, M, N) takes the place of storing C.
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(256, 1) gemm256_m16_kernel(GemmArgs g, X x) {
 #undef PRO_Q
   }
   if constexpr (X::kStarts) {
-    if (split == 0) x.template start<FP16>(acc, m0 + wm * 128, n0 + wn * 128, g.M, g.N);
+    if (split == 0) x.template start<FP16, true>(acc, m0 + wm * 128, n0 + wn * 128, g.M, g.N);
     PIN_ACC
   }
   dma_barrier_but<12>();
@@ -990,7 +990,7 @@ __global__ void __launch_bounds__(256, 1) gemm_ring_kernel(GemmArgs g, X x) {
   for (int i = 0; i < TI; ++i)
 #pragma unroll
     for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if constexpr (X::kStarts) x.template start<FP16>(acc, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
+  if constexpr (X::kStarts) x.template start<FP16, false>(acc, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
 
   // lane offsets of the fragments of k-step 0 (k-step 1: see frag): lane l
   // holds row l%16 of the block, k 8*(l/16) .. +7
@@ -1274,6 +1274,62 @@ inline GemmCut plan_cut(int64_t M, int64_t N, int64_t K, bool wide, GemmForm for
 // and a C extent plus one tile of rows below 2 GiB (their buffer offsets).
 inline bool wide_takes(int64_t M, int64_t N, int64_t ldc, int esz, bool c_vec) {
   return c_vec && ((M + 255) * ldc + N) * esz < (1LL << 31);
+}
+
+struct SplitSum {
+  const float* W;   // [splits][M][N] partial products
+  int splits;
+  int64_t stride;   // elements between splits
+  void* C;
+  int64_t ldc;
+  const uint16_t* bias;
+  int M, N;
+  int c_dtype, flags;
+  float alpha;
+};
+// C[m, n] (+)= alpha * sum_s W[s][m*N + n] (+ bias[n]), splits added in order
+// (deterministic) and rounded once.  Four columns a thread; the splits' loads
+// go out four at a time.
+template <bool FP16>
+__global__ void __launch_bounds__(256) splitk_sum_kernel(SplitSum g) {
+  const int nq = g.N / 4;
+  const int64_t total = (int64_t)g.M * nq;
+  for (int64_t q = blockIdx.x * 256LL + threadIdx.x; q < total; q += gridDim.x * 256LL) {
+    const int m = (int)(q / nq), n = (int)(q - (int64_t)m * nq) * 4;
+    const float* w = g.W + (int64_t)m * g.N + n;
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(w);
+    int s = 1;
+    for (; s + 3 < g.splits; s += 4) {
+      f32x4_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) u[e] = *reinterpret_cast<const f32x4_t*>(w + (s + e) * g.stride);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v += u[e];
+    }
+    for (; s < g.splits; ++s) v += *reinterpret_cast<const f32x4_t*>(w + s * g.stride);
+    float bn[4] = {0.f, 0.f, 0.f, 0.f};
+    if (g.bias) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bn[e] = FP16 ? h2f_bits(g.bias[n + e]) : bf2f(g.bias[n + e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = v[e] * g.alpha + bn[e];
+    const int64_t o = (int64_t)m * g.ldc + n;
+    if (g.c_dtype == ETH_F32) {
+      f32x4_t* c = reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(g.C) + o);
+      *c = (g.flags & ETH_GEMM_ACCUMULATE) ? *c + v : v;
+    } else {
+      u32x2_t r;
+      if (g.c_dtype == ETH_BF16) {
+        r.x = f2bf_pair(v[0], v[1]);
+        r.y = f2bf_pair(v[2], v[3]);
+      } else {
+        r.x = f2h_bits(v[0]) | ((uint32_t)f2h_bits(v[1]) << 16);
+        r.y = f2h_bits(v[2]) | ((uint32_t)f2h_bits(v[3]) << 16);
+      }
+      *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint16_t*>(g.C) + o) = r;
+    }
+  }
 }
 
 }  // namespace eth

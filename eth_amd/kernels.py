@@ -1019,6 +1019,118 @@ def linear_xent_bwd(hidden2d, weight, labels, lse, dloss, ignore_index=-100, nee
     return dhidden, dweight
 
 
+def _adapter_desc(x2d, weight, lora_a, lora_b, rows, *ts):
+    """(device index, descriptor) of an adapted projection's operands, for the
+    rows of `rows` (AdapterRows)."""
+    index = rows.device.index
+    _check_device(index, x2d, weight, lora_a, lora_b, *ts)
+    code = _HALF_CODES.get(x2d.dtype)
+    if code is None or any(t.dtype != x2d.dtype for t in (weight, lora_a, lora_b)):
+        raise ValueError(f"adapted projections need bf16 or fp16 tensors of one type, got "
+                         f"{', '.join(str(t.dtype) for t in (x2d, weight, lora_a, lora_b))}")
+    if x2d.dim() != 2 or weight.dim() != 2 or lora_a.dim() != 3 or lora_b.dim() != 3:
+        raise ValueError("x [rows, in], weight [out, in], lora_a [adapters, r, in] and lora_b [adapters, out, r] are needed")
+    M, K = x2d.shape
+    N = weight.shape[0]
+    adapters, r, _ = lora_a.shape
+    if weight.shape[1] != K or lora_a.shape[2] != K or lora_b.shape != (adapters, N, r) or M != rows.total:
+        raise ValueError(f"x {tuple(x2d.shape)}, weight {tuple(weight.shape)}, lora_a {tuple(lora_a.shape)}, lora_b "
+                         f"{tuple(lora_b.shape)} and {rows.total} rows do not match")
+    if K < 1 or N < 1 or K % 8 or N % 8:
+        raise ValueError(f"in and out must be multiples of 8 (got {K}, {N})")
+    if not 8 <= r <= 128 or r % 8:
+        raise ValueError(f"the rank must be a multiple of 8 up to 128 (got {r})")
+    if rows.n_listed > adapters or not 0 < adapters < 65536:
+        raise ValueError(f"rows use adapter {rows.n_listed - 1} of {adapters}")
+    desc = nat.AdapterDesc()
+    strides = []
+    for name, t in (("x", x2d), ("weight", weight)):
+        ld, s1 = t.stride()
+        ld = K if t.shape[0] <= 1 else ld
+        if s1 != 1 or ld < K or ld % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name}: rows must be contiguous, 16-byte aligned and apart")
+        strides.append(ld)
+    for name, t in (("lora_a", lora_a), ("lora_b", lora_b)):
+        if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+    desc.rows, desc.in_, desc.out, desc.ldx, desc.ldw = M, K, N, *strides
+    desc.tiles, desc.chunks, desc.first_chunk, desc.used, desc.of_row = rows.addresses
+    desc.n_tiles, desc.n_chunks, desc.n_used, desc.n_listed = rows.n_tiles, rows.n_chunks, rows.n_used, rows.n_listed
+    desc.adapters, desc.rank, desc.dtype = adapters, r, code
+    return index, desc
+
+
+def _adapter_workspace(desc, backward, device):
+    size = nat.value("eth_adapter_linear_workspace", ctypes.byref(desc), backward)
+    if size < 0:
+        raise ValueError(nat.load().eth_last_error().decode(errors="replace"))
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def adapter_linear_fwd(x2d, weight, bias, lora_a, lora_b, rows, save=False):
+    """(y [rows, out], saved): y = x2d weight^T + bias + scale (x2d A^T) B^T with
+    each row's adapter (A [r, in] and B [out, r] of lora_a and lora_b) and scale of
+    `rows` (AdapterRows); rows of no adapter without the last term.  saved: what
+    dB needs, or None without `save`."""
+    index, desc = _adapter_desc(x2d, weight, lora_a, lora_b, rows)
+    M, N, rp = desc.rows, desc.out, -(-desc.rank // 32) * 32
+    if bias is not None:
+        _check_device(index, bias)
+        if bias.dtype != x2d.dtype or bias.shape != (N,) or not bias.is_contiguous():
+            raise ValueError("bias must be a contiguous [out] tensor of the input type")
+    new = functools.partial(torch.empty, device=x2d.device)
+    y = new(M, N, dtype=x2d.dtype)
+    saved = None
+    if save:
+        saved = (new(rows.n_tiles, rp, nat.ADAPTER_TILE_ROWS, dtype=x2d.dtype),
+                 new(rows.n_tiles, dtype=torch.float32))
+    ut, tile_scale = saved or (None, None)
+    ws = _adapter_workspace(desc, 0, x2d.device)
+    rows.in_use()
+    _launch(index, "eth_adapter_linear_fwd", ctypes.byref(desc), x2d.data_ptr(), weight.data_ptr(), nat.ptr(bias),
+            lora_a.data_ptr(), lora_b.data_ptr(), y.data_ptr(), nat.ptr(ut), nat.ptr(tile_scale), ws.data_ptr())
+    return y, saved
+
+
+def adapter_linear_bwd(x2d, weight, lora_a, lora_b, dy, rows, saved=None, need_dx=True, da=None, db=None):
+    """dx [rows, in] (None without need_dx) of adapter_linear_fwd for contiguous dy
+    [rows, out].  da, db: pairs (tensor like lora_a / lora_b, in their type or fp32,
+    that the gradient is written to, whether it is added, fp32 alone), or None; db
+    needs the forward's `saved`.  Adapters without rows get zeros."""
+    index, desc = _adapter_desc(x2d, weight, lora_a, lora_b, rows, dy)
+    if dy.shape != (desc.rows, desc.out) or dy.dtype != x2d.dtype or not dy.is_contiguous() or dy.data_ptr() % 16:
+        raise ValueError("dy must be a contiguous, 16-byte aligned [rows, out] tensor of the input type")
+    grads = []
+    for name, pair, like in (("da", da, lora_a), ("db", db, lora_b)):
+        entry = nat.AdapterGrad()
+        if pair is not None:
+            t, accumulate = pair
+            _check_device(index, t)
+            if t.shape != like.shape or t.dtype not in (like.dtype, torch.float32) or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous tensor like its adapters, or fp32")
+            if t.data_ptr() % 16 or accumulate and t.dtype != torch.float32:
+                raise ValueError(f"{name} must be 16-byte aligned, and fp32 where it is added to")
+            entry.grad, entry.fp32, entry.accumulate = t.data_ptr(), t.dtype == torch.float32, bool(accumulate)
+        grads.append(entry)
+    ut, tile_scale = saved or (None, None)
+    if db is not None:
+        rp = -(-desc.rank // 32) * 32
+        if (saved is None or ut.shape != (rows.n_tiles, rp, nat.ADAPTER_TILE_ROWS) or ut.dtype != x2d.dtype
+                or not ut.is_contiguous() or tile_scale.shape != (rows.n_tiles,) or tile_scale.dtype != torch.float32
+                or not tile_scale.is_contiguous()):
+            raise ValueError("db needs what the forward saved")
+        _check_device(index, ut, tile_scale)
+    dx = torch.empty(desc.rows, desc.in_, dtype=x2d.dtype, device=x2d.device) if need_dx else None
+    if not need_dx and da is None and db is None:
+        return None
+    ws = _adapter_workspace(desc, 1, x2d.device)
+    rows.in_use()
+    _launch(index, "eth_adapter_linear_bwd", ctypes.byref(desc), x2d.data_ptr(), weight.data_ptr(), lora_a.data_ptr(),
+            lora_b.data_ptr(), dy.data_ptr(), nat.ptr(ut), nat.ptr(tile_scale), nat.ptr(dx), ctypes.byref(grads[0]),
+            ctypes.byref(grads[1]), ws.data_ptr())
+    return dx
+
+
 def synthetic_batch(sample_ids, seq, vocab, device):
     """tokens [b, s] int64, loss_mask [b, s] fp32, position_ids [b, s] int64
     of the deterministic synthetic batch, computed on the device in one

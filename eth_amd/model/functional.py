@@ -703,3 +703,61 @@ class LinearCrossEntropyFn(torch.autograd.Function):
             grad_written(weight)
             dw = None
         return None if dh is None else dh.view(ctx.shape), dw, None, None, None
+
+
+def _adapter_target(p, need):
+    """(pair for K.adapter_linear_bwd, gradient to return) of lora_a or lora_b."""
+    if not need:
+        return None, None
+    mg, accumulate = _fp32_accum_target(p)
+    if mg is not None:
+        return (mg, accumulate), None
+    new = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+    return (new, False), new
+
+
+class AdapterLinearFn(torch.autograd.Function):
+    """y = x @ W^T (+ bias) + scale (x @ A^T) @ B^T: LinearFn with each row's
+    low-rank adapter beside the shared weight; A [r, in] and B [out, r] of lora_a
+    [adapters, r, in] and lora_b [adapters, out, r], adapters and scales of the rows
+    by `rows` (eth_amd.packed.AdapterRows, whose total are x's rows).  Rows of no
+    adapter are LinearFn's."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, lora_a, lora_b, rows):
+        x2 = _aligned_rows(x)
+        y, saved = K.adapter_linear_fwd(x2, weight, bias, lora_a, lora_b, rows, save=ctx.needs_input_grad[4])
+        ctx.save_for_backward(x2, weight, bias, lora_a, lora_b, *(saved or ()))
+        ctx.rows, ctx.in_shape = rows, x.shape
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        x2, weight, bias, lora_a, lora_b, *saved = ctx.saved_tensors
+        x2, dy2 = _aligned_rows(x2), _whole(dy).view(-1, weight.shape[0])
+        needs = ctx.needs_input_grad
+        (da, ga), (db, gb) = (_adapter_target(p, need) for p, need in ((lora_a, needs[3]), (lora_b, needs[4])))
+        dx = K.adapter_linear_bwd(x2, weight, lora_a, lora_b, dy2, ctx.rows, tuple(t.contiguous() for t in saved) or None,
+                                  needs[0], da, db)
+        for p, pair, g in ((lora_a, da, ga), (lora_b, db, gb)):
+            if pair is not None and g is None:
+                grad_written(p)
+        dw = dbias = None
+        if needs[1]:
+            mg, accumulate = _fp32_accum_target(weight)
+            pad = -x2.shape[0] % 8  # (the product takes depths that are multiples of 8)
+            dyw, xw = (torch.nn.functional.pad(t, (0, 0, 0, pad)) if pad else t for t in (dy2, x2))
+            if mg is not None:
+                _wgrad(weight, dyw, xw, mg, accumulate)
+                grad_written(weight)
+            else:
+                dw = K.gemm(dyw.t(), xw, out_dtype=weight.dtype)
+        if bias is not None and needs[2]:
+            mg, accumulate = _fp32_accum_target(bias)
+            acc = mg if mg is not None else torch.empty(bias.shape, dtype=torch.float32, device=bias.device)
+            K.col_sum(dy2, acc, accumulate=accumulate)
+            if mg is None:
+                dbias = acc.to(bias.dtype)
+            else:
+                grad_written(bias)
+        return None if dx is None else dx.view(ctx.in_shape), dw, dbias, ga, gb, None

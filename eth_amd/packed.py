@@ -1,4 +1,4 @@
-"""Sequences of different lengths packed into one row dimension.
+"""Sequences and tasks of different lengths packed into one row dimension.
 
 `PackedSequences` is what the packed attention kernels need to know of a
 batch: which rows form which sequence, as device lists of tiles (blocks of
@@ -6,6 +6,8 @@ queries, blocks of keys, and blocks of rows that no sequence covers), built and
 checked once on the host and shared by every layer of the batch, forward and
 backward.  The lists are ordered by the length of a tile's chain, so that the
 longest start first.
+
+`AdapterRows` is the same for low-rank adapters: which rows use which adapter.
 """
 
 import operator
@@ -68,7 +70,50 @@ def split_chains(chain, heads, slots):
     return int(np.searchsorted(-chain, -steps, side="left")), -(-longest // steps), steps
 
 
-class PackedSequences:
+def _checked_lengths(lengths, what):
+    if isinstance(lengths, torch.Tensor):
+        if lengths.dim() != 1 or lengths.is_floating_point() or lengths.dtype == torch.bool:
+            raise ValueError("lengths must be a one-dimensional list of whole numbers")
+        lengths = lengths.tolist()
+    lengths = list(lengths)
+    for x in lengths:
+        if type(x) is not int and not isinstance(x, np.integer) or x < 0:
+            raise ValueError(f"a {what} length must be a whole number of at least 0, got {x!r}")
+    return tuple(int(x) for x in lengths)
+
+
+def _checked_total(total, covered, what):
+    if isinstance(total, (bool, float)):
+        raise ValueError(f"total must be a whole number, got {total!r}")
+    total = covered if total is None else operator.index(total)
+    if not covered <= total or not 0 < total < 2**31:
+        raise ValueError(f"total must be at least 1, at least the {covered} rows of the {what}, and below 2^31 "
+                         f"(got {total})")
+    return total
+
+
+def _checked_device(device, what):
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"{what} live on the GPU (no CPU fallback)")
+    return device if device.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
+class _DeviceLists:
+    """Lists of a batch's rows in device memory, uploaded once."""
+
+    def _upload(self, table):
+        self._table = nat.table_to_device(table, self.device)
+        self._home = nat.stream_ptr(self.device)
+
+    def in_use(self):
+        """A launch on the current stream is about to read the lists."""
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._home:
+            if not torch.cuda.is_current_stream_capturing():
+                self._table.record_stream(torch.cuda.current_stream(self.device))
+
+
+class PackedSequences(_DeviceLists):
     """Rows [0, lengths[0]) are the first sequence, the next lengths[1] rows
     the second, and so on; rows from sum(lengths) to `total` (default: none)
     belong to no sequence.  Lengths may be zero.  Device lists are uploaded
@@ -77,31 +122,12 @@ class PackedSequences:
     as long as a graph that was captured with it is replayed."""
 
     def __init__(self, lengths, total=None, device="cuda"):
-        if isinstance(lengths, torch.Tensor):
-            if lengths.dim() != 1 or lengths.is_floating_point() or lengths.dtype == torch.bool:
-                raise ValueError("lengths must be a one-dimensional list of whole numbers")
-            lengths = lengths.tolist()
-        lengths = list(lengths)
-        for x in lengths:
-            if type(x) is not int and not isinstance(x, np.integer) or x < 0:
-                raise ValueError(f"a sequence length must be a whole number of at least 0, got {x!r}")
-        self.lengths = tuple(int(x) for x in lengths)
-        covered = sum(self.lengths)
-        if isinstance(total, (bool, float)):
-            raise ValueError(f"total must be a whole number, got {total!r}")
-        self.total = covered if total is None else operator.index(total)
-        if not covered <= self.total or not 0 < self.total < 2**31:
-            raise ValueError(f"total must be at least 1, at least the {covered} rows of the sequences, and below 2^31 "
-                             f"(got {self.total})")
-        self.device = torch.device(device)
-        if self.device.type != "cuda":
-            raise ValueError("packed sequences live on the GPU (no CPU fallback)")
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.lengths = _checked_lengths(lengths, "sequence")
+        self.total = _checked_total(total, sum(self.lengths), "sequences")
+        self.device = _checked_device(device, "packed sequences")
         lists = {rows: _tile_list(self.lengths, self.total, rows, True) for rows in QUERY_TILE_ROWS}
         lists["keys"] = _tile_list(self.lengths, self.total, KEY_TILE_ROWS, False)
-        self._table = nat.table_to_device(np.concatenate([tiles for tiles, _ in lists.values()]), self.device)
-        self._home = nat.stream_ptr(self.device)
+        self._upload(np.concatenate([tiles for tiles, _ in lists.values()]))
         self._chains = {key: chain for key, (_, chain) in lists.items()}
         self._at, at = {}, self._table.data_ptr()
         for key, (tiles, _) in lists.items():
@@ -109,12 +135,6 @@ class PackedSequences:
             at += tiles.nbytes
         self._plans = {}
         self.descriptors = {}  # of calls with this plan, by shapes and strides
-
-    def in_use(self):
-        """A launch on the current stream is about to read the lists."""
-        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._home:
-            if not torch.cuda.is_current_stream_capturing():
-                self._table.record_stream(torch.cuda.current_stream(self.device))
 
     def plan(self, heads, kv_heads, head_dim):
         """(query list address and count, key list address and count, query
@@ -130,3 +150,72 @@ class PackedSequences:
             k_split = split_chains(self._chains["keys"] * (heads // kv_heads), kv_heads, (1 if head_dim > 96 else 2) * cus)
             plan = self._plans[heads, kv_heads, head_dim] = (*self._at[rows], *self._at["keys"], q_split, k_split)
         return plan
+
+
+MIN_CHUNK, MAX_CHUNK, CHUNKS = 4, 16, 16  # tiles of a partial gradient sum, and how many sums a batch is cut into
+
+
+def adapter_tiles(lengths, ids, scales, rows=nat.ADAPTER_TILE_ROWS):
+    """(tiles, chunks, first_chunk, used) of segments of the given lengths, adapter
+    ids (-1: none) and scales: up to `rows` rows of one segment a tile, ordered by
+    adapter; runs of tiles of one adapter, whose gradients are summed together;
+    where each adapter's chunks start; and the adapters that have rows."""
+    lengths, ids = np.asarray(lengths, dtype=np.int64).reshape(-1), np.asarray(ids, dtype=np.int64).reshape(-1)
+    begins = np.cumsum(lengths) - lengths
+    counts = np.where(ids >= 0, -(-lengths // rows), 0)
+    seg = np.repeat(np.arange(lengths.size), counts)
+    start = (np.arange(seg.size) - np.repeat(np.cumsum(counts) - counts, counts)) * rows
+    order = np.argsort(ids[seg], kind="stable")
+    seg, start = seg[order], start[order]
+    tiles = np.zeros(seg.size, dtype=nat.ADAPTER_TILE_DTYPE)
+    tiles["row"], tiles["rows"] = begins[seg] + start, np.minimum(rows, lengths[seg] - start)
+    tiles["adapter"], tiles["scale"] = ids[seg], np.asarray(scales, dtype=np.float32).reshape(-1)[seg]
+    per = max(MIN_CHUNK, min(MAX_CHUNK, -(-seg.size // CHUNKS)))
+    used, first, many = np.unique(tiles["adapter"], return_index=True, return_counts=True)
+    pieces = -(-many // per)
+    chunks = np.zeros(int(pieces.sum()), dtype=nat.ADAPTER_CHUNK_DTYPE)
+    at = (np.arange(chunks.size) - np.repeat(np.cumsum(pieces) - pieces, pieces)) * per
+    chunks["first"] = np.repeat(first, pieces) + at
+    chunks["tiles"] = np.minimum(per, np.repeat(many, pieces) - at)
+    listed = int(used[-1]) + 1 if used.size else 0
+    first_chunk = np.zeros(listed + 1, dtype=np.int32)
+    first_chunk[used.astype(np.int64) + 1] = pieces
+    return tiles, chunks, np.cumsum(first_chunk, dtype=np.int32), used.astype(np.int32)
+
+
+class AdapterRows(_DeviceLists):
+    """Rows [0, lengths[0]) use adapter ids[0] with scales[0] (default: one), the
+    next lengths[1] rows ids[1], and so on; id -1, and rows from sum(lengths) to
+    `total` (default: none), use no adapter.  Lengths may be zero, and an adapter
+    may serve several segments.  Device lists are uploaded here (the host waits for
+    the current stream), so make it ahead of the work that needs it and outside of a
+    graph capture, and keep it for as long as a graph that was captured with it is
+    replayed."""
+
+    def __init__(self, lengths, ids, scales=None, total=None, device="cuda"):
+        self.lengths = _checked_lengths(lengths, "segment")
+        ids = ids.tolist() if isinstance(ids, torch.Tensor) else list(ids)
+        scales = [1.0] * len(ids) if scales is None else scales.tolist() if isinstance(scales, torch.Tensor) else list(scales)
+        if not len(ids) == len(scales) == len(self.lengths):
+            raise ValueError(f"{len(self.lengths)} segments, {len(ids)} ids and {len(scales)} scales do not match")
+        for x in ids:
+            if type(x) is not int and not isinstance(x, np.integer) or not -1 <= x < 65535:
+                raise ValueError(f"an adapter id must be -1 or a whole number from 0 to 65534, got {x!r}")
+        self.ids, self.scales = tuple(int(x) for x in ids), tuple(float(x) for x in scales)
+        if not all(abs(x) <= 2.0**64 for x in self.scales):
+            raise ValueError("scales must be finite, up to 2^64")
+        self.total = _checked_total(total, sum(self.lengths), "segments")
+        self.device = _checked_device(device, "adapter rows")
+        tiles, chunks, first_chunk, used = adapter_tiles(self.lengths, self.ids, self.scales)
+        of_row = np.full(self.total, -1, dtype=np.int32)
+        of_row[: sum(self.lengths)] = np.repeat(np.asarray(self.ids, dtype=np.int32), self.lengths)
+        self.n_tiles, self.n_chunks, self.n_used, self.n_listed = tiles.size, chunks.size, used.size, first_chunk.size - 1
+        if self.n_tiles >= 2**23 or self.n_chunks >= 2**16:
+            raise ValueError(f"{self.n_tiles} tiles in {self.n_chunks} sums are too many for one call")
+        parts = [tiles, chunks, first_chunk, used, of_row]
+        self._upload(np.concatenate([np.ascontiguousarray(x).view(np.uint8) for x in parts]))
+        at = self._table.data_ptr()
+        self.addresses = []  # of tiles, chunks, first_chunk, used and of_row
+        for x in parts:
+            self.addresses.append(at)
+            at += x.nbytes

@@ -458,6 +458,69 @@ int eth_packed_attn_bwd(const eth_packed_attn_desc_t* desc, const void* q, const
                         float* delta, void* dq, void* dk, void* dv, void* workspace,
                         void* stream);
 
+/* Low-rank adapters of many tasks beside a shared projection, on x [rows, in] (row
+ * stride ldx), w [out, in] (row stride ldw), lora_a [adapters, rank, in] and lora_b
+ * [adapters, out, rank] (contiguous), all bf16 or fp16 (`dtype`), 16-byte aligned;
+ * in, out and strides multiples of 8, rank a multiple of 8 up to 128, operands below
+ * 2 GiB:
+ *   y = x w^T + bias + scale (x A_a^T) B_a^T   for rows of adapter a,
+ * without the last term for rows of none (bias [out] may be NULL; y contiguous).
+ *
+ * The lists are device memory and are not checked.  of_row [rows]: a row's adapter,
+ * -1 for none.  tiles [n_tiles]: up to 32 consecutive rows of one adapter and their
+ * scale, every adapted row in one tile, ordered by adapter.  chunks [n_chunks]:
+ * consecutive tiles of one adapter, every tile in one chunk, in the tiles' order (what
+ * one partial sum of a gradient is taken over).  first_chunk [n_listed + 1]:
+ * where an adapter's chunks start (those from n_listed on have none).  used [n_used]: the adapters that have tiles.  Adapters
+ * may have none, and n_tiles may be 0.
+ *
+ * The forward leaves in `ut` (n_tiles * 32 * rank rounded up to 32, 16-bit; NULL
+ * where no dB is wanted) and in fp16 tile_scale [n_tiles] what dB needs.  The
+ * backward writes dx [rows, in] (contiguous, or NULL) and the adapters' gradients
+ * (each NULL, in `dtype`, or fp32, then stored, or added to with `accumulate`), zeros
+ * for adapters without rows; dy is contiguous.  Sums are fp32, in a fixed order;
+ * x A^T and dy B are rounded to 16 bits for their second products (in fp16 times a
+ * power of two, so they keep their digits at any size).  Values that are not finite
+ * reach no other task's rows or gradients; one in an adapter makes its own rows NaN,
+ * in its column or, where they share 128 rows with another adapter's, in up to 128
+ * columns about it.  `workspace`: eth_adapter_linear_workspace bytes
+ * (-1: refused), 256-byte aligned. */
+#define ETH_ADAPTER_TILE_ROWS 32
+
+typedef struct eth_adapter_tile {
+  int32_t row, rows, adapter;
+  float scale;
+} eth_adapter_tile_t;
+
+typedef struct eth_adapter_chunk {
+  int32_t first, tiles;
+} eth_adapter_chunk_t;
+
+typedef struct eth_adapter_desc {
+  int64_t rows, in, out, ldx, ldw;
+  const eth_adapter_tile_t* tiles;
+  const eth_adapter_chunk_t* chunks;
+  const int32_t* first_chunk;
+  const int32_t* used;
+  const int32_t* of_row;
+  int32_t n_tiles, n_chunks, n_used, n_listed, adapters, rank, dtype, reserved;
+} eth_adapter_desc_t;
+
+typedef struct eth_adapter_grad {
+  void* grad;
+  int32_t fp32, accumulate;
+} eth_adapter_grad_t;
+
+int64_t eth_adapter_linear_workspace(const eth_adapter_desc_t* desc, int backward);
+int eth_adapter_linear_fwd(const eth_adapter_desc_t* desc, const void* x, const void* w,
+                           const void* bias, const void* lora_a, const void* lora_b, void* y,
+                           void* ut, float* tile_scale, void* workspace, void* stream);
+int eth_adapter_linear_bwd(const eth_adapter_desc_t* desc, const void* x, const void* w,
+                           const void* lora_a, const void* lora_b, const void* dy,
+                           const void* ut, const float* tile_scale, void* dx,
+                           const eth_adapter_grad_t* da, const eth_adapter_grad_t* db,
+                           void* workspace, void* stream);
+
 /* The norm behind a block, its gate, the scaled residual and the norm before the
  * next block, on contiguous [rows, cols] tensors of bf16 or fp16 (`dtype`; cols a
  * multiple of 8 up to 8192, rows below 2^26; 16-byte aligned):
