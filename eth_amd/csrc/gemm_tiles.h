@@ -220,12 +220,14 @@ struct GemmArgs {
   bool c_vec;        // C rows take 4-column vector accesses
   int k_split;              // split-K: k extent per split (0: one split of K)
   int64_t c_split_stride;   // split-K: elements between the splits' C slices
+  int splits;               // split-K: how many (read by kernels of device sizes)
 };
 
 // What a kernel adds to the plain product: a type X whose value is the
 // kernel's second argument.  Its flags compile in
 //  * kSized: size(g) puts sizes that only the device knows into g (at most
-//    those of the launch; row tiles past g.M leave at once);
+//    those of the launch; the tiles are those of g.M, workgroups past them leave
+//    at once: with the launch's tiles 3 empty rows of ten left two XCDs idle);
 //  * kGathers: row r of A lies at row rows[r];
 //  * kStarts: start<FP16, PINNED>(acc, row0, col0, M, N) adds to the zeros that
 //    the accumulators start at (split-K: in the first split);
@@ -308,18 +310,18 @@ __global__ void __launch_bounds__(256, 1) gemm256_m16_kernel(GemmArgs g, X x) {
   __shared__ __attribute__((aligned(16))) uint16_t smem[STAGE > EPI ? STAGE : EPI];
   __shared__ __attribute__((aligned(16))) uint16_t smem1[STAGE];
 
+  if constexpr (X::kSized) x.size(g);
   const int tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN;
   // split-K launches tiles * splits workgroups: split = blockIdx.x / tiles
   const int tiles = tiles_m * tiles_n;
+  if constexpr (X::kSized) {
+    if (tiles == 0 || blockIdx.x >= tiles * g.splits) return;
+  }
   const int split = blockIdx.x / tiles;
   const int kb = split * g.k_split;
   int tm, tn;
   tile_coords(blockIdx.x - split * tiles, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  if constexpr (X::kSized) {
-    x.size(g);
-    if (m0 >= g.M) return;
-  }
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid >> 1, wn = wid & 1;
   const int l16 = lane & 15, lg = lane >> 4;
@@ -954,14 +956,14 @@ __global__ void __launch_bounds__(256, 1) gemm_ring_kernel(GemmArgs g, X x) {
   __shared__ __attribute__((aligned(16))) uint16_t st2[STAGE];
   __shared__ __attribute__((aligned(16))) uint16_t st3[STAGE];
 
+  if constexpr (X::kSized) x.size(g);
   const int tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.N + BN - 1) / BN;
+  if constexpr (X::kSized) {
+    if (blockIdx.x >= tiles_m * tiles_n) return;
+  }
   int tm, tn;
   tile_coords(blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  if constexpr (X::kSized) {
-    x.size(g);
-    if (m0 >= g.M) return;
-  }
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int wm = wid >> 1, wn = wid & 1;
   const int l16 = lane & 15, lg = lane >> 4;

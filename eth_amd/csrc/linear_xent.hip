@@ -366,9 +366,11 @@ __global__ void __launch_bounds__(256) xent_finish_kernel(const int* at, const f
 
 // ------------------------------------------------------------------ host --
 template <bool A_K, bool B_K, bool FP16, bool SHORT, class X>
-static int launch_product(int tile, const GemmArgs& a, const X& x, hipStream_t s, int splits = 1) {
-  const int64_t tiles = (int64_t)((a.M + tile - 1) / tile) * ((a.N + tile - 1) / tile) * splits;
+static int launch_product(int tile, const GemmArgs& args, const X& x, hipStream_t s, int splits = 1) {
+  const int64_t tiles = (int64_t)((args.M + tile - 1) / tile) * ((args.N + tile - 1) / tile) * splits;
   const dim3 grid((unsigned)tiles);
+  GemmArgs a = args;
+  a.splits = splits;
   if (tile == 256) {
     if (SHORT || a.K % 64)  // (SHORT: the depth is the device's, its last k-tile of any length)
       gemm256_m16_kernel<A_K, B_K, FP16, true, X><<<grid, 256, 0, s>>>(a, x);
