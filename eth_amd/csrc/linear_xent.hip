@@ -33,9 +33,10 @@ namespace eth {
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // How a call's rows are listed: `count` rows take part, row r of the list
-// being row rows[r] of h with label[r] (clamped); `alpha` is dW's factor.
+// being row rows[r] of h with label[r] (clamped); `high` is the largest exponent
+// of their dloss, `alpha` dW's factor.
 struct XentHead {
-  int count;
+  int count, high;
   float alpha;
 };
 
@@ -79,6 +80,9 @@ struct XentStats {
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const int p = part0 + col0 / (TJ * 16);
     const bool edge = col0 + TJ * 16 > N;
+    int at_label[TI];  // (all in flight together: a row block at a time, each waits for its own)
+#pragma unroll
+    for (int i = 0; i < TI; ++i) at_label[i] = label[min(row0 + i * 16 + l16, M - 1)];
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       const int row = row0 + i * 16 + l16;
@@ -88,7 +92,7 @@ struct XentStats {
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[j * 4 + e] = acc[i][j][e];
-      const int t = (live ? label[row] : -1) - v0 - col0;
+      const int t = at_label[i] - v0 - col0;
       if (__ballot(live && t >= 0 && t < TJ * 16)) {
         // (one of a row's four lanes holds its label's logit; a column past N
         // is no label)
@@ -117,6 +121,7 @@ struct XentStats {
       for (int k = 0; k < TJ * 4; ++k) s += __builtin_amdgcn_exp2f(__builtin_fmaf(z[k], kLog2e, -at));
       s = row_sum(s);
       if (lg == 0 && live) part[((int64_t)(row >> 4) * parts + p) * 16 + l16] = XentPart{m2, s};
+      __builtin_amdgcn_sched_barrier(0);  // (a row block at a time, or its values are spilled)
     }
   }
 };
@@ -142,23 +147,39 @@ struct XentGrad {
   __device__ __forceinline__ void map(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int) const {
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const bool edge = col0 + TJ * 16 > n_real;
+    float at[TI], f[TI];
+    int t[TI];
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      const int row = row0 + i * 16 + l16;
-      const bool live = row < M;
-      const float at = live ? lse2[row] : 0.f, f = live ? mult[row] : 0.f;
-      const int t = (live ? label[row] : -1) - v0 - col0;
-      const bool here = __ballot(live && t >= 0 && t < TJ * 16) != 0;
+      const int row = min(row0 + i * 16 + l16, M - 1);  // (rows past M are not stored)
+      at[i] = lse2[row];
+      f[i] = mult[row];
+      t[i] = label[row] - v0 - col0;
+    }
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float d = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -at));
-          if (here && t == j * 16 + lg * 4 + e) d -= 1.f;
-          d *= f;
-          if (edge && col0 + j * 16 + lg * 4 + e >= n_real) d = 0.f;
-          acc[i][j][e] = d;
-        }
+        for (int e = 0; e < 4; ++e)
+          acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -at[i]));
+      if (__ballot(t[i] >= 0 && t[i] < TJ * 16)) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t[i] == j * 16 + lg * 4 + e) acc[i][j][e] -= 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] *= f[i];
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col0 + j * 16 + lg * 4 + e >= n_real) acc[i][j][e] = 0.f;
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -220,65 +241,74 @@ __device__ __forceinline__ int exponent_of(float v) {
 }
 
 __global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
-  __shared__ int sums[kListThreads / 64];
-  __shared__ int highs[kListThreads / 64];
+  constexpr int U = 8, WAVES = kListThreads / 64;  // rows of a thread a trip
+  __shared__ int counts[U * WAVES], highs[WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int64_t per = (g.n + kListThreads - 1) / kListThreads, a = tid * per, b = min(g.n, a + per);
   const bool back = g.dloss != nullptr;
-  int mine = 0, high = -1000;
-  for (int64_t r = a; r < b; ++r) {
-    if (g.labels[r] == g.ignore) continue;
-    if (back) {
-      const float d = g.dloss[r];
-      if (d == 0.f) continue;
-      if (__builtin_isfinite(d)) high = max(high, ilogbf(d));
-    }
-    ++mine;
-  }
-  // exclusive sum over the workgroup, and the largest exponent
-  int incl = mine;
+  int base = 0, high = -1000;
+  bool wild = false;
+  for (int64_t r0 = 0; r0 < g.n; r0 += U * kListThreads) {
+    int64_t t[U];
+    float d[U];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int v = __shfl_up(incl, o);
-    if (lane >= o) incl += v;
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * kListThreads + tid;
+      t[u] = r < g.n ? g.labels[r] : g.ignore;
+      d[u] = back && r < g.n ? g.dloss[r] : 1.f;
+    }
+    uint64_t on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      on[u] = __ballot(t[u] != g.ignore && d[u] != 0.f);
+      if (lane == 0) counts[u * WAVES + wid] = __popcll(on[u]);
+    }
+    __syncthreads();
+    // rows before each wave's of each step, in every wave: two entries a lane
+    static_assert(U * WAVES == 128, "two entries a lane");
+    const int c0 = counts[2 * lane], c1 = counts[2 * lane + 1];
+    int incl = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(incl, o);
+      if (lane >= o) incl += v;
+    }
+    const int excl = incl - c0 - c1, total = __shfl(incl, 63);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + u * kListThreads + tid;
+      const int entry = u * WAVES + wid, lo = __shfl(excl, entry >> 1), first = __shfl(c0, entry >> 1);
+      const int at = base + lo + (entry & 1 ? first : 0) + __popcll(on[u] & ((1ull << lane) - 1));
+      if (r >= g.n) continue;
+      if (!(on[u] >> lane & 1)) {
+        if (back)
+          g.at[r] = -1;
+        else
+          g.loss[r] = 0.f;
+        continue;
+      }
+      wild |= t[u] < 0 || t[u] >= g.vocab;
+      g.rows[at] = (int)r;
+      g.label[at] = (int)(t[u] < 0 ? 0 : t[u] >= g.vocab ? g.vocab - 1 : t[u]);
+      if (back) {
+        const int e = exponent_of(d[u]);
+        if (__builtin_isfinite(d[u])) high = max(high, e);
+        g.at[r] = at;
+        g.exps[at] = e;
+        g.lse2[at] = g.lse[r];
+        g.mult[at] = ldexpf(d[u], g.shift - e);
+        g.back[at] = ldexpf(1.f, e - g.shift);
+      }
+    }
+    base += total;
+    __syncthreads();  // (counts are free for the next trip)
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) high = max(high, __shfl_xor(high, o));
-  if (lane == 63) sums[wid] = incl;
   if (lane == 0) highs[wid] = high;
   __syncthreads();
-  int before = incl - mine, total = 0;
-  for (int w = 0; w < kListThreads / 64; ++w) {
-    if (w < wid) before += sums[w];
-    total += sums[w];
-    high = max(high, highs[w]);
-  }
+  for (int w = 0; w < WAVES; ++w) high = max(high, highs[w]);
   if (high == -1000) high = 0;
-  if (tid == 0) *g.head = XentHead{total, ldexpf(1.f, high - g.shift)};
-  bool wild = false;
-  for (int64_t r = a; r < b; ++r) {
-    const int64_t t = g.labels[r];
-    const float d = back ? g.dloss[r] : 1.f;
-    if (t == g.ignore || d == 0.f) {
-      if (back)
-        g.at[r] = -1;
-      else
-        g.loss[r] = 0.f;
-      continue;
-    }
-    wild |= t < 0 || t >= g.vocab;
-    g.rows[before] = (int)r;
-    g.label[before] = (int)(t < 0 ? 0 : t >= g.vocab ? g.vocab - 1 : t);
-    if (back) {
-      const int e = exponent_of(d);
-      g.at[r] = before;
-      g.exps[before] = e - high;
-      g.lse2[before] = g.lse[r];
-      g.mult[before] = ldexpf(d, g.shift - e);
-      g.back[before] = ldexpf(1.f, e - g.shift);
-    }
-    ++before;
-  }
+  if (tid == 0) *g.head = XentHead{base, high, ldexpf(1.f, high - g.shift)};
   if (wild && !back) *g.bad = 1;
 }
 
@@ -299,7 +329,15 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead*
   XentPart v{-INFINITY, 0.f};
   if (row < n) {
     const XentPart* mine = part + (int64_t)blockIdx.x * parts * 16 + r;
-    for (int p = k; p < parts; p += kJoinThreads / 16) v = join(v, mine[(int64_t)p * 16]);
+    constexpr int STEP = kJoinThreads / 16, U = 8;  // parts in flight
+    for (int p = k; p < parts; p += U * STEP) {
+      XentPart in[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        in[u] = p + u * STEP < parts ? mine[(int64_t)(p + u * STEP) * 16] : XentPart{-INFINITY, 0.f};
+#pragma unroll
+      for (int u = 0; u < U; ++u) v = join(v, in[u]);
+    }
   }
   red[k][r] = v;
   for (int half = kJoinThreads / 32; half; half >>= 1) {
@@ -324,7 +362,7 @@ __global__ void __launch_bounds__(256) xent_gather_kernel(const XentHead* head, 
   const int row = blockIdx.x;
   if (row >= head->count) return;
   const uint16_t* src = h + (int64_t)rows[row] * ldh;
-  const float f = ldexpf(1.f, exps[row]);
+  const float f = ldexpf(1.f, exps[row] - head->high);
   for (int c = threadIdx.x * 8; c < hidden; c += 256 * 8) {
     const uint4 raw = *reinterpret_cast<const uint4*>(src + c);
     const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
@@ -395,19 +433,41 @@ static int64_t room(int64_t bytes) { return up(bytes, 256); }
 // Columns of W that a launch's 32-bit offsets reach, whole 256s.
 static int64_t reach(int64_t ldw) { return std::max<int64_t>(256, kMaxBytes / (2 * ldw) / 256 * 256); }
 
+// The product [M, N] x K deep in whole rounds of 256x256 tiles and a rest along N
+// in its own best tile, where the time model promises 2 %: `first` columns, then the
+// others (`first` N: all in one).  (2048 rows of hidden 2048, vocabulary 50304: 1576
+// tiles, 6.2 rounds; as 1536 and a rest see the figures at the kernels' cases.)
+struct XentCut {
+  int64_t first;
+  int tile, rest;
+};
+static XentCut cut_columns(int64_t M, int64_t N, int64_t K, GemmForm form) {
+  XentCut c{N, plan_tile(M, N, K, true, form), 0};
+  const int64_t tm = (M + 255) / 256, tn = (N + 255) / 256, n1 = tm * tn / 256 * 256 / tm * 256;
+  if (c.tile != 256 || n1 <= 0 || n1 >= N) return c;
+  const int rest = plan_tile(M, N - n1, K, true, form);
+  if (tile_time(256, M, n1, K, 1, form) + tile_time(rest, M, N - n1, K, 1, form) <
+      0.98 * tile_time(256, M, N, K, 1, form))
+    c = XentCut{n1, 256, rest};
+  return c;
+}
+
 struct XentForward {
-  int tile;
-  int64_t chunk;  // columns of a launch
+  int64_t chunk;  // columns of a cut
   int64_t parts;  // of a row
   int64_t rows, label, picked, part, bytes;  // workspace offsets
 };
+// a wave has half a tile's columns
+static int64_t parts_of(int64_t cols, int tile) { return up(cols, tile) / (tile / 2); }
 static XentForward plan_forward(int64_t n, int64_t hidden, int64_t vocab, int64_t ldw) {
   XentForward p;
   p.chunk = std::min(vocab, reach(ldw));
-  p.tile = plan_tile(n, p.chunk, hidden, true, GemmForm{false, hidden % 64 != 0, 0});
-  const int64_t wide = p.tile / 2;  // columns of a wave
   p.parts = 0;
-  for (int64_t v = 0; v < vocab; v += p.chunk) p.parts += up(std::min(p.chunk, vocab - v), p.tile) / wide;
+  for (int64_t v = 0; v < vocab; v += p.chunk) {
+    const int64_t cols = std::min(p.chunk, vocab - v);
+    const XentCut c = cut_columns(n, cols, hidden, GemmForm{false, hidden % 64 != 0, 0});
+    p.parts += parts_of(c.first, c.tile) + (c.rest ? parts_of(cols - c.first, c.rest) : 0);
+  }
   int64_t o = room(sizeof(XentHead));
   p.rows = o, o += room(n * 4);
   p.label = o, o += room(n * 4);
@@ -418,24 +478,35 @@ static XentForward plan_forward(int64_t n, int64_t hidden, int64_t vocab, int64_
 }
 
 struct XentBackward {
-  int z_tile, w_tile;
   int splits;           // of dh's depth
-  int64_t piece, ldz;   // columns of a piece, of its rows
+  int64_t k_split;
+  int pieces;
+  int64_t piece, last, ldz;  // columns of a piece, of the last one, of their rows
   int64_t rows, label, at, exps, lse2, mult, back, gathered, dz, dh, bytes;
 };
 static XentBackward plan_backward(int64_t n, int64_t hidden, int64_t vocab, int64_t ldw, bool need_dh, bool need_dw) {
   XentBackward p;
   int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
   most = std::min(most, reach(std::max(ldw, hidden)));
-  const int64_t pieces = (vocab + most - 1) / most;
-  p.piece = std::min(up(vocab, 8), up((vocab + pieces - 1) / pieces, 256));
-  p.ldz = up(p.piece, 8);
-  p.z_tile = plan_tile(n, p.piece, hidden, true, GemmForm{false, hidden % 64 != 0, 0});
-  p.w_tile = plan_tile(p.piece, hidden, n, true, GemmForm{false, false, 0});
+  // whole rounds of dW's tiles where they fit
+  const int64_t tn = (hidden + 255) / 256;
+  int64_t unit = 256;
+  while (unit < 65536 && unit / 256 * tn % 256) unit *= 2;
+  const int64_t whole = most >= unit ? most / unit * unit : most;
+  // equal pieces of at most that, or whole ones and a last one of half to three halves
+  const int64_t many = std::max<int64_t>(1, (vocab + whole / 2 - 1) / whole);
+  p.piece = std::min(up(vocab, 8), whole);
+  p.last = vocab - (many - 1) * p.piece;
+  p.pieces = (int)many;
+  p.ldz = up(std::max(p.piece, p.last), 8);
   // dh has few tiles and a deep product: split until the chip is full
   const int64_t tiles = (n + 255) / 256 * ((hidden + 255) / 256);
   p.splits = 1;
-  while (p.splits < 16 && tiles * p.splits * 2 <= 256 && p.piece / (p.splits * 2) >= 512) p.splits *= 2;
+  // (the first piece fills every slice; the last may be deeper: its splits are)
+  const int64_t first = p.pieces > 1 ? p.piece : p.ldz;
+  while (p.splits < 16 && tiles * p.splits * 2 <= 256 && first / (p.splits * 2) >= 512) p.splits *= 2;
+  p.k_split = up((first + p.splits - 1) / p.splits, 64);
+  p.splits = (int)((first + p.k_split - 1) / p.k_split);
   int64_t o = room(sizeof(XentHead));
   for (int64_t* at : {&p.rows, &p.label, &p.at, &p.exps, &p.lse2, &p.mult, &p.back}) *at = o, o += room(n * 4);
   p.gathered = o, o += need_dw ? room(n * hidden * 2) : 0;
@@ -484,15 +555,20 @@ template <bool FP16>
 static int xent_forward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const XentForward& p, char* ws,
                         int64_t n, int64_t hidden, int64_t vocab, hipStream_t s) {
   int part0 = 0;
-  for (int64_t v0 = 0; v0 < vocab; v0 += p.chunk) {
-    const int64_t cols = std::min(p.chunk, vocab - v0);
+  auto columns = [&](int64_t v0, int64_t cols, int tile) {
     const GemmArgs a = product_args(h, (n - 1) * ldh + hidden, ldh, w + v0 * ldw, (cols - 1) * ldw + hidden, ldw, n,
                                     cols, hidden);
     const XentStats x{(const XentHead*)ws, (const int*)(ws + p.rows), (const int*)(ws + p.label),
                       (XentPart*)(ws + p.part), (float*)(ws + p.picked), (int)v0, part0, (int)p.parts};
-    const int rc = launch_product<true, true, FP16, false>(p.tile, a, x, s);
+    part0 += (int)parts_of(cols, tile);
+    return launch_product<true, true, FP16, false>(tile, a, x, s);
+  };
+  for (int64_t v0 = 0; v0 < vocab; v0 += p.chunk) {
+    const int64_t cols = std::min(p.chunk, vocab - v0);
+    const XentCut c = cut_columns(n, cols, hidden, GemmForm{false, hidden % 64 != 0, 0});
+    int rc = columns(v0, c.first, c.tile);
+    if (rc == ETH_OK && c.rest) rc = columns(v0 + c.first, cols - c.first, c.rest);
     if (rc != ETH_OK) return rc;
-    part0 += (int)(up(cols, p.tile) / (p.tile / 2));
   }
   return ETH_OK;
 }
@@ -512,18 +588,26 @@ static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int6
     ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
   }
   const int esz = dw_dtype == ETH_F32 ? 4 : 2;
-  for (int64_t v0 = 0; v0 < vocab; v0 += p.piece) {
-    const int64_t real = std::min(p.piece, vocab - v0), cols = up(real, 8);
+  for (int piece = 0; piece < p.pieces; ++piece) {
+    const int64_t v0 = piece * p.piece, real = piece == p.pieces - 1 ? p.last : p.piece, cols = up(real, 8);
     const uint16_t* wp = w + v0 * ldw;
     const int64_t w_elems = (real - 1) * ldw + hidden;
-    GemmArgs a = product_args(h, (n - 1) * ldh + hidden, ldh, wp, w_elems, ldw, n, cols, hidden);
-    a.C = dz;
-    a.ldc = p.ldz;
-    a.c_dtype = FP16 ? ETH_F16 : ETH_BF16;
-    a.c_vec = true;
-    const XentGrad grad{head, rows, (const int*)(ws + p.label), (const float*)(ws + p.lse2),
-                        (const float*)(ws + p.mult), (int)v0, (int)real};
-    int rc = launch_product<true, true, FP16, false>(p.z_tile, a, grad, s);
+    int rc = ETH_OK;
+    auto z_columns = [&](int64_t c0, int64_t many, int tile) {
+      const int64_t there = std::min(many, real - c0);
+      GemmArgs a = product_args(h, (n - 1) * ldh + hidden, ldh, wp + c0 * ldw, (there - 1) * ldw + hidden, ldw, n, many,
+                                hidden);
+      a.C = dz + c0;
+      a.ldc = p.ldz;
+      a.c_dtype = FP16 ? ETH_F16 : ETH_BF16;
+      a.c_vec = true;
+      const XentGrad grad{head, rows, (const int*)(ws + p.label), (const float*)(ws + p.lse2),
+                          (const float*)(ws + p.mult), (int)(v0 + c0), (int)there};
+      return launch_product<true, true, FP16, false>(tile, a, grad, s);
+    };
+    const XentCut zc = cut_columns(n, cols, hidden, GemmForm{false, hidden % 64 != 0, 0});
+    rc = z_columns(0, zc.first, zc.tile);
+    if (rc == ETH_OK && zc.rest) rc = z_columns(zc.first, cols - zc.first, zc.rest);
     if (rc != ETH_OK) return rc;
     if (dh) {
       GemmArgs d = product_args(dz, (n - 1) * p.ldz + cols, p.ldz, wp, w_elems, ldw, n, hidden, cols);
@@ -534,8 +618,9 @@ static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int6
       d.flags = v0 ? ETH_GEMM_ACCUMULATE : 0;
       const bool wide = wide_takes(n, hidden, hidden, 4, true);
       d.c_bytes = wide ? 1 : 0;
-      // the same split of the depth in every piece (the last may need fewer)
-      d.k_split = (int)up((p.piece + p.splits - 1) / p.splits, 64);
+      // (the same split of the depth in every piece: some need fewer splits)
+      const bool deeper = piece && cols > p.splits * p.k_split;
+      d.k_split = (int)(deeper ? up((cols + p.splits - 1) / p.splits, 64) : p.k_split);
       d.c_split_stride = n * hidden;
       const int splits = (int)((cols + d.k_split - 1) / d.k_split);
       if (!wide) d.k_split = 0;
@@ -543,23 +628,27 @@ static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int6
       if (rc != ETH_OK) return rc;
     }
     if (dw) {
-      GemmArgs d = product_args(dz, 0, p.ldz, gathered, 0, hidden, real, hidden, n);
-      d.C = (char*)dw + v0 * hidden * esz;
-      d.ldc = hidden;
-      d.c_dtype = dw_dtype;
-      d.flags = accumulate ? ETH_GEMM_ACCUMULATE : 0;
-      d.c_vec = true;
-      const bool wide = wide_takes(real, hidden, hidden, esz, true);
-      d.c_bytes = wide ? (uint32_t)(real * hidden * esz) : 0;
-      rc = launch_product<false, false, FP16, true>(wide || p.w_tile != 256 ? p.w_tile : 128, d, XentDepth{head}, s);
+      auto w_rows = [&](int64_t r0, int64_t many, int tile) {
+        GemmArgs d = product_args(dz + r0, 0, p.ldz, gathered, 0, hidden, many, hidden, n);
+        d.C = (char*)dw + (v0 + r0) * hidden * esz;
+        d.ldc = hidden;
+        d.c_dtype = dw_dtype;
+        d.flags = accumulate ? ETH_GEMM_ACCUMULATE : 0;
+        d.c_vec = true;
+        const bool wide = wide_takes(many, hidden, hidden, esz, true);
+        d.c_bytes = wide ? (uint32_t)(many * hidden * esz) : 0;
+        return launch_product<false, false, FP16, true>(wide || tile != 256 ? tile : 128, d, XentDepth{head}, s);
+      };
+      // (the same rule with dW's rows for columns)
+      const XentCut wc = cut_columns(hidden, real, n, GemmForm{esz == 4, false, 0});
+      rc = w_rows(0, wc.first, wc.tile);
+      if (rc == ETH_OK && wc.rest) rc = w_rows(wc.first, real - wc.first, wc.rest);
       if (rc != ETH_OK) return rc;
     }
   }
   if (dh) {
     const bool wide = wide_takes(n, hidden, hidden, 4, true);
-    // slices that the first, deepest piece filled
-    const int64_t k_split = up((p.piece + p.splits - 1) / p.splits, 64), first = up(std::min(p.piece, vocab), 8);
-    const int filled = wide ? (int)((first + k_split - 1) / k_split) : 1;
+    const int filled = wide ? p.splits : 1;
     xent_finish_kernel<FP16><<<(unsigned)n, 256, 0, s>>>((const int*)(ws + p.at), (const float*)(ws + p.back), slices,
                                                          filled, n * hidden, dh, (int)hidden);
     ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
