@@ -30,7 +30,6 @@ namespace eth {
 
 constexpr int kRnMaxCols = 8192;
 constexpr int kRnWaves = 4;     // rows of a forward workgroup
-constexpr int kRnBwdWaves = 8;  // waves of a backward workgroup
 
 template <bool FP16>
 __device__ __forceinline__ float rn_in(uint16_t v) {
@@ -161,16 +160,16 @@ __global__ void __launch_bounds__(64 * kRnWaves) rn_fwd_kernel(RnParams g, const
 }
 
 // Backward.  As in the LayerNorm backward, T waves share a row (a team), NVW
-// vectors of 512 columns each, a workgroup's teams walk the rows g, g + G, ...,
+// vectors of 512 columns each; a workgroup's W / T teams walk the rows g, g + G, ...,
 // the next row's loads are issued while one is computed, and column sums stay in
 // registers for all of a workgroup's rows.  Both norms' row sums meet in LDS, one
 // barrier each.
-template <int T, int NVW, bool FP16>
-__global__ void __launch_bounds__(64 * kRnBwdWaves) rn_bwd_kernel(
+template <int W, int T, int NVW, bool FP16>
+__global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
     RnParams p, const uint16_t* __restrict__ x, const uint16_t* __restrict__ h, const float* __restrict__ stats,
     const uint16_t* __restrict__ dh, const uint16_t* __restrict__ dy, uint16_t* __restrict__ dx,
     uint16_t* __restrict__ dres, float* __restrict__ part) {
-  constexpr int TEAMS = kRnBwdWaves / T;
+  constexpr int TEAMS = W / T;
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int team = wid / T, sub = wid - team * T;
@@ -197,7 +196,7 @@ __global__ void __launch_bounds__(64 * kRnBwdWaves) rn_bwd_kernel(
   const int nrows = (rows - g + G - 1) / G;
   const int iters = (nrows + TEAMS - 1) / TEAMS;  // equal for every wave of the workgroup
   const float inv_n = 1.0f / cols;
-  __shared__ float rsum[2][2][kRnBwdWaves][2];  // [norm][row parity]
+  __shared__ float rsum[2][2][W][2];  // [norm][row parity]
 
   rn_u32x4 nx[NVW], nh[NVW], nd[NVW], ny[NVW];
   auto load_row = [&](int k) __attribute__((always_inline)) {
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(64 * kRnBwdWaves) rn_bwd_kernel(
     }
   }
   // the teams' column sums, added in a fixed order: part[g][4][cols]
-  __shared__ float red[kRnBwdWaves][512];
+  __shared__ float red[W][512];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     float* dst = part + ((int64_t)blockIdx.x * 4 + q) * cols;
@@ -351,13 +350,12 @@ __global__ void __launch_bounds__(64 * kRnBwdWaves) rn_bwd_kernel(
       rw[0] = rn_f32x4{acc[q][i][0], acc[q][i][1], acc[q][i][2], acc[q][i][3]};
       rw[1] = rn_f32x4{acc[q][i][4], acc[q][i][5], acc[q][i][6], acc[q][i][7]};
       __syncthreads();
-#pragma unroll
-      for (int k = 0; k < T; ++k) {
-        const int c = (k * NVW + i) * 512 + (int)threadIdx.x;  // 512 threads: a column of sub k's vectors each
+      for (int n = threadIdx.x; n < T * 512; n += 64 * W) {
+        const int k = n / 512, e = n % 512, c = (k * NVW + i) * 512 + e;  // a column of sub k's vectors
         if (c < cols) {
           float a = 0.f;
 #pragma unroll
-          for (int t = 0; t < TEAMS; ++t) a += red[t * T + k][threadIdx.x];
+          for (int t = 0; t < TEAMS; ++t) a += red[t * T + k][e];
           dst[c] = a;
         }
       }
@@ -366,7 +364,7 @@ __global__ void __launch_bounds__(64 * kRnBwdWaves) rn_bwd_kernel(
 }
 
 // The parameters' gradients of the workgroups' column sums, added in a fixed
-// order: 64 columns and all four sums a workgroup, 16 threads a column quad and
+// order: 16 columns and all four sums a workgroup, 16 threads a column quad and
 // sum.
 struct RnGrads {
   eth_residual_norm_grad_t post_gamma, post_beta, gate, gamma, beta;
@@ -380,23 +378,33 @@ __device__ __forceinline__ void rn_put(const eth_residual_norm_grad_t& t, int c,
     store_elem(t.grad, c, dtype, v);
   }
 }
-__global__ void __launch_bounds__(1024) rn_grads_kernel(RnParams p, const float* __restrict__ part, int groups,
-                                                        RnGrads out, int dtype) {
-  __shared__ rn_f32x4 red[16][4][16];
-  const int quad = threadIdx.x & 15, q = (threadIdx.x >> 4) & 3, lane = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + quad * 4;
+constexpr int kRnGradCols = 16;
+__global__ void __launch_bounds__(256) rn_grads_kernel(RnParams p, const float* __restrict__ part, int groups,
+                                                       RnGrads out, int dtype) {
+  __shared__ rn_f32x4 red[16][4][4];
+  const int quad = threadIdx.x & 3, q = (threadIdx.x >> 2) & 3, lane = threadIdx.x >> 4;
+  const int c = blockIdx.x * kRnGradCols + quad * 4;
   rn_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (c < p.cols)
-    for (int g = lane; g < groups; g += 16)
-      v += *reinterpret_cast<const rn_f32x4*>(part + ((int64_t)g * 4 + q) * p.cols + c);
+  if (c < p.cols) {
+    const float* mine = part + (int64_t)q * p.cols + c;
+    for (int g = lane; g < groups; g += 16 * 8) {
+      rn_f32x4 in[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        in[u] = g + u * 16 < groups ? *reinterpret_cast<const rn_f32x4*>(mine + (int64_t)(g + u * 16) * 4 * p.cols)
+                                    : rn_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += in[u];
+    }
+  }
   red[lane][q][quad] = v;
   for (int half = 8; half; half >>= 1) {
     __syncthreads();
     if (lane < half) red[lane][q][quad] += red[lane + half][q][quad];
   }
   __syncthreads();
-  const int col = blockIdx.x * 64 + (int)threadIdx.x;
-  if (threadIdx.x < 64 && col < p.cols) {
+  const int col = blockIdx.x * kRnGradCols + (int)threadIdx.x;
+  if (threadIdx.x < kRnGradCols && col < p.cols) {
     float s[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) s[k] = red[0][k][threadIdx.x >> 2][threadIdx.x & 3];
@@ -410,10 +418,23 @@ __global__ void __launch_bounds__(1024) rn_grads_kernel(RnParams p, const float*
   }
 }
 
-inline int rn_team(int64_t cols) { return cols <= 1024 ? 1 : cols <= 2048 ? 2 : cols <= 4096 ? 4 : 8; }
+// Waves of a workgroup, waves that share a row, and vectors of 512 columns a wave
+// has of it: a vector a wave and as many rows as 16 waves take, but two vectors and
+// one wave for 513 to 1024 columns, which need no barrier (us, gradients of the
+// parameters included, two vectors a wave / one: [16384, 1024] 42.2 / 44.6, [8192,
+// 2048] 46.8 / 45.2, [4096, 4096] 49.8 / 47.1, [3001, 5120] 60.9 / 52.2).
+struct RnShape {
+  int waves, team, vectors;
+};
+inline RnShape rn_shape(int64_t cols) {
+  if (cols > 512 && cols <= 1024) return {8, 1, 2};
+  const int team = (int)((cols + 511) / 512);
+  return {team == 1 ? 8 : 16 / team * team, team, 1};
+}
 // at most a workgroup a compute unit, each with a row for every team
 inline int rn_groups(int64_t rows, int64_t cols) {
-  const int64_t teams = kRnBwdWaves / rn_team(cols), g = (rows + teams - 1) / teams;
+  const RnShape f = rn_shape(cols);
+  const int64_t teams = f.waves / f.team, g = (rows + teams - 1) / teams;
   return (int)(g > 256 ? 256 : g < 1 ? 1 : g);
 }
 
@@ -435,13 +456,17 @@ template <bool FP16>
 static void launch_rn_bwd(const RnParams& p, int groups, const uint16_t* x, const uint16_t* h, const float* stats,
                           const uint16_t* dh, const uint16_t* dy, uint16_t* dx, uint16_t* dres, float* part,
                           hipStream_t s) {
-#define ETH_RN_BWD(T, N) \
-  rn_bwd_kernel<T, N, FP16><<<groups, 64 * kRnBwdWaves, 0, s>>>(p, x, h, stats, dh, dy, dx, dres, part)
-  if (p.cols <= 512) ETH_RN_BWD(1, 1);
-  else if (p.cols <= 1024) ETH_RN_BWD(1, 2);
-  else if (p.cols <= 2048) ETH_RN_BWD(2, 2);
-  else if (p.cols <= 4096) ETH_RN_BWD(4, 2);
-  else ETH_RN_BWD(8, 2);
+  const RnShape f = rn_shape(p.cols);
+#define ETH_RN_BWD(W, T, N)                                                                        \
+  case T * 10 + N:                                                                                 \
+    rn_bwd_kernel<W, T, N, FP16><<<groups, 64 * W, 0, s>>>(p, x, h, stats, dh, dy, dx, dres, part); \
+    break;
+  switch (f.team * 10 + f.vectors) {
+    ETH_RN_BWD(8, 1, 1) ETH_RN_BWD(8, 1, 2) ETH_RN_BWD(15, 3, 1) ETH_RN_BWD(16, 4, 1) ETH_RN_BWD(15, 5, 1)
+    ETH_RN_BWD(12, 6, 1) ETH_RN_BWD(14, 7, 1) ETH_RN_BWD(16, 8, 1) ETH_RN_BWD(9, 9, 1) ETH_RN_BWD(10, 10, 1)
+    ETH_RN_BWD(11, 11, 1) ETH_RN_BWD(12, 12, 1) ETH_RN_BWD(13, 13, 1) ETH_RN_BWD(14, 14, 1) ETH_RN_BWD(15, 15, 1)
+    ETH_RN_BWD(16, 16, 1)
+  }
 #undef ETH_RN_BWD
 }
 
@@ -523,7 +548,7 @@ extern "C" int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const
   bool any = false;
   for (int i = 0; i < 5; ++i) any |= grads[i].grad != nullptr;
   if (any) {
-    rn_grads_kernel<<<(unsigned)((desc->cols + 63) / 64), 1024, 0, s>>>(
+    rn_grads_kernel<<<(unsigned)((desc->cols + kRnGradCols - 1) / kRnGradCols), 256, 0, s>>>(
         p, workspace, groups, RnGrads{grads[0], grads[1], grads[2], grads[3], grads[4]}, desc->dtype);
     ETH_CHECK_LAUNCH("eth_residual_norm_bwd gradients");
   }

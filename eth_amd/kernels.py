@@ -366,16 +366,18 @@ def residual_norm_bwd(x, h, stats, dh, dy, post_gamma, post_beta, gate, residual
     if stats.dtype != torch.float32 or stats.shape != (4, desc.rows) or not stats.is_contiguous():
         raise ValueError("stats must be the forward's fp32 [4, rows]")
     table = (nat.ResidualNormGrad * 5)()
-    for entry, pair, param in zip(table, grads, (post_gamma, post_beta, gate, gamma, beta)):
+    for i, (pair, param) in enumerate(zip(grads, (post_gamma, post_beta, gate, gamma, beta))):
         if pair is None:
             continue
         t, accumulate = pair
-        _check_device(index, t)
-        if param is None or t.dtype not in (x.dtype, torch.float32) or t.numel() != desc.cols or not t.is_contiguous():
+        fp32 = t.dtype == torch.float32
+        if param is None or not fp32 and t.dtype != x.dtype or t.numel() != desc.cols or not t.is_contiguous():
             raise ValueError("a parameter's gradient must be a contiguous [cols] tensor of its type or fp32")
-        if accumulate and t.dtype != torch.float32:
+        if accumulate and not fp32:
             raise ValueError("accumulate needs an fp32 gradient")
-        entry.grad, entry.fp32, entry.accumulate = t.data_ptr(), t.dtype == torch.float32, bool(accumulate)
+        if t.get_device() != index:
+            _check_device(index, t)
+        table[i] = (t.data_ptr(), fp32, bool(accumulate))
     dx = torch.empty_like(x) if need_dx else None
     dresidual = torch.empty_like(x) if need_dresidual else None
     if not desc.rows:

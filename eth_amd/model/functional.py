@@ -339,13 +339,16 @@ class GatedResidualNormFn(torch.autograd.Function):
             return (None,) * 10
         x, h, stats, *params = ctx.saved_tensors
         needs = ctx.needs_input_grad
+        wanted = needs[2], needs[3], needs[4], needs[6], needs[7]
+        # gradients that are returned share one allocation
+        new = iter(torch.empty(sum(wanted), x.shape[-1], dtype=x.dtype, device=x.device).unbind(0))
         targets, returned, places, added = [], [], set(), []
-        for p, need in zip(params, (needs[2], needs[3], needs[4], needs[6], needs[7])):
+        for p, need in zip(params, wanted):
             target = result = None
             if need:
                 mg, accumulate = _fp32_accum_target(p)
                 if mg is None:
-                    result = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+                    result = next(new)
                     target = result, False
                 elif mg.data_ptr() in places:
                     # (one parameter in two places of the call: its second gradient is added behind it)
