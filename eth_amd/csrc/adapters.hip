@@ -45,75 +45,28 @@ struct ShrinkArgs {
   float* row_scale;  // [rows] (fp16)
   uint16_t* ut;      // [tile][rp][32], zeros behind the tile's rows; or NULL
   float* tile_scale; // [tile] (fp16)
+  float* partials;   // [split][tile][32][16 RB]; NULL: the depth is in one piece
 };
 
-// RB: blocks of 16 ranks; W waves, each with a range of the depth.
-template <int RB, int W, bool FP16>
-__global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
-  constexpr int RS = RB * 16 + 4;  // padded row of the partial sums
-  __shared__ __attribute__((aligned(16))) float red[W][kTileRows][RS];
-  __shared__ float high[W];
-  const eth_adapter_tile_t t = g.tiles[blockIdx.x];
-  const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const rsrc_t xs = make_rsrc(g.x + (int64_t)t.row * g.ldx, (uint32_t)(((t.rows - 1) * g.ldx + g.K) * 2));
-  const rsrc_t as = make_rsrc(g.a + (int64_t)t.adapter * g.r * g.K, (uint32_t)(g.r * g.K * 2));
-  const bool second = t.rows > 16;
-  f32x4_t acc[2][RB];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < RB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int steps = (g.K + 31) / 32, per = (steps + W - 1) / W;
-  const int s0 = wid * per, s1 = min(steps, s0 + per);
-  int32_t xo[2], ao[RB];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) xo[i] = i * 16 + l16 < t.rows ? (int32_t)(((i * 16 + l16) * g.ldx + lg * 8) * 2) : kOob;
-#pragma unroll
-  for (int j = 0; j < RB; ++j) ao[j] = j * 16 + l16 < g.r ? ((j * 16 + l16) * g.K + lg * 8) * 2 : kOob;
-  constexpr int UN = RB >= 4 ? 2 : 4;  // steps whose loads are in flight together
-  for (int s = s0; s < s1; s += UN) {
-    uint4 fx[UN][2], fa[UN][RB];
-#pragma unroll
-    for (int n = 0; n < UN; ++n) {
-      // (past this wave's range, or the depth: zeros)
-      const bool in = s + n < s1 && (s + n) * 32 + lg * 8 < g.K;
-      const int32_t at = (s + n) * 64;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) fx[n][i] = load8(xs, in && xo[i] != kOob && (i == 0 || second) ? xo[i] + at : kOob);
-#pragma unroll
-      for (int j = 0; j < RB; ++j) fa[n][j] = load8(as, in && ao[j] != kOob ? ao[j] + at : kOob);
-    }
-#pragma unroll
-    for (int n = 0; n < UN; ++n)
-#pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        acc[0][j] = mfma16<FP16>(fa[n][j], fx[n][0], acc[0][j]);
-        if (second) acc[1][j] = mfma16<FP16>(fa[n][j], fx[n][1], acc[1][j]);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < RB; ++j)
-      *reinterpret_cast<f32x4_t*>(&red[wid][i * 16 + l16][j * 16 + lg * 4]) = acc[i][j];
-  __syncthreads();
-  // the waves' sums in order, the scale, and the largest value
+// A tile's u of its fp32 sums: the scale, the power of two, 16 bits, both layouts.
+// sum(row, j): four ranks of a row.  `turned`, `high`: LDS that nothing reads any
+// more behind the next barrier.
+template <int RB, int W, bool FP16, class F>
+__device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_tile_t& t, int tile, uint16_t* turned,
+                                       float* high, F&& sum) {
   constexpr int CELLS = kTileRows * RB * 4, PER = (CELLS + 64 * W - 1) / (64 * W);  // of four ranks
+  constexpr int TS = kTileRows + 8;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   f32x4_t v[PER];
   float top = 0.f;
 #pragma unroll
   for (int c = 0; c < PER; ++c) {
     const int cell = c * 64 * W + (int)threadIdx.x, row = cell / (RB * 4), j = cell % (RB * 4) * 4;
     if (cell >= CELLS) break;
-    f32x4_t s = *reinterpret_cast<const f32x4_t*>(&red[0][row][j]);
-#pragma unroll
-    for (int w = 1; w < W; ++w) s += *reinterpret_cast<const f32x4_t*>(&red[w][row][j]);
-    s *= t.scale;
-    v[c] = s;
+    v[c] = sum(row, j) * t.scale;
     if (FP16)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = __builtin_isfinite(s[e]) ? fmaxf(top, fabsf(s[e])) : top;
+      for (int e = 0; e < 4; ++e) top = __builtin_isfinite(v[c][e]) ? fmaxf(top, fabsf(v[c][e])) : top;
   }
   float down = 1.f, up = 1.f;  // what the stored u is times, and what brings it back
   if (FP16) {
@@ -127,12 +80,10 @@ __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
       down = ldexpf(1.f, -e);
       up = ldexpf(1.f, e);
     }
-    if (threadIdx.x == 0 && g.ut) g.tile_scale[blockIdx.x] = up;
+    if (threadIdx.x == 0 && g.ut) g.tile_scale[tile] = up;
     if ((int)threadIdx.x < t.rows) g.row_scale[t.row + threadIdx.x] = up;
   }
-  __syncthreads();  // (red is read no more: its first rows take u^T)
-  uint16_t* turned = reinterpret_cast<uint16_t*>(&red[0][0][0]);  // [RB * 16][32 + 8]
-  constexpr int TS = kTileRows + 8;
+  __syncthreads();
 #pragma unroll
   for (int c = 0; c < PER; ++c) {
     const int cell = c * 64 * W + (int)threadIdx.x, row = cell / (RB * 4), j = cell % (RB * 4) * 4;
@@ -161,12 +112,109 @@ __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
   }
   if (!g.ut) return;
   __syncthreads();
-  uint16_t* out = g.ut + (int64_t)blockIdx.x * g.rp * kTileRows;
+  uint16_t* out = g.ut + (int64_t)tile * g.rp * kTileRows;
   for (int c = threadIdx.x; c < g.rp * 4; c += 64 * W) {
     const int j = c / 4, row = c % 4 * 8;
     const uint4 o = j < RB * 16 ? *reinterpret_cast<const uint4*>(turned + j * TS + row) : make_uint4(0, 0, 0, 0);
     *reinterpret_cast<uint4*>(out + j * kTileRows + row) = o;
   }
+}
+
+// RB: blocks of 16 ranks; W waves, each with a range of the workgroup's depth
+// (blockIdx.y: of gridDim.y).
+template <int RB, int W, bool FP16>
+__global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
+  constexpr int RS = RB * 16 + 4;  // padded row of the partial sums
+  __shared__ __attribute__((aligned(16))) float red[W][kTileRows][RS];
+  __shared__ float high[W];
+  const eth_adapter_tile_t t = g.tiles[blockIdx.x];
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const rsrc_t xs = make_rsrc(g.x + (int64_t)t.row * g.ldx, (uint32_t)(((t.rows - 1) * g.ldx + g.K) * 2));
+  const rsrc_t as = make_rsrc(g.a + (int64_t)t.adapter * g.r * g.K, (uint32_t)(g.r * g.K * 2));
+  const bool second = t.rows > 16;
+  f32x4_t acc[2][RB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < RB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int pieces = W * gridDim.y, steps = (g.K + 31) / 32, per = (steps + pieces - 1) / pieces;
+  const int s0 = (blockIdx.y * W + wid) * per, s1 = min(steps, s0 + per);
+  int32_t xo[2], ao[RB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) xo[i] = i * 16 + l16 < t.rows ? (int32_t)(((i * 16 + l16) * g.ldx + lg * 8) * 2) : kOob;
+#pragma unroll
+  for (int j = 0; j < RB; ++j) ao[j] = j * 16 + l16 < g.r ? ((j * 16 + l16) * g.K + lg * 8) * 2 : kOob;
+  constexpr int UN = RB >= 4 ? 2 : 4;  // steps whose loads are in flight together, and as many ahead
+  struct Batch {
+    uint4 x[UN][2], a[UN][RB];
+  };
+  auto load = [&](Batch& f, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < UN; ++n) {
+      // (past this wave's range, or the depth: zeros)
+      const bool in = s + n < s1 && (s + n) * 32 + lg * 8 < g.K;
+      const int32_t at = (s + n) * 64;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f.x[n][i] = load8(xs, in && xo[i] != kOob && (i == 0 || second) ? xo[i] + at : kOob);
+#pragma unroll
+      for (int j = 0; j < RB; ++j) f.a[n][j] = load8(as, in && ao[j] != kOob ? ao[j] + at : kOob);
+    }
+  };
+  auto products = [&](const Batch& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < UN; ++n)
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        acc[0][j] = mfma16<FP16>(f.a[n][j], f.x[n][0], acc[0][j]);
+        if (second) acc[1][j] = mfma16<FP16>(f.a[n][j], f.x[n][1], acc[1][j]);
+      }
+  };
+  Batch one, two;
+  load(one, s0);
+  for (int s = s0; s < s1; s += 2 * UN) {
+    load(two, s + UN);
+    products(one);
+    load(one, s + 2 * UN);
+    products(two);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < RB; ++j)
+      *reinterpret_cast<f32x4_t*>(&red[wid][i * 16 + l16][j * 16 + lg * 4]) = acc[i][j];
+  __syncthreads();
+  // the waves' sums, in order
+  auto sum = [&](int row, int j) __attribute__((always_inline)) {
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(&red[0][row][j]);
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += *reinterpret_cast<const f32x4_t*>(&red[w][row][j]);
+    return v;
+  };
+  if (g.partials) {
+    float* out = g.partials + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kTileRows * RB * 16;
+    for (int cell = threadIdx.x; cell < kTileRows * RB * 4; cell += 64 * W) {
+      const int row = cell / (RB * 4), j = cell % (RB * 4) * 4;
+      *reinterpret_cast<f32x4_t*>(out + row * RB * 16 + j) = sum(row, j);
+    }
+    return;
+  }
+  narrow<RB, W, FP16>(g, t, blockIdx.x, reinterpret_cast<uint16_t*>(&red[0][0][0]), high, sum);
+}
+
+// The pieces of the depth joined, in order.
+template <int RB, bool FP16>
+__global__ void __launch_bounds__(256) adapter_narrow_kernel(ShrinkArgs g, int splits) {
+  __shared__ __attribute__((aligned(16))) uint16_t turned[RB * 16 * (kTileRows + 8)];
+  __shared__ float high[4];
+  const float* mine = g.partials + (int64_t)blockIdx.x * kTileRows * RB * 16;
+  const int64_t stride = (int64_t)gridDim.x * kTileRows * RB * 16;
+  narrow<RB, 4, FP16>(g, g.tiles[blockIdx.x], blockIdx.x, turned, high, [&](int row, int j) __attribute__((always_inline)) {
+    const float* at = mine + row * RB * 16 + j;
+    f32x4_t v = *reinterpret_cast<const f32x4_t*>(at);
+    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4_t*>(at + s * stride);
+    return v;
+  });
 }
 
 // --------------------------------------------------------------- product --
@@ -224,46 +272,66 @@ struct AdapterStart {
 #pragma unroll
     for (int i = 0; i < TI; ++i) same &= mine[i] == first || mine[i] == -2;
     const bool one = __ballot(!same) == 0;
-    // the least adapter of the wave's rows above `last`
+    // the least adapter of the wave's rows above `last` (a row of 16 lanes holds all)
     auto next = [&](int last) __attribute__((always_inline)) {
       int v = NONE;
 #pragma unroll
       for (int i = 0; i < TI; ++i) v = mine[i] > last ? min(v, mine[i]) : v;
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) v = min(v, __shfl_xor(v, o));
+      v = min(v, __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true));  // row_ror:8
+      v = min(v, __builtin_amdgcn_mov_dpp(v, 0x124, 0xf, 0xf, true));  // row_ror:4
+      v = min(v, __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true));   // quad_perm:[2,3,0,1]
+      v = min(v, __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true));   // quad_perm:[1,0,3,2]
       return __builtin_amdgcn_readfirstlane(v);
     };
+    // 32 ranks of an adapter at a time, the next ones' fragments under way
+    struct Frags {
+      uint4 e[TJ], u[TI];
+      int a;
+    };
+    auto load = [&](Frags& f, int a, int k) __attribute__((always_inline)) {
+      f.a = a;
+      if (a == NONE) return;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) f.e[j] = e_frag(a, col0 + j * 16 + l16, k + lg * 8, N);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) f.u[i] = u_frag(row0 + i * 16 + l16, k + lg * 8, mine[i] == a);
+    };
     int a = next(-1), k = 0;
-    while (a != NONE) {
-      uint4 fe[TJ], fu[TI];
-#pragma unroll
-      for (int j = 0; j < TJ; ++j) fe[j] = e_frag(a, col0 + j * 16 + l16, k + lg * 8, N);
-#pragma unroll
-      for (int i = 0; i < TI; ++i) fu[i] = u_frag(row0 + i * 16 + l16, k + lg * 8, mine[i] == a);
-      if (!one) {
-        // zero times another adapter's infinity or NaN is NaN: where its fragments
-        // hold one, zeros take their place, and its own rows become NaN
-        uint32_t wild = 0;
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) wild |= not_finite<FP16>(fe[j]);
-        if (__ballot((wild & 0x80008000u) != 0)) {
-#pragma unroll
-          for (int j = 0; j < TJ; ++j) fe[j] = make_uint4(0, 0, 0, 0);
-          const uint32_t nan = FP16 ? 0x7e007e00u : 0x7fc07fc0u;
-#pragma unroll
-          for (int i = 0; i < TI; ++i)
-            if (mine[i] == a) fu[i] = make_uint4(nan, nan, nan, nan);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < TI; ++i)
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) mul<FP16, PINNED>(acc[i][j], fe[j], fu[i]);
+    auto step = [&]() __attribute__((always_inline)) {
       k += 32;
       if (k >= rp) {
         k = 0;
         a = next(a);
       }
+    };
+    auto products = [&](Frags& f) __attribute__((always_inline)) {
+      if (!one) {
+        // zero times another adapter's infinity or NaN is NaN: where its fragments
+        // hold one, zeros take their place, and its own rows become NaN
+        uint32_t wild = 0;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wild |= not_finite<FP16>(f.e[j]);
+        if (__ballot((wild & 0x80008000u) != 0)) {
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) f.e[j] = make_uint4(0, 0, 0, 0);
+          const uint32_t nan = FP16 ? 0x7e007e00u : 0x7fc07fc0u;
+#pragma unroll
+          for (int i = 0; i < TI; ++i)
+            if (mine[i] == f.a) f.u[i] = make_uint4(nan, nan, nan, nan);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) mul<FP16, PINNED>(acc[i][j], f.e[j], f.u[i]);
+    };
+    Frags now, then;
+    load(now, a, k);
+    while (now.a != NONE) {
+      step();
+      load(then, a, k);
+      products(now);
+      now = then;
     }
     // asm MFMAs: wait states before anything reads their accumulators
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
@@ -280,58 +348,73 @@ struct AdapterStart {
 };
 
 // ------------------------------------------------------------- transpose --
-// [adapters][rows][cols] -> [adapters][cols][rows], 64 x 64 a workgroup, of the
-// adapters that are in use.
+// rows a (low) and b (high) of column h of two packed pairs
+__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, int h) {
+  return __builtin_amdgcn_perm(b, a, h ? 0x07060302u : 0x05040100u);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
+// column f of eight rows of eight 16-bit values
+__device__ __forceinline__ uint4 column_of(const uint4 (&row)[8], int f) {
+  const int w = f >> 1, h = f & 1;
+  return make_uint4(pair_of(word_of(row[0], w), word_of(row[1], w), h), pair_of(word_of(row[2], w), word_of(row[3], w), h),
+                    pair_of(word_of(row[4], w), word_of(row[5], w), h), pair_of(word_of(row[6], w), word_of(row[7], w), h));
+}
+
+// [adapters][rows][cols] -> [adapters][cols][rows] of the adapters that are in
+// use, both multiples of 8: an 8 x 8 block a thread.
 struct TurnArgs {
   const uint16_t* from;
   uint16_t* to;
   int rows, cols;
 };
-__global__ void __launch_bounds__(256) adapter_turn_kernel(TurnArgs a, TurnArgs b, const int* used, int a_tiles) {
-  __shared__ uint16_t tile[64][66];
-  const bool second = (int)blockIdx.x >= a_tiles;
+__global__ void __launch_bounds__(256) adapter_turn_kernel(TurnArgs a, TurnArgs b, const int* used, int a_blocks) {
+  int i = blockIdx.x * 256 + threadIdx.x;
+  const bool second = i >= a_blocks;
   const TurnArgs t = second ? b : a;
-  const int at = second ? blockIdx.x - a_tiles : blockIdx.x, wide = (t.cols + 63) / 64;
-  const int r0 = at / wide * 64, c0 = at % wide * 64;
+  if (second) i -= a_blocks;
+  if (i >= t.rows / 8 * (t.cols / 8)) return;
+  // neighbouring threads write side by side
+  const int r0 = i % (t.rows / 8) * 8, c0 = i / (t.rows / 8) * 8;
   const int64_t base = (int64_t)used[blockIdx.y] * t.rows * t.cols;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int r = r0 + i / 64, c = c0 + i % 64;
-    if (r < t.rows && c < t.cols) tile[i / 64][i % 64] = t.from[base + (int64_t)r * t.cols + c];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int c = c0 + i / 64, r = r0 + i % 64;
-    if (r < t.rows && c < t.cols) t.to[base + (int64_t)c * t.rows + r] = tile[i % 64][i / 64];
-  }
+  uint4 row[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    row[k] = *reinterpret_cast<const uint4*>(t.from + base + (int64_t)(r0 + k) * t.cols + c0);
+#pragma unroll
+  for (int f = 0; f < 8; ++f)
+    *reinterpret_cast<uint4*>(t.to + base + (int64_t)(c0 + f) * t.rows + r0) = column_of(row, f);
 }
 
 // ----------------------------------------------------------------- outer --
-// part[chunk][r][C] = sum over the chunk's tiles of u^T q: 128 columns a
-// workgroup, its four waves taking tiles in turn.
-struct OuterArgs {
-  const eth_adapter_tile_t* tiles;
-  const eth_adapter_chunk_t* chunks;
+// part[chunk][r][C] = sum over the chunk's tiles of u^T q, for dA (q = x) and dB
+// (q = dy) in one launch: 128 columns a workgroup, its four waves taking tiles in
+// turn.
+struct OuterSide {
   const uint16_t* ut;
   const float* tile_scale;  // (fp16)
   const uint16_t* q;        // [rows][ldq], C of it
   int64_t ldq;
-  int C, r, rp;
+  int C;
   float* part;
 };
-
-// rows a (low) and b (high) of column 2 w + h from the packed pairs
-__device__ __forceinline__ uint32_t pair_of(uint32_t a, uint32_t b, int h) {
-  return __builtin_amdgcn_perm(b, a, h ? 0x07060302u : 0x05040100u);
-}
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
+struct OuterArgs {
+  const eth_adapter_tile_t* tiles;
+  const eth_adapter_chunk_t* chunks;
+  int r, rp;
+  OuterSide a, b;
+  int a_blocks;  // workgroups along x of side a
+};
 
 template <int RB, bool FP16>
-__global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs g) {
+__global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
   __shared__ __attribute__((aligned(16))) float sum[RB * 16][128 + 4];
-  const eth_adapter_chunk_t c = g.chunks[blockIdx.y];
+  const bool second = (int)blockIdx.x >= args.a_blocks;
+  const OuterSide g = second ? args.b : args.a;
+  const int block = second ? blockIdx.x - args.a_blocks : blockIdx.x;
+  const eth_adapter_chunk_t c = args.chunks[blockIdx.y];
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = blockIdx.x * 128 + l16 * 8;
+  const int col = block * 128 + l16 * 8;
   // acc[j][f]: ranks 16 j + 4 (lane / 16) + 0..3, column col + f
   f32x4_t acc[RB][8];
 #pragma unroll
@@ -345,14 +428,14 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs g) {
     for (int k = 0; k < c.tiles; ++k) have = fmaxf(have, g.tile_scale[c.first + k]);
   for (int k = wid; k < c.tiles; k += 4) {
     const int at = c.first + k;
-    const eth_adapter_tile_t t = g.tiles[at];
+    const eth_adapter_tile_t t = args.tiles[at];
     const rsrc_t qs = make_rsrc(g.q + (int64_t)t.row * g.ldq, (uint32_t)(((t.rows - 1) * g.ldq + g.C) * 2));
     uint4 row[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       row[i] = load8(qs, lg * 8 + i < t.rows && col < g.C ? (int32_t)(((lg * 8 + i) * g.ldq + col) * 2) : kOob);
     uint4 fu[RB];
-    const uint16_t* ut = g.ut + (int64_t)at * g.rp * kTileRows + lg * 8;
+    const uint16_t* ut = g.ut + (int64_t)at * args.rp * kTileRows + lg * 8;
 #pragma unroll
     for (int j = 0; j < RB; ++j) fu[j] = *reinterpret_cast<const uint4*>(ut + (j * 16 + l16) * kTileRows);
     if (FP16) {
@@ -364,11 +447,7 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs g) {
     // eight rows of eight columns -> a column's eight rows
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
-      const int w = f >> 1, h = f & 1;
-      const uint4 fq = make_uint4(pair_of(word_of(row[0], w), word_of(row[1], w), h),
-                                  pair_of(word_of(row[2], w), word_of(row[3], w), h),
-                                  pair_of(word_of(row[4], w), word_of(row[5], w), h),
-                                  pair_of(word_of(row[6], w), word_of(row[7], w), h));
+      const uint4 fq = column_of(row, f);
 #pragma unroll
       for (int j = 0; j < RB; ++j) acc[j][f] = mfma16<FP16>(fu[j], fq, acc[j][f]);
     }
@@ -396,9 +475,9 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs g) {
     }
     __syncthreads();
   }
-  float* out = g.part + (int64_t)blockIdx.y * g.r * g.C;
-  for (int i = threadIdx.x; i < g.r * 32; i += 256) {
-    const int j = i / 32, q = i % 32 * 4, at = blockIdx.x * 128 + q;
+  float* out = g.part + (int64_t)blockIdx.y * args.r * g.C;
+  for (int i = threadIdx.x; i < args.r * 32; i += 256) {
+    const int j = i / 32, q = i % 32 * 4, at = block * 128 + q;
     if (at < g.C)
       *reinterpret_cast<f32x4_t*>(out + (int64_t)j * g.C + at) = *reinterpret_cast<const f32x4_t*>(&sum[j][q]);
   }
@@ -408,13 +487,18 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs g) {
 // An adapter's gradient: its chunks added in order; zeros where it has none.
 // dA [adapters][r][K] is stored as summed, dB [adapters][N][r] turned: a thread
 // has eight ranks of a column.
-struct JoinArgs {
+struct JoinSide {
   const float* part;
-  const int* first_chunk;  // [listed + 1]
-  int listed;              // adapters from there on have none
-  int C, r;
+  int C;
   void* out;
   int fp32, accumulate, turned;
+};
+struct JoinArgs {
+  const int* first_chunk;  // [listed + 1]
+  int listed;              // adapters from there on have none
+  int r, dtype;
+  JoinSide a, b;
+  int a_blocks;
 };
 __device__ __forceinline__ void put8(void* out, int64_t at, int fp32, int accumulate, int dtype, const float (&v)[8]) {
   if (fp32) {
@@ -435,18 +519,20 @@ __device__ __forceinline__ void put8(void* out, int64_t at, int fp32, int accumu
     w[k] = dtype == ETH_F16 ? f2h_pair(v[2 * k], v[2 * k + 1]) : f2bf_pair(v[2 * k], v[2 * k + 1]);
   *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + at) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__global__ void __launch_bounds__(256) adapter_join_kernel(JoinArgs g, int dtype) {
-  const int a = blockIdx.y, eights = g.r / 8 * g.C, i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= eights) return;
-  const int c0 = a < g.listed ? g.first_chunk[a] : 0, c1 = a < g.listed ? g.first_chunk[a + 1] : 0;
+__global__ void __launch_bounds__(256) adapter_join_kernel(JoinArgs args) {
+  const bool second = (int)blockIdx.x >= args.a_blocks;
+  const JoinSide g = second ? args.b : args.a;
+  const int r = args.r, a = blockIdx.y, i = (second ? blockIdx.x - args.a_blocks : blockIdx.x) * 256 + threadIdx.x;
+  if (i >= r / 8 * g.C) return;
+  const int c0 = a < args.listed ? args.first_chunk[a] : 0, c1 = a < args.listed ? args.first_chunk[a + 1] : 0;
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const int64_t chunk = (int64_t)g.r * g.C;
+  const int64_t chunk = (int64_t)r * g.C;
   if (g.turned) {
     const int j = i / g.C * 8, col = i % g.C;
     for (int c = c0; c < c1; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += g.part[c * chunk + (int64_t)(j + e) * g.C + col];
-    put8(g.out, (int64_t)a * chunk + (int64_t)col * g.r + j, g.fp32, g.accumulate, dtype, v);
+    put8(g.out, (int64_t)a * chunk + (int64_t)col * r + j, g.fp32, g.accumulate, args.dtype, v);
   } else {
     for (int c = c0; c < c1; ++c) {
       const float4* p = reinterpret_cast<const float4*>(g.part + c * chunk + (int64_t)i * 8);
@@ -454,7 +540,7 @@ __global__ void __launch_bounds__(256) adapter_join_kernel(JoinArgs g, int dtype
       v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
       v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
     }
-    put8(g.out, (int64_t)a * chunk + (int64_t)i * 8, g.fp32, g.accumulate, dtype, v);
+    put8(g.out, (int64_t)a * chunk + (int64_t)i * 8, g.fp32, g.accumulate, args.dtype, v);
   }
 }
 
@@ -524,13 +610,35 @@ static int launch_adapted(const ProductPlan& p, GemmArgs a, const X& x, float* p
   return ETH_OK;
 }
 
+// Pieces of the shrink's depth: as many as bring four workgroups a compute unit
+// (two from 33 ranks on, whose LDS leaves room for two), each of two trips of its
+// waves at least.
+struct ShrinkPlan {
+  int blocks, waves, splits;
+  int64_t workspace;
+};
+static ShrinkPlan plan_shrink(int64_t K, int r, int n_tiles) {
+  ShrinkPlan p{r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8, r <= 64 ? 8 : 4, 1, 0};
+  const int64_t trips = K / (p.waves * 32 * (p.blocks >= 4 ? 2 : 4)), slots = p.blocks >= 4 ? 512 : 1024;
+  if (n_tiles) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, slots / n_tiles), trips / 2));
+  if (p.splits > 1) p.workspace = (int64_t)p.splits * n_tiles * kTileRows * p.blocks * 16 * 4;
+  return p;
+}
 template <bool FP16>
-static int launch_shrink(const ShrinkArgs& g, int n_tiles, hipStream_t s) {
-#define ETH_SHRINK(RB, W) adapter_shrink_kernel<RB, W, FP16><<<n_tiles, 64 * W, 0, s>>>(g)
-  if (g.r <= 16) ETH_SHRINK(1, 8);
-  else if (g.r <= 32) ETH_SHRINK(2, 8);
-  else if (g.r <= 64) ETH_SHRINK(4, 8);
-  else ETH_SHRINK(8, 4);
+static int launch_shrink(ShrinkArgs g, int n_tiles, float* partials, hipStream_t s) {
+  const ShrinkPlan p = plan_shrink(g.K, g.r, n_tiles);
+  g.partials = p.splits > 1 ? partials : nullptr;
+  const dim3 grid((unsigned)n_tiles, (unsigned)p.splits);
+#define ETH_SHRINK(RB, W)                                                             \
+  {                                                                                   \
+    adapter_shrink_kernel<RB, W, FP16><<<grid, 64 * W, 0, s>>>(g);                    \
+    ETH_CHECK_LAUNCH("eth_adapter_linear");                                           \
+    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g, p.splits); \
+  }
+  if (p.blocks == 1) ETH_SHRINK(1, 8)
+  else if (p.blocks == 2) ETH_SHRINK(2, 8)
+  else if (p.blocks == 4) ETH_SHRINK(4, 8)
+  else ETH_SHRINK(8, 4)
 #undef ETH_SHRINK
   ETH_CHECK_LAUNCH("eth_adapter_linear");
   return ETH_OK;
@@ -538,7 +646,7 @@ static int launch_shrink(const ShrinkArgs& g, int n_tiles, hipStream_t s) {
 
 template <bool FP16>
 static int launch_outer(const OuterArgs& g, int n_chunks, hipStream_t s) {
-  const dim3 grid((unsigned)((g.C + 127) / 128), (unsigned)n_chunks);
+  const dim3 grid((unsigned)(g.a_blocks + (g.b.C + 127) / 128), (unsigned)n_chunks);
 #define ETH_OUTER(RB) adapter_outer_kernel<RB, FP16><<<grid, 256, 0, s>>>(g)
   if (g.r <= 16) ETH_OUTER(1);
   else if (g.r <= 32) ETH_OUTER(2);
@@ -582,12 +690,13 @@ static AdapterForward plan_adapter_fwd(const eth_adapter_desc_t* d) {
   int64_t o = 0;
   p.u = o, o += room(d->rows * padded_rank(d->rank) * 2);
   p.row_scale = o, o += room(d->rows * 4);
-  p.product = o, o += room(p.plan.workspace);
+  // (the shrink's partial sums, then the product's)
+  p.product = o, o += room(std::max(p.plan.workspace, plan_shrink(d->in, d->rank, d->n_tiles).workspace));
   p.bytes = o;
   return p;
 }
 struct AdapterBackward {
-  int64_t u, row_scale, ut, tile_scale, at, bt, part, product, bytes;
+  int64_t u, row_scale, ut, tile_scale, at, bt, part_a, part_b, product, bytes;
   ProductPlan plan;
 };
 static AdapterBackward plan_adapter_bwd(const eth_adapter_desc_t* d) {
@@ -601,11 +710,13 @@ static AdapterBackward plan_adapter_bwd(const eth_adapter_desc_t* d) {
   p.tile_scale = o, o += room((int64_t)d->n_tiles * 4);
   p.at = o, o += room((int64_t)d->adapters * d->rank * d->in * 2);
   p.bt = o, o += room((int64_t)d->adapters * d->rank * d->out * 2);
-  // dA's and dB's chunks, one after the other, and the product's partial sums
-  // (its stream order lets all three share)
-  p.part = o;
+  // the shrink's partial sums, the product's, then dA's and dB's chunks: each is
+  // read before the next is written
   p.product = o;
-  o += room(std::max((int64_t)d->n_chunks * d->rank * std::max(d->in, d->out) * 4, p.plan.workspace));
+  p.part_a = o;
+  p.part_b = o + room((int64_t)d->n_chunks * d->rank * d->in * 4);
+  o += std::max({room(p.plan.workspace), room(plan_shrink(d->out, d->rank, d->n_tiles).workspace),
+                 p.part_b - o + room((int64_t)d->n_chunks * d->rank * d->out * 4)});
   p.bytes = o;
   return p;
 }
@@ -642,8 +753,8 @@ static int adapter_forward(const eth_adapter_desc_t* d, const void* x, const voi
   const GemmArgs a = adapter_product(d, x, d->ldx, d->in, w, y, d->out, bias);
   if (!d->n_tiles) return launch_adapted<true, FP16>(p.plan, a, PlainProduct{}, (float*)(ws + p.product), s);
   const ShrinkArgs g{d->tiles, (const uint16_t*)x, (const uint16_t*)lora_a, d->ldx, (int)d->in, d->rank, rp,
-                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale};
-  const int rc = launch_shrink<FP16>(g, d->n_tiles, s);
+                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale, nullptr};
+  const int rc = launch_shrink<FP16>(g, d->n_tiles, (float*)(ws + p.product), s);
   if (rc != ETH_OK) return rc;
   const AdapterStart start{d->of_row, g.u, g.row_scale, (const uint16_t*)lora_b, d->rank, rp};
   return launch_adapted<true, FP16>(p.plan, a, start, (float*)(ws + p.product), s);
@@ -665,15 +776,14 @@ static int adapter_backward(const eth_adapter_desc_t* d, const void* x, const vo
     // A^T for the start of dx, B^T for u
     const TurnArgs turn_a{(const uint16_t*)lora_a, (uint16_t*)(ws + p.at), d->rank, (int)d->in};
     const TurnArgs turn_b{(const uint16_t*)lora_b, (uint16_t*)(ws + p.bt), (int)d->out, d->rank};
-    const int high = (d->rank + 63) / 64;
-    const int a_tiles = dx ? high * (int)((d->in + 63) / 64) : 0, b_tiles = high * (int)((d->out + 63) / 64);
-    adapter_turn_kernel<<<dim3((unsigned)(a_tiles + b_tiles), (unsigned)d->n_used), 256, 0, s>>>(turn_a, turn_b, d->used,
-                                                                                                a_tiles);
+    const int a_blocks = dx ? d->rank / 8 * (int)(d->in / 8) : 0, b_blocks = d->rank / 8 * (int)(d->out / 8);
+    adapter_turn_kernel<<<dim3((unsigned)((a_blocks + b_blocks + 255) / 256), (unsigned)d->n_used), 256, 0, s>>>(
+        turn_a, turn_b, d->used, a_blocks);
     ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
     const ShrinkArgs g{d->tiles, (const uint16_t*)dy, turn_b.to, d->out, (int)d->out, d->rank, rp,
                        (uint16_t*)(dx ? ws + p.u : nullptr), (float*)(ws + p.row_scale),
-                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale)};
-    rc = launch_shrink<FP16>(g, d->n_tiles, s);
+                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale), nullptr};
+    rc = launch_shrink<FP16>(g, d->n_tiles, (float*)(ws + p.product), s);
     if (rc != ETH_OK) return rc;
     if (dx) {
       const AdapterStart start{d->of_row, g.u, g.row_scale, turn_a.to, d->rank, rp};
@@ -681,22 +791,29 @@ static int adapter_backward(const eth_adapter_desc_t* d, const void* x, const vo
       if (rc != ETH_OK) return rc;
     }
   }
-  for (int which = 0; which < 2; ++which) {
-    const eth_adapter_grad_t* t = which ? db : da;
-    if (!t->grad) continue;
-    const int C = (int)(which ? d->out : d->in);
-    if (d->n_tiles) {
-      const OuterArgs g{d->tiles, d->chunks, which ? (const uint16_t*)ut : (const uint16_t*)(ws + p.ut),
-                        which ? tile_scale : (const float*)(ws + p.tile_scale),
-                        which ? (const uint16_t*)dy : (const uint16_t*)x, which ? d->out : d->ldx, C, d->rank, rp,
-                        (float*)(ws + p.part)};
-      rc = launch_outer<FP16>(g, d->n_chunks, s);
-      if (rc != ETH_OK) return rc;
+  const OuterSide none{};
+  if (d->n_tiles && (da->grad || db->grad)) {
+    OuterArgs g{d->tiles, d->chunks, d->rank, rp, none, none, 0};
+    if (da->grad) {
+      g.a = OuterSide{(const uint16_t*)(ws + p.ut), (const float*)(ws + p.tile_scale), (const uint16_t*)x, d->ldx,
+                      (int)d->in, (float*)(ws + p.part_a)};
+      g.a_blocks = (int)((d->in + 127) / 128);
     }
-    if (!d->n_tiles && t->accumulate) continue;
-    const JoinArgs j{(const float*)(ws + p.part), d->first_chunk, d->n_tiles ? d->n_listed : 0, C, d->rank, t->grad, t->fp32, t->accumulate, which};
-    adapter_join_kernel<<<dim3((unsigned)((d->rank / 8 * (int64_t)C + 255) / 256), (unsigned)d->adapters), 256, 0, s>>>(
-        j, d->dtype);
+    if (db->grad)
+      g.b = OuterSide{(const uint16_t*)ut, tile_scale, (const uint16_t*)dy, d->out, (int)d->out,
+                      (float*)(ws + p.part_b)};
+    rc = launch_outer<FP16>(g, d->n_chunks, s);
+    if (rc != ETH_OK) return rc;
+  }
+  // (without rows, what is added to stays as it is)
+  const bool join_a = da->grad && (d->n_tiles || !da->accumulate), join_b = db->grad && (d->n_tiles || !db->accumulate);
+  if (join_a || join_b) {
+    const int64_t a_blocks = join_a ? (d->rank / 8 * d->in + 255) / 256 : 0;
+    const int64_t b_blocks = join_b ? (d->rank / 8 * d->out + 255) / 256 : 0;
+    const JoinSide a{(const float*)(ws + p.part_a), (int)d->in, da->grad, da->fp32, da->accumulate, 0};
+    const JoinSide b{(const float*)(ws + p.part_b), (int)d->out, db->grad, db->fp32, db->accumulate, 1};
+    const JoinArgs j{d->first_chunk, d->n_tiles ? d->n_listed : 0, d->rank, d->dtype, a, b, (int)a_blocks};
+    adapter_join_kernel<<<dim3((unsigned)(a_blocks + b_blocks), (unsigned)d->adapters), 256, 0, s>>>(j);
     ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
   }
   return ETH_OK;
