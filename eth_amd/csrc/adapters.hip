@@ -46,6 +46,7 @@ struct ShrinkArgs {
   uint16_t* ut;      // [tile][rp][32], zeros behind the tile's rows; or NULL
   float* tile_scale; // [tile] (fp16)
   float* partials;   // [split][tile][32][16 RB]; NULL: the depth is in one piece
+  int splits;
 };
 
 // A tile's u of its fp32 sums: the scale, the power of two, 16 bits, both layouts.
@@ -120,14 +121,16 @@ __device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_ti
   }
 }
 
-// RB: blocks of 16 ranks; W waves, each with a range of the workgroup's depth
-// (blockIdx.y: of gridDim.y).
+// RB: blocks of 16 ranks; W waves, each with a range of the workgroup's depth.
+// Neighbouring workgroups have the pieces of a tile's depth: with eight, each XCD
+// reads its own piece of every adapter, which its L2 holds.
 template <int RB, int W, bool FP16>
 __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
   constexpr int RS = RB * 16 + 4;  // padded row of the partial sums
   __shared__ __attribute__((aligned(16))) float red[W][kTileRows][RS];
   __shared__ float high[W];
-  const eth_adapter_tile_t t = g.tiles[blockIdx.x];
+  const int tile = blockIdx.x / g.splits, piece = blockIdx.x - tile * g.splits;
+  const eth_adapter_tile_t t = g.tiles[tile];
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const rsrc_t xs = make_rsrc(g.x + (int64_t)t.row * g.ldx, (uint32_t)(((t.rows - 1) * g.ldx + g.K) * 2));
@@ -138,8 +141,8 @@ __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < RB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int pieces = W * gridDim.y, steps = (g.K + 31) / 32, per = (steps + pieces - 1) / pieces;
-  const int s0 = (blockIdx.y * W + wid) * per, s1 = min(steps, s0 + per);
+  const int pieces = W * g.splits, steps = (g.K + 31) / 32, per = (steps + pieces - 1) / pieces;
+  const int s0 = (piece * W + wid) * per, s1 = min(steps, s0 + per);
   int32_t xo[2], ao[RB];
 #pragma unroll
   for (int i = 0; i < 2; ++i) xo[i] = i * 16 + l16 < t.rows ? (int32_t)(((i * 16 + l16) * g.ldx + lg * 8) * 2) : kOob;
@@ -192,28 +195,34 @@ __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
     return v;
   };
   if (g.partials) {
-    float* out = g.partials + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kTileRows * RB * 16;
+    const int tiles = gridDim.x / g.splits;
+    float* out = g.partials + ((int64_t)piece * tiles + tile) * kTileRows * RB * 16;
     for (int cell = threadIdx.x; cell < kTileRows * RB * 4; cell += 64 * W) {
       const int row = cell / (RB * 4), j = cell % (RB * 4) * 4;
       *reinterpret_cast<f32x4_t*>(out + row * RB * 16 + j) = sum(row, j);
     }
     return;
   }
-  narrow<RB, W, FP16>(g, t, blockIdx.x, reinterpret_cast<uint16_t*>(&red[0][0][0]), high, sum);
+  narrow<RB, W, FP16>(g, t, tile, reinterpret_cast<uint16_t*>(&red[0][0][0]), high, sum);
 }
 
 // The pieces of the depth joined, in order.
+constexpr int kMaxSplits = 8;
 template <int RB, bool FP16>
-__global__ void __launch_bounds__(256) adapter_narrow_kernel(ShrinkArgs g, int splits) {
+__global__ void __launch_bounds__(256) adapter_narrow_kernel(ShrinkArgs g) {
   __shared__ __attribute__((aligned(16))) uint16_t turned[RB * 16 * (kTileRows + 8)];
   __shared__ float high[4];
   const float* mine = g.partials + (int64_t)blockIdx.x * kTileRows * RB * 16;
   const int64_t stride = (int64_t)gridDim.x * kTileRows * RB * 16;
   narrow<RB, 4, FP16>(g, g.tiles[blockIdx.x], blockIdx.x, turned, high, [&](int row, int j) __attribute__((always_inline)) {
     const float* at = mine + row * RB * 16 + j;
-    f32x4_t v = *reinterpret_cast<const f32x4_t*>(at);
-    for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4_t*>(at + s * stride);
-    return v;
+    f32x4_t in[kMaxSplits];
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s)
+      in[s] = s < g.splits ? *reinterpret_cast<const f32x4_t*>(at + s * stride) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 1; s < kMaxSplits; ++s) in[0] += in[s];
+    return in[0];
   });
 }
 
@@ -225,7 +234,7 @@ struct AdapterStart {
   static constexpr bool kSized = false, kGathers = false, kStarts = true, kMaps = false, kReduces = false;
   const int* of_row;
   const uint16_t* u;
-  const float* row_scale;
+  const float* row_scale;  // (fp16; NULL else)
   const uint16_t* e;
   int r, rp;
 
@@ -256,16 +265,27 @@ struct AdapterStart {
     return ((v.x & top) + one) | ((v.y & top) + one) | ((v.z & top) + one) | ((v.w & top) + one);
   }
 
-  template <bool FP16, bool PINNED, int TI, int TJ>
-  __device__ __forceinline__ void start(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int N) const {
-    const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
-    constexpr int NONE = 0x7fffffff;
-    int mine[TI];
+  template <int TI>
+  struct Early {
+    int mine[TI];     // the lane's rows' adapters (-1: none, -2: a row past M)
+    float scale[TI];  // (fp16)
+  };
+  template <int TI>
+  __device__ __forceinline__ void ask(Early<TI>& r, int row0, int M) const {
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      const int row = row0 + i * 16 + l16;
-      mine[i] = row < M ? of_row[row] : -2;
+      const int row = row0 + i * 16 + (threadIdx.x & 15);
+      r.mine[i] = row < M ? of_row[row] : -2;
+      r.scale[i] = row_scale && row < M ? row_scale[row] : 0.f;
     }
+  }
+
+  template <bool FP16, bool PINNED, int TI, int TJ>
+  __device__ __forceinline__ void start(f32x4_t (&acc)[TI][TJ], const Early<TI>& early, int row0, int col0, int M,
+                                        int N) const {
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
+    constexpr int NONE = 0x7fffffff;
+    const int(&mine)[TI] = early.mine;
     // whether all rows (but those past M) have one adapter
     const int first = __builtin_amdgcn_readfirstlane(mine[0]);
     bool same = true;
@@ -301,7 +321,7 @@ struct AdapterStart {
       k += 32;
       if (k >= rp) {
         k = 0;
-        a = next(a);
+        if (a != NONE) a = next(a);
       }
     };
     auto products = [&](Frags& f) __attribute__((always_inline)) {
@@ -325,20 +345,39 @@ struct AdapterStart {
 #pragma unroll
         for (int j = 0; j < TJ; ++j) mul<FP16, PINNED>(acc[i][j], f.e[j], f.u[i]);
     };
-    Frags now, then;
-    load(now, a, k);
-    while (now.a != NONE) {
+    // (small tiles, whose rows often have an adapter each, look further ahead)
+    constexpr int AHEAD = TI * TJ <= 4 ? 4 : 2;
+    Frags f[AHEAD];
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+      load(f[d], a, k);
       step();
-      load(then, a, k);
-      products(now);
-      now = then;
+    }
+    while (f[0].a != NONE) {
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        if (f[d].a != NONE) products(f[d]);
+        load(f[d], a, k);
+        step();
+      }
     }
     // asm MFMAs: wait states before anything reads their accumulators
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
     if (FP16) {
+      // (the products by f stay behind the waits by their operands, not by their
+      // place alone)
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) {
+          if constexpr (PINNED)
+            asm volatile("" : "+a"(acc[i][j]));
+          else
+            asm volatile("" : "+v"(acc[i][j]));
+        }
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
-        const float f = mine[i] >= 0 ? row_scale[row0 + i * 16 + l16] : 0.f;
+        const float f = mine[i] >= 0 ? early.scale[i] : 0.f;
 #pragma unroll
         for (int j = 0; j < TJ; ++j) acc[i][j] *= f;
         if (PINNED) __builtin_amdgcn_sched_barrier(0);  // (a row block at a time: 26 registers spilled else)
@@ -620,7 +659,7 @@ struct ShrinkPlan {
 static ShrinkPlan plan_shrink(int64_t K, int r, int n_tiles) {
   ShrinkPlan p{r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8, r <= 64 ? 8 : 4, 1, 0};
   const int64_t trips = K / (p.waves * 32 * (p.blocks >= 4 ? 2 : 4)), slots = p.blocks >= 4 ? 512 : 1024;
-  if (n_tiles) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, slots / n_tiles), trips / 2));
+  if (n_tiles) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSplits, slots / n_tiles), trips / 2));
   if (p.splits > 1) p.workspace = (int64_t)p.splits * n_tiles * kTileRows * p.blocks * 16 * 4;
   return p;
 }
@@ -628,12 +667,13 @@ template <bool FP16>
 static int launch_shrink(ShrinkArgs g, int n_tiles, float* partials, hipStream_t s) {
   const ShrinkPlan p = plan_shrink(g.K, g.r, n_tiles);
   g.partials = p.splits > 1 ? partials : nullptr;
-  const dim3 grid((unsigned)n_tiles, (unsigned)p.splits);
+  g.splits = p.splits;
+  const unsigned grid = (unsigned)(n_tiles * p.splits);
 #define ETH_SHRINK(RB, W)                                                             \
   {                                                                                   \
     adapter_shrink_kernel<RB, W, FP16><<<grid, 64 * W, 0, s>>>(g);                    \
     ETH_CHECK_LAUNCH("eth_adapter_linear");                                           \
-    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g, p.splits); \
+    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g);           \
   }
   if (p.blocks == 1) ETH_SHRINK(1, 8)
   else if (p.blocks == 2) ETH_SHRINK(2, 8)
@@ -753,10 +793,10 @@ static int adapter_forward(const eth_adapter_desc_t* d, const void* x, const voi
   const GemmArgs a = adapter_product(d, x, d->ldx, d->in, w, y, d->out, bias);
   if (!d->n_tiles) return launch_adapted<true, FP16>(p.plan, a, PlainProduct{}, (float*)(ws + p.product), s);
   const ShrinkArgs g{d->tiles, (const uint16_t*)x, (const uint16_t*)lora_a, d->ldx, (int)d->in, d->rank, rp,
-                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale, nullptr};
+                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale, nullptr, 1};
   const int rc = launch_shrink<FP16>(g, d->n_tiles, (float*)(ws + p.product), s);
   if (rc != ETH_OK) return rc;
-  const AdapterStart start{d->of_row, g.u, g.row_scale, (const uint16_t*)lora_b, d->rank, rp};
+  const AdapterStart start{d->of_row, g.u, FP16 ? g.row_scale : nullptr, (const uint16_t*)lora_b, d->rank, rp};
   return launch_adapted<true, FP16>(p.plan, a, start, (float*)(ws + p.product), s);
 }
 
@@ -782,11 +822,11 @@ static int adapter_backward(const eth_adapter_desc_t* d, const void* x, const vo
     ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
     const ShrinkArgs g{d->tiles, (const uint16_t*)dy, turn_b.to, d->out, (int)d->out, d->rank, rp,
                        (uint16_t*)(dx ? ws + p.u : nullptr), (float*)(ws + p.row_scale),
-                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale), nullptr};
+                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale), nullptr, 1};
     rc = launch_shrink<FP16>(g, d->n_tiles, (float*)(ws + p.product), s);
     if (rc != ETH_OK) return rc;
     if (dx) {
-      const AdapterStart start{d->of_row, g.u, g.row_scale, turn_a.to, d->rank, rp};
+      const AdapterStart start{d->of_row, g.u, FP16 ? g.row_scale : nullptr, turn_a.to, d->rank, rp};
       rc = launch_adapted<false, FP16>(p.plan, a, start, (float*)(ws + p.product), s);
       if (rc != ETH_OK) return rc;
     }

@@ -229,8 +229,10 @@ struct GemmArgs {
 //    those of the launch; the tiles are those of g.M, workgroups past them leave
 //    at once: with the launch's tiles 3 empty rows of ten left two XCDs idle);
 //  * kGathers: row r of A lies at row rows[r];
-//  * kStarts: start<FP16, PINNED>(acc, row0, col0, M, N) adds to the zeros that
-//    the accumulators start at (split-K: in the first split);
+//  * kStarts: start<FP16, PINNED>(acc, early, row0, col0, M, N) adds to the zeros
+//    that the accumulators start at (split-K: in the first split); ask(early,
+//    row0, M) fills an Early<TI> ahead of the k loop's first loads, behind which
+//    any later load returns;
 //  * kMaps: map(acc, row0, col0, M, N) changes the accumulators before C is
 //    stored;
 //  * kReduces: reduce(acc, row0, col0, M, N) takes the place of storing C.
@@ -239,6 +241,11 @@ struct GemmArgs {
 struct PlainProduct {
   static constexpr bool kSized = false, kGathers = false, kStarts = false, kMaps = false, kReduces = false;
 };
+
+template <class X, int TI, bool STARTS = X::kStarts>
+struct EarlyOf {};
+template <class X, int TI>
+struct EarlyOf<X, TI, true> : X::template Early<TI> {};
 
 // 256x256x64 tiles, 4 waves of 128x128 (one per SIMD).
 //
@@ -381,6 +388,8 @@ __global__ void __launch_bounds__(256, 1) gemm256_m16_kernel(GemmArgs g, X x) {
     }                                    \
   }
   LIMIT_IF(0)
+  [[maybe_unused]] EarlyOf<X, 8> early;
+  if constexpr (X::kStarts) x.ask(early, m0 + wm * 128, g.M);
   la.template issue<0, NA>(smem, ra, g.lda, kb);
   lb.template issue<0, NB>(smem + A_IMG, rb, g.ldb, kb);
   LIMIT_IF(1)
@@ -401,7 +410,7 @@ __global__ void __launch_bounds__(256, 1) gemm256_m16_kernel(GemmArgs g, X x) {
 #undef PRO_Q
   }
   if constexpr (X::kStarts) {
-    if (split == 0) x.template start<FP16, true>(acc, m0 + wm * 128, n0 + wn * 128, g.M, g.N);
+    if (split == 0) x.template start<FP16, true>(acc, early, m0 + wm * 128, n0 + wn * 128, g.M, g.N);
     PIN_ACC
   }
   dma_barrier_but<12>();
@@ -507,6 +516,8 @@ __global__ void __launch_bounds__(256, 1) gemm256_m16_kernel(GemmArgs g, X x) {
   }
   // asm MFMAs: wait states before any instruction reads their accumulators
   if constexpr (!A_K || TAIL) asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  // (what reads them is behind the waits by its operands, not by its place alone)
+  if constexpr (X::kMaps || X::kReduces) { PIN_ACC }
 #undef PIN_ACC
 #undef LIMIT_IF
 #undef ITER
@@ -982,6 +993,8 @@ __global__ void __launch_bounds__(256, 1) gemm_ring_kernel(GemmArgs g, X x) {
     la.issue(S, ra, g.lda, (KT) * 64, g.K);            \
     lb.issue((S) + A_IMG, rb, g.ldb, (KT) * 64, g.K);  \
   }
+  [[maybe_unused]] EarlyOf<X, TI> early;
+  if constexpr (X::kStarts) x.ask(early, m0 + wm * WM, g.M);
   RING_ISSUE(st0, 0)
   RING_ISSUE(st1, 1)
   RING_ISSUE(st2, 2)
@@ -992,7 +1005,7 @@ __global__ void __launch_bounds__(256, 1) gemm_ring_kernel(GemmArgs g, X x) {
   for (int i = 0; i < TI; ++i)
 #pragma unroll
     for (int j = 0; j < TJ; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if constexpr (X::kStarts) x.template start<FP16, false>(acc, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
+  if constexpr (X::kStarts) x.template start<FP16, false>(acc, early, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
 
   // lane offsets of the fragments of k-step 0 (k-step 1: see frag): lane l
   // holds row l%16 of the block, k 8*(l/16) .. +7
@@ -1063,6 +1076,12 @@ __global__ void __launch_bounds__(256, 1) gemm_ring_kernel(GemmArgs g, X x) {
   if (kt + 2 < nk) RING_STEP(st2, st3, kt + 2)
   // asm MFMAs: wait states before any instruction reads their accumulators
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+  if constexpr (X::kMaps || X::kReduces) {  // (behind the waits by its operands)
+#pragma unroll
+    for (int i = 0; i < TI; ++i)
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) asm volatile("" : "+v"(acc[i][j]));
+  }
 #undef RING_STEP
 #undef RING_ISSUE
   dma_barrier();  // every load landed, every wave done with the stages
