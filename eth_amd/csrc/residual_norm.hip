@@ -2,8 +2,8 @@
 // the next block in one pass over the rows, forward and backward:
 //
 //   n = (x - mu1) r1 post_gamma + post_beta        the block's output, normed
-//   h = residual_scale residual + gate n           the residual stream (stored in 16 bits)
-//   y = (h - mu2) r2 gamma + beta                  of the stored h
+//   h = residual_scale residual + gate n           the residual stream, stored in 16 bits
+//   y = (h - mu2) r2 gamma + beta                  of h before that rounding
 //
 // (root-mean-square norms: mu = 0, r = 1 / sqrt(mean of squares + eps), no
 // betas).  With D the gradient of h, from h's own consumers and through y,
@@ -15,15 +15,20 @@
 //   dpost_gamma = gate S1, dpost_beta = gate S2, dgate = post_gamma S1 +
 //   post_beta S2, dgamma = S3, dbeta = S4.
 //
+// The backward makes h again from x and the residual, with the forward's
+// operations, rather than read the rounded one: the same bytes, and h's rounding is
+// in no other result (read back, it took every result's error from 1 to 1.4
+// roundings, and to more where few rows or columns average it).
+//
 // Memory bounds it: 8 bytes an element forward (x and residual in, h and y
-// out), 12 backward (x, h, dh, dy in, dx, dresidual out).
+// out), 12 backward (x, residual, dh, dy in, dx, dresidual out).
 //
 // Beside the bias-dropout-add and LayerNorm of model/flex_ops.py:104-134 and
 // model/fused_layer_norm.py:62-89; no counterpart in the reference.
 #include "common.h"
 
-// As in the LayerNorm kernels: only the fused multiply-adds that are written are
-// fused, so y is what those kernels make of the stored h, bit for bit.
+// Only the fused multiply-adds that are written are fused, so the backward's h is
+// the forward's, bit for bit.
 #pragma clang fp contract(off)
 
 namespace eth {
@@ -63,6 +68,13 @@ struct RnParams {
 };
 
 // stats [4][rows]: mu1, r1, mu2, r2
+
+// h of an element of x and of the residual
+template <bool FP16>
+__device__ __forceinline__ float rn_stream(float x, float mu, float r, float gamma, float beta, float gate, float scale,
+                                           float res) {
+  return __builtin_fmaf(gate, __builtin_fmaf((x - mu) * r, gamma, beta), scale * res);
+}
 
 // One wave a row, NV vectors of 8 a lane.
 template <int NV, bool FP16>
@@ -118,17 +130,18 @@ __global__ void __launch_bounds__(64 * kRnWaves) rn_fwd_kernel(RnParams g, const
     for (int j = 0; j < 8; j += 2) {
       float t[2];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const float n = __builtin_fmaf((v[i][j + k] - mu1) * r1, rn_at<FP16>(ga, j + k), rn_at<FP16>(be, j + k));
-        t[k] = __builtin_fmaf(g.gate ? rn_at<FP16>(gv, j + k) : 1.f, n, g.scale * rn_at<FP16>(r16[i], j + k));
-      }
+      for (int k = 0; k < 2; ++k)
+        t[k] = rn_stream<FP16>(v[i][j + k], mu1, r1, rn_at<FP16>(ga, j + k), rn_at<FP16>(be, j + k),
+                               g.gate ? rn_at<FP16>(gv, j + k) : 1.f, g.scale, rn_at<FP16>(r16[i], j + k));
       o[j >> 1] = FP16 ? f2h_pair(t[0], t[1]) : f2bf_pair(t[0], t[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) v[i][j + k] = t[k];
     }
     __builtin_amdgcn_raw_buffer_store_b128(o, ho, off, 0, 0);
     const bool in = off < cols * 2;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[i][j] = in ? rn_at<FP16>(o, j) : 0.f;
+      v[i][j] = in ? v[i][j] : 0.f;
       s += v[i][j];
     }
   }
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(64 * kRnWaves) rn_fwd_kernel(RnParams g, const
 // barrier each.
 template <int W, int T, int NVW, bool FP16>
 __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
-    RnParams p, const uint16_t* __restrict__ x, const uint16_t* __restrict__ h, const float* __restrict__ stats,
+    RnParams p, const uint16_t* __restrict__ x, const uint16_t* __restrict__ res, const float* __restrict__ stats,
     const uint16_t* __restrict__ dh, const uint16_t* __restrict__ dy, uint16_t* __restrict__ dx,
     uint16_t* __restrict__ dres, float* __restrict__ part) {
   constexpr int TEAMS = W / T;
@@ -176,14 +189,15 @@ __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
   const int cols = p.cols, rows = p.rows;
   const bool rms = p.rms;
   const int voff = ((sub * NVW) * 64 + lane) * 16;
-  rn_u32x4 pg16[NVW], gt16[NVW], g216[NVW];
+  rn_u32x4 pg16[NVW], pb16[NVW], gt16[NVW], g216[NVW];
   float acc[4][NVW][8];
   {
     const __amdgpu_buffer_rsrc_t a = rn_row(p.post_gamma, 0, cols, true), b = rn_row(p.gate, 0, cols, p.gate),
-                                 c = rn_row(p.gamma, 0, cols, true);
+                                 c = rn_row(p.gamma, 0, cols, true), e = rn_row(p.post_beta, 0, cols, !rms);
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
       pg16[i] = rn_load(a, voff + i * 1024);
+      pb16[i] = rn_load(e, voff + i * 1024);
       gt16[i] = rn_load(b, voff + i * 1024);
       g216[i] = rn_load(c, voff + i * 1024);
 #pragma unroll
@@ -198,21 +212,21 @@ __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
   const float inv_n = 1.0f / cols;
   __shared__ float rsum[2][2][W][2];  // [norm][row parity]
 
-  rn_u32x4 nx[NVW], nh[NVW], nd[NVW], ny[NVW];
+  rn_u32x4 nx[NVW], nr[NVW], nd[NVW], ny[NVW];
   auto load_row = [&](int k) __attribute__((always_inline)) {
     const bool live = k < nrows;
     const int64_t r = g + (int64_t)k * G;
-    const __amdgpu_buffer_rsrc_t xr = rn_row(x, r, cols, live), hr = rn_row(h, r, cols, live),
+    const __amdgpu_buffer_rsrc_t xr = rn_row(x, r, cols, live), rr = rn_row(res, r, cols, live),
                                  dr = rn_row(dh, r, cols, live && dh), yr = rn_row(dy, r, cols, live && dy);
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
-      nh[i] = rn_load(hr, voff + i * 1024);
-      ny[i] = rn_load(yr, voff + i * 1024);
+      nx[i] = rn_load(xr, voff + i * 1024);
+      nr[i] = rn_load(rr, voff + i * 1024);
     }
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
+      ny[i] = rn_load(yr, voff + i * 1024);
       nd[i] = rn_load(dr, voff + i * 1024);
-      nx[i] = rn_load(xr, voff + i * 1024);
     }
   };
   // the team's sums of (a, b), in a fixed order
@@ -238,24 +252,27 @@ __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
     const int k = it * TEAMS + team;
     const int64_t r = g + (int64_t)k * G;
     const bool valid = k < nrows;
-    rn_u32x4 cx[NVW], ch[NVW], cd[NVW], cy[NVW];
+    rn_u32x4 cx[NVW], cr[NVW], cd[NVW], cy[NVW];
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
       cx[i] = nx[i];
-      ch[i] = nh[i];
+      cr[i] = nr[i];
       cd[i] = nd[i];
       cy[i] = ny[i];
     }
     const float mu1 = valid ? stats[r] : 0.f, r1 = valid ? stats[rows + r] : 0.f;
     const float mu2 = valid ? stats[2LL * rows + r] : 0.f, r2 = valid ? stats[3LL * rows + r] : 0.f;
     if (it + 1 < iters) load_row(k + TEAMS);
+    float hhat[NVW][8];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < NVW; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float dv = rn_at<FP16>(cy[i], j);
-        const float hh = (rn_at<FP16>(ch[i], j) - mu2) * r2;
+        const float h = rn_stream<FP16>(rn_at<FP16>(cx[i], j), mu1, r1, rn_at<FP16>(pg16[i], j), rn_at<FP16>(pb16[i], j),
+                                        p.gate ? rn_at<FP16>(gt16[i], j) : 1.f, p.scale, rn_at<FP16>(cr[i], j));
+        const float hh = hhat[i][j] = (h - mu2) * r2;
         const float dg = dv * rn_at<FP16>(g216[i], j);
         s1 += dg;
         s2 = __builtin_fmaf(dg, hh, s2);
@@ -268,8 +285,8 @@ __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
     // would not fit the registers
 #pragma unroll
     for (int i = 0; i < NVW; ++i) {
-      asm volatile("" : "+v"(ch[i]), "+v"(cy[i]));
-      asm volatile("" : "+v"(g216[i]));
+      asm volatile("" : "+v"(cx[i]), "+v"(cy[i]));
+      asm volatile("" : "+v"(g216[i]), "+v"(gt16[i]), "+v"(pg16[i]));
     }
     float d[NVW][8];
     float t1 = 0.f, t2 = 0.f;
@@ -278,7 +295,7 @@ __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float dv = rn_at<FP16>(cy[i], j);
-        const float hh = (rn_at<FP16>(ch[i], j) - mu2) * r2;
+        const float hh = hhat[i][j];
         const float through = r2 * __builtin_fmaf(-inv_n, __builtin_fmaf(hh, s2, s1), dv * rn_at<FP16>(g216[i], j));
         d[i][j] = rn_at<FP16>(cd[i], j) + through;
         const float xh = (rn_at<FP16>(cx[i], j) - mu1) * r1;
@@ -453,13 +470,13 @@ static void launch_rn_fwd(const RnParams& p, const uint16_t* x, const uint16_t* 
 }
 
 template <bool FP16>
-static void launch_rn_bwd(const RnParams& p, int groups, const uint16_t* x, const uint16_t* h, const float* stats,
+static void launch_rn_bwd(const RnParams& p, int groups, const uint16_t* x, const uint16_t* res, const float* stats,
                           const uint16_t* dh, const uint16_t* dy, uint16_t* dx, uint16_t* dres, float* part,
                           hipStream_t s) {
   const RnShape f = rn_shape(p.cols);
 #define ETH_RN_BWD(W, T, N)                                                                        \
   case T * 10 + N:                                                                                 \
-    rn_bwd_kernel<W, T, N, FP16><<<groups, 64 * W, 0, s>>>(p, x, h, stats, dh, dy, dx, dres, part); \
+    rn_bwd_kernel<W, T, N, FP16><<<groups, 64 * W, 0, s>>>(p, x, res, stats, dh, dy, dx, dres, part); \
     break;
   switch (f.team * 10 + f.vectors) {
     ETH_RN_BWD(8, 1, 1) ETH_RN_BWD(8, 1, 2) ETH_RN_BWD(15, 3, 1) ETH_RN_BWD(16, 4, 1) ETH_RN_BWD(15, 5, 1)
@@ -517,14 +534,14 @@ extern "C" int64_t eth_residual_norm_workspace(int64_t rows, int64_t cols) {
   return rows > 0 && cols > 0 ? (int64_t)rn_groups(rows, cols) * 4 * cols : 0;
 }
 
-extern "C" int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const void* x, const void* h,
+extern "C" int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const void* x, const void* residual,
                                      const float* stats, const void* dh, const void* dy, void* dx, void* dresidual,
                                      const eth_residual_norm_grad_t* grads, float* workspace, void* stream) {
   const int rc = check_rn("eth_residual_norm_bwd", desc);
   if (rc != ETH_OK) return rc;
   if (desc->rows == 0) return ETH_OK;
-  ETH_CHECK_ARG(x && h && stats && (dh || dy) && grads && workspace, "eth_residual_norm_bwd: null pointer");
-  ETH_CHECK_ARG((((uintptr_t)x | (uintptr_t)h | (uintptr_t)dh | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)dresidual |
+  ETH_CHECK_ARG(x && residual && stats && (dh || dy) && grads && workspace, "eth_residual_norm_bwd: null pointer");
+  ETH_CHECK_ARG((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)dh | (uintptr_t)dy | (uintptr_t)dx | (uintptr_t)dresidual |
                   (uintptr_t)workspace) & 15u) == 0, "eth_residual_norm_bwd: operands must be 16-byte aligned");
   ETH_CHECK_ARG((desc->gate || !grads[2].grad) && (!desc->rms || (!grads[1].grad && !grads[4].grad)),
                 "eth_residual_norm_bwd: a gradient of a parameter that is not there");
@@ -539,10 +556,10 @@ extern "C" int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const
   const int groups = rn_groups(desc->rows, desc->cols);
   hipStream_t s = (hipStream_t)stream;
   if (desc->dtype == ETH_F16)
-    launch_rn_bwd<true>(p, groups, (const uint16_t*)x, (const uint16_t*)h, stats, (const uint16_t*)dh,
+    launch_rn_bwd<true>(p, groups, (const uint16_t*)x, (const uint16_t*)residual, stats, (const uint16_t*)dh,
                         (const uint16_t*)dy, (uint16_t*)dx, (uint16_t*)dresidual, workspace, s);
   else
-    launch_rn_bwd<false>(p, groups, (const uint16_t*)x, (const uint16_t*)h, stats, (const uint16_t*)dh,
+    launch_rn_bwd<false>(p, groups, (const uint16_t*)x, (const uint16_t*)residual, stats, (const uint16_t*)dh,
                          (const uint16_t*)dy, (uint16_t*)dx, (uint16_t*)dresidual, workspace, s);
   ETH_CHECK_LAUNCH("eth_residual_norm_bwd");
   bool any = false;

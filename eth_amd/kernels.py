@@ -334,7 +334,7 @@ def _check_like(name, t, x):
 
 def residual_norm_fwd(x, residual, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps=1e-5, rms=False):
     """(h, y, stats): h = residual_scale * residual + gate * norm(x), y = norm(h)
-    of the stored h, each norm with its gamma and beta; gate None: one.  With
+    of h before its rounding, each norm with its gamma and beta; gate None: one.  With
     `rms` the norms are root-mean-square ones and have no betas (None).  stats
     [4, rows] fp32, for the backward."""
     index, desc = _norm_desc(x, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms)
@@ -348,7 +348,7 @@ def residual_norm_fwd(x, residual, post_gamma, post_beta, gate, residual_scale, 
     return h, y, stats
 
 
-def residual_norm_bwd(x, h, stats, dh, dy, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms, grads,
+def residual_norm_bwd(x, residual, stats, dh, dy, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps, rms, grads,
                       need_dx=True, need_dresidual=True):
     """(dx, dresidual) of residual_norm_fwd for the gradients dh of h and dy of y
     (one of them may be None), None where not needed.  `grads`: for post_gamma,
@@ -359,8 +359,8 @@ def residual_norm_bwd(x, h, stats, dh, dy, post_gamma, post_beta, gate, residual
     given = [t for t in (dh, dy) if t is not None]
     if not given:
         raise ValueError("residual_norm_bwd needs dh or dy")
-    _check_device(index, h, stats, *given)
-    for name, t in (("x", x), ("h", h), ("dh", dh), ("dy", dy)):
+    _check_device(index, residual, stats, *given)
+    for name, t in (("x", x), ("residual", residual), ("dh", dh), ("dy", dy)):
         if t is not None:
             _check_like(name, t, x)
     if stats.dtype != torch.float32 or stats.shape != (4, desc.rows) or not stats.is_contiguous():
@@ -386,8 +386,8 @@ def residual_norm_bwd(x, h, stats, dh, dy, post_gamma, post_beta, gate, residual
                 pair[0].zero_()
         return dx, dresidual
     ws = torch.empty(nat.value("eth_residual_norm_workspace", desc.rows, desc.cols), dtype=torch.float32, device=x.device)
-    _launch(index, "eth_residual_norm_bwd", ctypes.byref(desc), x.data_ptr(), h.data_ptr(), stats.data_ptr(), nat.ptr(dh),
-            nat.ptr(dy), nat.ptr(dx), nat.ptr(dresidual), table, ws.data_ptr())
+    _launch(index, "eth_residual_norm_bwd", ctypes.byref(desc), x.data_ptr(), residual.data_ptr(), stats.data_ptr(),
+            nat.ptr(dh), nat.ptr(dy), nat.ptr(dx), nat.ptr(dresidual), table, ws.data_ptr())
     return dx, dresidual
 
 

@@ -327,9 +327,9 @@ class GatedResidualNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if residual.shape != x.shape:
             raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
-        xc, scale = _whole(x), float(residual_scale)
-        h, y, stats = K.residual_norm_fwd(xc, _whole(residual), post_gamma, post_beta, gate, scale, gamma, beta, eps, rms)
-        ctx.save_for_backward(xc, h, stats, post_gamma, post_beta, gate, gamma, beta)
+        xc, rc, scale = _whole(x), _whole(residual), float(residual_scale)
+        h, y, stats = K.residual_norm_fwd(xc, rc, post_gamma, post_beta, gate, scale, gamma, beta, eps, rms)
+        ctx.save_for_backward(xc, rc, stats, post_gamma, post_beta, gate, gamma, beta)
         ctx.scale, ctx.eps, ctx.rms = scale, eps, rms
         return h, y
 
@@ -337,7 +337,7 @@ class GatedResidualNormFn(torch.autograd.Function):
     def backward(ctx, dh, dy):
         if dh is None and dy is None:
             return (None,) * 10
-        x, h, stats, *params = ctx.saved_tensors
+        x, residual, stats, *params = ctx.saved_tensors
         needs = ctx.needs_input_grad
         wanted = needs[2], needs[3], needs[4], needs[6], needs[7]
         # gradients that are returned share one allocation
@@ -360,7 +360,7 @@ class GatedResidualNormFn(torch.autograd.Function):
             targets.append(target)
             returned.append(result)
         pg, pb, gate, gamma, beta = params
-        dx, dres = K.residual_norm_bwd(_whole(x), _whole(h), stats, None if dh is None else _whole(dh),
+        dx, dres = K.residual_norm_bwd(_whole(x), _whole(residual), stats, None if dh is None else _whole(dh),
                                        None if dy is None else _whole(dy), pg, pb, gate, ctx.scale, gamma, beta, ctx.eps,
                                        ctx.rms, targets, needs[0], needs[1])
         for mg, extra in added:

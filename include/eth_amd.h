@@ -525,12 +525,12 @@ int eth_adapter_linear_bwd(const eth_adapter_desc_t* desc, const void* x, const 
  * next block, on contiguous [rows, cols] tensors of bf16 or fp16 (`dtype`; cols a
  * multiple of 8 up to 8192, rows below 2^26; 16-byte aligned):
  *   n = norm(x) post_gamma + post_beta,  h = residual_scale residual + gate n,
- *   y = norm(h) gamma + beta  (of the stored h),
+ *   y = norm(h) gamma + beta  (of h before it is rounded to 16 bits),
  * norm(v) = (v - mean) / sqrt(variance + eps), or with `rms` v / sqrt(mean of
  * squares + eps), then without betas (NULL).  gate [cols] NULL: one.
  * stats [4, rows] fp32: mean and inverse deviation of x, then of h, for the
  * backward (means 0 with rms).
- * The backward takes dh (the gradient of h from its other consumers) and dy, one
+ * The backward takes the forward's x, residual and stats, dh (the gradient of h from its other consumers) and dy, one
  * of which may be NULL (zero), writes dx and dresidual (either may be NULL), and
  * the gradients of the five parameters, grads[0..4] in the descriptor's order:
  * each NULL, in `dtype`, or in fp32 (stored, or added to with `accumulate`), no two
@@ -551,7 +551,7 @@ typedef struct eth_residual_norm_grad {
 int eth_residual_norm_fwd(const eth_residual_norm_desc_t* desc, const void* x, const void* residual,
                           void* h, void* y, float* stats, void* stream);
 int64_t eth_residual_norm_workspace(int64_t rows, int64_t cols);
-int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const void* x, const void* h,
+int eth_residual_norm_bwd(const eth_residual_norm_desc_t* desc, const void* x, const void* residual,
                           const float* stats, const void* dh, const void* dy, void* dx,
                           void* dresidual, const eth_residual_norm_grad_t* grads,
                           float* workspace, void* stream);

@@ -11,19 +11,22 @@ import torch
 STEP = 2.0**-23
 
 
-def _norm(v, eps, rms):
-    """(vhat, inverse deviation, bound of vhat) of rows v in fp32."""
+def _norm(v, eps, rms, ev=0.0):
+    """(vhat, inverse deviation, bound of vhat) of rows v in fp32, off by up to ev."""
     cols = v.shape[1]
     deep = (cols / 64 + 16) * STEP
+    ev = torch.zeros_like(v) + ev
     mu = torch.zeros_like(v[:, :1]) if rms else v.mean(1, keepdim=True)
     inv = 1.0 / torch.sqrt(((v - mu) ** 2).mean(1, keepdim=True) + eps)
     hat = (v - mu) * inv
-    off = torch.zeros_like(mu) if rms else inv * deep * v.abs().mean(1, keepdim=True)
-    return hat, inv, off + hat.abs() * deep
+    off = torch.zeros_like(mu) if rms else inv * (deep * v.abs().mean(1, keepdim=True) + ev.mean(1, keepdim=True))
+    # (the deviation's own change, relative to it: mean of |vhat| ev, over it)
+    return hat, inv, off + inv * ev + hat.abs() * (deep + inv * (hat.abs() * ev).mean(1, keepdim=True))
 
 
-def _back(g, eg, hat, ehat, inv, rms):
-    """(gradient of v, its bound) from that of vhat (g, off by up to eg)."""
+def _back(g, eg, hat, ehat, inv, rms, einv=0.0):
+    """(gradient of v, its bound) from that of vhat (g, off by up to eg); einv: what
+    inv is off by, relative to it, beyond its rounding."""
     deep = (g.shape[1] / 64 + 16) * STEP
     mean = lambda x: x.mean(1, keepdim=True)  # noqa: E731
     s1, s2 = (torch.zeros_like(inv) if rms else mean(g)), mean(g * hat)
@@ -31,40 +34,48 @@ def _back(g, eg, hat, ehat, inv, rms):
     e2 = mean(eg * hat.abs() + g.abs() * ehat) + deep * mean((g * hat).abs())
     out = inv * (g - s1 - hat * s2)
     size = g.abs() + s1.abs() + (hat * s2).abs()
-    return out, inv * (eg + e1 + hat.abs() * e2 + ehat * s2.abs() + deep * size)
+    return out, inv * (eg + e1 + hat.abs() * e2 + ehat * s2.abs() + (deep + einv) * size)
 
 
-def forward(x, residual, pg, pb, gate, scale, gamma, beta, eps, rms, u=0.0, least=0.0, stored=None):
-    """{"h", "y"} and their bounds; y is that of `stored`, the h that a kernel
-    rounded, where that is given."""
-    x, residual, pg, gamma = (t.double() for t in (x, residual, pg, gamma))
-    pb, beta = (0.0 if t is None else t.double() for t in (pb, beta))
-    gate = torch.ones_like(pg) if gate is None else gate.double()
-    hat, _, ehat = _norm(x, eps, rms)
+def _stream(x, residual, pg, pb, gate, scale, eps, rms):
+    """h in fp32 and its bound; xhat, its inverse deviation and its bound."""
+    hat, inv, ehat = _norm(x, eps, rms)
     n = hat * pg + pb
     h = scale * residual + gate * n
-    r = {"h": h}
-    r["bound_h"] = (gate * pg).abs() * ehat + 4 * STEP * ((gate * n).abs() + (gate * hat * pg).abs()
-                                                          + (scale * residual).abs()) + 1.001 * u * h.abs() + least
-    hat, _, ehat = _norm(h if stored is None else stored.double(), eps, rms)
+    eh = (gate * pg).abs() * ehat + 4 * STEP * ((gate * n).abs() + (gate * hat * pg).abs() + (scale * residual).abs())
+    return h, eh, hat, inv, ehat
+
+
+def _double(x, residual, pg, pb, gate, gamma):
+    x, residual, pg, gamma = (t.double() for t in (x, residual, pg, gamma))
+    pb = torch.zeros_like(pg) if pb is None else pb.double()
+    return x, residual, pg, pb, torch.ones_like(pg) if gate is None else gate.double(), gamma
+
+
+def forward(x, residual, pg, pb, gate, scale, gamma, beta, eps, rms, u=0.0, least=0.0):
+    """{"h", "y"} and their bounds; y is that of h before its rounding."""
+    x, residual, pg, pb, gate, gamma = _double(x, residual, pg, pb, gate, gamma)
+    beta = 0.0 if beta is None else beta.double()
+    h, eh, *_ = _stream(x, residual, pg, pb, gate, scale, eps, rms)
+    r = {"h": h, "bound_h": eh + 1.001 * u * h.abs() + least}
+    hat, _, ehat = _norm(h, eps, rms, eh)
     r["y"] = hat * gamma + beta
     r["bound_y"] = (gamma.abs() * ehat + 4 * STEP * ((hat * gamma).abs() + r["y"].abs())
                     + 1.001 * u * r["y"].abs() + least)
     return r
 
 
-def backward(x, h, dh, dy, pg, pb, gate, scale, gamma, eps, rms, u=0.0, least=0.0):
+def backward(x, residual, dh, dy, pg, pb, gate, scale, gamma, eps, rms, u=0.0, least=0.0):
     """{"dx", "dresidual", "dpost_gamma", "dpost_beta", "dgate", "dgamma",
-    "dbeta"} and their bounds, for a stored h; dh or dy may be None."""
-    x, h, pg, gamma = (t.double() for t in (x, h, pg, gamma))
-    pb = torch.zeros_like(pg) if pb is None else pb.double()
-    gate = torch.ones_like(pg) if gate is None else gate.double()
+    "dbeta"} and their bounds; dh or dy may be None."""
+    x, residual, pg, pb, gate, gamma = _double(x, residual, pg, pb, gate, gamma)
     dh, dy = (torch.zeros_like(x) if t is None else t.double() for t in (dh, dy))
     rows = x.shape[0]
-    hat1, inv1, ehat1 = _norm(x, eps, rms)
-    hat2, inv2, ehat2 = _norm(h, eps, rms)
+    h, eh, hat1, inv1, ehat1 = _stream(x, residual, pg, pb, gate, scale, eps, rms)
+    hat2, inv2, ehat2 = _norm(h, eps, rms, eh)
+    einv2 = inv2 * (hat2.abs() * eh).mean(1, keepdim=True)
     g2 = dy * gamma
-    through, ethrough = _back(g2, STEP * g2.abs(), hat2, ehat2, inv2, rms)
+    through, ethrough = _back(g2, STEP * g2.abs(), hat2, ehat2, inv2, rms, einv2)
     D = dh + through
     eD = ethrough + STEP * D.abs()
     g1 = D * gate * pg

@@ -66,10 +66,10 @@ def test_step(cuda, dtype):
     _within(loss, r, "loss")
     _within(dy, {"dy": r["dh"], "bound_dy": r["bound_dh"]}, "dy")
     _within(got["head"], {"head": r["dw"], "bound_head": r["bound_dw"]}, "head")
-    r = residual_norm.forward(z, v["x"], v["pg"], v["pb"], v["gate"], 0.5, v["gamma"], v["beta"], 1e-5, False, u, least, h)
+    r = residual_norm.forward(z, v["x"], v["pg"], v["pb"], v["gate"], 0.5, v["gamma"], v["beta"], 1e-5, False, u, least)
     _within(h, r, "h")
     _within(y, r, "y")
-    r = residual_norm.backward(z, h, None, dy, v["pg"], v["pb"], v["gate"], 0.5, v["gamma"], 1e-5, False, u, least)
+    r = residual_norm.backward(z, v["x"], None, dy, v["pg"], v["pb"], v["gate"], 0.5, v["gamma"], 1e-5, False, u, least)
     _within(dz, {"dz": r["dx"], "bound_dz": r["bound_dx"]}, "dz")
     for k, name in (("pg", "dpost_gamma"), ("pb", "dpost_beta"), ("gate", "dgate"), ("gamma", "dgamma"), ("beta", "dbeta")):
         _within(got[k], r, name)

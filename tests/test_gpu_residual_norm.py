@@ -37,9 +37,9 @@ def _forward(o, scale, eps, rms):
     return K.residual_norm_fwd(o["x"], o["residual"], o["pg"], o["pb"], o["gate"], scale, o["gamma"], o["beta"], eps, rms)
 
 
-def _backward(o, h, stats, dh, dy, scale, eps, rms, grads, **kw):
+def _backward(o, stats, dh, dy, scale, eps, rms, grads, **kw):
     pg, pb, gate, gamma, beta = _params(o)
-    return K.residual_norm_bwd(o["x"], h, stats, dh, dy, pg, pb, gate, scale, gamma, beta, eps, rms, grads, **kw)
+    return K.residual_norm_bwd(o["x"], o["residual"], stats, dh, dy, pg, pb, gate, scale, gamma, beta, eps, rms, grads, **kw)
 
 
 def _grads(o, fp32=False):
@@ -65,15 +65,13 @@ def test_forward_and_backward(cuda, dtype, rms, gate, scale, rows, cols):
     h, y, stats = _forward(o, scale, eps, rms)
     u, least = HALF_STEP[dtype], LEAST[dtype]
     r = oracle.forward(o["x"], o["residual"], o["pg"], o["pb"], o["gate"], scale, o["gamma"], o["beta"], eps, rms, u,
-                       least, stored=h)
+                       least)
     _within(h, r, "h")
     _within(y, r, "y")
-    if not rms:
-        assert torch.equal(y, K.layer_norm_fwd(h, o["gamma"], o["beta"], eps)[0])
     for dh, dy in ((o["dh"], o["dy"]), (o["dh"], None), (None, o["dy"])):
         grads = _grads(o)
-        dx, dres = _backward(o, h, stats, dh, dy, scale, eps, rms, grads)
-        r = oracle.backward(o["x"], h, dh, dy, o["pg"], o["pb"], o["gate"], scale, o["gamma"], eps, rms, u, least)
+        dx, dres = _backward(o, stats, dh, dy, scale, eps, rms, grads)
+        r = oracle.backward(o["x"], o["residual"], dh, dy, o["pg"], o["pb"], o["gate"], scale, o["gamma"], eps, rms, u, least)
         _within(dx, r, "dx")
         _within(dres, r, "dresidual")
         for name, pair in zip(NAMES, grads):
@@ -81,15 +79,15 @@ def test_forward_and_backward(cuda, dtype, rms, gate, scale, rows, cols):
                 _within(pair[0], r, name)
     # fp32 gradients, stored and added; nothing else asked for
     wide = _grads(o, fp32=True)
-    nothing = _backward(o, h, stats, None, o["dy"], scale, eps, rms, wide, need_dx=False, need_dresidual=False)
+    nothing = _backward(o, stats, None, o["dy"], scale, eps, rms, wide, need_dx=False, need_dresidual=False)
     assert nothing == (None, None)
-    r = oracle.backward(o["x"], h, None, o["dy"], o["pg"], o["pb"], o["gate"], scale, o["gamma"], eps, rms)
+    r = oracle.backward(o["x"], o["residual"], None, o["dy"], o["pg"], o["pb"], o["gate"], scale, o["gamma"], eps, rms)
     once = [None if p is None else p[0].clone() for p in wide]
     for name, pair in zip(NAMES, wide):
         if pair is not None:
             _within(pair[0], r, name)
     more = [None if p is None else (p[0], True) for p in wide]
-    _backward(o, h, stats, None, o["dy"], scale, eps, rms, more)
+    _backward(o, stats, None, o["dy"], scale, eps, rms, more)
     for pair, one in zip(wide, once):
         assert pair is None or torch.equal(pair[0], one + one)
 
@@ -100,14 +98,14 @@ def test_rows_stay_apart(cuda):
     for rms in (False, True):
         o = _operands(cuda, 12, 1032, torch.bfloat16, rms, True)
         clean = _forward(o, 0.7, 1e-5, rms)
-        want = _backward(o, clean[0], clean[2], o["dh"], o["dy"], 0.7, 1e-5, rms, _grads(o))
+        want = _backward(o, clean[2], o["dh"], o["dy"], 0.7, 1e-5, rms, _grads(o))
         bad = dict(o, x=o["x"].clone(), residual=o["residual"].clone(), dy=o["dy"].clone())
         bad["x"][2, 5], bad["residual"][4, 1000], bad["dy"][6, 0] = float("nan"), float("inf"), float("nan")
         h, y, stats = _forward(bad, 0.7, 1e-5, rms)
         fine = [i for i in range(12) if i not in (2, 4)]
         assert torch.equal(h[fine], clean[0][fine]) and torch.equal(y[fine], clean[1][fine])
         assert h[2].isnan().all() and y[4].isnan().any()
-        got = _backward(bad, h, stats, o["dh"], bad["dy"], 0.7, 1e-5, rms, _grads(o))
+        got = _backward(bad, stats, o["dh"], bad["dy"], 0.7, 1e-5, rms, _grads(o))
         fine.remove(6)
         for a, b in zip(got, want):
             assert torch.equal(a[fine], b[fine])
@@ -119,7 +117,7 @@ def test_rows_stay_apart(cuda):
     o["pb"].zero_()
     h, y, stats = _forward(o, 1.0, 1e-5, False)
     assert torch.equal(h, o["residual"]) and torch.equal(y, o["beta"].expand_as(y))
-    dx, dres = _backward(o, h, stats, o["dh"], None, 1.0, 1e-5, False, _grads(o))
+    dx, dres = _backward(o, stats, o["dh"], None, 1.0, 1e-5, False, _grads(o))
     assert dx.isfinite().all() and torch.equal(dres, o["dh"])
 
 
@@ -146,7 +144,7 @@ def test_autograd_main_grads_streams_and_replays(cuda):
     o = sets[0]
     h, y, stats = _forward(o, 0.7, 1e-5, False)
     grads = _grads(o)
-    dx, dres = _backward(o, h, stats, o["dh"], o["dy"], 0.7, 1e-5, False, grads)
+    dx, dres = _backward(o, stats, o["dh"], o["dy"], 0.7, 1e-5, False, grads)
     for a, b in zip(want[0], (h, y, dx, dres, *(g[0] for g in grads))):
         assert torch.equal(a, b)
     with torch.autograd.graph.save_on_cpu():
@@ -159,11 +157,11 @@ def test_autograd_main_grads_streams_and_replays(cuda):
     hh, yy = _apply(leaf)
     assert torch.equal(hh.transpose(0, 1).reshape(24, 520), h) and torch.equal(yy.transpose(0, 1).reshape(24, 520), y)
     (got,) = torch.autograd.grad(yy, leaf["x"], o["dy"].view(4, 6, 520).transpose(0, 1))
-    alone, _ = _backward(o, h, stats, None, o["dy"], 0.7, 1e-5, False, [None] * 5)
+    alone, _ = _backward(o, stats, None, o["dy"], 0.7, 1e-5, False, [None] * 5)
     assert torch.equal(got.transpose(0, 1).reshape(24, 520), alone)
     # main grads: added or, where stale, stored; one parameter in both places
     wide = _grads(o, fp32=True)
-    _backward(o, h, stats, o["dh"], o["dy"], 0.7, 1e-5, False, wide)
+    _backward(o, stats, o["dh"], o["dy"], 0.7, 1e-5, False, wide)
     params = {k: torch.nn.Parameter(o[k].clone()) for k in ("pg", "pb", "gate", "gamma", "beta")}
     for p in params.values():
         p.main_grad = torch.ones(520, device=cuda)
@@ -175,9 +173,9 @@ def test_autograd_main_grads_streams_and_replays(cuda):
     both = torch.nn.Parameter(o["gamma"].clone())
     both.main_grad = torch.ones(520, device=cuda)
     same = {**o, "pg": o["gamma"]}
-    h2, _, st2 = _forward(same, 0.7, 1e-5, False)
+    st2 = _forward(same, 0.7, 1e-5, False)[2]
     wide = _grads(same, fp32=True)
-    _backward(same, h2, st2, o["dh"], o["dy"], 0.7, 1e-5, False, wide)
+    _backward(same, st2, o["dh"], o["dy"], 0.7, 1e-5, False, wide)
     torch.autograd.backward(_apply({**o, "pg": both, "gamma": both}), (o["dh"], o["dy"]))
     assert torch.equal(both.main_grad, 1.0 + wide[0][0] + wide[3][0])
     streams, got = [torch.cuda.Stream() for _ in range(2)], []
@@ -193,7 +191,7 @@ def test_autograd_main_grads_streams_and_replays(cuda):
     def captured():
         h, y, stats = _forward(held, 0.7, 1e-5, False)
         grads = _grads(held)
-        dx, dres = _backward(held, h, stats, held["dh"], held["dy"], 0.7, 1e-5, False, grads)
+        dx, dres = _backward(held, stats, held["dh"], held["dy"], 0.7, 1e-5, False, grads)
         return h, y, dx, dres, *(g[0] for g in grads)
 
     side = torch.cuda.Stream()
@@ -237,13 +235,13 @@ def test_refusals(cuda):
                    dict(x=o["x"].cpu(), residual=o["residual"].cpu())):
         with pytest.raises(ValueError):
             K.residual_norm_fwd(**(good | change))
-    h, _, stats = K.residual_norm_fwd(**good)
+    stats = K.residual_norm_fwd(**good)[2]
     for kw in (dict(dh=None, dy=None), dict(dh=o["dh"].float()), dict(dy=o["dy"][:3]), dict(stats=stats[:3]),
-               dict(stats=stats.double()), dict(h=h.half()), dict(grads=[(o["pg"].clone(), True), *[None] * 4]),
+               dict(stats=stats.double()), dict(residual=o["residual"].half()), dict(grads=[(o["pg"].clone(), True), *[None] * 4]),
                dict(grads=[(torch.zeros(60, device=cuda), False), *[None] * 4]),
                dict(grads=[(s := torch.zeros(64, device=cuda), False), (s, False), *[None] * 3])):
-        args = dict(h=h, stats=stats, dh=o["dh"], dy=o["dy"], grads=[None] * 5) | kw
+        args = dict(residual=o["residual"], stats=stats, dh=o["dh"], dy=o["dy"], grads=[None] * 5) | kw
         with pytest.raises(ValueError):
-            _backward(o, args["h"], args["stats"], args["dh"], args["dy"], 1.0, 1e-5, False, args["grads"])
+            _backward({**o, "residual": args["residual"]}, args["stats"], args["dh"], args["dy"], 1.0, 1e-5, False, args["grads"])
     with pytest.raises(ValueError):
         GatedResidualNormFn.apply(o["x"], o["residual"][:2], o["pg"], o["pb"], None, 1.0, o["gamma"], o["beta"])

@@ -34,7 +34,7 @@ def test_c_entries_refuse_before_any_launch():
 
     def bwd(desc, table=None, **change):
         table = (nat.ResidualNormGrad * 5)() if table is None else table
-        args = dict(x=P, h=P, stats=P, dh=P, dy=P, dx=P, dres=P, grads=table, ws=P, stream=None) | change
+        args = dict(x=P, residual=P, stats=P, dh=P, dy=P, dx=P, dres=P, grads=table, ws=P, stream=None) | change
         nat.call("eth_residual_norm_bwd", ctypes.byref(desc) if desc else None, *args.values())
 
     for call in (fwd, bwd):
@@ -47,7 +47,7 @@ def test_c_entries_refuse_before_any_launch():
                    dict(y=P + 8)):
         with pytest.raises(ValueError):
             fwd(_desc(), **change)
-    for change in (dict(x=None), dict(h=None), dict(stats=None), dict(dh=None, dy=None), dict(grads=None), dict(ws=None),
+    for change in (dict(x=None), dict(residual=None), dict(stats=None), dict(dh=None, dy=None), dict(grads=None), dict(ws=None),
                    dict(dh=P + 2), dict(dx=P + 8), dict(ws=P + 4)):
         with pytest.raises(ValueError):
             bwd(_desc(), **change)
@@ -85,8 +85,7 @@ def test_oracle_gradients_equal_differences(rms, gated):
         r = oracle.forward(v["x"], v["residual"], v["pg"], v["pb"], v["gate"], 0.6, v["gamma"], v["beta"], 1e-5, rms)
         return (r["h"] * dh + r["y"] * dy).sum()
 
-    h = oracle.forward(v["x"], v["residual"], v["pg"], v["pb"], v["gate"], 0.6, v["gamma"], v["beta"], 1e-5, rms)["h"]
-    r = oracle.backward(v["x"], h, dh, dy, v["pg"], v["pb"], v["gate"], 0.6, v["gamma"], 1e-5, rms)
+    r = oracle.backward(v["x"], v["residual"], dh, dy, v["pg"], v["pb"], v["gate"], 0.6, v["gamma"], 1e-5, rms)
     for key, name in (("x", "dx"), ("residual", "dresidual"), ("pg", "dpost_gamma"), ("pb", "dpost_beta"),
                       ("gate", "dgate"), ("gamma", "dgamma"), ("beta", "dbeta")):
         if v[key] is None:
