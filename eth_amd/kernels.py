@@ -310,20 +310,23 @@ def _norm_desc(x, post_gamma, post_beta, gate, residual_scale, gamma, beta, eps,
         raise ValueError("root-mean-square norms have no betas")
     if not rms and (post_beta is None or beta is None):
         raise ValueError("betas are needed (but for root-mean-square norms)")
-    desc = nat.ResidualNormDesc()
+    at, dtype, shape = [], x.dtype, (cols,)
     for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("gate", gate), ("gamma", gamma),
                     ("beta", beta)):
-        if t is None and name in ("post_gamma", "gamma"):
-            raise ValueError(f"{name} is needed")
-        if t is not None:
-            if t.dtype != x.dtype or t.shape != (cols,) or not t.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous [{cols}] tensor of the input type")
-            if t.data_ptr() % 16:
-                raise ValueError(f"{name} must be 16-byte aligned")
+        if t is None:
+            if name in ("post_gamma", "gamma"):
+                raise ValueError(f"{name} is needed")
+            at.append(None)
+            continue
+        place = t.data_ptr()
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous [{cols}] tensor of the input type")
+        if place % 16:
+            raise ValueError(f"{name} must be 16-byte aligned")
+        if t.get_device() != index:
             _check_device(index, t)
-            setattr(desc, name, t.data_ptr())
-    desc.rows, desc.cols, desc.rms, desc.dtype = rows, cols, 1 if rms else 0, code
-    desc.residual_scale, desc.eps = float(residual_scale), float(eps)
+        at.append(place)
+    desc = nat.ResidualNormDesc(*at, rows, cols, float(residual_scale), float(eps), bool(rms), code)
     return index, desc
 
 
