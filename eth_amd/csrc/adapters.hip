@@ -899,6 +899,7 @@ extern "C" int eth_adapter_linear_bwd(const eth_adapter_desc_t* desc, const void
                   (uintptr_t)dx | (uintptr_t)da->grad | (uintptr_t)db->grad) & 15u) == 0 &&
                     ((uintptr_t)workspace & 255) == 0,
                 "eth_adapter_linear_bwd: operands must be 16-byte, the workspace 256-byte aligned");
+  ETH_CHECK_ARG(!da->grad || da->grad != db->grad, "eth_adapter_linear_bwd: dA and dB in one place");
   for (const eth_adapter_grad_t* t : {da, db})
     ETH_CHECK_ARG(!t->accumulate || t->fp32, "eth_adapter_linear_bwd: accumulate needs an fp32 gradient");
   return desc->dtype == ETH_F16

@@ -677,6 +677,16 @@ def _aligned_rows(x):
     return x2.clone() if x2.data_ptr() % 16 else x2
 
 
+def _aligned_target(mg, accumulate):
+    """(tensor for the kernel, whether it adds, what is called behind it) for a main
+    grad that may start anywhere in its buffer: itself where it is 16-byte aligned,
+    else a tensor that is stored or added there."""
+    if mg.data_ptr() % 16 == 0:
+        return mg, accumulate, lambda: None
+    own = torch.empty_like(mg)
+    return own, False, lambda: mg.add_(own) if accumulate else mg.copy_(own)
+
+
 class LinearCrossEntropyFn(torch.autograd.Function):
     """Per-token loss [...] (fp32) of the head's logits hidden [..., H] @
     weight[V, H]^T against int64 labels [...]: LinearFn and CrossEntropyFn in
@@ -698,25 +708,40 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         h, weight, lab, lse = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
         mg, accumulate = _fp32_accum_target(weight) if need_w else (None, False)
-        after = _chained(weight, h.device) if mg is not None else None
-        dh, dw = K.linear_xent_bwd(_aligned_rows(h), weight, lab, lse, _row_values(dloss.reshape(-1)), ctx.ignore_index,
-                                   need_h, need_w, mg, accumulate)
+        target = mg
         if mg is not None:
+            after = _chained(weight, h.device)
+            target, accumulate, settle = _aligned_target(mg, accumulate)
+        dh, dw = K.linear_xent_bwd(_aligned_rows(h), weight, lab, lse, _row_values(dloss.reshape(-1)), ctx.ignore_index,
+                                   need_h, need_w, target, accumulate)
+        if mg is not None:
+            settle()
             after()
             grad_written(weight)
             dw = None
         return None if dh is None else dh.view(ctx.shape), dw, None, None, None
 
 
-def _adapter_target(p, need):
-    """(pair for K.adapter_linear_bwd, gradient to return) of lora_a or lora_b."""
-    if not need:
-        return None, None
-    mg, accumulate = _fp32_accum_target(p)
-    if mg is not None:
-        return (mg, accumulate), None
-    new = torch.empty(p.shape, dtype=p.dtype, device=p.device)
-    return (new, False), new
+def _adapter_targets(params, needs):
+    """[(pair for K.adapter_linear_bwd, gradient to return, what is called behind
+    it)] of lora_a and lora_b."""
+    targets, places = [], set()
+    for p, need in zip(params, needs):
+        mg, accumulate = _fp32_accum_target(p) if need else (None, False)
+        if not need:
+            targets.append((None, None, lambda: None))
+        elif mg is None:
+            new = torch.empty(p.shape, dtype=p.dtype, device=p.device)
+            targets.append(((new, False), new, lambda: None))
+        elif mg.data_ptr() in places:
+            # (one parameter in both places: its second gradient is added behind the first)
+            new = torch.empty(p.shape, dtype=torch.float32, device=p.device)
+            targets.append(((new, False), None, lambda mg=mg, new=new: mg.add_(new)))
+        else:
+            places.add(mg.data_ptr())
+            target, accumulate, settle = _aligned_target(mg, accumulate)
+            targets.append(((target, accumulate), None, settle))
+    return targets
 
 
 class AdapterLinearFn(torch.autograd.Function):
@@ -739,9 +764,11 @@ class AdapterLinearFn(torch.autograd.Function):
         x2, weight, bias, lora_a, lora_b, *saved = ctx.saved_tensors
         x2, dy2 = _aligned_rows(x2), _whole(dy).view(-1, weight.shape[0])
         needs = ctx.needs_input_grad
-        (da, ga), (db, gb) = (_adapter_target(p, need) for p, need in ((lora_a, needs[3]), (lora_b, needs[4])))
+        (da, ga, settle_a), (db, gb, settle_b) = _adapter_targets((lora_a, lora_b), needs[3:5])
         dx = K.adapter_linear_bwd(x2, weight, lora_a, lora_b, dy2, ctx.rows, tuple(t.contiguous() for t in saved) or None,
                                   needs[0], da, db)
+        settle_a()
+        settle_b()
         for p, pair, g in ((lora_a, da, ga), (lora_b, db, gb)):
             if pair is not None and g is None:
                 grad_written(p)

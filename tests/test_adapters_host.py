@@ -71,7 +71,7 @@ def test_c_entries_refuse_before_any_launch():
         args = dict(x=P, w=P, bias=P, a=P, b=P, y=P, ut=P, scale=P, ws=P, stream=None) | change
         nat.call("eth_adapter_linear_fwd", ctypes.byref(desc) if desc else None, *args.values())
 
-    def bwd(desc, da=(P, 0, 0), db=(P, 0, 0), **change):
+    def bwd(desc, da=(P, 0, 0), db=(2 * P, 0, 0), **change):
         grads = [ctypes.byref(nat.AdapterGrad(*g)) if g else None for g in (da, db)]
         args = dict(x=P, w=P, a=P, b=P, dy=P, ut=P, scale=P, dx=P, da=grads[0], db=grads[1], ws=P, stream=None) | change
         nat.call("eth_adapter_linear_bwd", ctypes.byref(desc) if desc else None, *args.values())
@@ -94,7 +94,7 @@ def test_c_entries_refuse_before_any_launch():
     with pytest.raises(ValueError):
         fwd(_desc(dtype=nat.ETH_F16), scale=None)
     for change in (dict(dy=None), dict(dx=None, da=(0, 0, 0), db=(0, 0, 0)), dict(ut=None), dict(da=None), dict(db=None),
-                   dict(da=(P, 0, 1)), dict(db=(P + 4, 1, 0)), dict(dy=P + 2), dict(ws=P + 8)):
+                   dict(da=(P, 0, 1)), dict(db=(P + 4, 1, 0)), dict(db=(P, 0, 0)), dict(dy=P + 2), dict(ws=P + 8)):
         with pytest.raises(ValueError):
             bwd(_desc(), **change)
 

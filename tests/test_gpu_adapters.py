@@ -224,6 +224,33 @@ def test_autograd_strides_and_main_grads(cuda):
     assert (p["w"].main_grad.double() - 1.0 - dw).abs().max() < 2.0**-14
 
 
+def test_main_grads_anywhere(cuda):
+    """Main grads that start anywhere in a buffer, and one parameter in both places."""
+    announce("adapters main grads anywhere")
+    rows, *_ = _rows(cuda, [50, 30], [1, 0], 3)
+    o = _operands(cuda, 83, 64, 64, 64, 2, torch.bfloat16)
+    fa, fb = torch.empty(o["a"].shape, device=cuda), torch.empty(o["b"].shape, device=cuda)
+    saved = K.adapter_linear_fwd(o["x"], o["w"], None, o["a"], o["b"], rows, save=True)[1]
+    K.adapter_linear_bwd(o["x"], o["w"], o["a"], o["b"], o["dy"], rows, saved, False, (fa, False), (fb, False))
+    p = {k: torch.nn.Parameter(o[k].clone()) for k in ("a", "b")}
+    buffer = torch.ones(2 + 2 * fa.numel(), device=cuda)
+    p["a"].main_grad, p["b"].main_grad = buffer[2:].view(2, *fa.shape)
+    p["b"]._eth_main_grad_stale = True
+    for times in (1.0, 2.0):
+        AdapterLinearFn.apply(o["x"], o["w"], None, p["a"], p["b"], rows).backward(o["dy"])
+        assert torch.equal(p["a"].main_grad, 1.0 + fa if times == 1 else 1.0 + fa + fa)
+        assert torch.equal(p["b"].main_grad, times * fb) and (buffer[:2] == 1).all()
+    both = torch.nn.Parameter(o["a"].clone())
+    saved = K.adapter_linear_fwd(o["x"], o["w"], None, o["a"], o["a"], rows, save=True)[1]
+    K.adapter_linear_bwd(o["x"], o["w"], o["a"], o["a"], o["dy"], rows, saved, False, (fa, False), (fb, False))
+    both.main_grad = buffer[2 : 2 + fa.numel()].view(fa.shape)
+    both._eth_main_grad_stale = True
+    AdapterLinearFn.apply(o["x"], o["w"], None, both, both, rows).backward(o["dy"])
+    assert both.grad is None and torch.equal(both.main_grad, fa + fb)
+    with pytest.raises(ValueError):
+        K.adapter_linear_bwd(o["x"], o["w"], o["a"], o["a"], o["dy"], rows, saved, False, (fa, False), (fa, False))
+
+
 def test_streams_threads_and_replays(cuda):
     announce("adapters streams, threads, graphs")
     lens, ids = [60, 3, 41], [0, 1, 0]

@@ -228,6 +228,14 @@ def test_weight_gradients_into_main_grad(cuda, rows, H, V):
                 LinearFn.apply(x, w, None).backward(dy)
             torch.cuda.synchronize()
             assert torch.equal(w.main_grad, whole)
+    # one that starts anywhere in its buffer
+    buffer = torch.ones(V * H + 2, device=cuda)
+    w.main_grad = buffer[2:].view(V, H)
+    backward()
+    assert w.grad is None and torch.equal(w.main_grad, 1.0 + want)
+    w._eth_main_grad_stale = True
+    backward()
+    assert torch.equal(w.main_grad, want) and (buffer[:2] == 1).all()
     del w.main_grad
     backward()
     assert w.grad.dtype == torch.bfloat16
