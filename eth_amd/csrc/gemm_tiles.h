@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(256, 1) gemm256_m16_kernel(GemmArgs g, X x) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     return;
   }
-  if constexpr (X::kMaps) x.map(acc, m0 + wm * 128, n0 + wn * 128, g.M, g.N);
+  if constexpr (X::kMaps) x.template map<FP16>(acc, m0 + wm * 128, n0 + wn * 128, g.M, g.N);
 
   // Epilogue: each wave stages one 32-row slab of its 128x128 block at a
   // time in its own LDS region (fp32, padded rows) and writes it back as
@@ -1089,7 +1089,7 @@ __global__ void __launch_bounds__(256, 1) gemm_ring_kernel(GemmArgs g, X x) {
     x.reduce(acc, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
     return;
   }
-  if constexpr (X::kMaps) x.map(acc, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
+  if constexpr (X::kMaps) x.template map<FP16>(acc, m0 + wm * WM, n0 + wn * WN, g.M, g.N);
 
   // Epilogue: 16-row slabs of the wave's block through its own LDS region,
   // out in whole rows of WN columns

@@ -22,6 +22,11 @@
 // fp16 as in bf16.  (A row's share of dW loses digits where its dloss is 2^-14
 // of the largest and nothing else reaches the same row of dW.)
 //
+// dz's rounding is dh's and dW's largest error (1.4 roundings with their own). It
+// averages over the rows; where few take part they are listed twice, and dz is
+// stored in two parts, its rounding and what that left, which the same products
+// add up.
+//
 // No counterpart in the reference, whose head keeps the logits
 // (model/flex_ops.py:1976-1981 after language_model.py:24-38).
 #include <algorithm>
@@ -137,13 +142,14 @@ struct XentGrad {
   const float* mult;
   int v0;      // the piece's first column in the vocabulary
   int n_real;  // columns of the vocabulary in it
+  int twice;   // odd rows hold what the rounding of the even ones left
 
   __device__ __forceinline__ void size(GemmArgs& g) const {
     g.M = min(g.M, head->count);
     g.c_bytes = g.M > 0 ? (uint32_t)(((int64_t)(g.M - 1) * g.ldc + g.N) * 2) : 0;
   }
 
-  template <int TI, int TJ>
+  template <bool FP16, int TI, int TJ>
   __device__ __forceinline__ void map(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int) const {
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const bool edge = col0 + TJ * 16 > n_real;
@@ -178,6 +184,16 @@ struct XentGrad {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (col0 + j * 16 + lg * 4 + e >= n_real) acc[i][j][e] = 0.f;
+      }
+      if (twice) {
+        const bool rest = l16 & 1;
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = acc[i][j][e], high = FP16 ? h2f_bits(f2h_bits(v)) : bf2f(f2bf(v));
+            acc[i][j][e] = !rest ? v : __builtin_isfinite(high) ? v - high : 0.f;
+          }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -232,6 +248,7 @@ struct XentList {
   float* mult;
   float* back;
   int shift;  // dz's power of two
+  int twice;  // every row is listed twice (backward)
 };
 constexpr int kListThreads = 1024;
 
@@ -287,16 +304,19 @@ __global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
         continue;
       }
       wild |= t[u] < 0 || t[u] >= g.vocab;
-      g.rows[at] = (int)r;
-      g.label[at] = (int)(t[u] < 0 ? 0 : t[u] >= g.vocab ? g.vocab - 1 : t[u]);
+      const int e = exponent_of(d[u]), first_at = at << g.twice;
       if (back) {
-        const int e = exponent_of(d[u]);
         if (__builtin_isfinite(d[u])) high = max(high, e);
-        g.at[r] = at;
-        g.exps[at] = e;
-        g.lse2[at] = g.lse[r];
-        g.mult[at] = ldexpf(d[u], g.shift - e);
-        g.back[at] = ldexpf(1.f, e - g.shift);
+        g.at[r] = first_at;
+      }
+      for (int to = first_at; to <= first_at + g.twice; ++to) {
+        g.rows[to] = (int)r;
+        g.label[to] = (int)(t[u] < 0 ? 0 : t[u] >= g.vocab ? g.vocab - 1 : t[u]);
+        if (!back) continue;
+        g.exps[to] = e;
+        g.lse2[to] = g.lse[r];
+        g.mult[to] = ldexpf(d[u], g.shift - e);
+        g.back[to] = ldexpf(1.f, e - g.shift);
       }
     }
     base += total;
@@ -308,7 +328,7 @@ __global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
   __syncthreads();
   for (int w = 0; w < WAVES; ++w) high = max(high, highs[w]);
   if (high == -1000) high = 0;
-  if (tid == 0) *g.head = XentHead{base, high, ldexpf(1.f, high - g.shift)};
+  if (tid == 0) *g.head = XentHead{base << g.twice, high, ldexpf(1.f, high - g.shift)};
   if (wild && !back) *g.bad = 1;
 }
 
@@ -346,7 +366,7 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead*
   }
   if (k == 0 && row < n) {
     const XentPart t = red[0][r];
-    const float l = __builtin_amdgcn_logf(t.s);
+    const float l = log2f(t.s);  // (near one the instruction alone is off by more than s is)
     // (apart from each other the large terms cancel exactly first)
     const int64_t o = rows[row];
     loss[o] = kLn2 * (__builtin_fmaf(-picked[row], kLog2e, t.m2) + l);
@@ -376,11 +396,12 @@ __global__ void __launch_bounds__(256) xent_gather_kernel(const XentHead* head, 
   }
 }
 
-// dh of every row: the sum of its slices times its power of two, rounded once;
-// zeros where it took no part.
+// dh of every row: the sum of its slices (of both of its places, where it was
+// listed twice) times its power of two, rounded once; zeros where it took no part.
 template <bool FP16>
 __global__ void __launch_bounds__(256) xent_finish_kernel(const int* at, const float* back, const float* slices,
-                                                          int n_slices, int64_t stride, uint16_t* dh, int hidden) {
+                                                          int n_slices, int64_t stride, int twice, uint16_t* dh,
+                                                          int hidden) {
   const int64_t row = blockIdx.x;
   const int p = at[row];
   const float f = p < 0 ? 0.f : back[p];
@@ -388,8 +409,9 @@ __global__ void __launch_bounds__(256) xent_finish_kernel(const int* at, const f
     uint32_t o[4] = {0, 0, 0, 0};
     if (p >= 0) {
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      for (int s = 0; s < n_slices; ++s) {
-        const float4* src = reinterpret_cast<const float4*>(slices + s * stride + (int64_t)p * hidden + c);
+      for (int s = 0; s < n_slices << twice; ++s) {
+        const float4* src = reinterpret_cast<const float4*>(slices + (s >> twice) * stride +
+                                                            (int64_t)(p + (s & twice)) * hidden + c);
         const float4 x = src[0], y = src[1];
         v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
         v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
@@ -477,15 +499,26 @@ static XentForward plan_forward(int64_t n, int64_t hidden, int64_t vocab, int64_
   return p;
 }
 
+// Rows up to which each is listed twice: few enough not to average dz's roundings,
+// and for the products to wait for W and dW rather than for the matrix cores.
+// Backward of hidden 2048, vocabulary 50304, listed once / twice (us): 1 row 216 / 222,
+// 32 rows 217 / 223, 64 rows 221 / 247, 128 rows 239 / 282; of 4096, 65536: 461 / 478,
+// 470 / 490, 482 / 535, 520 / 622.
+constexpr int64_t kTwiceRows = 64;
+
 struct XentBackward {
+  int twice;
+  int64_t n;            // rows of the list, at most
   int splits;           // of dh's depth
   int64_t k_split;
   int pieces;
   int64_t piece, last, ldz;  // columns of a piece, of the last one, of their rows
   int64_t rows, label, at, exps, lse2, mult, back, gathered, dz, dh, bytes;
 };
-static XentBackward plan_backward(int64_t n, int64_t hidden, int64_t vocab, int64_t ldw, bool need_dh, bool need_dw) {
+static XentBackward plan_backward(int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw, bool need_dh, bool need_dw) {
   XentBackward p;
+  p.twice = rows <= kTwiceRows;
+  const int64_t n = p.n = rows << p.twice;
   int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
   most = std::min(most, reach(std::max(ldw, hidden)));
   // whole rounds of dW's tiles where they fit
@@ -575,8 +608,9 @@ static int xent_forward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64
 
 template <bool FP16>
 static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int64_t ldw, const XentBackward& p,
-                         char* ws, int64_t n, int64_t hidden, int64_t vocab, uint16_t* dh, void* dw, int dw_dtype,
+                         char* ws, int64_t n_rows, int64_t hidden, int64_t vocab, uint16_t* dh, void* dw, int dw_dtype,
                          int accumulate, hipStream_t s) {
+  const int64_t n = p.n;
   const XentHead* head = (const XentHead*)ws;
   const int* rows = (const int*)(ws + p.rows);
   uint16_t* gathered = (uint16_t*)(ws + p.gathered);
@@ -595,14 +629,14 @@ static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int6
     int rc = ETH_OK;
     auto z_columns = [&](int64_t c0, int64_t many, int tile) {
       const int64_t there = std::min(many, real - c0);
-      GemmArgs a = product_args(h, (n - 1) * ldh + hidden, ldh, wp + c0 * ldw, (there - 1) * ldw + hidden, ldw, n, many,
+      GemmArgs a = product_args(h, (n_rows - 1) * ldh + hidden, ldh, wp + c0 * ldw, (there - 1) * ldw + hidden, ldw, n, many,
                                 hidden);
       a.C = dz + c0;
       a.ldc = p.ldz;
       a.c_dtype = FP16 ? ETH_F16 : ETH_BF16;
       a.c_vec = true;
       const XentGrad grad{head, rows, (const int*)(ws + p.label), (const float*)(ws + p.lse2),
-                          (const float*)(ws + p.mult), (int)(v0 + c0), (int)there};
+                          (const float*)(ws + p.mult), (int)(v0 + c0), (int)there, p.twice};
       return launch_product<true, true, FP16, false>(tile, a, grad, s);
     };
     const XentCut zc = cut_columns(n, cols, hidden, GemmForm{false, hidden % 64 != 0, 0});
@@ -649,8 +683,8 @@ static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int6
   if (dh) {
     const bool wide = wide_takes(n, hidden, hidden, 4, true);
     const int filled = wide ? p.splits : 1;
-    xent_finish_kernel<FP16><<<(unsigned)n, 256, 0, s>>>((const int*)(ws + p.at), (const float*)(ws + p.back), slices,
-                                                         filled, n * hidden, dh, (int)hidden);
+    xent_finish_kernel<FP16><<<(unsigned)n_rows, 256, 0, s>>>((const int*)(ws + p.at), (const float*)(ws + p.back), slices,
+                                                         filled, n * hidden, p.twice, dh, (int)hidden);
     ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
   }
   return ETH_OK;
@@ -728,6 +762,7 @@ extern "C" int eth_linear_xent_bwd(const void* h, int64_t ldh, const void* w, in
   list.mult = (float*)(ws + p.mult);
   list.back = (float*)(ws + p.back);
   list.shift = dtype == ETH_F16 ? 14 : 0;
+  list.twice = p.twice;
   xent_list_kernel<<<1, kListThreads, 0, s>>>(list);
   ETH_CHECK_LAUNCH("eth_linear_xent_bwd");
   return dtype == ETH_F16 ? xent_backward<true>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden,

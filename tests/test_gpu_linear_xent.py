@@ -77,6 +77,26 @@ def test_loss_and_gradients(cuda, dtype, rows, H, V, ignored):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,H,V,ignored", [(1, 64, 3001, 0.0), (5, 128, 1000, 0.4), (64, 200, 2504, 0.0)])
+def test_few_rows_keep_more_of_dz(cuda, dtype, rows, H, V, ignored):
+    """Up to 64 rows dz is held in two parts: off by half a step of what half a
+    step left, the square of one rounding."""
+    announce(f"linear xent few rows {dtype} rows={rows}")
+    h, w, labels, dloss = _operands(cuda, rows, H, V, dtype, rows, ignored)
+    _, lse = K.linear_xent_fwd(h, w, labels, _bad(cuda))
+    dw = torch.empty(V, H, device=cuda)
+    dh, _ = K.linear_xent_bwd(h, w, labels, lse, dloss, dweight=dw)
+    r = linear_xent(h, w, labels, -100, dloss, HALF_STEP[dtype] ** 2, LEAST[dtype], FLOOR[dtype])
+    _within(dh, r["dh"], r["bound_dh"] + 1.001 * HALF_STEP[dtype] * r["dh"].abs(), "dh")
+    _within(dw, r["dw"], r["bound_dw"], "dw")
+    # a row without a finite gradient reaches itself alone
+    dloss[0] = float("inf")
+    if labels[0] != -100:
+        bad, _ = K.linear_xent_bwd(h, w, labels, lse, dloss, dweight=dw)
+        assert torch.equal(bad[1:], dh[1:]) and not bad[0].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_several_pieces_of_the_vocabulary(cuda, dtype):
     """32768 rows of 9001 logits: three pieces, the last of an odd width."""
     announce(f"linear xent in pieces {dtype}")
