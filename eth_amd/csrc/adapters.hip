@@ -15,7 +15,10 @@
 //             16-bit values transposed 8 x 8 in registers, memory-bound on x and dy
 //   join      an adapter's chunks added in order, rounded once
 //
-// u is rounded to 16 bits, the matrix cores' operand.  In fp16 a tile's u carries
+// u is rounded to 16 bits, the matrix cores' operand: with their own rounding dA
+// and dB are 1.4 roundings from exact.  It averages over the rows; tiles of up to 16
+// rows, half of whose depth in those products is free, hold there what it left.  In
+// fp16 a tile's u carries
 // a power of two that puts its largest value at 2^13 to 2^14, so that it keeps its
 // digits whatever the size of gradients and adapters.
 //
@@ -43,7 +46,8 @@ struct ShrinkArgs {
   int K, r, rp;
   uint16_t* u;       // [rows][rp]: rp the rank rounded up to 32, zeros behind it
   float* row_scale;  // [rows] (fp16)
-  uint16_t* ut;      // [tile][rp][32], zeros behind the tile's rows; or NULL
+  uint16_t* ut;      // [tile][rp][32], zeros behind the tile's rows (at 16 and on, of up to 16
+                     // rows, what their rounding left); or NULL
   float* tile_scale; // [tile] (fp16)
   float* partials;   // [split][tile][32][16 RB]; NULL: the depth is in one piece
   int splits;
@@ -69,6 +73,7 @@ __device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_ti
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = __builtin_isfinite(v[c][e]) ? fmaxf(top, fabsf(v[c][e])) : top;
   }
+  const bool both = t.rows <= kTileRows / 2;
   float down = 1.f, up = 1.f;  // what the stored u is times, and what brings it back
   if (FP16) {
     top = wave_max(top);
@@ -101,10 +106,16 @@ __device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_ti
       u32x2_t o = {lo, hi};
       *reinterpret_cast<u32x2_t*>(g.u + (int64_t)(t.row + row) * g.rp + j) = o;
     }
-    turned[(j + 0) * TS + row] = (uint16_t)lo;
-    turned[(j + 1) * TS + row] = (uint16_t)(lo >> 16);
-    turned[(j + 2) * TS + row] = (uint16_t)hi;
-    turned[(j + 3) * TS + row] = (uint16_t)(hi >> 16);
+    if (both && row >= kTileRows / 2) continue;
+    const uint16_t at[4] = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      turned[(j + e) * TS + row] = at[e];
+      if (!both) continue;
+      const float had = FP16 ? v[c][e] * down : v[c][e], is = FP16 ? h2f_bits(at[e]) : bf2f(at[e]);
+      const float left = __builtin_isfinite(is) ? had - is : 0.f;
+      turned[(j + e) * TS + kTileRows / 2 + row] = FP16 ? f2h_bits(left) : f2bf(left);
+    }
   }
   if (RB == 1 && g.u) {  // (rp 32: the second half of a row of 16 ranks)
     for (int c = threadIdx.x; c < kTileRows * 2; c += 64 * W)
@@ -470,9 +481,10 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
     const eth_adapter_tile_t t = args.tiles[at];
     const rsrc_t qs = make_rsrc(g.q + (int64_t)t.row * g.ldq, (uint32_t)(((t.rows - 1) * g.ldq + g.C) * 2));
     uint4 row[8];
+    const int r0 = t.rows <= kTileRows / 2 ? lg * 8 % (kTileRows / 2) : lg * 8;  // (16 rows: twice)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      row[i] = load8(qs, lg * 8 + i < t.rows && col < g.C ? (int32_t)(((lg * 8 + i) * g.ldq + col) * 2) : kOob);
+      row[i] = load8(qs, r0 + i < t.rows && col < g.C ? (int32_t)(((r0 + i) * g.ldq + col) * 2) : kOob);
     uint4 fu[RB];
     const uint16_t* ut = g.ut + (int64_t)at * args.rp * kTileRows + lg * 8;
 #pragma unroll

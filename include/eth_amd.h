@@ -471,16 +471,17 @@ int eth_packed_attn_bwd(const eth_packed_attn_desc_t* desc, const void* q, const
  * scale, every adapted row in one tile, ordered by adapter.  chunks [n_chunks]:
  * consecutive tiles of one adapter, every tile in one chunk, in the tiles' order (what
  * one partial sum of a gradient is taken over).  first_chunk [n_listed + 1]:
- * where an adapter's chunks start (those from n_listed on have none).  used [n_used]: the adapters that have tiles.  Adapters
- * may have none, and n_tiles may be 0.
+ * where an adapter's chunks start (those from n_listed on have none).  used [n_used]:
+ * the adapters that have tiles.  Adapters may have none, and n_tiles may be 0.
  *
  * The forward leaves in `ut` (n_tiles * 32 * rank rounded up to 32, 16-bit; NULL
  * where no dB is wanted) and in fp16 tile_scale [n_tiles] what dB needs.  The
  * backward writes dx [rows, in] (contiguous, or NULL) and the adapters' gradients
  * (each NULL, in `dtype`, or fp32, then stored, or added to with `accumulate`), zeros
- * for adapters without rows; dy is contiguous.  Sums are fp32, in a fixed order;
- * x A^T and dy B are rounded to 16 bits for their second products (in fp16 times a
- * power of two, so they keep their digits at any size).  Values that are not finite
+ * for adapters without rows, in two places; dy is contiguous.  Sums are fp32, in a
+ * fixed order; x A^T and dy B are rounded to 16 bits for their second products (in
+ * fp16 times a power of two, so they keep their digits at any size; for the gradients
+ * of tiles of up to 16 rows in two parts).  Values that are not finite
  * reach no other task's rows or gradients; one in an adapter makes its own rows NaN,
  * in its column or, where they share 128 rows with another adapter's, in up to 128
  * columns about it.  `workspace`: eth_adapter_linear_workspace bytes

@@ -224,6 +224,24 @@ def test_autograd_strides_and_main_grads(cuda):
     assert (p["w"].main_grad.double() - 1.0 - dw).abs().max() < 2.0**-14
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,k,n,r", [([1], 64, 72, 8), ([16, 3, 1], 264, 128, 16), ([5, 16], 2048, 512, 64),
+                                        ([2, 9], 128, 1032, 128)])
+def test_few_rows_keep_more_of_their_products(cuda, dtype, lens, k, n, r):
+    """Segments of up to 16 rows: x A^T and dy B are held in two parts for dA and dB,
+    off by half a step of what half a step left, the square of one rounding."""
+    announce(f"adapters few rows {dtype} {lens} {k} {n} {r}")
+    rows, of_row, scale = _rows(cuda, lens, list(range(len(lens))), 2)
+    o = _operands(cuda, sum(lens) + 2, k, n, r, len(lens), dtype)
+    saved = K.adapter_linear_fwd(o["x"], o["w"], None, o["a"], o["b"], rows, save=True)[1]
+    da, db = torch.empty(o["a"].shape, device=cuda), torch.empty(o["b"].shape, device=cuda)
+    K.adapter_linear_bwd(o["x"], o["w"], o["a"], o["b"], o["dy"], rows, saved, False, (da, False), (db, False))
+    r = adapter_linear(o["x"], o["w"], None, o["a"], o["b"], of_row, scale, o["dy"], HALF_STEP[dtype] ** 2, LEAST[dtype],
+                       FLOOR[dtype])
+    _within(da, r, "da")
+    _within(db, r, "db")
+
+
 def test_main_grads_anywhere(cuda):
     """Main grads that start anywhere in a buffer, and one parameter in both places."""
     announce("adapters main grads anywhere")
