@@ -50,7 +50,7 @@ struct ShrinkArgs {
                      // rows, what their rounding left); or NULL
   float* tile_scale; // [tile] (fp16)
   float* partials;   // [split][tile][32][16 RB]; NULL: the depth is in one piece
-  int splits;
+  int splits, n_tiles;
 };
 
 // A tile's u of its fp32 sums: the scale, the power of two, 16 bits, both layouts.
@@ -138,86 +138,109 @@ __device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_ti
 // TB/s of x; rank 64, [3000, 4096] 8.9, where every tile reads its adapter's 512 KB.
 // Neighbouring workgroups have the pieces of a tile's depth: with eight, each XCD
 // reads its own piece of every adapter, which its L2 holds.
-template <int RB, int W, bool FP16>
+// P: tiles of a workgroup, in one pass over the depth where they are one adapter's.
+template <int RB, int W, int P, bool FP16>
 __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
   constexpr int RS = RB * 16 + 4;  // padded row of the partial sums
   __shared__ __attribute__((aligned(16))) float red[W][kTileRows][RS];
   __shared__ float high[W];
-  const int tile = blockIdx.x / g.splits, piece = blockIdx.x - tile * g.splits;
-  const eth_adapter_tile_t t = g.tiles[tile];
+  const int group = blockIdx.x / g.splits, piece = blockIdx.x - group * g.splits;
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const rsrc_t xs = make_rsrc(g.x + (int64_t)t.row * g.ldx, (uint32_t)(((t.rows - 1) * g.ldx + g.K) * 2));
-  const rsrc_t as = make_rsrc(g.a + (int64_t)t.adapter * g.r * g.K, (uint32_t)(g.r * g.K * 2));
-  const bool second = t.rows > 16;
-  f32x4_t acc[2][RB];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < RB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const int pieces = W * g.splits, steps = (g.K + 31) / 32, per = (steps + pieces - 1) / pieces;
   const int s0 = (piece * W + wid) * per, s1 = min(steps, s0 + per);
-  int32_t xo[2], ao[RB];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) xo[i] = i * 16 + l16 < t.rows ? (int32_t)(((i * 16 + l16) * g.ldx + lg * 8) * 2) : kOob;
-#pragma unroll
-  for (int j = 0; j < RB; ++j) ao[j] = j * 16 + l16 < g.r ? ((j * 16 + l16) * g.K + lg * 8) * 2 : kOob;
-  constexpr int UN = RB >= 4 ? 2 : 4;  // steps whose loads are in flight together, and as many ahead
-  struct Batch {
-    uint4 x[UN][2], a[UN][RB];
-  };
-  auto load = [&](Batch& f, int s) __attribute__((always_inline)) {
-#pragma unroll
-    for (int n = 0; n < UN; ++n) {
-      // (past this wave's range, or the depth: zeros)
-      const bool in = s + n < s1 && (s + n) * 32 + lg * 8 < g.K;
-      const int32_t at = (s + n) * 64;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) f.x[n][i] = load8(xs, in && xo[i] != kOob && (i == 0 || second) ? xo[i] + at : kOob);
-#pragma unroll
-      for (int j = 0; j < RB; ++j) f.a[n][j] = load8(as, in && ao[j] != kOob ? ao[j] + at : kOob);
+  // steps whose loads are in flight together, and as many ahead (at 128 ranks two take
+  // the registers of a second workgroup: [8192, 4096] 1 to 2 us more)
+  constexpr int UN = RB >= 8 ? 1 : RB >= 4 ? 2 : 4;
+  const int last = min(g.n_tiles, (group + 1) * P);
+  for (int tile = group * P, many; tile < last; tile += many) {
+    eth_adapter_tile_t t[P];
+    rsrc_t xs[P];
+    t[0] = g.tiles[tile];
+    many = 1;
+    if (P > 1) {
+      t[P - 1] = g.tiles[min(tile + 1, last - 1)];
+      if (tile + 1 < last && t[P - 1].adapter == t[0].adapter) many = 2;
     }
-  };
-  auto products = [&](const Batch& f) __attribute__((always_inline)) {
+    const rsrc_t as = make_rsrc(g.a + (int64_t)t[0].adapter * g.r * g.K, (uint32_t)(g.r * g.K * 2));
+    bool live[2 * P];  // blocks of 16 rows
+    int32_t xo[2 * P], ao[RB];
+    f32x4_t acc[2 * P][RB];
 #pragma unroll
-    for (int n = 0; n < UN; ++n)
+    for (int q = 0; q < P; ++q) {
+      xs[q] = make_rsrc(g.x + (int64_t)t[q].row * g.ldx, (uint32_t)(((t[q].rows - 1) * g.ldx + g.K) * 2));
 #pragma unroll
-      for (int j = 0; j < RB; ++j) {
-        acc[0][j] = mfma16<FP16>(f.a[n][j], f.x[n][0], acc[0][j]);
-        if (second) acc[1][j] = mfma16<FP16>(f.a[n][j], f.x[n][1], acc[1][j]);
+      for (int h = 0; h < 2; ++h) {
+        const int i = q * 2 + h, row = h * 16 + l16;
+        live[i] = q < many && t[q].rows > h * 16;
+        xo[i] = live[i] && row < t[q].rows ? (int32_t)((row * g.ldx + lg * 8) * 2) : kOob;
+#pragma unroll
+        for (int j = 0; j < RB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
-  };
-  Batch one, two;
-  load(one, s0);
-  for (int s = s0; s < s1; s += 2 * UN) {
-    load(two, s + UN);
-    products(one);
-    load(one, s + 2 * UN);
-    products(two);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < RB; ++j)
-      *reinterpret_cast<f32x4_t*>(&red[wid][i * 16 + l16][j * 16 + lg * 4]) = acc[i][j];
-  __syncthreads();
-  // the waves' sums, in order
-  auto sum = [&](int row, int j) __attribute__((always_inline)) {
-    f32x4_t v = *reinterpret_cast<const f32x4_t*>(&red[0][row][j]);
-#pragma unroll
-    for (int w = 1; w < W; ++w) v += *reinterpret_cast<const f32x4_t*>(&red[w][row][j]);
-    return v;
-  };
-  if (g.partials) {
-    const int tiles = gridDim.x / g.splits;
-    float* out = g.partials + ((int64_t)piece * tiles + tile) * kTileRows * RB * 16;
-    for (int cell = threadIdx.x; cell < kTileRows * RB * 4; cell += 64 * W) {
-      const int row = cell / (RB * 4), j = cell % (RB * 4) * 4;
-      *reinterpret_cast<f32x4_t*>(out + row * RB * 16 + j) = sum(row, j);
     }
-    return;
+#pragma unroll
+    for (int j = 0; j < RB; ++j) ao[j] = j * 16 + l16 < g.r ? ((j * 16 + l16) * g.K + lg * 8) * 2 : kOob;
+    struct Batch {
+      uint4 x[UN][2 * P], a[UN][RB];
+    };
+    auto load = [&](Batch& f, int s) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        // (past this wave's range, or the depth: zeros)
+        const bool in = s + n < s1 && (s + n) * 32 + lg * 8 < g.K;
+        const int32_t at = (s + n) * 64;
+#pragma unroll
+        for (int i = 0; i < 2 * P; ++i) f.x[n][i] = load8(xs[i / 2], in && xo[i] != kOob ? xo[i] + at : kOob);
+#pragma unroll
+        for (int j = 0; j < RB; ++j) f.a[n][j] = load8(as, in && ao[j] != kOob ? ao[j] + at : kOob);
+      }
+    };
+    auto products = [&](const Batch& f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n)
+#pragma unroll
+        for (int i = 0; i < 2 * P; ++i)
+          if (i == 0 || live[i]) {
+#pragma unroll
+            for (int j = 0; j < RB; ++j) acc[i][j] = mfma16<FP16>(f.a[n][j], f.x[n][i], acc[i][j]);
+          }
+    };
+    Batch one, two;
+    load(one, s0);
+    for (int s = s0; s < s1; s += 2 * UN) {
+      load(two, s + UN);
+      products(one);
+      load(one, s + 2 * UN);
+      products(two);
+    }
+    // the waves' sums, in order
+    auto sum = [&](int row, int j) __attribute__((always_inline)) {
+      f32x4_t v = *reinterpret_cast<const f32x4_t*>(&red[0][row][j]);
+#pragma unroll
+      for (int w = 1; w < W; ++w) v += *reinterpret_cast<const f32x4_t*>(&red[w][row][j]);
+      return v;
+    };
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      if (q >= many) break;
+      if (P > 1) __syncthreads();  // (the tile before is out)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+          *reinterpret_cast<f32x4_t*>(&red[wid][h * 16 + l16][j * 16 + lg * 4]) = acc[q * 2 + h][j];
+      __syncthreads();
+      if (g.partials) {
+        float* out = g.partials + ((int64_t)piece * g.n_tiles + tile + q) * kTileRows * RB * 16;
+        for (int cell = threadIdx.x; cell < kTileRows * RB * 4; cell += 64 * W) {
+          const int row = cell / (RB * 4), j = cell % (RB * 4) * 4;
+          *reinterpret_cast<f32x4_t*>(out + row * RB * 16 + j) = sum(row, j);
+        }
+      } else {
+        narrow<RB, W, FP16>(g, t[q], tile + q, reinterpret_cast<uint16_t*>(&red[0][0][0]), high, sum);
+      }
+    }
   }
-  narrow<RB, W, FP16>(g, t, tile, reinterpret_cast<uint16_t*>(&red[0][0][0]), high, sum);
 }
 
 // The pieces of the depth joined, in order (4 to 5 us, a launch and its latency).
@@ -672,17 +695,27 @@ static int launch_adapted(const ProductPlan& p, GemmArgs a, const X& x, float* p
   return ETH_OK;
 }
 
+// From this many tiles on, and 33 ranks, a workgroup of the shrink takes two: their
+// adapter's values, which L2 hands out again for every tile, serve both.  One / two
+// (us, the whole of the adapters' share of a forward call): [16384, 4096] rank 128
+// 80 / 65, [8192, 4096] 48 / 40, rank 64 33 / 30; of fewer tiles the depth's pieces
+// get shorter, and of short segments pairs are often of two adapters, taken one after
+// the other: [4000, 4096] rank 64 of one adapter 22 / 18, [3000, 4096] of four 14 / 21.
+constexpr int kPairedTiles = 128;
+
 // Pieces of the shrink's depth: as many as bring four workgroups a compute unit
 // (two from 33 ranks on, whose LDS leaves room for two), each of two trips of its
 // waves at least.
 struct ShrinkPlan {
-  int blocks, waves, splits;
+  int blocks, waves, splits, pairs;
   int64_t workspace;
 };
 static ShrinkPlan plan_shrink(int64_t K, int r, int n_tiles) {
-  ShrinkPlan p{r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8, r <= 64 ? 8 : 4, 1, 0};
+  ShrinkPlan p{r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8, r <= 64 ? 8 : 4, 1, 0, 0};
+  p.pairs = p.blocks >= 4 && n_tiles >= kPairedTiles;
+  const int groups = p.pairs ? (n_tiles + 1) / 2 : n_tiles;
   const int64_t trips = K / (p.waves * 32 * (p.blocks >= 4 ? 2 : 4)), slots = p.blocks >= 4 ? 512 : 1024;
-  if (n_tiles) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSplits, slots / n_tiles), trips / 2));
+  if (n_tiles) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSplits, slots / groups), trips / 2));
   if (p.splits > 1) p.workspace = (int64_t)p.splits * n_tiles * kTileRows * p.blocks * 16 * 4;
   return p;
 }
@@ -691,17 +724,20 @@ static int launch_shrink(ShrinkArgs g, int n_tiles, float* partials, hipStream_t
   const ShrinkPlan p = plan_shrink(g.K, g.r, n_tiles);
   g.partials = p.splits > 1 ? partials : nullptr;
   g.splits = p.splits;
-  const unsigned grid = (unsigned)(n_tiles * p.splits);
-#define ETH_SHRINK(RB, W)                                                             \
-  {                                                                                   \
-    adapter_shrink_kernel<RB, W, FP16><<<grid, 64 * W, 0, s>>>(g);                    \
-    ETH_CHECK_LAUNCH("eth_adapter_linear");                                           \
-    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g);           \
+  g.n_tiles = n_tiles;
+  const unsigned grid = (unsigned)((p.pairs ? (n_tiles + 1) / 2 : n_tiles) * p.splits);
+#define ETH_SHRINK(RB, W, P)                                                      \
+  {                                                                               \
+    adapter_shrink_kernel<RB, W, P, FP16><<<grid, 64 * W, 0, s>>>(g);             \
+    ETH_CHECK_LAUNCH("eth_adapter_linear");                                       \
+    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g); \
   }
-  if (p.blocks == 1) ETH_SHRINK(1, 8)
-  else if (p.blocks == 2) ETH_SHRINK(2, 8)
-  else if (p.blocks == 4) ETH_SHRINK(4, 8)
-  else ETH_SHRINK(8, 4)
+  if (p.blocks == 1) ETH_SHRINK(1, 8, 1)
+  else if (p.blocks == 2) ETH_SHRINK(2, 8, 1)
+  else if (p.blocks == 4 && p.pairs) ETH_SHRINK(4, 8, 2)
+  else if (p.blocks == 4) ETH_SHRINK(4, 8, 1)
+  else if (p.pairs) ETH_SHRINK(8, 4, 2)
+  else ETH_SHRINK(8, 4, 1)
 #undef ETH_SHRINK
   ETH_CHECK_LAUNCH("eth_adapter_linear");
   return ETH_OK;
@@ -816,7 +852,7 @@ static int adapter_forward(const eth_adapter_desc_t* d, const void* x, const voi
   const GemmArgs a = adapter_product(d, x, d->ldx, d->in, w, y, d->out, bias);
   if (!d->n_tiles) return launch_adapted<true, FP16>(p.plan, a, PlainProduct{}, (float*)(ws + p.product), s);
   const ShrinkArgs g{d->tiles, (const uint16_t*)x, (const uint16_t*)lora_a, d->ldx, (int)d->in, d->rank, rp,
-                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale, nullptr, 1};
+                     (uint16_t*)(ws + p.u), (float*)(ws + p.row_scale), (uint16_t*)ut, tile_scale, nullptr, 1, 0};
   const int rc = launch_shrink<FP16>(g, d->n_tiles, (float*)(ws + p.product), s);
   if (rc != ETH_OK) return rc;
   const AdapterStart start{d->of_row, g.u, FP16 ? g.row_scale : nullptr, (const uint16_t*)lora_b, d->rank, rp};
@@ -845,7 +881,7 @@ static int adapter_backward(const eth_adapter_desc_t* d, const void* x, const vo
     ETH_CHECK_LAUNCH("eth_adapter_linear_bwd");
     const ShrinkArgs g{d->tiles, (const uint16_t*)dy, turn_b.to, d->out, (int)d->out, d->rank, rp,
                        (uint16_t*)(dx ? ws + p.u : nullptr), (float*)(ws + p.row_scale),
-                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale), nullptr, 1};
+                       (uint16_t*)(da->grad ? ws + p.ut : nullptr), (float*)(ws + p.tile_scale), nullptr, 1, 0};
     rc = launch_shrink<FP16>(g, d->n_tiles, (float*)(ws + p.product), s);
     if (rc != ETH_OK) return rc;
     if (dx) {

@@ -71,6 +71,8 @@ def _check(o, of_row, scale, got, bias=True):
     # the wide tiles, whole and with short ends; the depth in splits
     ([900, 1100, 700, 1400], [0, 1, 0, 2], 19, 3, 320, 2056, 16), ([2048, 2300], [1, 0], 0, 2, 128, 2048, 64),
     ([400, 120], [0, 1], 0, 2, 8192, 512, 32), ([130, 390], [1, 0], 0, 2, 512, 8192, 16),
+    # two tiles a workgroup: of one adapter, of two, an odd last one; in pieces of the depth too
+    ([2000, 33, 1, 2050, 64], [0, 1, 0, 2, 1], 3, 3, 64, 72, 40), ([4090, 17, 3], [1, 0, 2], 0, 3, 2056, 264, 128),
 ])
 def test_forward_and_backward(cuda, dtype, lens, ids, tail, adapters, k, n, r):
     announce(f"adapters {dtype} lens={lens} ids={ids} tail={tail} k={k} n={n} r={r}")
