@@ -149,10 +149,10 @@ __global__ void __launch_bounds__(64 * W) adapter_shrink_kernel(ShrinkArgs g) {
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int pieces = W * g.splits, steps = (g.K + 31) / 32, per = (steps + pieces - 1) / pieces;
   const int s0 = (piece * W + wid) * per, s1 = min(steps, s0 + per);
-  // steps whose loads are in flight together, and as many ahead (at 128 ranks two take
-  // the registers of a second workgroup: [8192, 4096] 1 to 2 us more)
+  // steps whose loads are in flight together, and as many ahead (two at 128 ranks: 1 us
+  // more at [3000, 4096] and [8192, 4096])
   constexpr int UN = RB >= 8 ? 1 : RB >= 4 ? 2 : 4;
-  const int last = min(g.n_tiles, (group + 1) * P);
+  const int last = P == 1 ? group + 1 : min(g.n_tiles, (group + 1) * P);
   for (int tile = group * P, many; tile < last; tile += many) {
     eth_adapter_tile_t t[P];
     rsrc_t xs[P];
