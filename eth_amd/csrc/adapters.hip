@@ -268,9 +268,9 @@ __global__ void __launch_bounds__(256) adapter_narrow_kernel(ShrinkArgs g) {
 // A transposed): for each adapter of the wave's rows (mostly one) the product of
 // all its rows, zeros in the place of the others', by fragments from memory (L2):
 // r / 32 k-steps of latency ahead of the main loop, whose first loads are under way
-// meanwhile.  Rank 16, [8192, 2048 -> 8192]: 218 us for the plain product's 195 (four
-// rounds of tiles); rank 64, [3000, 4096 -> 4096]: 99 for 82; eight rows of eight
-// adapters, rank 16, [2048 -> 6144]: 13.5 for 9.
+// meanwhile.  Rank 16, [8192, 2048 -> 8192]: 217 us for the plain product's 198 (four
+// rounds of tiles); rank 64, [3000, 4096 -> 4096]: 91 for 82; eight rows of eight
+// adapters, rank 16, [2048 -> 6144]: 13 for 9.
 struct AdapterStart {
   static constexpr bool kSized = false, kGathers = false, kStarts = true, kMaps = false, kReduces = false;
   const int* of_row;
