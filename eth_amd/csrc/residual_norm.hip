@@ -494,9 +494,9 @@ static void launch_rn_bwd(const RnParams& p, int groups, const uint16_t* x, cons
 static int check_rn(const char* name, const eth_residual_norm_desc_t* d) {
   ETH_CHECK_ARG(d, "%s: null descriptor", name);
   ETH_CHECK_ARG(d->dtype == ETH_BF16 || d->dtype == ETH_F16, "%s: dtype must be bf16 or fp16", name);
-  // (a grid of 2^32 threads and more is taken modulo 2^32)
-  ETH_CHECK_ARG(d->rows >= 0 && d->rows < (1LL << 26) && d->cols > 0 && d->cols <= kRnMaxCols && d->cols % 8 == 0,
-                "%s: cols must be a positive multiple of 8 up to %d, rows below 2^26 (got %lld, %lld)", name, kRnMaxCols,
+  // (a grid of 2^32 threads and more is taken modulo 2^32: 64 threads a row, rounded up to four rows)
+  ETH_CHECK_ARG(d->rows >= 0 && d->rows <= (1LL << 26) - 4 && d->cols > 0 && d->cols <= kRnMaxCols && d->cols % 8 == 0,
+                "%s: cols must be a positive multiple of 8 up to %d, rows up to 2^26 - 4 (got %lld, %lld)", name, kRnMaxCols,
                 (long long)d->cols, (long long)d->rows);
   ETH_CHECK_ARG(d->post_gamma && d->gamma && (d->rms ? !d->post_beta && !d->beta : d->post_beta && d->beta),
                 "%s: gammas are needed, and betas exactly where the norms are not root-mean-square", name);

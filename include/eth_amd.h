@@ -524,7 +524,7 @@ int eth_adapter_linear_bwd(const eth_adapter_desc_t* desc, const void* x, const 
 
 /* The norm behind a block, its gate, the scaled residual and the norm before the
  * next block, on contiguous [rows, cols] tensors of bf16 or fp16 (`dtype`; cols a
- * multiple of 8 up to 8192, rows below 2^26; 16-byte aligned):
+ * multiple of 8 up to 8192, rows up to 2^26 - 4; 16-byte aligned):
  *   n = norm(x) post_gamma + post_beta,  h = residual_scale residual + gate n,
  *   y = norm(h) gamma + beta  (of h before it is rounded to 16 bits),
  * norm(v) = (v - mean) / sqrt(variance + eps), or with `rms` v / sqrt(mean of
@@ -671,7 +671,8 @@ int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_
  * is not wanted; dw in `dtype`, or fp32 (then stored, or added to with `accumulate`).
  * Rows that are ignored or whose dloss is zero get dh 0 and take no part in dw.
  * dz is rounded to 16 bits for the products (a row's dloss enters as a mantissa, so
- * gradients of any size keep their digits); sums are fp32, in a fixed order.
+ * gradients of any size keep their digits; up to 64 rows in two parts); sums are fp32,
+ * in a fixed order.
  * `workspace`: eth_linear_xent_workspace bytes, 256-byte aligned (grads: 0 for the
  * forward, or 1 for dh + 2 for dw; at most about 256 MiB for a piece of dz, or 512
  * bytes a row, beside a row of fp32 dh for up to 16 splits and a copy of h). */

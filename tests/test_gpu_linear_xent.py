@@ -131,6 +131,28 @@ def test_rows_and_weights_of_wider_buffers(cuda, dtype):
         assert dx.shape == x.shape
 
 
+def test_weights_and_gradients_beyond_two_gibibytes(cuda):
+    """A head whose rows lie 64 KiB apart, 2.6 GB in all, and fp32 gradients of 2.3 GB."""
+    announce("linear xent beyond 2 GiB")
+    h, w, labels, dloss = _operands(cuda, 33, 64, 40000, torch.bfloat16, 21)
+    labels[:3] = torch.tensor([39999, 32768, 32767])
+    wide = torch.empty(40000, 32768, dtype=torch.bfloat16, device=cuda)[:, 8:72].copy_(w)
+    loss, lse = K.linear_xent_fwd(h, wide, labels, _bad(cuda))
+    dh, dw = K.linear_xent_bwd(h, wide, labels, lse, dloss)
+    _check(h, w, labels, loss, dloss, dh, dw)
+    del wide
+    gen = torch.Generator(device=cuda).manual_seed(22)
+    randn = lambda *s: torch.randn(*s, generator=gen, device=cuda).bfloat16()  # noqa: E731
+    h, w, labels = randn(3, 4096), randn(140000, 4096) * 2.0**-6, torch.tensor([139999, 0, 131072], device=cuda)
+    loss, lse = K.linear_xent_fwd(h, w, labels, _bad(cuda))
+    dw = torch.ones(140000, 4096, device=cuda)
+    dh, _ = K.linear_xent_bwd(h, w, labels, lse, dloss[:3], dweight=dw, accumulate=True)
+    dw -= 1.0  # (exact but for the rounding of the sum, 2^-24 of at most 8)
+    r = linear_xent(h, w, labels, -100, dloss[:3], HALF_STEP[torch.bfloat16], LEAST[torch.bfloat16])
+    _within(dh, r["dh"], r["bound_dh"], "dh")
+    _within(dw, r["dw"], r["bound_dw"] + 2.0**-21, "dw")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_rows_that_take_no_part(cuda, dtype):
     """What ignored rows, and backward rows without upstream gradient, hold

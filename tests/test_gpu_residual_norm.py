@@ -121,6 +121,24 @@ def test_rows_stay_apart(cuda):
     assert dx.isfinite().all() and torch.equal(dres, o["dh"])
 
 
+def test_rows_beyond_two_gibibytes(cuda):
+    """The last rows of 2.3 GB tensors: those of a call with them alone."""
+    announce("residual norm beyond 2 GiB")
+    rows, cols = 140000, 8192
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    few = _operands(cuda, 9, cols, torch.float16, False, True)
+    big = {k: v if v is None or v.dim() == 1 else torch.randn(rows, cols, generator=gen, device=cuda, dtype=v.dtype)
+           for k, v in few.items()}
+    for k in ("x", "residual", "dh", "dy"):
+        big[k][-9:] = few[k]
+    h, y, stats = _forward(big, 0.7, 1e-5, False)
+    want = _forward(few, 0.7, 1e-5, False)
+    assert torch.equal(h[-9:], want[0]) and torch.equal(y[-9:], want[1]) and torch.equal(stats[:, -9:], want[2])
+    got = _backward(big, stats, big["dh"], big["dy"], 0.7, 1e-5, False, [None] * 5)
+    want = _backward(few, want[2], few["dh"], few["dy"], 0.7, 1e-5, False, [None] * 5)
+    assert all(torch.equal(a[-9:], b) for a, b in zip(got, want))
+
+
 def _leaves(o):
     return {k: None if v is None or k in ("dh", "dy") else v.detach().clone().requires_grad_(True) for k, v in o.items()}
 

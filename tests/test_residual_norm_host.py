@@ -21,7 +21,7 @@ def _desc(**change):
     return d
 
 
-BAD = [dict(dtype=nat.ETH_F32), dict(rows=-1), dict(rows=2**26), dict(cols=0), dict(cols=60), dict(cols=8200),
+BAD = [dict(dtype=nat.ETH_F32), dict(rows=-1), dict(rows=2**26), dict(rows=2**26 - 3), dict(cols=0), dict(cols=60), dict(cols=8200),
        dict(post_gamma=None), dict(gamma=None), dict(beta=None), dict(post_beta=None), dict(rms=1), dict(gate=P + 2),
        dict(gamma=P + 8), dict(eps=-1.0), dict(eps=float("inf")), dict(eps=float("nan")),
        dict(residual_scale=float("nan")), dict(residual_scale=float("inf"))]
