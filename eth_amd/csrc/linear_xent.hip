@@ -347,24 +347,29 @@ __global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
 }
 
 // ------------------------------------------------------------------ join --
-// A workgroup joins 16 rows: 64 threads a row, each every 64th part, eight in
-// flight, then a tree.  `lse` in the log2 domain.  Latency: 6.0 us for one row's 1572
-// parts, 4.0 for 2048 rows of 393 (16 in flight: 0.9 us more).
+// A workgroup joins R rows: 1024 / R threads a row, some parts of each in flight,
+// then a tree.  `lse` in the log2 domain.  Latency: 4.0 us for 2048 rows of 393 parts.
+// A whole 16 rows' lines lie together, but few rows of many parts are done sooner two
+// a workgroup (forward, 16 / 2, us): one row of 50304 44.6 / 42.8, of 131072 35.2 /
+// 30.6, 64 rows 47.7 / 46.4 and 34.5 / 31.5; 64 rows of 1000 12.0 / 12.3, 256 of 131072
+// 40.5 / 41.5.
 constexpr int kJoinThreads = 1024;
+constexpr int64_t kFewRows = 64, kManyParts = 256;
 __device__ __forceinline__ XentPart join(XentPart a, XentPart b) {
   const float m = fmaxf(a.m2, b.m2), at = m == -INFINITY ? 0.f : m;
   return XentPart{m, a.s * __builtin_amdgcn_exp2f(a.m2 - at) + b.s * __builtin_amdgcn_exp2f(b.m2 - at)};
 }
+template <int R>
 __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead* head, const int* rows,
                                                                  const XentPart* part, const float* picked, int parts,
                                                                  float* loss, float* lse) {
-  __shared__ XentPart red[kJoinThreads / 16][16];
-  const int r = threadIdx.x & 15, k = threadIdx.x >> 4, row = blockIdx.x * 16 + r, n = head->count;
-  if ((int)blockIdx.x * 16 >= n) return;
+  __shared__ XentPart red[kJoinThreads / R][R];
+  const int r = threadIdx.x % R, k = threadIdx.x / R, row = blockIdx.x * R + r, n = head->count;
+  if ((int)blockIdx.x * R >= n) return;
   XentPart v{-INFINITY, 0.f};
   if (row < n) {
-    const XentPart* mine = part + (int64_t)blockIdx.x * parts * 16 + r;
-    constexpr int STEP = kJoinThreads / 16, U = 8;  // parts in flight
+    const XentPart* mine = part + (int64_t)(row >> 4) * parts * 16 + (row & 15);
+    constexpr int STEP = kJoinThreads / R, U = R == 16 ? 8 : 4;  // parts in flight
     for (int p = k; p < parts; p += U * STEP) {
       XentPart in[U];
 #pragma unroll
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead*
     }
   }
   red[k][r] = v;
-  for (int half = kJoinThreads / 32; half; half >>= 1) {
+  for (int half = kJoinThreads / R / 2; half; half >>= 1) {
     __syncthreads();
     if (k < half) red[k][r] = join(red[k][r], red[k + half][r]);
   }
@@ -743,7 +748,9 @@ extern "C" int eth_linear_xent_fwd(const void* h, int64_t ldh, const void* w, in
                        ? xent_forward<true>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden, vocab, s)
                        : xent_forward<false>((const uint16_t*)h, ldh, (const uint16_t*)w, ldw, p, ws, rows, hidden, vocab, s);
   if (done != ETH_OK) return done;
-  xent_join_kernel<<<(unsigned)((rows + 15) / 16), kJoinThreads, 0, s>>>(
+  const bool few = rows <= kFewRows && p.parts >= kManyParts;
+  const auto join_rows = few ? xent_join_kernel<2> : xent_join_kernel<16>;
+  join_rows<<<(unsigned)(few ? (rows + 1) / 2 : (rows + 15) / 16), kJoinThreads, 0, s>>>(
       (const XentHead*)ws, (const int*)(ws + p.rows), (const XentPart*)(ws + p.part), (const float*)(ws + p.picked),
       (int)p.parts, loss, lse);
   ETH_CHECK_LAUNCH("eth_linear_xent_fwd");

@@ -58,7 +58,7 @@ def _check(h, w, labels, loss, dloss, dh, dw, dw_type=None):
 @pytest.mark.parametrize("rows,H,V,ignored", [
     (1, 8, 1, 0.0), (1, 64, 2, 0.0), (2, 8, 7, 0.0), (3, 72, 129, 0.0), (16, 64, 256, 0.5), (17, 136, 1001, 0.3),
     (64, 128, 5000, 0.0), (65, 40, 4097, 0.1), (130, 256, 3001, 0.6), (300, 200, 2500, 0.0), (257, 1024, 513, 0.02),
-    (1000, 64, 9000, 0.2), (700, 96, 20001, 0.0),
+    (1000, 64, 9000, 0.2), (700, 96, 20001, 0.0), (1, 16, 40001, 0.0), (37, 24, 30000, 0.1),
 ])
 def test_loss_and_gradients(cuda, dtype, rows, H, V, ignored):
     announce(f"linear xent {dtype} rows={rows} H={H} V={V} ignored={ignored}")
