@@ -134,8 +134,8 @@ __device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_ti
 
 // RB: blocks of 16 ranks; W waves, each with a range of the workgroup's depth: 32
 // rows alone would be 32 x r / 256 results a workgroup for a depth of thousands, so
-// the depth is what is shared.  Rank 16, [8192, 2048] 14.6 us, [8192, 8192] 41, 3.3
-// TB/s of x; rank 64, [3000, 4096] 8.9, where every tile reads its adapter's 512 KB.
+// the depth is what is shared.  Rank 16, [8192, 2048] 14 us, [8192, 8192] 34, 3.9
+// TB/s of x; rank 64, [3000, 4096] 9, where every tile reads its adapter's 512 KB.
 // Neighbouring workgroups have the pieces of a tile's depth: with eight, each XCD
 // reads its own piece of every adapter, which its L2 holds.
 // P: tiles of a workgroup, in one pass over the depth where they are one adapter's.
@@ -697,25 +697,33 @@ static int launch_adapted(const ProductPlan& p, GemmArgs a, const X& x, float* p
 
 // From this many tiles on, and 33 ranks, a workgroup of the shrink takes two: their
 // adapter's values, which L2 hands out again for every tile, serve both.  One / two
-// (us, the whole of the adapters' share of a forward call): [16384, 4096] rank 128
-// 80 / 65, [8192, 4096] 48 / 40, rank 64 33 / 30; of fewer tiles the depth's pieces
-// get shorter, and of short segments pairs are often of two adapters, taken one after
-// the other: [4000, 4096] rank 64 of one adapter 22 / 18, [3000, 4096] of four 14 / 21.
+// (us, the adapters' share of a forward call): [16384, 4096] rank 128 78 / 54, rank 64
+// 48 / 36, [8192, 4096] rank 128 42 / 37, rank 64 26 / 27.  Of short segments pairs are
+// often of two adapters, taken one after the other: [3000, 4096] of four of rank 64
+// 14 / 21.
 constexpr int kPairedTiles = 128;
 
-// Pieces of the shrink's depth: as many as bring four workgroups a compute unit
-// (two from 33 ranks on, whose LDS leaves room for two), each of two trips of its
-// waves at least.
+// Pieces of the shrink's depth: as many as bring three workgroups a compute unit
+// (one from 33 ranks on, where every workgroup reads its adapter's values anew), each
+// of two trips of its waves at least; a depth of fewer than eight trips, 2048 at rank
+// 16, is not worth the second launch (3 us of the host).  One workgroup / two (us, the adapters' share
+// of a forward call): [16384, 4096] rank 128 54 / 65, rank 64 36 / 48, [8192, 4096] 27
+// / 28, [2000, 8192] 25 / 26; below 33 ranks two / three / four: [8192, 8192] rank 16 46
+// / 39 / 37, [16384, 4096] rank 16 26 / 26 / 30, rank 32 33 / 33 / 37.  Four waves a
+// workgroup: with eight, whose sums meet in twice the LDS, [500, 4096] rank 64 took 12.8
+// for 9.9, [2000, 2048] 13.5 for 11.3, [8192, 8192] rank 16 41 for 37 ([3000, 4096]
+// rank 16 11.5 for 12.6).
+constexpr int kShrinkWaves = 4;
 struct ShrinkPlan {
-  int blocks, waves, splits, pairs;
+  int blocks, splits, pairs;
   int64_t workspace;
 };
 static ShrinkPlan plan_shrink(int64_t K, int r, int n_tiles) {
-  ShrinkPlan p{r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8, r <= 64 ? 8 : 4, 1, 0, 0};
+  ShrinkPlan p{r <= 16 ? 1 : r <= 32 ? 2 : r <= 64 ? 4 : 8, 1, 0, 0};
   p.pairs = p.blocks >= 4 && n_tiles >= kPairedTiles;
   const int groups = p.pairs ? (n_tiles + 1) / 2 : n_tiles;
-  const int64_t trips = K / (p.waves * 32 * (p.blocks >= 4 ? 2 : 4)), slots = p.blocks >= 4 ? 512 : 1024;
-  if (n_tiles) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSplits, slots / groups), trips / 2));
+  const int64_t trips = K / (kShrinkWaves * 32 * (p.blocks >= 4 ? 2 : 4)), slots = p.blocks >= 4 ? 256 : 768;
+  if (n_tiles && trips >= 8) p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(kMaxSplits, slots / groups), trips / 2));
   if (p.splits > 1) p.workspace = (int64_t)p.splits * n_tiles * kTileRows * p.blocks * 16 * 4;
   return p;
 }
@@ -726,18 +734,18 @@ static int launch_shrink(ShrinkArgs g, int n_tiles, float* partials, hipStream_t
   g.splits = p.splits;
   g.n_tiles = n_tiles;
   const unsigned grid = (unsigned)((p.pairs ? (n_tiles + 1) / 2 : n_tiles) * p.splits);
-#define ETH_SHRINK(RB, W, P)                                                      \
-  {                                                                               \
-    adapter_shrink_kernel<RB, W, P, FP16><<<grid, 64 * W, 0, s>>>(g);             \
-    ETH_CHECK_LAUNCH("eth_adapter_linear");                                       \
-    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g); \
+#define ETH_SHRINK(RB, P)                                                                   \
+  {                                                                                         \
+    adapter_shrink_kernel<RB, kShrinkWaves, P, FP16><<<grid, 64 * kShrinkWaves, 0, s>>>(g); \
+    ETH_CHECK_LAUNCH("eth_adapter_linear");                                                 \
+    if (p.splits > 1) adapter_narrow_kernel<RB, FP16><<<n_tiles, 256, 0, s>>>(g);           \
   }
-  if (p.blocks == 1) ETH_SHRINK(1, 8, 1)
-  else if (p.blocks == 2) ETH_SHRINK(2, 8, 1)
-  else if (p.blocks == 4 && p.pairs) ETH_SHRINK(4, 8, 2)
-  else if (p.blocks == 4) ETH_SHRINK(4, 8, 1)
-  else if (p.pairs) ETH_SHRINK(8, 4, 2)
-  else ETH_SHRINK(8, 4, 1)
+  if (p.blocks == 1) ETH_SHRINK(1, 1)
+  else if (p.blocks == 2) ETH_SHRINK(2, 1)
+  else if (p.blocks == 4 && p.pairs) ETH_SHRINK(4, 2)
+  else if (p.blocks == 4) ETH_SHRINK(4, 1)
+  else if (p.pairs) ETH_SHRINK(8, 2)
+  else ETH_SHRINK(8, 1)
 #undef ETH_SHRINK
   ETH_CHECK_LAUNCH("eth_adapter_linear");
   return ETH_OK;
