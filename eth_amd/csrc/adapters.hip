@@ -134,7 +134,7 @@ __device__ __forceinline__ void narrow(const ShrinkArgs& g, const eth_adapter_ti
 
 // RB: blocks of 16 ranks; W waves, each with a range of the workgroup's depth: 32
 // rows alone would be 32 x r / 256 results a workgroup for a depth of thousands, so
-// the depth is what is shared.  Rank 16, [8192, 2048] 14 us, [8192, 8192] 34, 3.9
+// the depth is what is shared.  Rank 16, [8192, 2048] 14 us, [8192, 8192] 39, 3.4
 // TB/s of x; rank 64, [3000, 4096] 9, where every tile reads its adapter's 512 KB.
 // Neighbouring workgroups have the pieces of a tile's depth: with eight, each XCD
 // reads its own piece of every adapter, which its L2 holds.
