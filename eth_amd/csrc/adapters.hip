@@ -504,11 +504,6 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
   for (int j = 0; j < RB; ++j)
 #pragma unroll
     for (int f = 0; f < 8; ++f) acc[j][f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // (fp16) the chunk's largest power of two: its sums are without it, and tiles of
-  // smaller ones are taken down to it (losing what the sums would not hold)
-  float have = 0.f;
-  if (FP16)
-    for (int k = 0; k < c.tiles; ++k) have = fmaxf(have, g.tile_scale[c.first + k]);
   for (int k = wid; k < c.tiles; k += 4) {
     const int at = c.first + k;
     const eth_adapter_tile_t t = args.tiles[at];
@@ -522,22 +517,43 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
     const uint16_t* ut = g.ut + (int64_t)at * args.rp * kTileRows + lg * 8;
 #pragma unroll
     for (int j = 0; j < RB; ++j) fu[j] = *reinterpret_cast<const uint4*>(ut + (j * 16 + l16) * kTileRows);
-    if (FP16) {
-      typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-      const _Float16 f = (_Float16)(g.tile_scale[at] / have);
-#pragma unroll
-      for (int j = 0; j < RB; ++j) fu[j] = __builtin_bit_cast(uint4, __builtin_bit_cast(half8, fu[j]) * f);
-    }
+    // (fp16) a tile's products get its power of two in fp32: brought to that of other
+    // tiles in u's 16 bits, small tiles beside large ones or zeros lost their digits
+    const float scale = FP16 ? g.tile_scale[at] : 1.f;
     // eight rows of eight columns -> a column's eight rows
+    f32x4_t had[RB];
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
       const uint4 fq = column_of(row, f);
+      if (!FP16) {
 #pragma unroll
-      for (int j = 0; j < RB; ++j) acc[j][f] = mfma16<FP16>(fu[j], fq, acc[j][f]);
+        for (int j = 0; j < RB; ++j) acc[j][f] = mfma16<FP16>(fu[j], fq, acc[j][f]);
+        continue;
+      }
+      f32x4_t now[RB];
+#pragma unroll
+      for (int j = 0; j < RB; ++j) now[j] = mfma16<FP16>(fu[j], fq, f32x4_t{0.f, 0.f, 0.f, 0.f});
+      // (up to 64 ranks a column's products are under way while those of the one before
+      // are added, 45.3 -> 43.1 us of rank 64's gradients; above, registers are short:
+      // 182 -> 202 us)
+      if (RB >= 8) {
+#pragma unroll
+        for (int j = 0; j < RB; ++j) acc[j][f] += now[j] * scale;
+        continue;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < RB; ++j) {
+        if (f) acc[j][f - 1] += had[j] * scale;
+        had[j] = now[j];
+      }
+    }
+    if (FP16 && RB < 8) {
+#pragma unroll
+      for (int j = 0; j < RB; ++j) acc[j][7] += had[j] * scale;
     }
   }
   // the waves' sums, one wave after the other
-  const float back = FP16 ? have : 1.f;
   for (int w = 0; w < 4; ++w) {
     if (w == wid) {
 #pragma unroll
@@ -547,8 +563,6 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
           f32x4_t* s = reinterpret_cast<f32x4_t*>(&sum[j * 16 + lg * 4 + e][l16 * 8]);
           f32x4_t lo = {acc[j][0][e], acc[j][1][e], acc[j][2][e], acc[j][3][e]};
           f32x4_t hi = {acc[j][4][e], acc[j][5][e], acc[j][6][e], acc[j][7][e]};
-          lo *= back;
-          hi *= back;
           if (w) {
             lo += s[0];
             hi += s[1];
