@@ -514,9 +514,10 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
     for (int i = 0; i < 8; ++i)
       row[i] = load8(qs, r0 + i < t.rows && col < g.C ? (int32_t)(((r0 + i) * g.ldq + col) * 2) : kOob);
     uint4 fu[RB];
-    const uint16_t* ut = g.ut + (int64_t)at * args.rp * kTileRows + lg * 8;
+    // (zeros past the tile's rp ranks: 72 to 96 ranks are 96 there and 128 here)
+    const rsrc_t us = make_rsrc(g.ut + (int64_t)at * args.rp * kTileRows, (uint32_t)(args.rp * kTileRows * 2));
 #pragma unroll
-    for (int j = 0; j < RB; ++j) fu[j] = *reinterpret_cast<const uint4*>(ut + (j * 16 + l16) * kTileRows);
+    for (int j = 0; j < RB; ++j) fu[j] = load8(us, ((j * 16 + l16) * kTileRows + lg * 8) * 2);
     // (fp16) a tile's products get its power of two in fp32: brought to that of other
     // tiles in u's 16 bits, small tiles beside large ones or zeros lost their digits
     const float scale = FP16 ? g.tile_scale[at] : 1.f;
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(256) adapter_outer_kernel(OuterArgs args) {
       for (int j = 0; j < RB; ++j) now[j] = mfma16<FP16>(fu[j], fq, f32x4_t{0.f, 0.f, 0.f, 0.f});
       // (up to 64 ranks a column's products are under way while those of the one before
       // are added, 45.3 -> 43.1 us of rank 64's gradients; above, registers are short:
-      // 182 -> 202 us)
+      // 179 -> 202 us)
       if (RB >= 8) {
 #pragma unroll
         for (int j = 0; j < RB; ++j) acc[j][f] += now[j] * scale;
