@@ -510,7 +510,7 @@ using namespace eth;
 
 extern "C" {
 
-int eth_abi_version(void) { return 1; }
+int eth_abi_version(void) { return 2; }
 
 const char* eth_last_error(void) { return g_last_error.c_str(); }
 

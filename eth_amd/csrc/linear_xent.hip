@@ -28,6 +28,10 @@
 // fp16 as in bf16.  (A row's share of dW loses digits where its dloss is 2^-14
 // of the largest and nothing else reaches the same row of dW.)
 //
+// The label's dz, p - 1, is the forward's loss: -(1 - exp(-loss)).  By way of lse,
+// whose rounding is up to 2^-24 of it, 1 - p of a confident row would be that far off:
+// at a logit of 100 by 5e-6, 5 % of a 1 - p of 1e-4.
+//
 // dz's rounding is dh's and dW's largest error (1.4 roundings with their own). It
 // averages over the rows; where few take part they are listed twice, and dz is
 // stored in two parts, its rounding and what that left, which the same products
@@ -141,8 +145,8 @@ struct XentStats {
 };
 
 // (362 us for 2048 rows, hidden 2048, vocabulary 50304, where the product that
-// stores z takes 346.)  dz in place of z: mult (2^(z log2 e - lse2) - [v = label]), zero past the
-// vocabulary.
+// stores z takes 346.)  dz in place of z: mult 2^(z log2 e - lse2), of the label mult
+// (p - 1), zero past the vocabulary.
 struct XentGrad {
   static constexpr bool kSized = true, kGathers = true, kStarts = false, kMaps = true, kReduces = false;
   const XentHead* head;
@@ -150,6 +154,7 @@ struct XentGrad {
   const int* label;
   const float* lse2;
   const float* mult;
+  const float* miss;  // the label's p - 1
   int v0;      // the piece's first column in the vocabulary
   int n_real;  // columns of the vocabulary in it
   int twice;   // odd rows hold what the rounding of the even ones left
@@ -163,13 +168,14 @@ struct XentGrad {
   __device__ __forceinline__ void map(f32x4_t (&acc)[TI][TJ], int row0, int col0, int M, int) const {
     const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
     const bool edge = col0 + TJ * 16 > n_real;
-    float at[TI], f[TI];
+    float at[TI], f[TI], q[TI];
     int t[TI];
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       const int row = min(row0 + i * 16 + l16, M - 1);  // (rows past M are not stored)
       at[i] = lse2[row];
       f[i] = mult[row];
+      q[i] = miss[row];
       t[i] = label[row] - v0 - col0;
     }
 #pragma unroll
@@ -184,7 +190,7 @@ struct XentGrad {
         for (int j = 0; j < TJ; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (t[i] == j * 16 + lg * 4 + e) acc[i][j][e] -= 1.f;
+            if (t[i] == j * 16 + lg * 4 + e) acc[i][j][e] = q[i];
       }
 #pragma unroll
       for (int j = 0; j < TJ; ++j) acc[i][j] *= f[i];
@@ -255,11 +261,12 @@ struct XentList {
   float* loss;  // forward
   int* bad;
   const float* dloss;  // backward
-  const float* lse;
+  const float* lse;    // [2][n], the loss behind it
   int* at;
   int* exps;
   float* lse2;
   float* mult;
+  float* miss;
   float* back;
   int shift;  // dz's power of two
   int twice;  // every row is listed twice (backward)
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
         if (!back) continue;
         g.exps[to] = e;
         g.lse2[to] = g.lse[r];
+        g.miss[to] = expm1f(-g.lse[g.n + r]);
         g.mult[to] = ldexpf(d[u], g.shift - e);
         g.back[to] = ldexpf(1.f, e - g.shift);
       }
@@ -348,7 +356,7 @@ __global__ void __launch_bounds__(kListThreads) xent_list_kernel(XentList g) {
 
 // ------------------------------------------------------------------ join --
 // A workgroup joins R rows: 1024 / R threads a row, some parts of each in flight,
-// then a tree.  `lse` in the log2 domain.  Latency: 4.0 us for 2048 rows of 393 parts.
+// then a tree.  `lse` [2][n]: in the log2 domain, then the loss.  Latency: 4.0 us for 2048 rows of 393 parts.
 // A whole 16 rows' lines lie together, but few rows of many parts are done sooner two
 // a workgroup (forward, 16 / 2, us): one row of 50304 44.6 / 42.8, of 131072 35.2 /
 // 30.6, 64 rows 47.7 / 46.4 and 34.5 / 31.5; 64 rows of 1000 12.0 / 12.3, 256 of 131072
@@ -362,7 +370,7 @@ __device__ __forceinline__ XentPart join(XentPart a, XentPart b) {
 template <int R>
 __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead* head, const int* rows,
                                                                  const XentPart* part, const float* picked, int parts,
-                                                                 float* loss, float* lse) {
+                                                                 float* loss, float* lse, int64_t n_rows) {
   __shared__ XentPart red[kJoinThreads / R][R];
   const int r = threadIdx.x % R, k = threadIdx.x / R, row = blockIdx.x * R + r, n = head->count;
   if ((int)blockIdx.x * R >= n) return;
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(kJoinThreads) xent_join_kernel(const XentHead*
     const float l = log2f(t.s);  // (near one the instruction alone is off by more than s is)
     // (apart from each other the large terms cancel exactly first)
     const int64_t o = rows[row];
-    loss[o] = kLn2 * (__builtin_fmaf(-picked[row], kLog2e, t.m2) + l);
+    loss[o] = lse[n_rows + o] = kLn2 * (__builtin_fmaf(-picked[row], kLog2e, t.m2) + l);
     lse[o] = t.m2 + l;
   }
 }
@@ -536,7 +544,7 @@ struct XentBackward {
   int64_t k_split;
   int pieces;
   int64_t piece, last, ldz;  // columns of a piece, of the last one, of their rows
-  int64_t rows, label, at, exps, lse2, mult, back, gathered, dz, dh, bytes;
+  int64_t rows, label, at, exps, lse2, mult, miss, back, gathered, dz, dh, bytes;
 };
 static XentBackward plan_backward(int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw, bool need_dh, bool need_dw) {
   XentBackward p;
@@ -564,7 +572,7 @@ static XentBackward plan_backward(int64_t rows, int64_t hidden, int64_t vocab, i
   p.k_split = up((first + p.splits - 1) / p.splits, 64);
   p.splits = (int)((first + p.k_split - 1) / p.k_split);
   int64_t o = room(sizeof(XentHead));
-  for (int64_t* at : {&p.rows, &p.label, &p.at, &p.exps, &p.lse2, &p.mult, &p.back}) *at = o, o += room(n * 4);
+  for (int64_t* at : {&p.rows, &p.label, &p.at, &p.exps, &p.lse2, &p.mult, &p.miss, &p.back}) *at = o, o += room(n * 4);
   p.gathered = o, o += need_dw ? room(n * hidden * 2) : 0;
   p.dz = o, o += room(n * p.ldz * 2);
   p.dh = o, o += need_dh ? room(p.splits * n * hidden * 4) : 0;
@@ -659,7 +667,7 @@ static int xent_backward(const uint16_t* h, int64_t ldh, const uint16_t* w, int6
       a.c_dtype = FP16 ? ETH_F16 : ETH_BF16;
       a.c_vec = true;
       const XentGrad grad{head, rows, (const int*)(ws + p.label), (const float*)(ws + p.lse2),
-                          (const float*)(ws + p.mult), (int)(v0 + c0), (int)there, p.twice};
+                          (const float*)(ws + p.mult), (const float*)(ws + p.miss), (int)(v0 + c0), (int)there, p.twice};
       return launch_product<true, true, FP16, false>(tile, a, grad, s);
     };
     const XentCut zc = cut_columns(n, cols, hidden, GemmForm{false, hidden % 64 != 0, 0});
@@ -752,7 +760,7 @@ extern "C" int eth_linear_xent_fwd(const void* h, int64_t ldh, const void* w, in
   const auto join_rows = few ? xent_join_kernel<2> : xent_join_kernel<16>;
   join_rows<<<(unsigned)(few ? (rows + 1) / 2 : (rows + 15) / 16), kJoinThreads, 0, s>>>(
       (const XentHead*)ws, (const int*)(ws + p.rows), (const XentPart*)(ws + p.part), (const float*)(ws + p.picked),
-      (int)p.parts, loss, lse);
+      (int)p.parts, loss, lse, rows);
   ETH_CHECK_LAUNCH("eth_linear_xent_fwd");
   return ETH_OK;
 }
@@ -785,6 +793,7 @@ extern "C" int eth_linear_xent_bwd(const void* h, int64_t ldh, const void* w, in
   list.exps = (int*)(ws + p.exps);
   list.lse2 = (float*)(ws + p.lse2);
   list.mult = (float*)(ws + p.mult);
+  list.miss = (float*)(ws + p.miss);
   list.back = (float*)(ws + p.back);
   list.shift = dtype == ETH_F16 ? 14 : 0;
   list.twice = p.twice;

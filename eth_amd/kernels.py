@@ -974,14 +974,16 @@ def _check_head(hidden2d, weight, labels, *ts):
 
 
 def linear_xent_fwd(hidden2d, weight, labels, bad_flag, ignore_index=-100):
-    """(loss [rows], lse [rows]) in fp32 of the cross entropy of logits hidden2d
-    [rows, H] @ weight[V, H]^T, which are not kept, against int64 labels [rows].
+    """(loss [rows], lse [2, rows]) in fp32 of the cross entropy of logits hidden2d
+    [rows, H] @ weight[V, H]^T, which are not kept, against int64 labels [rows]; lse,
+    for the backward, is the logits' logsumexp (log2 domain) and the loss again.
     Rows with label `ignore_index` have loss 0 and are not read; other labels
     outside the vocabulary are clamped and flagged in `bad_flag`."""
     index, code, rows, H, V, ldh, ldw = _check_head(hidden2d, weight, labels, bad_flag)
     if bad_flag.dtype != torch.int32 or bad_flag.numel() < 1:
         raise ValueError("bad_flag must be an int32 tensor")
-    loss, lse = torch.empty(2, rows, dtype=torch.float32, device=hidden2d.device)
+    loss = torch.empty(rows, dtype=torch.float32, device=hidden2d.device)
+    lse = torch.empty(2, rows, dtype=torch.float32, device=hidden2d.device)
     if rows:
         ws = nat.value("eth_linear_xent_workspace", rows, H, V, ldw, 0)
         ws = torch.empty(ws, dtype=torch.uint8, device=hidden2d.device)
@@ -997,7 +999,8 @@ def linear_xent_bwd(hidden2d, weight, labels, lse, dloss, ignore_index=-100, nee
     needed: in the operands' type, or dweight into a given fp32 tensor, stored or
     added."""
     index, code, rows, H, V, ldh, ldw = _check_head(hidden2d, weight, labels, lse, dloss)
-    _check_row_values("lse", lse, rows)
+    if lse.dtype != torch.float32 or lse.shape != (2, rows) or not lse.is_contiguous():
+        raise ValueError("lse must be the forward's fp32 [2, rows]")
     _check_row_values("dloss", dloss, rows)
     if dweight is not None:
         _check_device(index, dweight)
