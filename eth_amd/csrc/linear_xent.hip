@@ -551,16 +551,21 @@ static XentBackward plan_backward(int64_t rows, int64_t hidden, int64_t vocab, i
   p.twice = rows <= kTwiceRows;
   const int64_t n = p.n = rows << p.twice;
   int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
-  most = std::min(most, reach(std::max(ldw, hidden)));
+  const int64_t within = reach(std::max(ldw, hidden));
+  most = std::min(most, within);
   // whole rounds of dW's tiles where they fit
   const int64_t tn = (hidden + 255) / 256;
   int64_t unit = 256;
   while (unit < 65536 && unit / 256 * tn % 256) unit *= 2;
   const int64_t whole = most >= unit ? most / unit * unit : most;
   // equal pieces of at most that, or whole ones and a last one of half to three halves
-  const int64_t many = std::max<int64_t>(1, (vocab + whole / 2 - 1) / whole);
+  int64_t many = std::max<int64_t>(1, (vocab + whole / 2 - 1) / whole);
   p.piece = std::min(up(vocab, 8), whole);
   p.last = vocab - (many - 1) * p.piece;
+  if (p.last > within) {  // (what a launch's offsets do not reach is a short piece of its own)
+    ++many;
+    p.last -= p.piece;
+  }
   p.pieces = (int)many;
   p.ldz = up(std::max(p.piece, p.last), 8);
   // dh has few tiles and a deep product: split until the chip is full

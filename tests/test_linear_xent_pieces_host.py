@@ -1,0 +1,33 @@
+"""CPU: the pieces of the vocabulary that the linear head's cross entropy takes in
+its backward.  A launch reaches a piece's weights by 32-bit offsets whose upper half
+stands for "not there, zero": every piece, the last and longest too, lies within 2 GiB."""
+
+import itertools
+
+import pytest
+
+from eth_amd import _native as nat
+
+REACH = 2**31 - 1
+
+
+def _columns(rows, hidden, vocab, ldw):
+    """At least so many columns the longest piece has, by the workspace (lists, the
+    rows of h, and dz [rows, the longest piece in 8s], each in 256s)."""
+    n = 2 * rows if rows <= 64 else rows
+    room = lambda b: -(-b // 256) * 256  # noqa: E731
+    rest = room(12) + 8 * room(4 * n) + room(2 * n * hidden)
+    dz = nat.value("eth_linear_xent_workspace", rows, hidden, vocab, ldw, 2) - rest
+    assert dz >= 2 * n * min(vocab, 256)
+    return max(min(vocab, 256), (dz - 255) // (2 * n) - 7)
+
+
+@pytest.mark.parametrize("hidden", [64, 2048, 4096, 5376, 8192, 12288, 16384, 65536])
+def test_pieces_lie_within_reach(hidden):
+    for rows, vocab in itertools.product((1, 33, 64, 65, 128, 500, 700, 1024, 1500, 2048, 8192, 16384),
+                                         (1, 257, 32000, 50304, 65537, 100000, 128000, 131073, 152064, 196609, 262144, 2**24)):
+        if rows * hidden > 2**30:
+            continue
+        for ldw in {hidden, hidden + 8, 2 * hidden, 32768 if hidden < 32768 else hidden}:
+            columns = _columns(rows, hidden, vocab, ldw)
+            assert 2 * ((columns - 1) * ldw + hidden) <= REACH, (rows, hidden, vocab, ldw, columns)
