@@ -482,8 +482,9 @@ constexpr int64_t kPieceBytes = 256LL << 20;
 static int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 static int64_t room(int64_t bytes) { return up(bytes, 256); }
 
-// Columns of W that a launch's 32-bit offsets reach, whole 256s.
-static int64_t reach(int64_t ldw) { return std::max<int64_t>(256, kMaxBytes / (2 * ldw) / 256 * 256); }
+// Columns of W that a launch's 32-bit offsets reach, whole 256s (check_xent: one of them
+// at least).
+static int64_t reach(int64_t ldw) { return std::max<int64_t>(256, kMaxBytes / 2 / ldw / 256 * 256); }
 
 // The product [M, N] x K deep in whole rounds of 256x256 tiles and a rest along N
 // in its own best tile, where the time model promises 2 %: `first` columns, then the
@@ -592,6 +593,10 @@ static int check_xent(const char* name, const void* h, int64_t ldh, const void* 
   ETH_CHECK_ARG(n > 0 && hidden > 0 && vocab > 0 && n < (1LL << 21) && vocab <= (1LL << 24) && hidden < (1LL << 20),
                 "%s: bad shape: %lld rows, hidden %lld, vocabulary %lld", name, (long long)n, (long long)hidden,
                 (long long)vocab);
+  // (a launch takes 256 rows of W at least)
+  const int64_t apart = std::min<int64_t>(vocab, 256) - 1;
+  ETH_CHECK_ARG(apart == 0 || ldw <= (kMaxBytes / 2 - hidden) / apart,
+                "%s: rows of W %lld elements apart: 256 of them above 2 GiB are not supported", name, (long long)ldw);
   ETH_CHECK_ARG(h && w && labels && workspace, "%s: null operand", name);
   ETH_CHECK_ARG(hidden % 8 == 0 && ldh % 8 == 0 && ldw % 8 == 0 && ldh >= hidden && ldw >= hidden,
                 "%s: hidden (%lld) and row strides (%lld, %lld) must be multiples of 8", name, (long long)hidden,

@@ -660,7 +660,8 @@ int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_
 /* Cross entropy of a linear head whose logits z = h w^T are never kept:
  * h [rows, hidden] (row stride ldh), w [vocab, hidden] (row stride ldw), both bf16
  * or fp16 (`dtype`), 16-byte aligned, hidden and strides multiples of 8; rows below
- * 2^21 and 2 GiB, vocab up to 2^24 (w of any size).  Per row, in fp32:
+ * 2^21 and 2 GiB, vocab up to 2^24 (w of any size, 256 of its rows within 2 GiB).  Per
+ * row, in fp32:
  *   loss = log sum exp z - z[label],
  * and for the backward lse [2, rows]: log sum exp z (log2 domain), then the loss again.
  * Rows whose label is `ignore_index` are not read and have loss 0 (their lse is

@@ -31,3 +31,22 @@ def test_pieces_lie_within_reach(hidden):
         for ldw in {hidden, hidden + 8, 2 * hidden, 32768 if hidden < 32768 else hidden}:
             columns = _columns(rows, hidden, vocab, ldw)
             assert 2 * ((columns - 1) * ldw + hidden) <= REACH, (rows, hidden, vocab, ldw, columns)
+
+
+def _call(name, rows, hidden, vocab, ldw, h):
+    P = 1 << 20
+    last = (rows, hidden, vocab, P, nat.ETH_BF16, None) if name.endswith("fwd") else (rows, hidden, vocab, nat.ETH_BF16, None)
+    first = (h, hidden, P, ldw, P, -100, P, P)
+    nat.call(name, *first, *((P,) if name.endswith("fwd") else (P, P, nat.ETH_BF16, 0, P)), *last)
+
+
+@pytest.mark.parametrize("name", ["eth_linear_xent_fwd", "eth_linear_xent_bwd"])
+def test_weights_too_far_apart_are_refused(name):
+    """256 rows of W, the least that a launch takes, within 2 GiB; what is within
+    is refused for its null operand alone, ahead of any launch."""
+    for vocab, ldw in ((256, 2**22 + 2**15), (300, 2**22 + 2**15), (50304, 2**23), (2**24, 2**40), (2, 2**30 - 64), (2, 2**62)):
+        with pytest.raises(ValueError, match="apart"):
+            _call(name, 4, 64, vocab, ldw, 1 << 20)
+    for vocab, ldw in ((1, 2**40), (2, 2**30 - 72), (256, 2**22), (50304, 2**22)):
+        with pytest.raises(ValueError, match="null"):
+            _call(name, 4, 64, vocab, ldw, None)
