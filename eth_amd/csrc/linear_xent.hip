@@ -476,7 +476,8 @@ static int launch_product(int tile, const GemmArgs& args, const X& x, hipStream_
 }
 
 constexpr int64_t kMaxBytes = (1LL << 31) - 1;
-// Workspace for a piece of dz, at most (a piece is 256 columns at least).
+// Workspace for a piece of dz, the last one apart, which may be half as long again (a
+// piece is 256 columns at least).
 constexpr int64_t kPieceBytes = 256LL << 20;
 
 static int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }

@@ -676,7 +676,7 @@ int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_
  * gradients of any size keep their digits; up to 64 rows in two parts); sums are fp32,
  * in a fixed order.
  * `workspace`: eth_linear_xent_workspace bytes, 256-byte aligned (grads: 0 for the
- * forward, or 1 for dh + 2 for dw; at most about 256 MiB for a piece of dz, or 512
+ * forward, or 1 for dh + 2 for dw; at most about 384 MiB for a piece of dz, or 768
  * bytes a row, beside a row of fp32 dh for up to 16 splits and a copy of h). */
 int64_t eth_linear_xent_workspace(int64_t rows, int64_t hidden, int64_t vocab, int64_t ldw,
                                   int grads);

@@ -50,3 +50,19 @@ def test_weights_too_far_apart_are_refused(name):
     for vocab, ldw in ((1, 2**40), (2, 2**30 - 72), (256, 2**22), (50304, 2**22)):
         with pytest.raises(ValueError, match="null"):
             _call(name, 4, 64, vocab, ldw, None)
+
+
+def test_stated_workspace():
+    """Without dh: a piece of dz, whole ones of 256 MiB (or of 256 columns, 512 bytes
+    a row) and a last one half as long again, a copy of h, and the lists."""
+    worst = 0.0
+    for rows, vocab in itertools.product((1, 64, 65, 1000, 2047, 2048, 4096, 8192, 16384, 30000, 2**19, 2**21 - 1),
+                                         (1, 1000, 24575, 24576, 50257, 98303, 151936, 262143, 2**20)):
+        for hidden in (64, 512, 2048, 4096):
+            n = 2 * rows if rows <= 64 else rows
+            lists = 8 * (4 * n + 256) + 512
+            dz = nat.value("eth_linear_xent_workspace", rows, hidden, vocab, hidden, 2) - lists - 2 * n * hidden
+            most = max(384 << 20, 768 * n) + 16 * n
+            assert dz <= most, (rows, hidden, vocab, dz >> 20)
+            worst = max(worst, dz / most)
+    assert worst > 0.9
