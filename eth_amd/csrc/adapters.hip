@@ -18,9 +18,9 @@
 // u is rounded to 16 bits, the matrix cores' operand: with their own rounding dA
 // and dB are 1.4 roundings from exact.  It averages over the rows; tiles of up to 16
 // rows, half of whose depth in those products is free, hold there what it left.  In
-// fp16 a tile's u carries
-// a power of two that puts its largest value at 2^13 to 2^14, so that it keeps its
-// digits whatever the size of gradients and adapters.
+// fp16 a tile's u carries a power of two that puts its largest value at 2^13 to 2^14,
+// taken back in fp32 from each tile's products, so that it keeps its digits whatever
+// the size of gradients and adapters, and of the tiles beside it.
 //
 // No counterpart in the reference, whose linear layers (mpu/layers.py:357-370,
 // 452-470) have one weight for all rows.
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(256) adapter_turn_kernel(TurnArgs a, TurnArgs 
 // part[chunk][r][C] = sum over the chunk's tiles of u^T q, for dA (q = x) and dB
 // (q = dy) in one launch: 128 columns a workgroup, its four waves taking tiles in
 // turn.  Rank 16, x [8192, 2048] and dy [8192, 8192]: 30.4 us, 5.5 TB/s; rank 64, 2000
-// rows of 8192 and 2048 in a chunk for each of eight adapters: 21.2 us, 640 workgroups
+// rows of 8192 and 2048 in a chunk for each of eight adapters: 19.8 us, 640 workgroups
 // whose waves have one or two tiles: latency.
 struct OuterSide {
   const uint16_t* ut;

@@ -673,8 +673,9 @@ int eth_topk_distill_bwd(const void* logits, int64_t ld, const int64_t* teacher_
  * is not wanted; dw in `dtype`, or fp32 (then stored, or added to with `accumulate`).
  * Rows that are ignored or whose dloss is zero get dh 0 and take no part in dw.
  * dz is rounded to 16 bits for the products (a row's dloss enters as a mantissa, so
- * gradients of any size keep their digits; up to 64 rows in two parts); sums are fp32,
- * in a fixed order.
+ * gradients of any size keep their digits, but in fp16 dw's share of a row whose dloss
+ * is below 2^-14 of the largest; up to 64 rows in two parts); sums are fp32, in a fixed
+ * order.
  * `workspace`: eth_linear_xent_workspace bytes, 256-byte aligned (grads: 0 for the
  * forward, or 1 for dh + 2 for dw; at most about 384 MiB for a piece of dz, or 768
  * bytes a row, beside a row of fp32 dh for up to 16 splits and a copy of h). */
